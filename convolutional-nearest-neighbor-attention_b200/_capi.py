@@ -79,6 +79,15 @@ SIGNATURES = {
                                              c_i64, c_i64, c_i32, c_void]),
     "convnn_b200_linear": (ctypes.c_int, [ctypes.c_int, c_void, c_i64, c_void, c_void, c_void, c_i64, c_void, c_i64,
                                           c_i64, c_i32, c_i32, c_i32, c_void]),
+    "convnn_b200_rms_norm": (ctypes.c_int, [ctypes.c_int, c_void, c_i64, c_void, c_i64, c_void, ctypes.c_float, c_void, c_i64,
+                                            c_void, c_i64, c_i64, c_i32, c_void]),
+    "convnn_b200_rms_norm_fp8": (ctypes.c_int, [ctypes.c_int, c_void, c_i64, c_void, c_i64, c_void, ctypes.c_float, c_void,
+                                                c_i64, c_void, c_i64, c_void, c_i64, c_i64, c_i64, c_i32, c_void]),
+    "convnn_b200_quantize_fp8": (ctypes.c_int, [ctypes.c_int, c_void, c_i64, c_i32, c_void, c_i64, c_void, c_i64, c_i64, c_i64,
+                                                c_i32, c_void]),
+    "convnn_b200_linear_fp8": (ctypes.c_int, [c_void, c_i64, c_void, c_i64, c_i64, c_void, c_i64, c_void, c_i64, c_i64,
+                                              ctypes.c_int, c_void, c_void, c_i64, c_void, c_i64, c_void, c_i64, c_i64, c_i64,
+                                              c_i32, c_i32, c_i32, c_void]),
     "convnn_b200_patchify": (ctypes.c_int, [ctypes.c_int, c_void, c_void, c_i32, c_i32, c_i32, c_i32, c_i32, c_void]),
     "convnn_b200_patchify_u8": (ctypes.c_int, [ctypes.c_int, c_void, c_void, c_void, c_void, c_i32, c_i32, c_i32, c_i32,
                                                c_i32, c_void]),

@@ -242,6 +242,7 @@ int convnn_b200_device_status(int* code) {
     if (!c && (rc = read_mlp_tc_status(&c))) return rc;
     if (!c && (rc = read_conv_std_status(&c))) return rc;
     if (!c && (rc = read_conv1d_tc_status(&c))) return rc;
+    if (!c && (rc = read_linear_fp8_status(&c))) return rc;
     *code = a ? a : (b ? b : c);
     return CONVNN_OK;
 }
@@ -544,6 +545,95 @@ int convnn_b200_linear(int dtype, const void* a, int64_t lda, const void* w, con
                        int64_t ldr, void* out, int64_t ldo, int64_t M, int32_t N, int32_t K, int32_t gelu,
                        void* stream) {
     return linear(dtype, a, lda, w, bias, residual, ldr, out, ldo, M, N, K, gelu, false, stream);
+}
+
+// ---- 8-bit values with a scale per block of 128 ---------------------------------------------------
+
+// Strides of (rows, blocks) float32 scales, in elements; written scales may not share an address.
+static int scales_ok(const char* what, const float* s, int64_t row, int64_t block, bool written) {
+    if (reinterpret_cast<uintptr_t>(s) & 3u) return set_error(CONVNN_E_ALIGN, "%s: scales must be 4-byte aligned", what);
+    if (row < (written ? 1 : 0) || block < (written ? 1 : 0))
+        return set_error(CONVNN_E_INVALID, "%s: strides %lld, %lld of the scales", what, (long long)row, (long long)block);
+    return CONVNN_OK;
+}
+
+static int rms_norm_impl(const char* what, int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                         const void* weight, float eps, void* sum, int64_t lds, void* y, void* q, int64_t ldy, float* scales,
+                         int64_t scale_row, int64_t scale_block, int64_t rows, int32_t D, void* stream) {
+    if (dtype != CONVNN_F32 && dtype != CONVNN_BF16) return set_error(CONVNN_E_INVALID, "unknown dtype %d", dtype);
+    if (!x || !weight || !(q ? (void*)scales : y)) return set_error(CONVNN_E_NULL, "%s: a required pointer is NULL", what);
+    if (!residual != !sum) return set_error(CONVNN_E_NULL, "%s: a residual comes with room for its sum, and no sum without", what);
+    if (rows < 0 || D < 1 || D > (1 << 30) || ldx < D || ldy < D || (residual && (ldr < D || lds < D)))
+        return set_error(CONVNN_E_INVALID, "%s: bad shape", what);
+    if (!(eps >= 0.f)) return set_error(CONVNN_E_INVALID, "%s: eps must not be negative", what);
+    const uintptr_t elt = dtype == CONVNN_F32 ? 3u : 1u;
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(weight) |
+         reinterpret_cast<uintptr_t>(sum) | reinterpret_cast<uintptr_t>(y)) & elt)
+        return set_error(CONVNN_E_ALIGN, "%s: a pointer is not aligned to its type", what);
+    int rc;
+    if (q && (rc = scales_ok(what, scales, scale_row, scale_block, true))) return rc;
+    if ((rc = check_device())) return rc;
+    if (rows == 0) return CONVNN_OK;
+    return launch_rms_norm(dtype, x, ldx, residual, ldr, weight, eps, sum, lds, y, q, ldy, scales, scale_row, scale_block, rows, D,
+                           static_cast<cudaStream_t>(stream));
+}
+
+int convnn_b200_rms_norm(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, float eps,
+                         void* sum, int64_t lds, void* y, int64_t ldy, int64_t rows, int32_t D, void* stream) {
+    return rms_norm_impl("rms_norm", dtype, x, ldx, residual, ldr, weight, eps, sum, lds, y, nullptr, ldy, nullptr, 0, 0, rows, D,
+                         stream);
+}
+
+int convnn_b200_rms_norm_fp8(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                             float eps, void* sum, int64_t lds, void* q, int64_t ldq, float* scales, int64_t scale_row,
+                             int64_t scale_block, int64_t rows, int32_t D, void* stream) {
+    if (!q) return set_error(CONVNN_E_NULL, "rms_norm_fp8: a required pointer is NULL");
+    return rms_norm_impl("rms_norm_fp8", dtype, x, ldx, residual, ldr, weight, eps, sum, lds, nullptr, q, ldq, scales, scale_row,
+                         scale_block, rows, D, stream);
+}
+
+int convnn_b200_quantize_fp8(int dtype, const void* x, int64_t ldx, int32_t block_rows, void* q, int64_t ldq, float* scales,
+                             int64_t scale_row, int64_t scale_block, int64_t rows, int32_t D, void* stream) {
+    if (dtype != CONVNN_F32 && dtype != CONVNN_BF16) return set_error(CONVNN_E_INVALID, "unknown dtype %d", dtype);
+    REQUIRE_PTR(x); REQUIRE_PTR(q); REQUIRE_PTR(scales);
+    if (rows < 0 || D < 1 || D > (1 << 30) || ldx < D || ldq < D) return set_error(CONVNN_E_INVALID, "quantize_fp8: bad shape");
+    if (block_rows != 1 && block_rows != 128)
+        return set_error(CONVNN_E_INVALID, "quantize_fp8: a scale belongs to 1 or 128 rows, not %d", block_rows);
+    if (reinterpret_cast<uintptr_t>(x) & (dtype == CONVNN_F32 ? 3u : 1u))
+        return set_error(CONVNN_E_ALIGN, "quantize_fp8: x is not aligned to its type");
+    int rc = scales_ok("quantize_fp8", scales, scale_row, scale_block, true);
+    if (rc || (rc = check_device())) return rc;
+    if (rows == 0) return CONVNN_OK;
+    return launch_quantize_fp8(dtype, x, ldx, block_rows, q, ldq, scales, scale_row, scale_block, rows, D,
+                               static_cast<cudaStream_t>(stream));
+}
+
+int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, int64_t a_scale_row, int64_t a_scale_block,
+                           const void* w, int64_t ldw, const float* w_scales, int64_t w_scale_row, int64_t w_scale_block,
+                           int dtype, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
+                           float* out_scales, int64_t out_scale_row, int64_t out_scale_block, int64_t M, int32_t N, int32_t K,
+                           int32_t gelu, void* stream) {
+    if (dtype != CONVNN_F32 && dtype != CONVNN_BF16) return set_error(CONVNN_E_INVALID, "unknown dtype %d", dtype);
+    REQUIRE_PTR(a); REQUIRE_PTR(a_scales); REQUIRE_PTR(w); REQUIRE_PTR(w_scales); REQUIRE_PTR(out);
+    if (M < 0 || N < 1 || K < 1 || K > (1 << 30) || N > (1 << 30) || lda < K || ldw < K || ldo < N || (residual && ldr < N))
+        return set_error(CONVNN_E_INVALID, "linear_fp8: bad shape");
+    if (M > (1ll << 30)) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %lld rows", (long long)M);
+    if (!aligned16(a) || !aligned16(w) || lda % 16 || ldw % 16)
+        return set_error(CONVNN_E_ALIGN, "linear_fp8: rows of a and w must start on 16-byte boundaries");
+    const uintptr_t elt = dtype == CONVNN_F32 ? 3u : 1u;
+    if ((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(residual) |
+         (out_scales ? (uintptr_t)0 : reinterpret_cast<uintptr_t>(out))) & elt)
+        return set_error(CONVNN_E_ALIGN, "linear_fp8: a pointer is not aligned to its type");
+    int rc;
+    if ((rc = scales_ok("linear_fp8: a", a_scales, a_scale_row, a_scale_block, false)) ||
+        (rc = scales_ok("linear_fp8: w", w_scales, w_scale_row, w_scale_block, false)) ||
+        (out_scales && (rc = scales_ok("linear_fp8: out", out_scales, out_scale_row, out_scale_block, true))))
+        return rc;
+    if ((rc = check_device())) return rc;
+    if (M == 0) return CONVNN_OK;
+    return launch_linear_fp8(a, lda, a_scales, a_scale_row, a_scale_block, w, ldw, w_scales, w_scale_row, w_scale_block, bias,
+                             residual, ldr, dtype, out, ldo, out_scales, out_scale_row, out_scale_block, (int)M, N, K, gelu,
+                             static_cast<cudaStream_t>(stream));
 }
 
 // ---- LayerNorm folded into the GEMM that consumes it ----------------------------------------------

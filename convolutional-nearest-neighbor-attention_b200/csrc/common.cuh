@@ -313,6 +313,19 @@ int softmax_attention(int dtype, const void* x, int64_t ldx, const void* w_qkv, 
 int conv1d_attention(int dtype, const void* x, int64_t ldx, const void* w_x, const void* b_x, const void* w_conv, const void*
                      b_conv, const void* w_o, const void* b_o, void* out, int64_t ldo, int32_t B, int32_t T, int32_t D,
                      int32_t H, int32_t kernel_size, void* workspace, size_t workspace_bytes, bool at_rest, void* stream);
+// Root-mean-square norm (norm_fp8.cu): y in dtype, or where q is given in 8 bits with scales[row * scale_row + block * scale_block];
+// `ldy` is the row stride of whichever it is.
+int launch_rms_norm(int dtype, const void* x, long long ldx, const void* residual, long long ldr, const void* weight, float eps,
+                    void* sum, long long lds, void* y, void* q, long long ldy, float* scales, long long scale_row,
+                    long long scale_block, long long rows, int D, cudaStream_t st);
+int launch_quantize_fp8(int dtype, const void* x, long long ldx, int block_rows, void* q, long long ldq, float* scales,
+                        long long scale_row, long long scale_block, long long rows, int D, cudaStream_t st);
+// 8-bit product (linear_fp8.cu); io: the type of bias, residual and, where no output scales are given, of the output.
+int launch_linear_fp8(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
+                      long long ldw, const float* sw, long long sw_row, long long sw_block, const void* bias, const void* residual,
+                      long long ldr, int io, void* out, long long ldo, float* so, long long so_row, long long so_block, int M, int N,
+                      int K, int gelu, cudaStream_t st);
+int read_linear_fp8_status(int* out);
 int launch_row_moments(const void* x, long long ldx, long long rows, int D, float* moments, cudaStream_t st);
 int launch_fold_layernorm(const void* w, const void* bias, const void* gamma, const void* beta, int N, int K,
                           void* w_folded, void* w_extra, cudaStream_t st);

@@ -1,0 +1,430 @@
+// Matrix product of 8-bit values (e4m3) with a float32 scale per row of A and block of 128 channels, and per 128 x 128 block of W:
+//   out[m, n] = [gelu](sum_b sa[m, b] sw[n / 128, b] (sum_{k in b} a[m, k] w[n, k]) + bias[n]) + residual[m, n]
+// The inner sums run on tcgen05 (kind::f8f6f4, 128 channels = four instructions = one row of a 128-byte-swizzled tile) into an
+// accumulator of their own in TMEM, which the epilogue warps add up in registers, scaled, in ascending b, while the next block
+// is multiplied into the next buffer.  The scales are any float32 values, so they cannot be the tensor cores' own powers of two.
+// Everything after the sum stays in float32 until the one rounding of the store: to bfloat16, not at all, or to e4m3 under the
+// scale of the row's block of 128 columns.
+//
+// One CTA has a tile of 128 x BN: 128 rows of P, whose rows are TMEM lanes, times BN rows of Q.  P are the activations and
+// BN = 128 (more rows), or P are the weights and Q 16, 32 or 64 tokens (SWAP).  Where tiles are few the CTAs of a cluster share
+// a tile's blocks of k; their partial tiles, in shared memory, are added up in rank order.
+//   warp 0     TMA producer (ring of P and Q blocks)
+//   warp 1     MMA issuer
+//   warps 2-9  scaled sums (two warps per lane quarter, half of the columns each), then with the others the output
+// Every mbarrier wait is bounded (see sm100.cuh); an expiry latches the device status.
+#include "common.cuh"
+#include "sm100.cuh"
+#include "f32x2.cuh"
+#include "fp8.cuh"
+
+namespace convnn {
+
+__device__ int g_linear_fp8_status = 0;   // error latch of this translation unit
+
+namespace {
+
+using namespace sm100;
+
+constexpr int BP = 128;                   // rows of P in a tile
+constexpr int KB = kFp8Block;             // channels (= bytes) of a block
+constexpr int NTHREADS = 320;
+constexpr int MAX_STAGES = 12;
+
+enum OutKind : int { OUT_F32 = 0, OUT_BF16 = 1, OUT_E4M3 = 2 };
+
+struct LinearFp8Params {
+    const float *sa, *sw;                 // scales; strides in elements
+    long long sa_row, sa_block, sw_row, sw_block;
+    const void *bias, *residual;          // of `io`
+    void* out;
+    float* so;                            // OUT_E4M3: scales out
+    long long ldr, ldo, so_row, so_block;
+    int M, N, blocks;                     // blocks of k
+    int out_kind, io, gelu;               // io: convnn_dtype of bias, residual (and out)
+    int stages, splits;                   // CTAs of the cluster
+    bool vec;                             // rows of out and residual, and bias, can be read eight values at a time
+};
+
+__device__ __forceinline__ void fail(volatile int* abort_flag, int code) {
+    *abort_flag = 1;
+    atomicCAS(&g_linear_fp8_status, 0, code);
+}
+
+// D format F32 (bit 4), A / B format E4M3 (0 in bits 7-9, 10-12), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) {
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+
+// x * Phi(x)
+__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+
+template <typename T>
+__device__ __forceinline__ void load8(const void* base, long long at, int valid, bool vec, float (&v)[8]) {
+    const T* p = static_cast<const T*>(base) + at;
+    if (vec && valid >= 8) {
+        uint4 raw[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+        const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < valid ? to_f32<T>(p[j]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* base, long long at, int valid, bool vec, const float (&v)[8]) {
+    T* p = static_cast<T*>(base) + at;
+    if (vec && valid >= 8) {
+        uint4 raw[sizeof(T) / 2];
+        T* e = reinterpret_cast<T*>(raw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) p[j] = from_f32<T>(v[j]);
+    }
+}
+
+// Eight neighbouring outputs of row m from column n on, from their sums.  Sixteen neighbouring lanes hold a row's block of 128
+// columns and come here together.
+__device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, int n, bool row_valid, float (&v)[8]) {
+    const int valid = row_valid ? p.N - n : 0;               // may be <= 0
+    if (p.bias && valid > 0) {
+        float b[8];
+        if (p.io == CONVNN_F32) load8<float>(p.bias, n, valid, p.vec, b);
+        else load8<__nv_bfloat16>(p.bias, n, valid, p.vec, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += b[j];
+    }
+    if (p.gelu) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = gelu_erf(v[j]);
+    }
+    if (p.residual && valid > 0) {
+        float r[8];
+        if (p.io == CONVNN_F32) load8<float>(p.residual, m * p.ldr + n, valid, p.vec, r);
+        else load8<__nv_bfloat16>(p.residual, m * p.ldr + n, valid, p.vec, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    if (p.out_kind == OUT_E4M3) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) top = max(top, abs_bits(v[j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float scale = fp8_scale(top), inv = __frcp_rn(scale);
+        if (valid > 0) {
+            uint2 w;
+            w.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+            w.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+            uint8_t* q = static_cast<uint8_t*>(p.out) + m * p.ldo + n;
+            if (p.vec && valid >= 8) *reinterpret_cast<uint2*>(q) = w;
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < valid) q[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+            }
+            if (n % KB == 0) p.so[m * p.so_row + (n / KB) * p.so_block] = scale;
+        }
+    } else if (valid > 0) {
+        if (p.out_kind == OUT_F32) store8<float>(p.out, m * p.ldo + n, valid, p.vec, v);
+        else store8<__nv_bfloat16>(p.out, m * p.ldo + n, valid, p.vec, v);
+    }
+}
+
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(NTHREADS, SWAP ? 1 : 2)
+linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const LinearFp8Params p) {
+    static_assert(SWAP ? BN <= 64 : BN == 128, "see the scales of the two forms");
+    constexpr int CW = BN / 2;                               // columns of a warp
+    constexpr int NBUF = BN == 128 ? 2 : 4;
+    constexpr uint32_t TCOLS = NBUF * BN < 32 ? 32 : NBUF * BN;
+    constexpr int AHEAD = 4;                                 // scales requested so many blocks before their use
+    // the summed tile, rows of the output by its columns
+    constexpr int ROWS = SWAP ? BN : BP, COLS = SWAP ? BP : BN, PITCH = COLS + 4;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr uint32_t P_BYTES = BP * KB, Q_BYTES = BN * KB;
+    const uint32_t STAGES = p.stages;
+    uint8_t* sP = smem;
+    uint8_t* sQ = sP + STAGES * P_BYTES;
+    float* tile = reinterpret_cast<float*>(smem);            // in the place of the ring, once that is read
+    __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[NBUF], tempty[NBUF];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    __shared__ __align__(16) float col_scale[SWAP ? 8 : 1][2][SWAP ? 32 : 1];
+    volatile int* abort_flag = &abort_word;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = p.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int unit = blockIdx.x / p.splits;
+    // tiles of one block of weights after another, or of one block of rows after another
+    const int n_q = SWAP ? (p.M + BN - 1) / BN : (p.N + BN - 1) / BN;
+    const int pt = unit / n_q, qt = unit - pt * n_q;
+    const int kb0 = (int)((long long)p.blocks * rank / p.splits), kb1 = (int)((long long)p.blocks * (rank + 1) / p.splits);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < NBUF; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 8); }
+        abort_word = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmP);
+        prefetch_tensormap(&tmQ);
+    }
+    if (warp == 1) { tmem_alloc(&tmem_slot, TCOLS); tmem_relinquish(); }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_slot;
+    chain_begin();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            int kb = kb0;
+            for (; kb < kb1; ++kb) {
+                if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) { fail(abort_flag, 121); break; }
+                mbar_expect_tx(&full[s], P_BYTES + Q_BYTES);
+                tma_load_2d(sP + s * P_BYTES, &tmP, &full[s], kb * KB, pt * BP);
+                tma_load_2d(sQ + s * Q_BYTES, &tmQ, &full[s], kb * KB, qt * BN);
+                if (++s == STAGES) { s = 0; ph ^= 1u; }
+            }
+            if (kb < kb1) {                                  // gave up: what is on its way lands before the CTA leaves
+                int never = 0;
+                for (uint32_t i = 0; i < STAGES && kb > kb0; ++i, --kb) {
+                    if (s == 0) { s = STAGES; ph ^= 1u; }
+                    --s;
+                    mbar_wait(&full[s], ph, &never);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = idesc_e4m3_f32(BP, BN);
+        const uint64_t hi = kmajor_desc_hi(KB);
+        const uint32_t full0 = smem_u32(full), tempty0 = smem_u32(tempty), empty0 = smem_u32(empty), tfull0 = smem_u32(tfull);
+        const uint32_t sP0 = smem_u32(sP), sQ0 = smem_u32(sQ);
+        uint32_t s = 0, ph = 0, buf = 0, tph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait_warp(tempty0 + 8 * buf, tph ^ 1u, abort_flag)) { if (lane == 0) fail(abort_flag, 122); break; }
+            if (!mbar_wait_warp(full0 + 8 * s, ph, abort_flag)) { if (lane == 0) fail(abort_flag, 123); break; }
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const uint64_t ad = hi | (uint64_t)(((sP0 + s * P_BYTES) & 0x3FFFFu) >> 4);
+                const uint64_t bd = hi | (uint64_t)(((sQ0 + s * Q_BYTES) & 0x3FFFFu) >> 4);
+                const uint32_t d = tmem_base + buf * BN;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma_e4m3_ss(d, ad + 2 * i, bd + 2 * i, idesc, i > 0);
+                mma_commit_a(empty0 + 8 * s);
+                mma_commit_a(tfull0 + 8 * buf);
+            }
+            __syncwarp();
+            if (++s == STAGES) { s = 0; ph ^= 1u; }
+            if (++buf == NBUF) { buf = 0; tph ^= 1u; }
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;   // (a warp reads the TMEM lanes of its number mod 4)
+        const int c0 = half * CW, row = quarter * 32 + lane;
+        f32x2 acc[CW / 2];
+#pragma unroll
+        for (int j = 0; j < CW / 2; ++j) acc[j] = pack2(0.f, 0.f);
+        // The scale of this lane's row (its column, where SWAP) times the one that the whole tile shares.  Rows past the end hold
+        // zeros and are never stored.
+        const int mine = SWAP ? qt * BN + c0 + lane : pt * BP + row;
+        const bool have = mine < p.M && (!SWAP || lane < CW);
+        const float* sa = p.sa + (have ? (long long)mine * p.sa_row : 0);
+        const float* sw = p.sw + (long long)(SWAP ? pt : qt) * p.sw_row;
+        auto scale_of = [&](int kb) {
+            if (!have || kb >= kb1) return 0.f;
+            return sa[kb * p.sa_block] * sw[kb * p.sw_block];
+        };
+        float next[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) next[i] = scale_of(kb0 + i);
+        uint32_t buf = 0, tph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const float s = next[0];
+#pragma unroll
+            for (int i = 0; i + 1 < AHEAD; ++i) next[i] = next[i + 1];
+            next[AHEAD - 1] = scale_of(kb + AHEAD);
+            float* sc = SWAP ? col_scale[warp - 2][kb & 1] : nullptr;
+            if (SWAP) {
+                sc[lane] = s;
+                __syncwarp();
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[buf], tph, abort_flag))) { if (lane == 0) fail(abort_flag, 124); break; }
+            tc_fence_after_sync();
+            const uint32_t t = tmem_base + buf * BN + c0 + ((uint32_t)(quarter * 32) << 16);
+            constexpr int STEP = CW < 16 ? CW : 16;
+#pragma unroll
+            for (int c = 0; c < CW; c += STEP) {
+                uint32_t r[STEP];
+                if constexpr (STEP == 8) tmem_ld_x8(t + c, r);
+                else tmem_ld_x16(t + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < STEP; j += 2) {
+                    const f32x2 part = pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+                    const f32x2 by = SWAP ? *reinterpret_cast<const f32x2*>(sc + c + j) : pack2(s, s);
+                    acc[(c + j) / 2] = fma2(part, by, acc[(c + j) / 2]);
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[buf]);
+            if (++buf == NBUF) { buf = 0; tph ^= 1u; }
+        }
+        // The last product has read the ring, and nothing more is copied into it.
+#pragma unroll
+        for (int j = 0; j < CW / 2; ++j) {
+            float a, b;
+            unpack2(acc[j], a, b);
+            if (SWAP) {
+                tile[(c0 + 2 * j) * PITCH + row] = a;
+                tile[(c0 + 2 * j + 1) * PITCH + row] = b;
+            } else {
+                *reinterpret_cast<float2*>(tile + row * PITCH + c0 + 2 * j) = make_float2(a, b);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    if (p.splits > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, TCOLS);
+    // After a wait that gave up, the tiles of the cluster are not whole, and what is written is undefined.
+    const int row_a = ROWS * rank / p.splits, row_b = ROWS * (rank + 1) / p.splits;
+    constexpr int GROUPS = COLS / 8;                         // sixteen, in both forms
+    static_assert(GROUPS == 16, "sixteen lanes hold a row");
+    const uint32_t tile0 = smem_u32(tile);
+    // (every warp goes round as often as the others: the lanes of a row exchange their largest values)
+    for (int u = row_a * GROUPS + (int)threadIdx.x; u - lane < row_b * GROUPS; u += NTHREADS) {
+        const int r = u / GROUPS, g = u % GROUPS;
+        const bool inside = r < row_b;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        if (inside) {
+            const uint32_t off = tile0 + (r * PITCH + g * 8) * 4;
+            if (p.splits == 1) {
+                const float4 a = *reinterpret_cast<const float4*>(tile + r * PITCH + g * 8);
+                const float4 b = *reinterpret_cast<const float4*>(tile + r * PITCH + g * 8 + 4);
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            } else {
+                for (int c = 0; c < p.splits; ++c) {
+                    const uint32_t at = map_to_cta(off, c);
+                    const float4 a = ld_cluster_f32x4(at), b = ld_cluster_f32x4(at + 16);
+                    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+                }
+            }
+        }
+        const long long m = (long long)(SWAP ? qt * BN : pt * BP) + r;
+        finish8(p, m, (SWAP ? pt * BP : qt * BN) + g * 8, inside && m < p.M, v);
+    }
+    if (p.splits > 1) cluster_sync_all();                    // the others may still read this CTA's tile
+}
+
+template <int BN, bool SWAP>
+int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params p, cudaStream_t st) {
+    constexpr size_t STAGE = (size_t)(BP + BN) * KB;
+    constexpr size_t TILE = (size_t)(SWAP ? BN * (BP + 4) : BP * (BN + 4)) * 4;
+    const long long tiles = SWAP ? (long long)((p.N + BP - 1) / BP) * ((p.M + BN - 1) / BN)
+                                 : (long long)((p.M + BP - 1) / BP) * ((p.N + BN - 1) / BN);
+    if (tiles * 8 > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %d x %d is too many tiles", p.M, p.N);
+    const int sms = device_sms();
+    p.splits = 1;
+    while (p.splits < 8 && tiles * p.splits * 2 <= sms && p.blocks >= 4 * p.splits) p.splits *= 2;
+    const int per = (p.blocks + p.splits - 1) / p.splits;
+    p.stages = SWAP ? MAX_STAGES : 3;
+    while (p.stages > per && p.stages > 2) --p.stages;
+    while (p.stages * STAGE > 200 * 1024) --p.stages;
+    size_t smem = p.stages * STAGE;
+    if (smem < TILE) smem = TILE;
+    smem += 1024;
+    auto kern = linear_fp8_kernel<BN, SWAP>;
+    CONVNN_ENSURE_SMEM(kern, smem);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0] = chained_attribute(st);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(tiles * p.splits)); cfg.blockDim = dim3(NTHREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = p.splits > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tmP, tmQ, p);
+    if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "linear_fp8 launch: %s", cudaGetErrorString(e));
+    CONVNN_CHECK_LAUNCH("linear_fp8");
+    return CONVNN_OK;
+}
+
+bool encode_rows(CUtensorMap* m, const void* base, long long rows, int K, long long ld, int box_rows) {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)ld};
+    const uint32_t box[2] = {(uint32_t)KB, (uint32_t)box_rows};
+    return encode_tensor_map_u8(m, base, 2, dims, strides, box, 128);
+}
+
+}  // namespace
+
+int launch_linear_fp8(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
+                      long long ldw, const float* sw, long long sw_row, long long sw_block, const void* bias, const void* residual,
+                      long long ldr, int io, void* out, long long ldo, float* so, long long so_row, long long so_block, int M, int N,
+                      int K, int gelu, cudaStream_t st) {
+    LinearFp8Params p{};
+    p.sa = sa; p.sa_row = sa_row; p.sa_block = sa_block;
+    p.sw = sw; p.sw_row = sw_row; p.sw_block = sw_block;
+    p.bias = bias; p.residual = residual; p.out = out; p.so = so;
+    p.ldr = ldr; p.ldo = ldo; p.so_row = so_row; p.so_block = so_block;
+    p.M = M; p.N = N; p.blocks = (K + KB - 1) / KB;
+    p.io = io; p.gelu = gelu;
+    p.out_kind = so ? OUT_E4M3 : io == CONVNN_F32 ? OUT_F32 : OUT_BF16;
+    const long long per16 = io == CONVNN_F32 ? 4 : 8;
+    p.vec = (so ? ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0 : ldo % per16 == 0 && aligned16(out)) &&
+            (!bias || aligned16(bias)) && (!residual || (aligned16(residual) && ldr % per16 == 0));
+    const bool swap = M <= 64;
+    const int bn = !swap ? 128 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    CUtensorMap tmP, tmQ;
+    if (!encode_rows(&tmP, swap ? w : a, swap ? N : M, K, swap ? ldw : lda, BP)) return CONVNN_E_CUDA;
+    if (!encode_rows(&tmQ, swap ? a : w, swap ? M : N, K, swap ? lda : ldw, bn)) return CONVNN_E_CUDA;
+    if (bn == 16) return launch_tiles<16, true>(tmP, tmQ, p, st);
+    if (bn == 32) return launch_tiles<32, true>(tmP, tmQ, p, st);
+    if (bn == 64) return launch_tiles<64, true>(tmP, tmQ, p, st);
+    return launch_tiles<128, false>(tmP, tmQ, p, st);
+}
+
+int read_linear_fp8_status(int* out) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_linear_fp8_status, sizeof(int));
+    if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
+    *out = v;
+    return CONVNN_OK;
+}
+
+}  // namespace convnn

@@ -64,6 +64,12 @@ bool encode_tensor_map_bf16(CUtensorMap* out, const void* base, int rank, const 
     return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides_bytes, box, swizzle_bytes);
 }
 
+// 8-bit elements of any kind
+bool encode_tensor_map_u8(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
+                          const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes) {
+    return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box, swizzle_bytes);
+}
+
 // float32 elements, no swizzle (the row moments of the pre-norm fold)
 bool encode_tensor_map_f32(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                            const uint64_t* strides_bytes, const uint32_t* box) {

@@ -108,7 +108,7 @@ int convnn_b200_forwards_in_flight(int32_t n);
 /* No reference counterpart: reads the device-side error latch (synchronises the device).
  * 0 = no kernel gave up; otherwise the code of the first bounded wait that expired inside
  * a tensor-core kernel (similarity: 1 producer, 2/3 MMA issuer, 4 epilogue; GEMM: 11-16; pair
- * similarity: 21-26; streaming depthwise conv: 31).  A wait gives up after 250 ms.  Results of
+ * similarity: 21-26; streaming depthwise conv: 31; 8-bit product: 121-124).  A wait gives up after 250 ms.  Results of
  * a call that latched a code are undefined. */
 int convnn_b200_device_status(int* code);
 
@@ -219,6 +219,45 @@ int convnn_b200_layernorm(int dtype, const void* x, int64_t ldx, const void* gam
 int convnn_b200_linear(int dtype, const void* a, int64_t lda, const void* w, const void* bias,
                        const void* residual, int64_t ldr, void* out, int64_t ldo,
                        int64_t M, int32_t N, int32_t K, int32_t gelu, void* stream);
+
+/* ---- 8-bit values (e4m3) with a float32 scale per block of 128 channels --------------------
+ * No reference counterpart: the encoder's norm -> Linear -> Linear served in 8 bits.  A value is
+ * stored as q and means q * scale, with scale = max(amax|block| / 448, 2^-126), q = e4m3(v / scale)
+ * (rounded to nearest even).  A block is 128 neighbouring channels (the last one of a row may be
+ * shorter) of one row, or of 128 rows in a weight.  scales[row_block * *_scale_row + channel_block *
+ * *_scale_block]: strides in elements, any order; the kernels read and write them fastest where
+ * the scales of neighbouring rows lie side by side.  A block that holds a NaN or an infinity means
+ * NaN throughout.  Row counts may be 0. */
+
+/* y = s * (mean(s^2) + eps)^-1/2 * weight over the last dimension, s = x or, with a residual, x +
+ * residual rounded to dtype, which is then also written to `sum` (both or neither NULL).  rows x D,
+ * strides in elements, statistics in fp32. */
+int convnn_b200_rms_norm(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                         const void* weight, float eps, void* sum, int64_t lds, void* y, int64_t ldy,
+                         int64_t rows, int32_t D, void* stream);
+/* The same with y in 8 bits (from its float32 values: no rounding in between), a scale per row and
+ * 128 channels; q (rows, D), row stride ldq bytes. */
+int convnn_b200_rms_norm_fp8(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                             const void* weight, float eps, void* sum, int64_t lds, void* q, int64_t ldq,
+                             float* scales, int64_t scale_row, int64_t scale_block, int64_t rows,
+                             int32_t D, void* stream);
+/* x (rows, D) in 8 bits, a scale per block of block_rows rows (1: activations, 128: weights) and
+ * 128 channels. */
+int convnn_b200_quantize_fp8(int dtype, const void* x, int64_t ldx, int32_t block_rows, void* q, int64_t ldq,
+                             float* scales, int64_t scale_row, int64_t scale_block, int64_t rows, int32_t D,
+                             void* stream);
+/* out = [GELU](a w^T + bias) [+ residual] with a (M, K) in 8 bits, a scale per row and 128 channels,
+ * and w (N, K) in 8 bits, a scale per 128 x 128 block.  Sums, bias, GELU (erf form) and residual in
+ * float32, one rounding at the store.  bias (N) and residual (M, N) in dtype, or NULL.  out (M, N) in
+ * dtype or, where out_scales is given, in 8 bits with a scale per row and 128 columns (the next
+ * product's a).  Rows of a and w must start on 16-byte boundaries (lda, ldw multiples of 16).
+ * out may be the residual itself, nothing else of the inputs. */
+int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, int64_t a_scale_row,
+                           int64_t a_scale_block, const void* w, int64_t ldw, const float* w_scales,
+                           int64_t w_scale_row, int64_t w_scale_block, int dtype, const void* bias,
+                           const void* residual, int64_t ldr, void* out, int64_t ldo, float* out_scales,
+                           int64_t out_scale_row, int64_t out_scale_block, int64_t M, int32_t N, int32_t K,
+                           int32_t gelu, void* stream);
 
 /* Unfold non-overlapping P x P patches: img (B, C, Hh, Ww) -> out (B * Hh/P * Ww/P, C*P*P),
  * the im2col of Conv2d(kernel = stride = P) (vit.py:99, 105-107). */
