@@ -3,10 +3,11 @@
 //   s = x + residual (rounded to the storage type once: what is stored is what is normalised)
 //   y = s * (mean(s^2) + eps)^-1/2 * weight,  in float32, rounded once: to the storage type, or straight to e4m3 under the
 //   block's scale (a rounding to bfloat16 in between would move one value in 16 by a step of e4m3)
-// A warp reads a block of 128 channels at once, four channels a lane: a block's largest magnitude is one warp reduction, its
-// 8-bit result one 128-byte store.  All kernels are bound by memory: every input is read once, into registers, however
-// often it is used.
+// A lane reads eight neighbouring channels at once, sixteen lanes a block: its largest magnitude is four exchanges, its 8-bit
+// result one 128-byte store.  All kernels are bound by memory as long as their loads are all requested before the first is used (raw,
+// into registers: every input is read once) and their instructions stay under about 90 per 256 channels.
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "fp8.cuh"
 
 namespace convnn {
@@ -31,128 +32,169 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// A lane has four neighbouring channels of the block that starts at channel c0, read and written at once (VEC: D a multiple of four
-// and every row on a boundary of four values) or one by one: the sums, and so the results, are the same bits either way.
-template <typename T> struct Raw4;
-template <> struct Raw4<float> { float4 v; };
-template <> struct Raw4<__nv_bfloat16> { uint2 v; };
+// Eight neighbouring channels as they are stored, and as four pairs of float32.  VEC: D a multiple of eight and every row on a
+// 16-byte boundary; otherwise one by one, into the same places, so that the sums and the results are the same bits.
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* row, int c0, int lane, int D, float (&v)[4]) {
+__device__ __forceinline__ Raw8<T> load8(const T* p, int valid) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = make_uint4(0, 0, 0, 0);
     if (VEC) {
-        v[0] = v[1] = v[2] = v[3] = 0.f;
-        if (c0 + 4 * lane < D) {
-            const Raw4<T> r = *reinterpret_cast<const Raw4<T>*>(row + c0 + 4 * lane);
-            const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = to_f32<T>(e[j]);
-        }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            if (valid > 0) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
+        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 4 * lane + j;
-            v[j] = c < D ? to_f32<T>(row[c]) : 0.f;
-        }
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) e[j] = p[j];
+    }
+    return r;
+}
+__device__ __forceinline__ void widen(const Raw8<__nv_bfloat16>& r, f32x2 (&v)[4]) { bf16x8_to_f32x2(r.v[0], v); }
+__device__ __forceinline__ void widen(const Raw8<float>& r, f32x2 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v[2 * i] = pack2(__uint_as_float(r.v[i].x), __uint_as_float(r.v[i].y));
+        v[2 * i + 1] = pack2(__uint_as_float(r.v[i].z), __uint_as_float(r.v[i].w));
+    }
+}
+__device__ __forceinline__ void narrow(const f32x2 (&v)[4], Raw8<__nv_bfloat16>& r) { r.v[0] = f32x2_to_bf16x8(v); }
+__device__ __forceinline__ void narrow(const f32x2 (&v)[4], Raw8<float>& r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float f[4];
+        unpack2(v[2 * i], f[0], f[1]);
+        unpack2(v[2 * i + 1], f[2], f[3]);
+        r.v[i] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
     }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T* row, int c0, int lane, int D, const float (&v)[4]) {
+__device__ __forceinline__ void store8(T* p, int valid, const Raw8<T>& r) {
     if (VEC) {
-        if (c0 + 4 * lane < D) {
-            Raw4<T> r;
-            T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = from_f32<T>(v[j]);
-            *reinterpret_cast<Raw4<T>*>(row + c0 + 4 * lane) = r;
-        }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            if (valid > 0) reinterpret_cast<uint4*>(p)[i] = r.v[i];
     } else {
+        const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 4 * lane + j;
-            if (c < D) row[c] = from_f32<T>(v[j]);
-        }
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) p[j] = e[j];
     }
 }
-// The warp's block v under its scale, which is returned.
+__device__ __forceinline__ uint32_t amax8(const f32x2 (&v)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack2(v[i], a, b);
+        m = max(m, max(abs_bits(a), abs_bits(b)));
+    }
+    return m;
+}
+// Over the sixteen lanes of a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
 template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* row, int c0, int lane, int D, const float (&v)[4], float scale) {
+__device__ __forceinline__ void store_e4m3(uint8_t* p, int valid, const f32x2 (&v)[4], float scale) {
     const float inv = __frcp_rn(scale);
-    const uint32_t w = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(mul2(v[i], pack2(inv, inv)), f[2 * i], f[2 * i + 1]);
+    const uint2 w = make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
     if (VEC) {
-        if (c0 + 4 * lane < D) *reinterpret_cast<uint32_t*>(row + c0 + 4 * lane) = w;
+        if (valid > 0) *reinterpret_cast<uint2*>(p) = w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 4 * lane + j;
-            if (c < D) row[c] = (uint8_t)(w >> (8 * j));
-        }
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) p[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
     }
-}
-__device__ __forceinline__ uint32_t amax4(const float (&v)[4]) {
-    return max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
 }
 
-// x + residual as it is stored.
+// x + residual as it is stored, widened again.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_sum(const NormParams& p, long long row, int c0, int lane, float (&v)[4]) {
-    load4<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx, c0, lane, p.D, v);
-    if (p.residual) {
-        float r[4];
-        load4<T, VEC>(static_cast<const T*>(p.residual) + row * p.ldr, c0, lane, p.D, r);
+__device__ __forceinline__ void add_residual(const NormParams& p, long long row, int c, int valid, const Raw8<T>& res, f32x2 (&v)[4]) {
+    f32x2 r[4];
+    widen(res, r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = to_f32<T>(from_f32<T>(v[j] + r[j]));
-    }
+    for (int i = 0; i < 4; ++i) v[i] = add2(v[i], r[i]);
+    Raw8<T> s;
+    narrow(v, s);
+    widen(s, v);
+    store8<T, VEC>(static_cast<T*>(p.sum) + row * p.lds + c, valid, s);
+}
+__device__ __forceinline__ float squares(const f32x2 (&v)[4], float ss) {
+    f32x2 a = mul2(v[0], v[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) a = fma2(v[i], v[i], a);
+    float x, y;
+    unpack2(a, x, y);
+    return ss + (x + y);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void finish_block(const NormParams& p, long long row, int b, int lane, const float (&v)[4],
-                                             const float (&w)[4], float rstd) {
-    const int c0 = b * kFp8Block;
-    float y[4];
+__device__ __forceinline__ void finish8(const NormParams& p, long long row, int c, int valid, bool inside, const f32x2 (&v)[4],
+                                        const f32x2 (&w)[4], float rstd) {
+    f32x2 y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = v[j] * rstd * w[j];
+    for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(v[i], pack2(rstd, rstd)), w[i]);
     if (p.q) {
-        const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, amax4(y)));
-        store_e4m3<VEC>(p.q + row * p.ldy, c0, lane, p.D, y, scale);
-        if (lane == 0) p.scales[row * p.scale_row + b * p.scale_block] = scale;
-    } else {
-        store4<T, VEC>(static_cast<T*>(p.y) + row * p.ldy, c0, lane, p.D, y);
+        const float scale = fp8_scale(block_max(amax8(y)));
+        if (!inside) return;
+        store_e4m3<VEC>(p.q + row * p.ldy + c, valid, y, scale);
+        if (valid > 0 && c % kFp8Block == 0) p.scales[row * p.scale_row + c / kFp8Block * p.scale_block] = scale;
+    } else if (inside) {
+        Raw8<T> o;
+        narrow(y, o);
+        store8<T, VEC>(static_cast<T*>(p.y) + row * p.ldy + c, valid, o);
     }
 }
 
-// WPR warps per row, each with NB blocks of it in registers; R rows at a time, where a row is short.
-template <typename T, int NB, int R, int WPR, bool VEC>
+// WPR warps per row, each with NV vectors of 256 channels of it in registers; R rows at a time, where a row is short.
+template <typename T, int NV, int R, int WPR, bool VEC>
 __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) {
     static_assert(WPR == 1 || R == 1, "rows shared by warps come one at a time");
     __shared__ float part[kWarps];
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPR;
     const long long row0 = ((long long)blockIdx.x * (kWarps / WPR) + warp / WPR) * R;
-    const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    float v[R][NB][4];
-    float w[NB][4];
+    const T* x = static_cast<const T*>(p.x);
+    const T* res = static_cast<const T*>(p.residual);
+    Raw8<T> raw[R][NV], extra[R][NV], wr[NV];
+    int c[NV], valid[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        c[i] = ((wi + WPR * i) * 32 + lane) * 8;
+        valid[i] = p.D - c[i];
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int b = wi + WPR * i;
-            if (row0 + r < p.rows && b < blocks) load_sum<T, VEC>(p, row0 + r, b * kFp8Block, lane, v[r][i]);
-            else v[r][i][0] = v[r][i][1] = v[r][i][2] = v[r][i][3] = 0.f;
-        }
+        for (int i = 0; i < NV; ++i)
+            raw[r][i] = load8<T, VEC>(x + (row0 + r) * p.ldx + c[i], row0 + r < p.rows ? valid[i] : 0);
+    if (res) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int b = wi + WPR * i;
-        if (b < blocks) load4<T, VEC>(static_cast<const T*>(p.weight), b * kFp8Block, lane, p.D, w[i]);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                extra[r][i] = load8<T, VEC>(res + (row0 + r) * p.ldr + c[i], row0 + r < p.rows ? valid[i] : 0);
     }
 #pragma unroll
+    for (int i = 0; i < NV; ++i) wr[i] = load8<T, VEC>(static_cast<const T*>(p.weight) + c[i], valid[i]);
+#pragma unroll
     for (int r = 0; r < R; ++r) {
+        const bool inside = row0 + r < p.rows;
+        f32x2 v[NV][4];
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int b = wi + WPR * i;
-            if (p.residual && row0 + r < p.rows && b < blocks)
-                store4<T, VEC>(static_cast<T*>(p.sum) + (row0 + r) * p.lds, b * kFp8Block, lane, p.D, v[r][i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ss = fmaf(v[r][i][j], v[r][i][j], ss);
+        for (int i = 0; i < NV; ++i) {
+            widen(raw[r][i], v[i]);
+            if (res) add_residual<T, VEC>(p, row0 + r, c[i], inside ? valid[i] : 0, extra[r][i], v[i]);
+            ss = squares(v[i], ss);
         }
         ss = warp_sum(ss);
         if (WPR > 1) {
@@ -164,9 +206,10 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) 
         }
         const float rstd = rsqrtf(ss * p.inv_d + p.eps);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int b = wi + WPR * i;
-            if (row0 + r < p.rows && b < blocks) finish_block<T, VEC>(p, row0 + r, b, lane, v[r][i], w[i], rstd);
+        for (int i = 0; i < NV; ++i) {
+            f32x2 w[4];
+            widen(wr[i], w);
+            finish8<T, VEC>(p, row0 + r, c[i], valid[i], inside, v[i], w, rstd);
         }
     }
 }
@@ -178,27 +221,40 @@ __global__ void __launch_bounds__(kThreads) rms_norm_wide_kernel(const NormParam
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = blockIdx.x;
-    const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    float ss = 0.f;
-    for (int b = warp; b < blocks; b += kWarps) {
-        float v[4];
-        load_sum<T, VEC>(p, row, b * kFp8Block, lane, v);
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+    const int steps = (p.D + 8 * kThreads - 1) / (8 * kThreads);
+    float rstd = 0.f;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        float ss = 0.f;
+#pragma unroll 2
+        for (int k = 0; k < steps; ++k) {
+            const int c = (k * kThreads + threadIdx.x) * 8, valid = p.D - c;
+            const Raw8<T> raw = load8<T, VEC>(x + c, valid);
+            f32x2 v[4];
+            widen(raw, v);
+            if (res) {
+                const Raw8<T> extra = load8<T, VEC>(res + c, valid);
+                add_residual<T, VEC>(p, row, c, pass ? valid : 0, extra, v);
+            }
+            if (!pass) {
+                ss = squares(v, ss);
+            } else {
+                f32x2 w[4];
+                widen(load8<T, VEC>(static_cast<const T*>(p.weight) + c, valid), w);
+                finish8<T, VEC>(p, row, c, valid, true, v, w, rstd);
+            }
+        }
+        if (!pass) {
+            ss = warp_sum(ss);
+            if (lane == 0) part[warp] = ss;
+            __syncthreads();
+            ss = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ss = fmaf(v[j], v[j], ss);
-    }
-    ss = warp_sum(ss);
-    if (lane == 0) part[warp] = ss;
-    __syncthreads();
-    ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) ss += part[k];
-    const float rstd = rsqrtf(ss * p.inv_d + p.eps);
-    for (int b = warp; b < blocks; b += kWarps) {
-        float v[4], w[4];
-        load_sum<T, VEC>(p, row, b * kFp8Block, lane, v);
-        if (p.residual) store4<T, VEC>(static_cast<T*>(p.sum) + row * p.lds, b * kFp8Block, lane, p.D, v);
-        load4<T, VEC>(static_cast<const T*>(p.weight), b * kFp8Block, lane, p.D, w);
-        finish_block<T, VEC>(p, row, b, lane, v, w, rstd);
+            for (int k = 0; k < kWarps; ++k) ss += part[k];
+            rstd = rsqrtf(ss * p.inv_d + p.eps);
+        }
     }
 }
 
@@ -210,38 +266,46 @@ struct QuantParams {
     int D;
 };
 
-// A scale per row and block: a warp takes eight blocks of the flattened (row, block) list, all requested before the first is
-// used.
+// A scale per row and block: a half-warp takes every other block of sixteen of the flattened (row, block) list.
 constexpr int kTasks = 8;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantParams p) {
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    const long long t0 = ((long long)blockIdx.x * kWarps + warp) * kTasks;
+    const long long t0 = ((long long)blockIdx.x * kWarps + warp) * (2 * kTasks) + (lane >> 4);
     const long long first = t0 / blocks;
-    float v[kTasks][4];
+    const int b0 = (int)(t0 - first * blocks), at = (lane & 15) * 8;
+    auto on = [&](long long& row, int& b) {                  // two blocks on
+        b += 2;
+        if (b >= blocks) { b -= blocks; ++row; }
+        if (b >= blocks) { b -= blocks; ++row; }
+    };
+    Raw8<T> raw[kTasks];
     long long row = first;
-    int b = (int)(t0 - first * blocks);
+    int b = b0;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        if (row < p.rows) load4<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx, b * kFp8Block, lane, p.D, v[t]);
-        if (++b == blocks) { b = 0; ++row; }
+        const int c = b * kFp8Block + at;
+        raw[t] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx + c, row < p.rows ? p.D - c : 0);
+        on(row, b);
     }
     row = first;
-    b = (int)(t0 - first * blocks);
+    b = b0;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        if (row < p.rows) {
-            const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, amax4(v[t])));
-            store_e4m3<VEC>(p.q + row * p.ldq, b * kFp8Block, lane, p.D, v[t], scale);
-            if (lane == 0) p.scales[row * p.scale_row + b * p.scale_block] = scale;
-        }
-        if (++b == blocks) { b = 0; ++row; }
+        const int c = b * kFp8Block + at;
+        f32x2 v[4];
+        widen(raw[t], v);
+        const float scale = fp8_scale(block_max(amax8(v)));
+        const int valid = row < p.rows ? p.D - c : 0;
+        store_e4m3<VEC>(p.q + row * p.ldq + c, valid, v, scale);
+        if (valid > 0 && at == 0) p.scales[row * p.scale_row + b * p.scale_block] = scale;
+        on(row, b);
     }
 }
 
-// A scale per 128 x 128 block: a CTA holds the block in registers, sixteen rows a warp.
+// A scale per 128 x 128 block: a CTA holds the block in registers, eight rows a half-warp.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantParams p) {
     __shared__ uint32_t top[kWarps];
@@ -249,18 +313,22 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantPa
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
     const long long rb = blockIdx.x / blocks;
-    const int b = (int)(blockIdx.x - rb * blocks), c0 = b * kFp8Block;
-    constexpr int N = kFp8Block / kWarps;
-    float v[N][4];
+    const int b = (int)(blockIdx.x - rb * blocks), c = b * kFp8Block + (lane & 15) * 8;
+    constexpr int N = kFp8Block / (2 * kWarps);
+    const long long row0 = rb * kFp8Block + 2 * warp + (lane >> 4);
+    Raw8<T> raw[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const long long row = rb * kFp8Block + warp + kWarps * i;
-        if (row < p.rows) load4<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx, c0, lane, p.D, v[i]);
-        else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+        const long long row = row0 + 2 * kWarps * i;
+        raw[i] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx + c, row < p.rows ? p.D - c : 0);
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = max(m, amax4(v[i]));
+    for (int i = 0; i < N; ++i) {
+        f32x2 v[4];
+        widen(raw[i], v);
+        m = max(m, amax8(v));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) top[warp] = m;
     __syncthreads();
@@ -271,38 +339,40 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantPa
     if (threadIdx.x == 0) p.scales[rb * p.scale_row + b * p.scale_block] = scale;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const long long row = rb * kFp8Block + warp + kWarps * i;
-        if (row < p.rows) store_e4m3<VEC>(p.q + row * p.ldq, c0, lane, p.D, v[i], scale);
+        const long long row = row0 + 2 * kWarps * i;
+        f32x2 v[4];
+        widen(raw[i], v);
+        store_e4m3<VEC>(p.q + row * p.ldq + c, row < p.rows ? p.D - c : 0, v, scale);
     }
 }
 
-// Whether rows of `elt`-byte values can be read four at a time.
-bool fours(const void* p, long long ld, size_t elt) {
-    return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (4 * elt - 1)) == 0;
+// Whether rows of `elt`-byte values can be read 16 bytes at a time (8-bit ones: written eight).
+bool eights(const void* p, long long ld, size_t elt) {
+    return ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & (elt == 1 ? 7u : 15u)) == 0;
 }
 
-template <typename T, int NB, int R, int WPR>
+template <typename T, int NV, int R, int WPR>
 int launch_norm(const NormParams& p, bool vec, cudaStream_t st) {
     const long long per = (long long)(kWarps / WPR) * R, grid = (p.rows + per - 1) / per;
     if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "rms_norm: %lld rows", p.rows);
-    if (vec) launch_chained(rms_norm_kernel<T, NB, R, WPR, true>, (unsigned)grid, kThreads, 0, st, p);
-    else launch_chained(rms_norm_kernel<T, NB, R, WPR, false>, (unsigned)grid, kThreads, 0, st, p);
+    if (vec) launch_chained(rms_norm_kernel<T, NV, R, WPR, true>, (unsigned)grid, kThreads, 0, st, p);
+    else launch_chained(rms_norm_kernel<T, NV, R, WPR, false>, (unsigned)grid, kThreads, 0, st, p);
     CONVNN_CHECK_LAUNCH("rms_norm");
     return CONVNN_OK;
 }
 
 template <typename T>
 int norm_of(const NormParams& p, cudaStream_t st) {
-    const bool vec = p.D % 4 == 0 && fours(p.x, p.ldx, sizeof(T)) && fours(p.weight, 0, sizeof(T)) &&
-                     (!p.residual || (fours(p.residual, p.ldr, sizeof(T)) && fours(p.sum, p.lds, sizeof(T)))) &&
-                     (p.q ? fours(p.q, p.ldy, 1) : fours(p.y, p.ldy, sizeof(T)));
-    const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    if (blocks <= 1) return launch_norm<T, 1, 8, 1>(p, vec, st);
-    if (blocks <= 2) return launch_norm<T, 2, 4, 1>(p, vec, st);
-    if (blocks <= 4) return launch_norm<T, 4, 2, 1>(p, vec, st);
-    if (blocks <= 8) return launch_norm<T, 8, 1, 1>(p, vec, st);
-    if (blocks <= 32) return launch_norm<T, 4, 1, 8>(p, vec, st);
-    if (blocks <= 64) return launch_norm<T, 8, 1, 8>(p, vec, st);
+    const bool vec = p.D % 8 == 0 && eights(p.x, p.ldx, sizeof(T)) && eights(p.weight, 0, sizeof(T)) &&
+                     (!p.residual || (eights(p.residual, p.ldr, sizeof(T)) && eights(p.sum, p.lds, sizeof(T)))) &&
+                     (p.q ? eights(p.q, p.ldy, 1) : eights(p.y, p.ldy, sizeof(T)));
+    const int vectors = (p.D + 255) / 256;
+    if (vectors <= 1) return launch_norm<T, 1, 4, 1>(p, vec, st);
+    if (vectors <= 2) return launch_norm<T, 2, 2, 1>(p, vec, st);
+    if (vectors <= 3) return launch_norm<T, 3, 1, 1>(p, vec, st);
+    if (vectors <= 4) return launch_norm<T, 4, 1, 1>(p, vec, st);
+    if (vectors <= 16) return launch_norm<T, 2, 1, 8>(p, vec, st);
+    if (vectors <= 32) return launch_norm<T, 4, 1, 8>(p, vec, st);
     if (p.rows > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "rms_norm: %lld rows", p.rows);
     if (vec) launch_chained(rms_norm_wide_kernel<T, true>, (unsigned)p.rows, kThreads, 0, st, p);
     else launch_chained(rms_norm_wide_kernel<T, false>, (unsigned)p.rows, kThreads, 0, st, p);
@@ -312,9 +382,9 @@ int norm_of(const NormParams& p, cudaStream_t st) {
 
 template <typename T>
 int quantize_of(const QuantParams& p, int block_rows, cudaStream_t st) {
-    const bool vec = p.D % 4 == 0 && fours(p.x, p.ldx, sizeof(T)) && fours(p.q, p.ldq, 1);
+    const bool vec = p.D % 8 == 0 && eights(p.x, p.ldx, sizeof(T)) && eights(p.q, p.ldq, 1);
     const long long blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    const long long grid = block_rows == 1 ? (p.rows * blocks + kWarps * kTasks - 1) / (kWarps * kTasks)
+    const long long grid = block_rows == 1 ? (p.rows * blocks + 2 * kWarps * kTasks - 1) / (2 * kWarps * kTasks)
                                            : (p.rows + kFp8Block - 1) / kFp8Block * blocks;
     if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "quantize_fp8: %lld rows of %d", p.rows, p.D);
     if (block_rows == 1) {
