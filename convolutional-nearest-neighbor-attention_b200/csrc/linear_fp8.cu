@@ -6,12 +6,9 @@
 // Everything after the sum stays in float32 until the one rounding of the store: to bfloat16, not at all, or to e4m3 under the
 // scale of the row's block of 128 columns.
 //
-// One CTA has a tile of 128 x BN: 128 rows of P, whose rows are TMEM lanes, times BN rows of Q.  P are the activations and
-// BN = 128 (more rows), or P are the weights and Q 16, 32 or 64 tokens (SWAP).  Where tiles are few the CTAs of a cluster share
-// a tile's blocks of k; their partial tiles, in shared memory, are added up in rank order.
-//   warp 0     TMA producer (ring of P and Q blocks)
-//   warp 1     MMA issuer
-//   warps 2-9  scaled sums (two warps per lane quarter, half of the columns each), then with the others the output
+// Two kernels, by the number of tiles (see launch_linear_fp8):
+//   linear_fp8_kernel: one CTA, or a cluster that shares the blocks of k, per tile of 128 x BN; few tiles
+//   linear_fp8_pair_kernel: persistent CTA pairs on tiles of 256 x 256; many tiles
 // Every mbarrier wait is bounded (see sm100.cuh); an expiry latches the device status.
 #include "common.cuh"
 #include "sm100.cuh"
@@ -43,7 +40,7 @@ struct LinearFp8Params {
     int M, N, blocks;                     // blocks of k
     int out_kind, io, gelu;               // io: convnn_dtype of bias, residual (and out)
     int stages, splits;                   // CTAs of the cluster
-    bool vec;                             // rows of out and residual, and bias, can be read eight values at a time
+    bool vec;                             // bias and the rows of out and residual start on 16-byte boundaries
 };
 
 __device__ __forceinline__ void fail(volatile int* abort_flag, int code) {
@@ -76,8 +73,28 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     return v;
 }
 
-// x * Phi(x)
+// x * Phi(x), for results that stay in float32.
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 12 in a / 2.5 - 1
+// that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 6.4e-7; off by 8.5e-7 *
+// |x| at most as it is evaluated here).  Sixteen instructions on pairs instead of erff's ~30 on one value.
+__device__ __forceinline__ f32x2 gelu_poly(f32x2 x) {
+    constexpr float C[13] = {0.00621029362f, -0.0438225605f, 0.136878088f, -0.239581555f, 0.232788831f, -0.0657733977f, -0.131332964f,
+                             0.163930997f, -0.0241190977f, -0.0787944123f, 0.0401191078f, 0.0140417274f, -0.0105441259f};
+    float x0, x1;
+    unpack2(x, x0, x1);
+    const float a0 = fminf(fabsf(x0), 5.0f), a1 = fminf(fabsf(x1), 5.0f);
+    const f32x2 u = fma2(pack2(a0, a1), pack2(0.4f, 0.4f), pack2(-1.0f, -1.0f));
+    f32x2 q = pack2(C[12], C[12]);
+#pragma unroll
+    for (int i = 11; i >= 0; --i) q = fma2(q, u, pack2(C[i], C[i]));
+    return fma2(pack2(-a0, -a1), q, pack2(max_nan(x0, 0.f), max_nan(x1, 0.f)));
+}
 
 template <typename T>
 __device__ __forceinline__ void load8(const void* base, long long at, int valid, bool vec, float (&v)[8]) {
@@ -122,9 +139,12 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += b[j];
     }
-    if (p.gelu) {
+    if (p.gelu && p.out_kind == OUT_F32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = gelu_erf(v[j]);
+    } else if (p.gelu) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) unpack2(gelu_poly(pack2(v[j], v[j + 1])), v[j], v[j + 1]);
     }
     if (p.residual && valid > 0) {
         float r[8];
@@ -160,6 +180,12 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
     }
 }
 
+// Tiles of 128 x BN: 128 rows of P, whose rows are TMEM lanes, times BN rows of Q.  P are the activations and BN = 128 (more rows),
+// or P are the weights and Q 16, 32 or 64 tokens (SWAP).  Where tiles are few the CTAs of a cluster share a tile's blocks of k;
+// their partial tiles, in shared memory, are added up in rank order.
+//   warp 0     TMA producer (ring of P and Q blocks)
+//   warp 1     MMA issuer
+//   warps 2-9  scaled sums (two warps per lane quarter, half of the columns each), then with the others the output
 template <int BN, bool SWAP>
 __global__ void __launch_bounds__(NTHREADS, SWAP ? 1 : 2)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const LinearFp8Params p) {
@@ -385,6 +411,397 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
     return CONVNN_OK;
 }
 
+// ---- CTA pairs ------------------------------------------------------------------------------------------------------
+// Two CTAs of a cluster (cta_group::2) have tiles of 256 x 256: 128 rows of a each, whose sums are in their own TMEM, and half of
+// the rows of w each, so that a CTA copies 32 KB for 512 cycles of products (a lone CTA's 128 x 256 tile: 48 KB).
+//   warp 0      TMA producer of its CTA's operands, credited to the even CTA's barriers
+//   warp 1      MMA issuer (even CTA), a block of k into one of two buffers of 256 columns
+//   warps 4-19  epilogue: a warp has 32 rows and 64 columns, its sums in registers (64 of 112), and after the last block bias, GELU,
+//               residual, rounding; the 32 x 64 results leave through its 4 KB of shared memory, rows of 128 bytes.  Meanwhile the
+//               next tile's first two blocks are multiplied.
+// Twenty warps are launched with 96 registers a thread; the first four keep 32, which leaves the others 112: 4 * 32 * 32 + 16 * 32 * 112
+// = 20 * 32 * 96.
+// No role waits for a warp outside an mbarrier, except the two warps that share a row's block of 128 columns for its largest value
+// (8-bit output), and those never leave their loop early.
+constexpr int PAIR_WARPS = 16, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
+constexpr int PAIR_N = 256;
+constexpr uint32_t PAIR_STAGE = 2 * BP * KB, SLAB = 4096;
+constexpr int PAIR_STAGES = 5;
+
+__device__ __forceinline__ void mma_e4m3_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// 16 bytes of a warp's slab: row r of 128 bytes, slot s of 16, so placed that neither eight lanes on neighbouring rows nor eight on one
+// row meet in a bank.
+__device__ __forceinline__ uint32_t slab_at(uint32_t slab, int r, int s) { return slab + r * 128 + ((s ^ (r & 7)) << 4); }
+
+template <typename T> struct Values16 { static constexpr int N = 16 / sizeof(T); };
+// 16 bytes of T at column n of a row that ends at column N, zeros beyond.
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p, int valid, bool vec) {
+    if (vec && valid >= Values16<T>::N) return *reinterpret_cast<const uint4*>(p);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int j = 0; j < Values16<T>::N; ++j)
+        if (j < valid) e[j] = p[j];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int valid, bool vec, const uint4& v) {
+    if (vec && valid >= Values16<T>::N) {
+        *reinterpret_cast<uint4*>(p) = v;
+    } else {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int j = 0; j < Values16<T>::N; ++j)
+            if (j < valid) p[j] = e[j];
+    }
+}
+__device__ __forceinline__ void widen16(const uint4& v, f32x2 (&f)[4], __nv_bfloat16) { bf16x8_to_f32x2(v, f); }
+__device__ __forceinline__ void widen16(const uint4& v, f32x2 (&f)[2], float) {
+    f[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+}
+
+// A warp's 64 columns: bias and GELU.
+template <typename T>
+__device__ __forceinline__ void add_bias(const LinearFp8Params& p, int n, f32x2 (&acc)[32]) {
+    constexpr int V = Values16<T>::N;
+#pragma unroll
+    for (int c = 0; c < 64; c += V) {
+        if (n + c < p.N) {
+            f32x2 b[V / 2];
+            widen16(load16<T>(static_cast<const T*>(p.bias) + n + c, p.N - n - c, p.vec), b, T());
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) acc[c / 2 + j] = add2(acc[c / 2 + j], b[j]);
+        }
+    }
+}
+// The residual of 32 rows and 128 bytes of columns (V * 8), from column n on, through the slab to the lanes that own the rows.
+template <typename T>
+__device__ __forceinline__ void add_residual(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane,
+                                             f32x2* acc) {
+    constexpr int V = Values16<T>::N;
+    const int col = n + (lane & 7) * V;
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+        uint4 r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long m = m0 + (h + i) * 4 + (lane >> 3);
+            r[i] = load16<T>(static_cast<const T*>(p.residual) + m * p.ldr + col, m < p.M ? p.N - col : 0, p.vec);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sts128(slab_at(slab, (h + i) * 4 + (lane >> 3), lane & 7), r[i]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        f32x2 f[V / 2];
+        widen16(lds128(slab_at(slab, lane, s)), f, T());
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) acc[s * (V / 2) + j] = add2(acc[s * (V / 2) + j], f[j]);
+    }
+}
+// The slab's rows of SLOTS * 16 bytes -> out, from column n on.
+template <typename T, int SLOTS>
+__device__ __forceinline__ void store_slab(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane) {
+    constexpr int V = Values16<T>::N, ROWS = 32 / SLOTS;
+    const int col = n + (lane % SLOTS) * V;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32 / ROWS; ++i) {
+        const int r = i * ROWS + lane / SLOTS;
+        const uint4 v = lds128(slab_at(slab, r, lane % SLOTS));
+        if (m0 + r < p.M) store16<T>(static_cast<T*>(p.out) + (m0 + r) * p.ldo + col, p.N - col, p.vec, v);
+    }
+}
+
+template <int OUT, bool GELU>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const LinearFp8Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* slabs = smem + PAIR_STAGES * PAIR_STAGE;
+    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 2 * PAIR_WARPS); }
+        abort_word = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmW);
+    }
+    __syncthreads();
+    if (warp == 1) { tmem_alloc_pair(&tmem_slot, 512); tmem_relinquish_pair(); }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();                                      // both CTAs' barriers exist before any remote signal
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_slot;
+    const uint32_t peer_abort = map_to_cta(smem_u32(&abort_word), rank ^ 1u);
+    auto give_up = [&](int code) {
+        st_cluster_u32(peer_abort, 1u);
+        fail(abort_flag, code);
+    };
+    chain_begin();
+
+    const int n_n = (p.N + PAIR_N - 1) / PAIR_N, n_m = (p.M + 2 * BP - 1) / (2 * BP);
+    const int tiles = n_n * n_m, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), tfull0 = smem_u32(tfull), tempty0 = smem_u32(tempty);
+    const uint32_t s0 = smem_u32(smem);
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == 0) {
+            const uint32_t lead_full0 = map_to_cta(full0, 0);
+            uint32_t s = 0, ph = 0, fills = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step) {
+                const int m0 = t / n_n * 2 * BP + (int)rank * BP, n0 = t % n_n * PAIR_N + (int)rank * BP;
+                for (int kb = 0; kb < p.blocks; ++kb) {
+                    if (!mbar_wait_warp(empty0 + 8 * s, ph ^ 1u, abort_flag)) { if (lane == 0) give_up(125); ok = false; break; }
+                    if (elect_one()) {
+                        if (rank == 0) mbar_expect_tx_a(full0 + 8 * s, 2 * PAIR_STAGE);
+                        tma_load_2d_pair(s0 + s * PAIR_STAGE, &tmA, lead_full0 + 8 * s, kb * KB, m0);
+                        tma_load_2d_pair(s0 + s * PAIR_STAGE + BP * KB, &tmW, lead_full0 + 8 * s, kb * KB, n0);
+                    }
+                    __syncwarp();
+                    ++fills;
+                    if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+                }
+            }
+            // the last signals to this CTA's barriers have come before it leaves
+            for (uint32_t i = 0; i < PAIR_STAGES && i < fills && ok; ++i) {
+                if (s == 0) { s = PAIR_STAGES; ph ^= 1u; }
+                --s;
+                ok = mbar_wait_warp(empty0 + 8 * s, ph, abort_flag);
+            }
+        } else if (warp == 1) {
+            if (rank == 0) {
+                constexpr uint32_t idesc = idesc_e4m3_f32(2 * BP, PAIR_N);
+                const uint64_t hi = kmajor_desc_hi(KB);
+                uint32_t s = 0, ph = 0, buf = 0, tph = 0;
+                bool ok = true;
+                for (int t = first; t < tiles && ok; t += step) {
+                    for (int kb = 0; kb < p.blocks; ++kb) {
+                        if (!mbar_wait_warp(tempty0 + 8 * buf, tph ^ 1u, abort_flag)) { if (lane == 0) give_up(126); ok = false; break; }
+                        if (!mbar_wait_warp(full0 + 8 * s, ph, abort_flag)) { if (lane == 0) give_up(127); ok = false; break; }
+                        tc_fence_after_sync();
+                        if (elect_one()) {
+                            const uint64_t ad = hi | (uint64_t)(((s0 + s * PAIR_STAGE) & 0x3FFFFu) >> 4);
+                            const uint64_t bd = hi | (uint64_t)(((s0 + s * PAIR_STAGE + BP * KB) & 0x3FFFFu) >> 4);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                mma_e4m3_ss_pair(tmem_base + buf * PAIR_N, ad + 2 * i, bd + 2 * i, idesc, i > 0);
+                            mma_commit_pair_both(empty0 + 8 * s);
+                            mma_commit_pair_both(tfull0 + 8 * buf);
+                        }
+                        __syncwarp();
+                        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+                        buf ^= 1u;
+                        if (buf == 0) tph ^= 1u;
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        const int quarter = warp & 3, cg = (warp - 4) >> 2, row = quarter * 32 + lane;
+        const uint32_t slab = smem_u32(slabs) + (warp - 4) * SLAB;
+        const uint32_t lead_tempty0 = map_to_cta(tempty0, 0);
+        const uint32_t taddr = tmem_base + cg * 64 + ((uint32_t)(quarter * 32) << 16);
+        // The scales, AHEAD blocks before their use, across tiles.
+        constexpr int AHEAD = 4;
+        int ft = first, fkb = 0;
+        const float *fa = nullptr, *fw = nullptr;            // nullptr: outside
+        auto enter = [&]() {                                 // tile ft
+            const int m = ft / n_n * 2 * BP + (int)rank * BP + row, n = ft % n_n * PAIR_N + cg * 64;
+            fa = nullptr;
+            if (ft < tiles && m < p.M && n < p.N) {
+                fa = p.sa + (long long)m * p.sa_row;
+                fw = p.sw + (long long)(n / KB) * p.sw_row;
+            }
+        };
+        auto fetch = [&]() {
+            float v = 0.f;
+            if (fa) {
+                v = *fa * *fw;
+                fa += p.sa_block;
+                fw += p.sw_block;
+            }
+            if (++fkb == p.blocks) { fkb = 0; ft += step; enter(); }
+            return v;
+        };
+        enter();
+        float next[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) next[i] = fetch();
+        uint32_t buf = 0, tph = 0;
+        bool ok = true;
+        for (int t = first; t < tiles; t += step) {
+            f32x2 acc[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = pack2(0.f, 0.f);
+            for (int kb = 0; kb < p.blocks; ++kb) {
+                const f32x2 by = pack2(next[0], next[0]);
+#pragma unroll
+                for (int i = 0; i + 1 < AHEAD; ++i) next[i] = next[i + 1];
+                next[AHEAD - 1] = fetch();
+                if (ok && !mbar_wait_warp(tfull0 + 8 * buf, tph, abort_flag)) { if (lane == 0) give_up(128); ok = false; }
+                tc_fence_after_sync();
+#pragma unroll
+                for (int c = 0; c < 64; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld_x16(taddr + buf * PAIR_N + c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2)
+                        acc[(c + j) / 2] = fma2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), by, acc[(c + j) / 2]);
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8 * buf);
+                buf ^= 1u;
+                if (buf == 0) tph ^= 1u;
+            }
+            const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
+            const int n = t % n_n * PAIR_N + cg * 64;
+            if (p.bias) {
+                if (p.io == CONVNN_F32) add_bias<float>(p, n, acc);
+                else add_bias<__nv_bfloat16>(p, n, acc);
+            }
+            if (GELU && OUT == OUT_F32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float a, b;
+                    unpack2(acc[j], a, b);
+                    acc[j] = pack2(gelu_erf(a), gelu_erf(b));
+                }
+            } else if (GELU) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[j] = gelu_poly(acc[j]);
+            }
+            if (p.residual) {
+                if (p.io == CONVNN_F32) {
+                    add_residual<float>(p, m0, n, slab, lane, acc);
+                    add_residual<float>(p, m0, n + 32, slab, lane, acc + 16);
+                } else {
+                    add_residual<__nv_bfloat16>(p, m0, n, slab, lane, acc);
+                }
+            }
+            __syncwarp();                                    // the slab has been read
+            if (OUT == OUT_BF16) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    const f32x2 four[4] = {acc[4 * s], acc[4 * s + 1], acc[4 * s + 2], acc[4 * s + 3]};
+                    sts128(slab_at(slab, lane, s), f32x2_to_bf16x8(four));
+                }
+                store_slab<__nv_bfloat16, 8>(p, m0, n, slab, lane);
+            } else if (OUT == OUT_F32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h) __syncwarp();
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) {
+                        float f[4];
+                        unpack2(acc[16 * h + 2 * s], f[0], f[1]);
+                        unpack2(acc[16 * h + 2 * s + 1], f[2], f[3]);
+                        sts128(slab_at(slab, lane, s), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                                                  __float_as_uint(f[3])));
+                    }
+                    store_slab<float, 8>(p, m0, n + 32 * h, slab, lane);
+                }
+            } else {
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float a, b;
+                    unpack2(acc[j], a, b);
+                    if (n + 2 * j < p.N) top = max(top, abs_bits(a));
+                    if (n + 2 * j + 1 < p.N) top = max(top, abs_bits(b));
+                }
+                const int pair = 1 + quarter * 2 + (cg >> 1);
+                // through the slabs, which are free; the other half's warp is four further or four back
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(slab + 4 * lane), "r"(top) : "memory");
+                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+                uint32_t other;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(other) : "r"(slab + (cg & 1 ? -4 : 4) * (int)SLAB + 4 * lane) : "memory");
+                top = max(top, other);
+                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");      // read before the slabs are written
+                const float scale = fp8_scale(top), inv = __frcp_rn(scale);
+                const f32x2 by = pack2(inv, inv);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float f[4];
+                        unpack2(mul2(acc[8 * s + 2 * i], by), f[0], f[1]);
+                        unpack2(mul2(acc[8 * s + 2 * i + 1], by), f[2], f[3]);
+                        w[i] = e4m3x4(f[0], f[1], f[2], f[3]);
+                    }
+                    sts128(slab_at(slab, lane, s), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+                if ((cg & 1) == 0 && m0 + lane < p.M && n < p.N) p.so[(m0 + lane) * p.so_row + n / KB * p.so_block] = scale;
+                store_slab<uint8_t, 4>(p, m0, n, slab, lane);
+            }
+            __syncwarp();                                    // the slab has been read
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();                                      // the peer no longer signals or reads this CTA
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+template <int OUT, bool GELU>
+int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8Params& p, cudaStream_t st) {
+    constexpr size_t smem = PAIR_STAGES * PAIR_STAGE + PAIR_WARPS * SLAB + 1024;
+    const long long tiles = (long long)((p.M + 2 * BP - 1) / (2 * BP)) * ((p.N + PAIR_N - 1) / PAIR_N);
+    if (tiles > 0x3fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %d x %d is too many tiles", p.M, p.N);
+    auto kern = linear_fp8_pair_kernel<OUT, GELU>;
+    CONVNN_ENSURE_SMEM(kern, smem);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(PAIR_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(2);
+    static ClusterLimit fit{};
+    int pairs = 0;
+    if (const int rc = fit.query(reinterpret_cast<const void*>(kern), &cfg, &pairs)) return rc;
+    cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs));
+    attr[1] = chained_attribute(st); cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tmA, tmW, p);
+    if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "linear_fp8 pair launch: %s", cudaGetErrorString(e));
+    CONVNN_CHECK_LAUNCH("linear_fp8_pair");
+    return CONVNN_OK;
+}
+
 bool encode_rows(CUtensorMap* m, const void* base, long long rows, int K, long long ld, int box_rows) {
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)rows}, strides[1] = {(uint64_t)ld};
     const uint32_t box[2] = {(uint32_t)KB, (uint32_t)box_rows};
@@ -406,8 +823,16 @@ int launch_linear_fp8(const void* a, long long lda, const float* sa, long long s
     p.io = io; p.gelu = gelu;
     p.out_kind = so ? OUT_E4M3 : io == CONVNN_F32 ? OUT_F32 : OUT_BF16;
     const long long per16 = io == CONVNN_F32 ? 4 : 8;
-    p.vec = (so ? ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0 : ldo % per16 == 0 && aligned16(out)) &&
+    p.vec = (so ? ldo % 16 == 0 : ldo % per16 == 0) && aligned16(out) &&
             (!bias || aligned16(bias)) && (!residual || (aligned16(residual) && ldr % per16 == 0));
+    const long long pair_tiles = (long long)((M + 2 * BP - 1) / (2 * BP)) * ((N + PAIR_N - 1) / PAIR_N);
+    if (pair_tiles >= device_sms() / 2) {
+        CUtensorMap tmA, tmW;
+        if (!encode_rows(&tmA, a, M, K, lda, BP) || !encode_rows(&tmW, w, N, K, ldw, BP)) return CONVNN_E_CUDA;
+        if (p.out_kind == OUT_F32) return gelu ? launch_pairs<OUT_F32, true>(tmA, tmW, p, st) : launch_pairs<OUT_F32, false>(tmA, tmW, p, st);
+        if (p.out_kind == OUT_BF16) return gelu ? launch_pairs<OUT_BF16, true>(tmA, tmW, p, st) : launch_pairs<OUT_BF16, false>(tmA, tmW, p, st);
+        return gelu ? launch_pairs<OUT_E4M3, true>(tmA, tmW, p, st) : launch_pairs<OUT_E4M3, false>(tmA, tmW, p, st);
+    }
     const bool swap = M <= 64;
     const int bn = !swap ? 128 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
     CUtensorMap tmP, tmQ;

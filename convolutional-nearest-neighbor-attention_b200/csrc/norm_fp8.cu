@@ -32,26 +32,67 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Eight neighbouring channels as they are stored, and as four pairs of float32.  VEC: D a multiple of eight and every row on a
-// 16-byte boundary; otherwise one by one, into the same places, so that the sums and the results are the same bits.
+// Eight neighbouring channels as they are stored, and as four pairs of float32.
 template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T* p, int valid) {
-    Raw8<T> r;
+// What a lane requests of SEG lanes' 8 * SEG channels, and how it comes to its own eight.  VEC: D a multiple of eight and rows on
+// 16-byte boundaries (8-bit rows: 8), read and written eight values at a time, without a branch for a tail (which kept the loads
+// from being requested together: 131072 x 768 107 -> 116 us).  Otherwise the lanes read value by value side by side and exchange them through shared memory (`room`, 8 *
+// 32 values a warp): 4099 x 1001 float32 26 -> 9.8 us against eight strided reads and writes a lane.  The sums, and so the results, are
+// the same bits either way.
+template <typename T, bool VEC> struct Held { Raw8<T> raw; };
+template <typename T> struct Held<T, false> { T e[8]; };
+
+template <typename T, bool VEC, int SEG>
+__device__ __forceinline__ Held<T, VEC> fetch(const T* row, int c0, int lane, int D) {
+    Held<T, VEC> h;
+    if constexpr (VEC) {
+        const int c = c0 + 8 * (lane % SEG);
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = make_uint4(0, 0, 0, 0);
-    if (VEC) {
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) h.raw.v[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            if (valid > 0) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+            if (c < D) h.raw.v[i] = reinterpret_cast<const uint4*>(row + c)[i];
     } else {
-        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < valid) e[j] = p[j];
+        for (int j = 0; j < 8; ++j) {
+            const int c = c0 + SEG * j + lane % SEG;
+            h.e[j] = c < D ? row[c] : from_f32<T>(0.f);
+        }
     }
-    return r;
+    return h;
+}
+template <typename T, bool VEC, int SEG>
+__device__ __forceinline__ Raw8<T> own8(const Held<T, VEC>& h, T* room, int lane) {
+    if constexpr (VEC) {
+        return h.raw;
+    } else {
+        T* seg = room + lane / SEG * (8 * SEG);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seg[SEG * j + lane % SEG] = h.e[j];
+        __syncwarp();
+        return *reinterpret_cast<const Raw8<T>*>(seg + 8 * (lane % SEG));
+    }
+}
+// 32 lanes' eight channels each from c0 on -> row.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store256(T* row, int c0, int lane, int D, const Raw8<T>& r, T* room) {
+    if constexpr (VEC) {
+        const int c = c0 + 8 * lane;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            if (c < D) reinterpret_cast<uint4*>(row + c)[i] = r.v[i];
+    } else {
+        __syncwarp();
+        *reinterpret_cast<Raw8<T>*>(room + 8 * lane) = r;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = c0 + 32 * j + lane;
+            if (c < D) row[c] = room[32 * j + lane];
+        }
+    }
 }
 __device__ __forceinline__ void widen(const Raw8<__nv_bfloat16>& r, f32x2 (&v)[4]) { bf16x8_to_f32x2(r.v[0], v); }
 __device__ __forceinline__ void widen(const Raw8<float>& r, f32x2 (&v)[4]) {
@@ -69,19 +110,6 @@ __device__ __forceinline__ void narrow(const f32x2 (&v)[4], Raw8<float>& r) {
         unpack2(v[2 * i], f[0], f[1]);
         unpack2(v[2 * i + 1], f[2], f[3]);
         r.v[i] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int valid, const Raw8<T>& r) {
-    if (VEC) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            if (valid > 0) reinterpret_cast<uint4*>(p)[i] = r.v[i];
-    } else {
-        const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < valid) p[j] = e[j];
     }
 }
 __device__ __forceinline__ uint32_t amax8(const f32x2 (&v)[4]) {
@@ -117,8 +145,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, int valid, const f32x2 (&
 }
 
 // x + residual as it is stored, widened again.
-template <typename T, bool VEC>
-__device__ __forceinline__ void add_residual(const NormParams& p, long long row, int c, int valid, const Raw8<T>& res, f32x2 (&v)[4]) {
+template <typename T>
+__device__ __forceinline__ Raw8<T> add_residual(const Raw8<T>& res, f32x2 (&v)[4]) {
     f32x2 r[4];
     widen(res, r);
 #pragma unroll
@@ -126,7 +154,7 @@ __device__ __forceinline__ void add_residual(const NormParams& p, long long row,
     Raw8<T> s;
     narrow(v, s);
     widen(s, v);
-    store8<T, VEC>(static_cast<T*>(p.sum) + row * p.lds + c, valid, s);
+    return s;
 }
 __device__ __forceinline__ float squares(const f32x2 (&v)[4], float ss) {
     f32x2 a = mul2(v[0], v[0]);
@@ -136,21 +164,22 @@ __device__ __forceinline__ float squares(const f32x2 (&v)[4], float ss) {
     unpack2(a, x, y);
     return ss + (x + y);
 }
+// The result of a warp's 256 channels from c0 on.
 template <typename T, bool VEC>
-__device__ __forceinline__ void finish8(const NormParams& p, long long row, int c, int valid, bool inside, const f32x2 (&v)[4],
-                                        const f32x2 (&w)[4], float rstd) {
+__device__ __forceinline__ void finish256(const NormParams& p, long long row, int c0, int lane, bool inside, const f32x2 (&v)[4],
+                                          const f32x2 (&w)[4], float rstd, T* room) {
     f32x2 y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = mul2(mul2(v[i], pack2(rstd, rstd)), w[i]);
     if (p.q) {
         const float scale = fp8_scale(block_max(amax8(y)));
-        if (!inside) return;
+        const int c = c0 + 8 * lane, valid = inside ? p.D - c : 0;
         store_e4m3<VEC>(p.q + row * p.ldy + c, valid, y, scale);
-        if (valid > 0 && c % kFp8Block == 0) p.scales[row * p.scale_row + c / kFp8Block * p.scale_block] = scale;
+        if (valid > 0 && lane % 16 == 0) p.scales[row * p.scale_row + c / kFp8Block * p.scale_block] = scale;
     } else if (inside) {
         Raw8<T> o;
         narrow(y, o);
-        store8<T, VEC>(static_cast<T*>(p.y) + row * p.ldy + c, valid, o);
+        store256<T, VEC>(static_cast<T*>(p.y) + row * p.ldy, c0, lane, p.D, o, room);
     }
 }
 
@@ -159,32 +188,31 @@ template <typename T, int NV, int R, int WPR, bool VEC>
 __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) {
     static_assert(WPR == 1 || R == 1, "rows shared by warps come one at a time");
     __shared__ float part[kWarps];
+    __shared__ __align__(16) T rooms[VEC ? 1 : kWarps][VEC ? 1 : 256];
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPR;
+    T* room = rooms[VEC ? 0 : warp];
     const long long row0 = ((long long)blockIdx.x * (kWarps / WPR) + warp / WPR) * R;
     const T* x = static_cast<const T*>(p.x);
     const T* res = static_cast<const T*>(p.residual);
-    Raw8<T> raw[R][NV], extra[R][NV], wr[NV];
-    int c[NV], valid[NV];
+    Held<T, VEC> raw[R][NV], extra[R][NV], wr[NV];
+    int c0[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        c[i] = ((wi + WPR * i) * 32 + lane) * 8;
-        valid[i] = p.D - c[i];
-    }
+    for (int i = 0; i < NV; ++i) c0[i] = (wi + WPR * i) * 256;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            raw[r][i] = load8<T, VEC>(x + (row0 + r) * p.ldx + c[i], row0 + r < p.rows ? valid[i] : 0);
+            raw[r][i] = fetch<T, VEC, 32>(x + (row0 + r) * p.ldx, c0[i], lane, row0 + r < p.rows ? p.D : 0);
     if (res) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                extra[r][i] = load8<T, VEC>(res + (row0 + r) * p.ldr + c[i], row0 + r < p.rows ? valid[i] : 0);
+                extra[r][i] = fetch<T, VEC, 32>(res + (row0 + r) * p.ldr, c0[i], lane, row0 + r < p.rows ? p.D : 0);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) wr[i] = load8<T, VEC>(static_cast<const T*>(p.weight) + c[i], valid[i]);
+    for (int i = 0; i < NV; ++i) wr[i] = fetch<T, VEC, 32>(static_cast<const T*>(p.weight), c0[i], lane, p.D);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const bool inside = row0 + r < p.rows;
@@ -192,8 +220,11 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) 
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            widen(raw[r][i], v[i]);
-            if (res) add_residual<T, VEC>(p, row0 + r, c[i], inside ? valid[i] : 0, extra[r][i], v[i]);
+            widen(own8<T, VEC, 32>(raw[r][i], room, lane), v[i]);
+            if (res) {
+                const Raw8<T> s = add_residual<T>(own8<T, VEC, 32>(extra[r][i], room, lane), v[i]);
+                if (inside) store256<T, VEC>(static_cast<T*>(p.sum) + (row0 + r) * p.lds, c0[i], lane, p.D, s, room);
+            }
             ss = squares(v[i], ss);
         }
         ss = warp_sum(ss);
@@ -208,8 +239,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             f32x2 w[4];
-            widen(wr[i], w);
-            finish8<T, VEC>(p, row0 + r, c[i], valid[i], inside, v[i], w, rstd);
+            widen(own8<T, VEC, 32>(wr[i], room, lane), w);
+            finish256<T, VEC>(p, row0 + r, c0[i], lane, inside, v[i], w, rstd, room);
         }
     }
 }
@@ -218,32 +249,35 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const NormParams p) 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) rms_norm_wide_kernel(const NormParams p) {
     __shared__ float part[kWarps];
+    __shared__ __align__(16) T rooms[VEC ? 1 : kWarps][VEC ? 1 : 256];
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    T* room = rooms[VEC ? 0 : warp];
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
-    const int steps = (p.D + 8 * kThreads - 1) / (8 * kThreads);
     float rstd = 0.f;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         float ss = 0.f;
 #pragma unroll 2
-        for (int k = 0; k < steps; ++k) {
-            const int c = (k * kThreads + threadIdx.x) * 8, valid = p.D - c;
-            const Raw8<T> raw = load8<T, VEC>(x + c, valid);
+        for (int c0 = warp * 256; c0 < p.D; c0 += kWarps * 256) {
+            const Held<T, VEC> raw = fetch<T, VEC, 32>(x, c0, lane, p.D);
+            Held<T, VEC> extra, wr;
+            if (res) extra = fetch<T, VEC, 32>(res, c0, lane, p.D);
+            if (pass) wr = fetch<T, VEC, 32>(static_cast<const T*>(p.weight), c0, lane, p.D);
             f32x2 v[4];
-            widen(raw, v);
+            widen(own8<T, VEC, 32>(raw, room, lane), v);
             if (res) {
-                const Raw8<T> extra = load8<T, VEC>(res + c, valid);
-                add_residual<T, VEC>(p, row, c, pass ? valid : 0, extra, v);
+                const Raw8<T> s = add_residual<T>(own8<T, VEC, 32>(extra, room, lane), v);
+                if (pass) store256<T, VEC>(static_cast<T*>(p.sum) + row * p.lds, c0, lane, p.D, s, room);
             }
             if (!pass) {
                 ss = squares(v, ss);
             } else {
                 f32x2 w[4];
-                widen(load8<T, VEC>(static_cast<const T*>(p.weight) + c, valid), w);
-                finish8<T, VEC>(p, row, c, valid, true, v, w, rstd);
+                widen(own8<T, VEC, 32>(wr, room, lane), w);
+                finish256<T, VEC>(p, row, c0, lane, true, v, w, rstd, room);
             }
         }
         if (!pass) {
@@ -270,8 +304,10 @@ struct QuantParams {
 constexpr int kTasks = 8;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantParams p) {
+    __shared__ __align__(16) T rooms[VEC ? 1 : kWarps][VEC ? 1 : 256];
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    T* room = rooms[VEC ? 0 : warp];
     const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
     const long long t0 = ((long long)blockIdx.x * kWarps + warp) * (2 * kTasks) + (lane >> 4);
     const long long first = t0 / blocks;
@@ -281,13 +317,12 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
         if (b >= blocks) { b -= blocks; ++row; }
         if (b >= blocks) { b -= blocks; ++row; }
     };
-    Raw8<T> raw[kTasks];
+    Held<T, VEC> raw[kTasks];
     long long row = first;
     int b = b0;
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
-        const int c = b * kFp8Block + at;
-        raw[t] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx + c, row < p.rows ? p.D - c : 0);
+        raw[t] = fetch<T, VEC, 16>(static_cast<const T*>(p.x) + row * p.ldx, b * kFp8Block, lane, row < p.rows ? p.D : 0);
         on(row, b);
     }
     row = first;
@@ -296,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
     for (int t = 0; t < kTasks; ++t) {
         const int c = b * kFp8Block + at;
         f32x2 v[4];
-        widen(raw[t], v);
+        widen(own8<T, VEC, 16>(raw[t], room, lane), v);
         const float scale = fp8_scale(block_max(amax8(v)));
         const int valid = row < p.rows ? p.D - c : 0;
         store_e4m3<VEC>(p.q + row * p.ldq + c, valid, v, scale);
@@ -309,23 +344,27 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantPara
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantParams p) {
     __shared__ uint32_t top[kWarps];
+    __shared__ __align__(16) T rooms[VEC ? 1 : kWarps][VEC ? 1 : 256];
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    T* room = rooms[VEC ? 0 : warp];
     const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
     const long long rb = blockIdx.x / blocks;
     const int b = (int)(blockIdx.x - rb * blocks), c = b * kFp8Block + (lane & 15) * 8;
     constexpr int N = kFp8Block / (2 * kWarps);
     const long long row0 = rb * kFp8Block + 2 * warp + (lane >> 4);
-    Raw8<T> raw[N];
+    Held<T, VEC> held[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const long long row = row0 + 2 * kWarps * i;
-        raw[i] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.ldx + c, row < p.rows ? p.D - c : 0);
+        held[i] = fetch<T, VEC, 16>(static_cast<const T*>(p.x) + row * p.ldx, b * kFp8Block, lane, row < p.rows ? p.D : 0);
     }
+    Raw8<T> raw[N];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         f32x2 v[4];
+        raw[i] = own8<T, VEC, 16>(held[i], room, lane);
         widen(raw[i], v);
         m = max(m, amax8(v));
     }
@@ -346,10 +385,10 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantPa
     }
 }
 
-// Whether rows of `elt`-byte values can be read 16 bytes at a time (8-bit ones: written eight).
-bool eights(const void* p, long long ld, size_t elt) {
-    return ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & (elt == 1 ? 7u : 15u)) == 0;
+bool on_boundary(const void* p, long long ld_bytes, int bytes) {
+    return ld_bytes % bytes == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
+template <typename T> bool rows16(const void* p, long long ld) { return on_boundary(p, ld * (long long)sizeof(T), 16); }
 
 template <typename T, int NV, int R, int WPR>
 int launch_norm(const NormParams& p, bool vec, cudaStream_t st) {
@@ -363,9 +402,9 @@ int launch_norm(const NormParams& p, bool vec, cudaStream_t st) {
 
 template <typename T>
 int norm_of(const NormParams& p, cudaStream_t st) {
-    const bool vec = p.D % 8 == 0 && eights(p.x, p.ldx, sizeof(T)) && eights(p.weight, 0, sizeof(T)) &&
-                     (!p.residual || (eights(p.residual, p.ldr, sizeof(T)) && eights(p.sum, p.lds, sizeof(T)))) &&
-                     (p.q ? eights(p.q, p.ldy, 1) : eights(p.y, p.ldy, sizeof(T)));
+    const bool vec = p.D % 8 == 0 && rows16<T>(p.x, p.ldx) && rows16<T>(p.weight, 0) &&
+                     (!p.residual || (rows16<T>(p.residual, p.ldr) && rows16<T>(p.sum, p.lds))) &&
+                     (p.q ? on_boundary(p.q, p.ldy, 8) : rows16<T>(p.y, p.ldy));
     const int vectors = (p.D + 255) / 256;
     if (vectors <= 1) return launch_norm<T, 1, 4, 1>(p, vec, st);
     if (vectors <= 2) return launch_norm<T, 2, 2, 1>(p, vec, st);
@@ -382,7 +421,7 @@ int norm_of(const NormParams& p, cudaStream_t st) {
 
 template <typename T>
 int quantize_of(const QuantParams& p, int block_rows, cudaStream_t st) {
-    const bool vec = p.D % 8 == 0 && eights(p.x, p.ldx, sizeof(T)) && eights(p.q, p.ldq, 1);
+    const bool vec = p.D % 8 == 0 && rows16<T>(p.x, p.ldx) && on_boundary(p.q, p.ldq, 8);
     const long long blocks = (p.D + kFp8Block - 1) / kFp8Block;
     const long long grid = block_rows == 1 ? (p.rows * blocks + 2 * kWarps * kTasks - 1) / (2 * kWarps * kTasks)
                                            : (p.rows + kFp8Block - 1) / kFp8Block * blocks;

@@ -6,6 +6,7 @@ back to torch ops.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
@@ -520,23 +521,26 @@ FP8_BLOCK = 128
 
 
 def _forward_only(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
-                           "(training / backward is outside this library)")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
+                               "(training / backward is outside this library)")
 
 
-def _same_device(like: torch.Tensor, *tensors) -> None:
-    """All on ``like``'s CUDA device."""
-    _require_cuda(like, *tensors)
+def _device_of(like: torch.Tensor, *tensors) -> int:
+    """The index of ``like``'s CUDA device, on which all of them are."""
     index = like.get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:
+            _require_cuda(like, *tensors)
             raise RuntimeError(f"all tensors must be on one device, got {like.device} and {t.device}")
+    if index < 0:
+        _require_cuda(like)
+    return index
 
 
-def _launch(like: torch.Tensor, fn, *args) -> None:
-    """``fn(*args, stream)`` with ``like``'s device current, on its current stream."""
-    index = like.get_device()
+def _launch(index: int, fn, *args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current, on its current stream."""
     if torch._C._cuda_getDevice() == index:
         rc = fn(*args, _raw_stream(index))
     else:
@@ -546,42 +550,40 @@ def _launch(like: torch.Tensor, fn, *args) -> None:
         _capi.check(rc)
 
 
-def _rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+def _rows_of(t: torch.Tensor, shape) -> Tuple[torch.Tensor, int, int]:
     """``_flat_rows`` without a division by the width (there may be no rows)."""
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t, t.shape[0], t.stride(0)
-    D = t.shape[-1]
-    rows = 1
-    for n in t.shape[:-1]:
-        rows *= n
+    D = shape[-1]
+    if len(shape) == 2:
+        ld, unit = t.stride()
+        if unit == 1 and ld >= D:
+            return t, shape[0], ld
+    rows = math.prod(shape[:-1])
     if t.is_contiguous():
         return t, rows, D
-    if t.dim() == 3:
+    if len(shape) == 3:
         v, ld = _rows_view(t)
         return v, rows, ld
     return t.contiguous(), rows, D
 
 
-def _fp8_empty(lead, D: int, device) -> Tuple[torch.Tensor, int, torch.Tensor, int]:
-    """Room for 8-bit rows with a scale per row and block: values (its rows on 16-byte boundaries, as ``linear_fp8`` reads
-    them), their stride, scales (those of one block of channels side by side), rows."""
-    rows = 1
-    for n in lead:
-        rows *= n
-    ld = (D + 15) // 16 * 16
-    values = torch.empty(*lead, ld, dtype=torch.float8_e4m3fn, device=device)
-    if ld != D:
-        values = values[..., :D]
-    scales = torch.empty((D + FP8_BLOCK - 1) // FP8_BLOCK, rows, dtype=torch.float32, device=device).t()
-    if len(lead) != 1:
-        scales = scales.view(*lead, scales.shape[1])
-    return values, ld, scales, rows
+def _fp8_empty(shape, rows: int, device) -> Tuple[torch.Tensor, int, torch.Tensor]:
+    """Room for 8-bit rows with a scale per row and block: values (rows on 16-byte boundaries, as ``linear_fp8`` reads them),
+    their stride, scales (those of one block of channels side by side)."""
+    D = shape[-1]
+    ld, blocks = -(-D // 16) * 16, -(-D // FP8_BLOCK)
+    if len(shape) == 2:
+        lead = (1,)
+    else:
+        lead = tuple(math.prod(shape[i + 1:-1]) for i in range(len(shape) - 1))
+    values = torch.empty_strided(shape, (*[n * ld for n in lead], 1), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty_strided((*shape[:-1], blocks), (*lead, max(rows, 1)), dtype=torch.float32, device=device)
+    return values, ld, scales
 
 
-def _channels(x: torch.Tensor, what: str) -> int:
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{what} needs a last dimension of at least one channel, got shape {tuple(x.shape)}")
-    return x.shape[-1]
+def _channels(shape, what: str) -> int:
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"{what} needs a last dimension of at least one channel, got shape {tuple(shape)}")
+    return shape[-1]
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
@@ -589,78 +591,82 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``s * rsqrt(mean(s * s) + eps) * weight`` over the last dimension, ``s = x``, or with ``residual`` the sum ``x +
     residual`` rounded to ``x``'s type (float32 or bfloat16).  -> y, in ``x``'s type or with ``quantize`` as ``Fp8Blocks``
     (from the float32 values) for ``linear_fp8``; with ``residual`` -> (y, s)."""
-    _forward_only(x, weight, residual)
-    _same_device(x, weight, residual)
-    D = _channels(x, "rms_norm")
-    dt = _dtype_code(x.dtype)
-    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
-        raise TypeError(f"weight and residual must have x's type, {x.dtype}")
+    if torch.is_grad_enabled():
+        _forward_only(x, weight, residual)
+    index = _device_of(x, weight, residual)
+    shape, dtype = x.shape, x.dtype
+    D = _channels(shape, "rms_norm")
+    dt = _dtype_code(dtype)
+    if weight.dtype != dtype or (residual is not None and residual.dtype != dtype):
+        raise TypeError(f"weight and residual must have x's type, {dtype}")
     if weight.shape != (D,):
         raise ValueError(f"weight must have shape ({D},), got {tuple(weight.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-    L = _capi.lib()
-    xv, rows, ldx = _rows_of(x)
-    w = weight if weight.stride(0) == 1 else weight.contiguous()
-    res, ldr, total = None, 0, None
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    xv, rows, ldx = _rows_of(x, shape)
+    res, ldr, total, sum_ptr = None, 0, None, None
     if residual is not None:
-        res, _, ldr = _rows_of(residual)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    common = (dt, xv.data_ptr(), ldx, _capi.ptr(res), ldr, w.data_ptr(), float(eps), _capi.ptr(total), D)
+        if residual.shape != shape:
+            raise ValueError(f"residual must have x's shape {tuple(shape)}, got {tuple(residual.shape)}")
+        residual, _, ldr = _rows_of(residual, shape)
+        res = residual.data_ptr()
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
+        sum_ptr = total.data_ptr()
+    L = _capi.lib()
     if quantize:
-        values, ld, scales, _ = _fp8_empty(x.shape[:-1], D, x.device)
+        values, ld, scales = _fp8_empty(shape, rows, x.device)
         y = Fp8Blocks(values, scales)
         if rows:
-            _launch(x, L.convnn_b200_rms_norm_fp8, *common, values.data_ptr(), ld, scales.data_ptr(), 1, rows, rows, D)
+            _launch(index, L.convnn_b200_rms_norm_fp8, dt, xv.data_ptr(), ldx, res, ldr, weight.data_ptr(), eps, sum_ptr, D,
+                    values.data_ptr(), ld, scales.data_ptr(), 1, rows, rows, D)
     else:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         if rows:
-            _launch(x, L.convnn_b200_rms_norm, *common, y.data_ptr(), D, rows, D)
-    return y if residual is None else (y, total)
+            _launch(index, L.convnn_b200_rms_norm, dt, xv.data_ptr(), ldx, res, ldr, weight.data_ptr(), eps, sum_ptr, D,
+                    y.data_ptr(), D, rows, D)
+    return y if total is None else (y, total)
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
     """``x`` (float32 or bfloat16) in 8 bits with a scale per row and 128 channels (``block_rows`` 1: activations (..., D)), or
     per 128 x 128 block (``block_rows`` 128: a weight (N, D)), for ``linear_fp8``."""
-    _forward_only(x)
-    _require_cuda(x)
-    D = _channels(x, "quantize_fp8")
+    if torch.is_grad_enabled():
+        _forward_only(x)
+    index = _device_of(x)
+    shape = x.shape
+    D = _channels(shape, "quantize_fp8")
     dt = _dtype_code(x.dtype)
-    if block_rows not in (1, FP8_BLOCK):
-        raise ValueError(f"a scale belongs to 1 or {FP8_BLOCK} rows, not {block_rows}")
-    if block_rows != 1 and x.dim() != 2:
-        raise ValueError(f"a weight is (N, D), got shape {tuple(x.shape)}")
-    L = _capi.lib()
-    xv, rows, ldx = _rows_of(x)
+    xv, rows, ldx = _rows_of(x, shape)
     if block_rows == 1:
-        values, ld, scales, _ = _fp8_empty(x.shape[:-1], D, x.device)
+        values, ld, scales = _fp8_empty(shape, rows, x.device)
         row, block = 1, rows
+    elif block_rows == FP8_BLOCK:
+        if len(shape) != 2:
+            raise ValueError(f"a weight is (N, D), got shape {tuple(shape)}")
+        ld, block, row = -(-D // 16) * 16, 1, -(-D // FP8_BLOCK)
+        values = torch.empty_strided(shape, (ld, 1), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty_strided((-(-rows // FP8_BLOCK), row), (row, 1), dtype=torch.float32, device=x.device)
     else:
-        ld = (D + 15) // 16 * 16
-        values = torch.empty(rows, ld, dtype=torch.float8_e4m3fn, device=x.device)[:, :D]
-        block, row = 1, (D + FP8_BLOCK - 1) // FP8_BLOCK
-        scales = torch.empty((rows + FP8_BLOCK - 1) // FP8_BLOCK, row, dtype=torch.float32, device=x.device)
+        raise ValueError(f"a scale belongs to 1 or {FP8_BLOCK} rows, not {block_rows}")
     if rows:
-        _launch(x, L.convnn_b200_quantize_fp8, dt, xv.data_ptr(), ldx, block_rows, values.data_ptr(), ld, scales.data_ptr(), row,
-                block, rows, D)
+        _launch(index, _capi.lib().convnn_b200_quantize_fp8, dt, xv.data_ptr(), ldx, block_rows, values.data_ptr(), ld,
+                scales.data_ptr(), row, block, rows, D)
     return Fp8Blocks(values, scales)
 
 
-def _fp8_rows(v: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(..., K) 8-bit values -> (tensor, row stride), rows on 16-byte boundaries: as they are, or copied."""
-    K = v.shape[-1]
-    if v.dim() != 2 or v.stride(1) != 1 or v.stride(0) < K:
-        v, rows, ld = _rows_of(v)
-    else:
-        rows, ld = v.shape[0], v.stride(0)
+def _fp8_rows(v: torch.Tensor, shape) -> Tuple[torch.Tensor, int, int, int]:
+    """(..., K) 8-bit values -> (tensor, its address, row stride, rows), rows on 16-byte boundaries: as they are, or copied."""
+    v, rows, ld = _rows_of(v, shape)
     if rows <= 1:
-        ld = (ld + 15) // 16 * 16                # (one row has no next)
-    if ld % 16 == 0 and v.data_ptr() % 16 == 0:
-        return v, ld
-    ld = (K + 15) // 16 * 16
+        ld = -(-ld // 16) * 16                   # (one row has no next)
+    at = v.data_ptr()
+    if ld % 16 == 0 and at % 16 == 0:
+        return v, at, ld, rows
+    K = shape[-1]
+    ld = -(-K // 16) * 16
     room = torch.empty(rows, ld, dtype=torch.uint8, device=v.device)
     room[:, :K].copy_(v.view(torch.uint8).reshape(rows, K))
-    return room, ld
+    return room, room.data_ptr(), ld, rows
 
 
 def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, residual: Optional[torch.Tensor] = None,
@@ -670,48 +676,52 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     bfloat16).  -> (..., N) in ``dtype``, summed in float32 and rounded once, or with ``quantize`` as ``Fp8Blocks`` for the
     next product."""
     (av, sa), (wv, sw) = a, w
-    _forward_only(bias, residual)
-    _same_device(av, sa, wv, sw, bias, residual)
+    if torch.is_grad_enabled():
+        _forward_only(bias, residual, sa, sw)
+    index = _device_of(av, sa, wv, sw, bias, residual)
     io = _dtype_code(dtype)
     if av.dtype != torch.float8_e4m3fn or wv.dtype != torch.float8_e4m3fn:
         raise TypeError(f"the values of a and w must be float8_e4m3fn, got {av.dtype} and {wv.dtype}")
     if sa.dtype != torch.float32 or sw.dtype != torch.float32:
         raise TypeError(f"the scales of a and w must be float32, got {sa.dtype} and {sw.dtype}")
-    K = _channels(av, "linear_fp8")
-    if wv.dim() != 2 or wv.shape[1] != K or wv.shape[0] < 1:
-        raise ValueError(f"w must be (N, {K}), got {tuple(wv.shape)}")
-    N, blocks, lead = wv.shape[0], (K + FP8_BLOCK - 1) // FP8_BLOCK, av.shape[:-1]
-    if sa.shape[-1:] != (blocks,) or sa.shape[:-1] != lead:
+    shape, wshape = av.shape, wv.shape
+    K = _channels(shape, "linear_fp8")
+    if len(wshape) != 2 or wshape[1] != K or wshape[0] < 1:
+        raise ValueError(f"w must be (N, {K}), got {tuple(wshape)}")
+    N, blocks, lead = wshape[0], -(-K // FP8_BLOCK), shape[:-1]
+    if sa.shape != (*lead, blocks):
         raise ValueError(f"the scales of a must have shape {(*lead, blocks)}, got {tuple(sa.shape)}")
-    if sw.shape != ((N + FP8_BLOCK - 1) // FP8_BLOCK, blocks):
-        raise ValueError(f"the scales of w must have shape {((N + FP8_BLOCK - 1) // FP8_BLOCK, blocks)}, got {tuple(sw.shape)}")
+    if sw.shape != (-(-N // FP8_BLOCK), blocks):
+        raise ValueError(f"the scales of w must have shape {(-(-N // FP8_BLOCK), blocks)}, got {tuple(sw.shape)}")
+    out_shape = (*lead, N)
+    bias_ptr, res, ldr = None, None, 0
     if bias is not None:
         if bias.dtype != dtype or bias.shape != (N,):
             raise ValueError(f"bias must be ({N},) in {dtype}, got {tuple(bias.shape)} in {bias.dtype}")
-        if bias.stride(0) != 1:
+        if not bias.is_contiguous():
             bias = bias.contiguous()
-    if residual is not None and (residual.dtype != dtype or residual.shape != (*lead, N)):
-        raise ValueError(f"residual must be {(*lead, N)} in {dtype}, got {tuple(residual.shape)} in {residual.dtype}")
-    L = _capi.lib()
-    out_scales, so_row, so_block = None, 0, 0
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        if residual.dtype != dtype or residual.shape != out_shape:
+            raise ValueError(f"residual must be {out_shape} in {dtype}, got {tuple(residual.shape)} in {residual.dtype}")
+        residual, _, ldr = _rows_of(residual, out_shape)
+        res = residual.data_ptr()
+    av, a_ptr, lda, M = _fp8_rows(av, shape)
+    wv, w_ptr, ldw, _ = _fp8_rows(wv, wshape)
+    out_scales, so_ptr, so_block, ldo = None, None, 0, N
     if quantize:
-        out, ldo, out_scales, M = _fp8_empty(lead, N, av.device)
-        so_row, so_block = 1, M
+        out, ldo, out_scales = _fp8_empty(out_shape, M, av.device)
+        so_ptr, so_block = out_scales.data_ptr(), M
     else:
-        out, ldo, M = torch.empty(*lead, N, dtype=dtype, device=av.device), N, 1
-        for n in lead:
-            M *= n
+        out = (torch.empty_strided(out_shape, (N, 1), dtype=dtype, device=av.device) if len(out_shape) == 2 else
+               torch.empty(out_shape, dtype=dtype, device=av.device))
     if M:
-        av, lda = _fp8_rows(av)
-        wv, ldw = _fp8_rows(wv)
-        if sa.dim() != 2:
+        if len(shape) != 2:
             sa = sa.reshape(M, blocks)
-        res, ldr = None, 0
-        if residual is not None:
-            res, _, ldr = _rows_of(residual)
-        _launch(av, L.convnn_b200_linear_fp8, av.data_ptr(), lda, sa.data_ptr(), sa.stride(0), sa.stride(1), wv.data_ptr(), ldw,
-                sw.data_ptr(), sw.stride(0), sw.stride(1), io, _capi.ptr(bias), _capi.ptr(res), ldr, out.data_ptr(), ldo,
-                _capi.ptr(out_scales), so_row, so_block, M, N, K, int(gelu))
+        sa_row, sa_block = sa.stride()
+        sw_row, sw_block = sw.stride()
+        _launch(index, _capi.lib().convnn_b200_linear_fp8, a_ptr, lda, sa.data_ptr(), sa_row, sa_block, w_ptr, ldw, sw.data_ptr(),
+                sw_row, sw_block, io, bias_ptr, res, ldr, out.data_ptr(), ldo, so_ptr, 1, so_block, M, N, K, int(gelu))
     return Fp8Blocks(out, out_scales) if quantize else out
 
 

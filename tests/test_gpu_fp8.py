@@ -283,6 +283,43 @@ def test_linear_many_rows_of_a_long_batch():
     check_linear(a, w, randn(768, seed=8, dtype=BF16), gelu=True, quantize=True)
 
 
+# shapes of at least 74 tiles of 256 x 256, the persistent pairs' form
+PAIR_SIZES = [(256 * 74, 256, 128), (256 * 73 + 1, 200, 100), (256 * 40 - 3, 257, 300), (2500, 2000, 1333), (5000, 1111, 640), (2304, 2304, 4096),
+              (100, 20000, 200)]
+
+
+@pytest.mark.parametrize("M,N,K", PAIR_SIZES)
+@pytest.mark.parametrize("dtype,quantize", [(BF16, False), (F32, False), (BF16, True)])
+def test_linear_many_tiles(M, N, K, dtype, quantize):
+    a, w = operands(M, N, K, seed=M + N)
+    check_linear(a, w, dtype=dtype, quantize=quantize)
+    bias, res = randn(N, seed=8, dtype=dtype), randn(M, N, seed=9, dtype=dtype)
+    check_linear(a, w, bias, False, res, dtype, quantize)
+    check_linear(a, w, bias, True, None, dtype, quantize)
+    check_linear(a, w, None, True, res, dtype, quantize)
+
+
+def test_linear_many_tiles_strides_and_nan():
+    M, N, K = 4000, 1300, 400
+    a, w = operands(M, N, K, seed=2)
+    res = randn(M, N + 3, seed=6)[:, 3:]
+    bias = randn(N + 1, seed=5)[1:]
+    want = ops.linear_fp8(a, w, bias=bias.clone(), residual=res.contiguous(), dtype=F32)
+    got = ops.linear_fp8((a.values, a.scales.contiguous()), w, bias=bias, residual=res, dtype=F32)
+    assert torch.equal(got, want)
+    a.scales[7, 1] = float("nan")
+    got = ops.linear_fp8(a, w, bias=bias, residual=res, dtype=F32)
+    assert got[7].isnan().all() and torch.equal(got[:7], want[:7]) and torch.equal(got[8:], want[8:])
+    q = ops.linear_fp8(a, w, gelu=True, quantize=True)
+    assert meant(q)[7].isnan().all() and meant(q)[8:].isfinite().all()
+    out = torch.full((M, N + 5), 3.0, device=DEV)            # rows of another stride, the rest left alone
+    L = _capi.lib()
+    _capi.check(L.convnn_b200_linear_fp8(a.values.data_ptr(), 400, a.scales.data_ptr(), *a.scales.stride(), w.values.data_ptr(), 400,
+                                         w.scales.data_ptr(), *w.scales.stride(), _capi.F32, None, None, 0, out.data_ptr(), N + 5, None,
+                                         0, 0, M, N, K, 0, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[8:, :N], ops.linear_fp8(a, w, dtype=F32)[8:]) and (out[:, N:] == 3).all()
+
+
 @pytest.mark.parametrize("M", [5, 40, 150])
 def test_linear_strides_and_shapes(M):
     N, K = 160, 400
