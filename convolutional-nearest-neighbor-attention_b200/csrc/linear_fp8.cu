@@ -416,17 +416,19 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 // the rows of w each, so that a CTA copies 32 KB for 512 cycles of products (a lone CTA's 128 x 256 tile: 48 KB).
 //   warp 0      TMA producer of its CTA's operands, credited to the even CTA's barriers
 //   warp 1      MMA issuer (even CTA), a block of k into one of two buffers of 256 columns
-//   warps 4-19  epilogue: a warp has 32 rows and 64 columns, its sums in registers (64 of 112), and after the last block bias, GELU,
-//               residual, rounding; the 32 x 64 results leave through its 4 KB of shared memory, rows of 128 bytes.  Meanwhile the
-//               next tile's first two blocks are multiplied.
-// Twenty warps are launched with 96 registers a thread; the first four keep 32, which leaves the others 112: 4 * 32 * 32 + 16 * 32 * 112
-// = 20 * 32 * 96.
-// No role waits for a warp outside an mbarrier, except the two warps that share a row's block of 128 columns for its largest value
-// (8-bit output), and those never leave their loop early.
-constexpr int PAIR_WARPS = 16, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
+//   warps 2, 3  scales: each the products of the rows' scales and that of one half of the columns, four blocks of k at a time
+//   warps 4-11  epilogue: a warp has 32 rows and 128 columns, its sums in registers (128 of 224), and after the last block bias, GELU,
+//               residual, rounding; the results leave through its 4 KB of shared memory, rows of 128 bytes.  Meanwhile the next
+//               tile's first two blocks are multiplied.
+// Twelve warps are launched with 168 registers a thread; the first four keep 56, which leaves the others 224: 4 * 32 * 56 + 8 * 32 * 224
+// = 12 * 32 * 168.  (Sixteen epilogue warps of 64 columns took 1350 cycles a block of k, 720 of them for loads and sums, the rest around
+// barriers; the products take 512.)
+constexpr int PAIR_WARPS = 8, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 constexpr int PAIR_N = 256;
 constexpr uint32_t PAIR_STAGE = 2 * BP * KB, SLAB = 4096;
 constexpr int PAIR_STAGES = 5;
+constexpr int SCALE_GROUP = 4, SCALE_SLOTS = 2;              // blocks of k whose scales come together, and how many times that is held
+constexpr uint32_t SCALE_BYTES = SCALE_GROUP * 2 * BP * 4;
 
 __device__ __forceinline__ void mma_e4m3_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                                  uint32_t accumulate) {
@@ -436,6 +438,10 @@ __device__ __forceinline__ void mma_e4m3_ss_pair(uint32_t tmem_d, uint64_t adesc
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[16], float scale) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = fmaf(__uint_as_float(part[j]), scale, acc[j]);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
     uint4 v;
@@ -472,30 +478,33 @@ __device__ __forceinline__ void store16(T* p, int valid, bool vec, const uint4& 
             if (j < valid) p[j] = e[j];
     }
 }
-__device__ __forceinline__ void widen16(const uint4& v, f32x2 (&f)[4], __nv_bfloat16) { bf16x8_to_f32x2(v, f); }
-__device__ __forceinline__ void widen16(const uint4& v, f32x2 (&f)[2], float) {
-    f[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
-    f[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+// acc += the values of 16 bytes.
+__device__ __forceinline__ void add16(const uint4& v, float* acc, __nv_bfloat16) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        acc[2 * i] += __uint_as_float(w[i] << 16);
+        acc[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void add16(const uint4& v, float* acc, float) {
+    acc[0] += __uint_as_float(v.x); acc[1] += __uint_as_float(v.y);
+    acc[2] += __uint_as_float(v.z); acc[3] += __uint_as_float(v.w);
 }
 
-// A warp's 64 columns: bias and GELU.
+// A warp's 128 columns.
 template <typename T>
-__device__ __forceinline__ void add_bias(const LinearFp8Params& p, int n, f32x2 (&acc)[32]) {
+__device__ __forceinline__ void add_bias(const LinearFp8Params& p, int n, float (&acc)[128]) {
     constexpr int V = Values16<T>::N;
 #pragma unroll
-    for (int c = 0; c < 64; c += V) {
-        if (n + c < p.N) {
-            f32x2 b[V / 2];
-            widen16(load16<T>(static_cast<const T*>(p.bias) + n + c, p.N - n - c, p.vec), b, T());
-#pragma unroll
-            for (int j = 0; j < V / 2; ++j) acc[c / 2 + j] = add2(acc[c / 2 + j], b[j]);
-        }
+    for (int c = 0; c < 128; c += V) {
+        if (n + c < p.N) add16(load16<T>(static_cast<const T*>(p.bias) + n + c, p.N - n - c, p.vec), acc + c, T());
     }
 }
 // The residual of 32 rows and 128 bytes of columns (V * 8), from column n on, through the slab to the lanes that own the rows.
 template <typename T>
 __device__ __forceinline__ void add_residual(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane,
-                                             f32x2* acc) {
+                                             float* acc) {
     constexpr int V = Values16<T>::N;
     const int col = n + (lane & 7) * V;
     __syncwarp();
@@ -512,23 +521,18 @@ __device__ __forceinline__ void add_residual(const LinearFp8Params& p, long long
     }
     __syncwarp();
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        f32x2 f[V / 2];
-        widen16(lds128(slab_at(slab, lane, s)), f, T());
-#pragma unroll
-        for (int j = 0; j < V / 2; ++j) acc[s * (V / 2) + j] = add2(acc[s * (V / 2) + j], f[j]);
-    }
+    for (int s = 0; s < 8; ++s) add16(lds128(slab_at(slab, lane, s)), acc + s * V, T());
 }
-// The slab's rows of SLOTS * 16 bytes -> out, from column n on.
-template <typename T, int SLOTS>
+// The slab's 32 rows of 128 bytes -> out, from column n on.
+template <typename T>
 __device__ __forceinline__ void store_slab(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane) {
-    constexpr int V = Values16<T>::N, ROWS = 32 / SLOTS;
-    const int col = n + (lane % SLOTS) * V;
+    constexpr int V = Values16<T>::N;
+    const int col = n + (lane & 7) * V;
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32 / ROWS; ++i) {
-        const int r = i * ROWS + lane / SLOTS;
-        const uint4 v = lds128(slab_at(slab, r, lane % SLOTS));
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        const uint4 v = lds128(slab_at(slab, r, lane & 7));
         if (m0 + r < p.M) store16<T>(static_cast<T*>(p.out) + (m0 + r) * p.ldo + col, p.N - col, p.vec, v);
     }
 }
@@ -539,7 +543,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* slabs = smem + PAIR_STAGES * PAIR_STAGE;
-    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2];
+    float* scales = reinterpret_cast<float*>(slabs + PAIR_WARPS * SLAB);       // [slot][block of the group][half of the columns][row]
+    __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2], sfull[SCALE_SLOTS], sempty[SCALE_SLOTS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
@@ -549,6 +554,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     if (threadIdx.x == 0) {
         for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 2 * PAIR_WARPS); }
+        for (int b = 0; b < SCALE_SLOTS; ++b) { mbar_init(&sfull[b], 2); mbar_init(&sempty[b], PAIR_WARPS); }
         abort_word = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmA);
@@ -574,7 +580,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     const uint32_t s0 = smem_u32(smem);
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
             const uint32_t lead_full0 = map_to_cta(full0, 0);
             uint32_t s = 0, ph = 0, fills = 0;
@@ -626,149 +632,160 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                     }
                 }
             }
+        } else {
+            const int half = warp - 2;
+            const long long rows32 = 32 * p.sa_row;
+            uint32_t slot = 0, ph = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += step) {
+                const int m0 = t / n_n * 2 * BP + (int)rank * BP + lane, n = t % n_n * PAIR_N + half * KB;
+                const float* sa = p.sa + (long long)m0 * p.sa_row;
+                const float* sw = p.sw + (long long)(n / KB) * p.sw_row;
+                for (int kb0 = 0; kb0 < p.blocks; kb0 += SCALE_GROUP) {
+                    // (all requested before the first is used)
+                    float v[SCALE_GROUP][4], w[SCALE_GROUP];
+#pragma unroll
+                    for (int i = 0; i < SCALE_GROUP; ++i) {
+                        const bool in = kb0 + i < p.blocks && n < p.N;
+                        w[i] = 0.f;
+                        if (in) w[i] = sw[i * p.sw_block];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            v[i][j] = 0.f;
+                            if (in && m0 + 32 * j < p.M) v[i][j] = sa[j * rows32 + i * p.sa_block];
+                        }
+                    }
+                    sa += SCALE_GROUP * p.sa_block;
+                    sw += SCALE_GROUP * p.sw_block;
+                    if (!mbar_wait_warp(smem_u32(&sempty[slot]), ph ^ 1u, abort_flag)) { if (lane == 0) give_up(129); ok = false; break; }
+                    float* to = scales + slot * (SCALE_BYTES / 4) + half * BP + lane;
+#pragma unroll
+                    for (int i = 0; i < SCALE_GROUP; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) to[i * 2 * BP + 32 * j] = v[i][j] * w[i];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[slot]);
+                    if (++slot == SCALE_SLOTS) { slot = 0; ph ^= 1u; }
+                }
+            }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-        const int quarter = warp & 3, cg = (warp - 4) >> 2, row = quarter * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
         const uint32_t slab = smem_u32(slabs) + (warp - 4) * SLAB;
         const uint32_t lead_tempty0 = map_to_cta(tempty0, 0);
-        const uint32_t taddr = tmem_base + cg * 64 + ((uint32_t)(quarter * 32) << 16);
-        // The scales, AHEAD blocks before their use, across tiles.
-        constexpr int AHEAD = 4;
-        int ft = first, fkb = 0;
-        const float *fa = nullptr, *fw = nullptr;            // nullptr: outside
-        auto enter = [&]() {                                 // tile ft
-            const int m = ft / n_n * 2 * BP + (int)rank * BP + row, n = ft % n_n * PAIR_N + cg * 64;
-            fa = nullptr;
-            if (ft < tiles && m < p.M && n < p.N) {
-                fa = p.sa + (long long)m * p.sa_row;
-                fw = p.sw + (long long)(n / KB) * p.sw_row;
-            }
-        };
-        auto fetch = [&]() {
-            float v = 0.f;
-            if (fa) {
-                v = *fa * *fw;
-                fa += p.sa_block;
-                fw += p.sw_block;
-            }
-            if (++fkb == p.blocks) { fkb = 0; ft += step; enter(); }
-            return v;
-        };
-        enter();
-        float next[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) next[i] = fetch();
-        uint32_t buf = 0, tph = 0;
+        const uint32_t taddr = tmem_base + half * KB + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t sc0 = smem_u32(scales) + (half * BP + row) * 4, sfull0 = smem_u32(sfull);
+        uint32_t slot = 0, sph = 0, buf = 0, tph = 0;
         bool ok = true;
+        uint32_t even[16], odd[16];
         for (int t = first; t < tiles; t += step) {
-            f32x2 acc[32];
+            float acc[128];                                  // (pairs, as elsewhere, do not stay in registers here)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[j] = pack2(0.f, 0.f);
+            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) odd[j] = 0u;
+            float last = 0.f;
+#pragma unroll 1
             for (int kb = 0; kb < p.blocks; ++kb) {
-                const f32x2 by = pack2(next[0], next[0]);
-#pragma unroll
-                for (int i = 0; i + 1 < AHEAD; ++i) next[i] = next[i + 1];
-                next[AHEAD - 1] = fetch();
+                const int in_group = kb % SCALE_GROUP;
+                if (in_group == 0 && ok && !mbar_wait_warp(sfull0 + 8 * slot, sph, abort_flag)) { if (lane == 0) give_up(130); ok = false; }
+                float scale;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(sc0 + slot * SCALE_BYTES + in_group * (2 * BP * 4)) : "memory");
                 if (ok && !mbar_wait_warp(tfull0 + 8 * buf, tph, abort_flag)) { if (lane == 0) give_up(128); ok = false; }
                 tc_fence_after_sync();
+                // sixteen columns are added up while the next are on their way, the last under the next block's first
+                const uint32_t from = taddr + buf * PAIR_N;
+                tmem_ld_x16(from, even);
+                add_scaled(acc + 112, odd, last);
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    uint32_t r[16];
-                    tmem_ld_x16(taddr + buf * PAIR_N + c, r);
+                for (int c = 0; c < 8; c += 2) {
                     tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2)
-                        acc[(c + j) / 2] = fma2(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), by, acc[(c + j) / 2]);
+                    tmem_ld_x16(from + 16 * (c + 1), odd);
+                    add_scaled(acc + 16 * c, even, scale);
+                    tmem_ld_wait();
+                    if (c == 6) break;
+                    tmem_ld_x16(from + 16 * (c + 2), even);
+                    add_scaled(acc + 16 * (c + 1), odd, scale);
                 }
+                last = scale;
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8 * buf);
                 buf ^= 1u;
                 if (buf == 0) tph ^= 1u;
+                if (in_group == SCALE_GROUP - 1 || kb == p.blocks - 1) {
+                    if (lane == 0) mbar_arrive(&sempty[slot]);
+                    if (++slot == SCALE_SLOTS) { slot = 0; sph ^= 1u; }
+                }
             }
+            add_scaled(acc + 112, odd, last);
             const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
-            const int n = t % n_n * PAIR_N + cg * 64;
+            const int n = t % n_n * PAIR_N + half * KB;
             if (p.bias) {
                 if (p.io == CONVNN_F32) add_bias<float>(p, n, acc);
                 else add_bias<__nv_bfloat16>(p, n, acc);
             }
             if (GELU && OUT == OUT_F32) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float a, b;
-                    unpack2(acc[j], a, b);
-                    acc[j] = pack2(gelu_erf(a), gelu_erf(b));
-                }
+                for (int j = 0; j < 128; ++j) acc[j] = gelu_erf(acc[j]);
             } else if (GELU) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) acc[j] = gelu_poly(acc[j]);
+                for (int j = 0; j < 128; j += 2) unpack2(gelu_poly(pack2(acc[j], acc[j + 1])), acc[j], acc[j + 1]);
             }
             if (p.residual) {
                 if (p.io == CONVNN_F32) {
-                    add_residual<float>(p, m0, n, slab, lane, acc);
-                    add_residual<float>(p, m0, n + 32, slab, lane, acc + 16);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) add_residual<float>(p, m0, n + 32 * q, slab, lane, acc + 32 * q);
                 } else {
-                    add_residual<__nv_bfloat16>(p, m0, n, slab, lane, acc);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) add_residual<__nv_bfloat16>(p, m0, n + 64 * q, slab, lane, acc + 64 * q);
                 }
             }
-            __syncwarp();                                    // the slab has been read
             if (OUT == OUT_BF16) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    const f32x2 four[4] = {acc[4 * s], acc[4 * s + 1], acc[4 * s + 2], acc[4 * s + 3]};
-                    sts128(slab_at(slab, lane, s), f32x2_to_bf16x8(four));
-                }
-                store_slab<__nv_bfloat16, 8>(p, m0, n, slab, lane);
-            } else if (OUT == OUT_F32) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h) __syncwarp();
+                for (int q = 0; q < 2; ++q) {
+                    __syncwarp();                            // the slab has been read
 #pragma unroll
                     for (int s = 0; s < 8; ++s) {
-                        float f[4];
-                        unpack2(acc[16 * h + 2 * s], f[0], f[1]);
-                        unpack2(acc[16 * h + 2 * s + 1], f[2], f[3]);
+                        const float* v = acc + 64 * q + 8 * s;
+                        const f32x2 four[4] = {pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
+                        sts128(slab_at(slab, lane, s), f32x2_to_bf16x8(four));
+                    }
+                    store_slab<__nv_bfloat16>(p, m0, n + 64 * q, slab, lane);
+                }
+            } else if (OUT == OUT_F32) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    __syncwarp();
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) {
+                        const float* f = acc + 32 * q + 4 * s;
                         sts128(slab_at(slab, lane, s), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
                                                                   __float_as_uint(f[3])));
                     }
-                    store_slab<float, 8>(p, m0, n + 32 * h, slab, lane);
+                    store_slab<float>(p, m0, n + 32 * q, slab, lane);
                 }
             } else {
                 uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float a, b;
-                    unpack2(acc[j], a, b);
-                    if (n + 2 * j < p.N) top = max(top, abs_bits(a));
-                    if (n + 2 * j + 1 < p.N) top = max(top, abs_bits(b));
-                }
-                const int pair = 1 + quarter * 2 + (cg >> 1);
-                // through the slabs, which are free; the other half's warp is four further or four back
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(slab + 4 * lane), "r"(top) : "memory");
-                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-                uint32_t other;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(other) : "r"(slab + (cg & 1 ? -4 : 4) * (int)SLAB + 4 * lane) : "memory");
-                top = max(top, other);
-                asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");      // read before the slabs are written
+                for (int j = 0; j < 128; ++j)
+                    if (n + j < p.N) top = max(top, abs_bits(acc[j]));
                 const float scale = fp8_scale(top), inv = __frcp_rn(scale);
-                const f32x2 by = pack2(inv, inv);
+                __syncwarp();
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
+                for (int s = 0; s < 8; ++s) {
                     uint32_t w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float f[4];
-                        unpack2(mul2(acc[8 * s + 2 * i], by), f[0], f[1]);
-                        unpack2(mul2(acc[8 * s + 2 * i + 1], by), f[2], f[3]);
-                        w[i] = e4m3x4(f[0], f[1], f[2], f[3]);
+                        const float* f = acc + 16 * s + 4 * i;
+                        w[i] = e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
                     }
                     sts128(slab_at(slab, lane, s), make_uint4(w[0], w[1], w[2], w[3]));
                 }
-                if ((cg & 1) == 0 && m0 + lane < p.M && n < p.N) p.so[(m0 + lane) * p.so_row + n / KB * p.so_block] = scale;
-                store_slab<uint8_t, 4>(p, m0, n, slab, lane);
+                if (m0 + lane < p.M && n < p.N) p.so[(m0 + lane) * p.so_row + n / KB * p.so_block] = scale;
+                store_slab<uint8_t>(p, m0, n, slab, lane);
             }
-            __syncwarp();                                    // the slab has been read
         }
     }
     __syncwarp();
@@ -780,7 +797,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 
 template <int OUT, bool GELU>
 int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8Params& p, cudaStream_t st) {
-    constexpr size_t smem = PAIR_STAGES * PAIR_STAGE + PAIR_WARPS * SLAB + 1024;
+    constexpr size_t smem = PAIR_STAGES * PAIR_STAGE + PAIR_WARPS * SLAB + SCALE_SLOTS * SCALE_BYTES + 1024;
     const long long tiles = (long long)((p.M + 2 * BP - 1) / (2 * BP)) * ((p.N + PAIR_N - 1) / PAIR_N);
     if (tiles > 0x3fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %d x %d is too many tiles", p.M, p.N);
     auto kern = linear_fp8_pair_kernel<OUT, GELU>;
