@@ -82,18 +82,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 12 in a / 2.5 - 1
 // that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 6.4e-7; off by 8.5e-7 *
-// |x| at most as it is evaluated here).  Sixteen instructions on pairs instead of erff's ~30 on one value.
-__device__ __forceinline__ f32x2 gelu_poly(f32x2 x) {
+// |x| at most as it is evaluated here).  Sixteen instructions instead of erff's ~30; single ones, whose constants are immediates, not
+// pairs, whose constants take registers.
+// Eight values side by side: the steps of one wait for one another.
+__device__ __forceinline__ void gelu_poly8(float* x) {
     constexpr float C[13] = {0.00621029362f, -0.0438225605f, 0.136878088f, -0.239581555f, 0.232788831f, -0.0657733977f, -0.131332964f,
                              0.163930997f, -0.0241190977f, -0.0787944123f, 0.0401191078f, 0.0140417274f, -0.0105441259f};
-    float x0, x1;
-    unpack2(x, x0, x1);
-    const float a0 = fminf(fabsf(x0), 5.0f), a1 = fminf(fabsf(x1), 5.0f);
-    const f32x2 u = fma2(pack2(a0, a1), pack2(0.4f, 0.4f), pack2(-1.0f, -1.0f));
-    f32x2 q = pack2(C[12], C[12]);
+    float a[8], u[8], q[8];
 #pragma unroll
-    for (int i = 11; i >= 0; --i) q = fma2(q, u, pack2(C[i], C[i]));
-    return fma2(pack2(-a0, -a1), q, pack2(max_nan(x0, 0.f), max_nan(x1, 0.f)));
+    for (int j = 0; j < 8; ++j) {
+        a[j] = fminf(fabsf(x[j]), 5.0f);
+        u[j] = fmaf(a[j], 0.4f, -1.0f);
+        q[j] = fmaf(u[j], C[12], C[11]);
+    }
+#pragma unroll
+    for (int i = 10; i >= 0; --i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = fmaf(q[j], u[j], C[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(-a[j], q[j], max_nan(x[j], 0.f));
 }
 
 template <typename T>
@@ -143,8 +150,7 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = gelu_erf(v[j]);
     } else if (p.gelu) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) unpack2(gelu_poly(pack2(v[j], v[j + 1])), v[j], v[j + 1]);
+        gelu_poly8(v);
     }
     if (p.residual && valid > 0) {
         float r[8];
@@ -418,15 +424,16 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 //   warp 1      MMA issuer (even CTA), a block of k into one of two buffers of 256 columns
 //   warps 2, 3  scales: each the products of the rows' scales and that of one half of the columns, four blocks of k at a time
 //   warps 4-11  epilogue: a warp has 32 rows and 128 columns, its sums in registers (128 of 224), and after the last block bias, GELU,
-//               residual, rounding; the results leave through its 4 KB of shared memory, rows of 128 bytes.  Meanwhile the next
-//               tile's first two blocks are multiplied.
+//               residual, rounding; the results leave through its two slabs of shared memory, 32 rows of 128 bytes in the order
+//               of the 128-byte swizzle, by TMA where rows start on 16-byte boundaries.  Meanwhile the next tile's first two
+//               blocks are multiplied.
 // Twelve warps are launched with 168 registers a thread; the first four keep 56, which leaves the others 224: 4 * 32 * 56 + 8 * 32 * 224
 // = 12 * 32 * 168.  (Sixteen epilogue warps of 64 columns took 1350 cycles a block of k, 720 of them for loads and sums, the rest around
 // barriers; the products take 512.)
 constexpr int PAIR_WARPS = 8, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 constexpr int PAIR_N = 256;
 constexpr uint32_t PAIR_STAGE = 2 * BP * KB, SLAB = 4096;
-constexpr int PAIR_STAGES = 5;
+constexpr int PAIR_STAGES = 4;
 constexpr int SCALE_GROUP = 4, SCALE_SLOTS = 2;              // blocks of k whose scales come together, and how many times that is held
 constexpr uint32_t SCALE_BYTES = SCALE_GROUP * 2 * BP * 4;
 
@@ -439,9 +446,26 @@ __device__ __forceinline__ void mma_e4m3_ss_pair(uint32_t tmem_d, uint64_t adesc
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ void tma_store_2d_a(const CUtensorMap* m, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(m)), "r"(src), "r"(c0), "r"(c1)
+                 : "memory");
+}
 __device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[16], float scale) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[j] = fmaf(__uint_as_float(part[j]), scale, acc[j]);
+}
+// Whether a phase is over, without waiting for it.
+__device__ __forceinline__ bool mbar_test_a(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
     uint4 v;
@@ -451,33 +475,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
 __device__ __forceinline__ void sts128(uint32_t at, const uint4& v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// 16 bytes of a warp's slab: row r of 128 bytes, slot s of 16, so placed that neither eight lanes on neighbouring rows nor eight on one
-// row meet in a bank.
+// 16 bytes of a warp's slab: row r of 128 bytes, slot s of 16, placed as the 128-byte swizzle does: neither eight lanes on neighbouring
+// rows nor eight on one row meet in a bank.
 __device__ __forceinline__ uint32_t slab_at(uint32_t slab, int r, int s) { return slab + r * 128 + ((s ^ (r & 7)) << 4); }
 
 template <typename T> struct Values16 { static constexpr int N = 16 / sizeof(T); };
-// 16 bytes of T at column n of a row that ends at column N, zeros beyond.
-template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int valid, bool vec) {
-    if (vec && valid >= Values16<T>::N) return *reinterpret_cast<const uint4*>(p);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-    for (int j = 0; j < Values16<T>::N; ++j)
-        if (j < valid) e[j] = p[j];
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ void store16(T* p, int valid, bool vec, const uint4& v) {
-    if (vec && valid >= Values16<T>::N) {
-        *reinterpret_cast<uint4*>(p) = v;
-    } else {
-        const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int j = 0; j < Values16<T>::N; ++j)
-            if (j < valid) p[j] = e[j];
-    }
-}
 // acc += the values of 16 bytes.
 __device__ __forceinline__ void add16(const uint4& v, float* acc, __nv_bfloat16) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -491,59 +493,79 @@ __device__ __forceinline__ void add16(const uint4& v, float* acc, float) {
     acc[0] += __uint_as_float(v.x); acc[1] += __uint_as_float(v.y);
     acc[2] += __uint_as_float(v.z); acc[3] += __uint_as_float(v.w);
 }
-
-// A warp's 128 columns.
+// The residual of 32 rows and 128 bytes of columns from column n on into the slab: asked for here, there after residual_arrived().
 template <typename T>
-__device__ __forceinline__ void add_bias(const LinearFp8Params& p, int n, float (&acc)[128]) {
+__device__ __forceinline__ void request_residual(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane) {
     constexpr int V = Values16<T>::N;
+    const int col = n + (lane & 7) * V, valid = p.N - col;
+    const T* from = static_cast<const T*>(p.residual) + (m0 + (lane >> 3)) * p.ldr + col;
 #pragma unroll
-    for (int c = 0; c < 128; c += V) {
-        if (n + c < p.N) add16(load16<T>(static_cast<const T*>(p.bias) + n + c, p.N - n - c, p.vec), acc + c, T());
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        const bool in = m0 + r < p.M && valid > 0;
+        const uint32_t to = slab_at(slab, r, lane & 7);
+        if (p.vec) {
+            const uint32_t bytes = in ? min(16u, (uint32_t)valid * (uint32_t)sizeof(T)) : 0u;      // the rest is filled with zeros
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? from : static_cast<const T*>(p.residual)),
+                         "r"(bytes)
+                         : "memory");
+        } else {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            T* e = reinterpret_cast<T*>(&v);
+            if (in) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j < valid) e[j] = from[j];
+            }
+            sts128(to, v);
+        }
+        from += 4 * p.ldr;
     }
 }
-// The residual of 32 rows and 128 bytes of columns (V * 8), from column n on, through the slab to the lanes that own the rows.
+__device__ __forceinline__ void residual_arrived() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+}
+// acc += this lane's row of the slab.
 template <typename T>
-__device__ __forceinline__ void add_residual(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane,
-                                             float* acc) {
-    constexpr int V = Values16<T>::N;
-    const int col = n + (lane & 7) * V;
-    __syncwarp();
+__device__ __forceinline__ void add_row(uint32_t slab, int lane, float* acc) {
 #pragma unroll
-    for (int h = 0; h < 8; h += 4) {
-        uint4 r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long long m = m0 + (h + i) * 4 + (lane >> 3);
-            r[i] = load16<T>(static_cast<const T*>(p.residual) + m * p.ldr + col, m < p.M ? p.N - col : 0, p.vec);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sts128(slab_at(slab, (h + i) * 4 + (lane >> 3), lane & 7), r[i]);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int s = 0; s < 8; ++s) add16(lds128(slab_at(slab, lane, s)), acc + s * V, T());
+    for (int s = 0; s < 8; ++s) add16(lds128(slab_at(slab, lane, s)), acc + s * Values16<T>::N, T());
 }
 // The slab's 32 rows of 128 bytes -> out, from column n on.
 template <typename T>
-__device__ __forceinline__ void store_slab(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane) {
+__device__ __forceinline__ void store_slab(const LinearFp8Params& p, const CUtensorMap* tmO, long long m0, int n, uint32_t slab, int lane) {
     constexpr int V = Values16<T>::N;
     const int col = n + (lane & 7) * V;
+    if (p.vec) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && m0 < p.M && n < p.N) tma_store_2d_a(tmO, slab, n, (int)m0);
+        if (lane == 0) tma_store_commit();
+        return;
+    }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = i * 4 + (lane >> 3);
         const uint4 v = lds128(slab_at(slab, r, lane & 7));
-        if (m0 + r < p.M) store16<T>(static_cast<T*>(p.out) + (m0 + r) * p.ldo + col, p.N - col, p.vec, v);
+        const T* e = reinterpret_cast<const T*>(&v);
+        T* to = static_cast<T*>(p.out) + (m0 + r) * p.ldo + col;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (m0 + r < p.M && col + j < p.N) to[j] = e[j];
     }
+    __syncwarp();
 }
 
 template <int OUT, bool GELU>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
-linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const LinearFp8Params p) {
+linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmO, const LinearFp8Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t* slabs = smem + PAIR_STAGES * PAIR_STAGE;
-    float* scales = reinterpret_cast<float*>(slabs + PAIR_WARPS * SLAB);       // [slot][block of the group][half of the columns][row]
+    uint8_t* slabs = smem + PAIR_STAGES * PAIR_STAGE;         // two a warp
+    float* scales = reinterpret_cast<float*>(slabs + 2 * PAIR_WARPS * SLAB);       // [slot][block of the group][half of the columns][row]
     __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2], sfull[SCALE_SLOTS], sempty[SCALE_SLOTS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -559,6 +581,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         fence_barrier_init();
         prefetch_tensormap(&tmA);
         prefetch_tensormap(&tmW);
+        prefetch_tensormap(&tmO);
     }
     __syncthreads();
     if (warp == 1) { tmem_alloc_pair(&tmem_slot, 512); tmem_relinquish_pair(); }
@@ -613,8 +636,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 bool ok = true;
                 for (int t = first; t < tiles && ok; t += step) {
                     for (int kb = 0; kb < p.blocks; ++kb) {
-                        if (!mbar_wait_warp(tempty0 + 8 * buf, tph ^ 1u, abort_flag)) { if (lane == 0) give_up(126); ok = false; break; }
                         if (!mbar_wait_warp(full0 + 8 * s, ph, abort_flag)) { if (lane == 0) give_up(127); ok = false; break; }
+                        if (!mbar_wait_warp(tempty0 + 8 * buf, tph ^ 1u, abort_flag)) { if (lane == 0) give_up(126); ok = false; break; }
                         tc_fence_after_sync();
                         if (elect_one()) {
                             const uint64_t ad = hi | (uint64_t)(((s0 + s * PAIR_STAGE) & 0x3FFFFu) >> 4);
@@ -672,30 +695,72 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-        const uint32_t slab = smem_u32(slabs) + (warp - 4) * SLAB;
+        const uint32_t slab0 = smem_u32(slabs) + (warp - 4) * (2 * SLAB);
+        const uint32_t bias0 = smem_u32(scales) + SCALE_SLOTS * SCALE_BYTES + (warp - 4) * 512;
         const uint32_t lead_tempty0 = map_to_cta(tempty0, 0);
         const uint32_t taddr = tmem_base + half * KB + ((uint32_t)(quarter * 32) << 16);
         const uint32_t sc0 = smem_u32(scales) + (half * BP + row) * 4, sfull0 = smem_u32(sfull);
         uint32_t slot = 0, sph = 0, buf = 0, tph = 0;
         bool ok = true;
         uint32_t even[16], odd[16];
+        // The scale of block kb; a group of them is waited for with its first one, which comes when the last group has been read.
+        auto scale_of = [&](int kb) {
+            const int i = kb % SCALE_GROUP;
+            if (i == 0) {
+                if (kb > 0) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[slot]);
+                    if (++slot == SCALE_SLOTS) { slot = 0; sph ^= 1u; }
+                }
+                if (ok && !mbar_wait_warp(sfull0 + 8 * slot, sph, abort_flag)) { if (lane == 0) give_up(130); ok = false; }
+            }
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sc0 + slot * SCALE_BYTES + i * (2 * BP * 4)) : "memory");
+            return v;
+        };
         for (int t = first; t < tiles; t += step) {
+            const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
+            const int n = t % n_n * PAIR_N + half * KB;
+            if (lane == 0) tma_store_wait_read<0>();         // the last tile's results have left the slabs
+            __syncwarp();
+            if (p.residual) {
+                if (p.io == CONVNN_F32) {
+                    request_residual<float>(p, m0, n, slab0, lane);
+                    request_residual<float>(p, m0, n + 32, slab0 + SLAB, lane);
+                } else {
+                    request_residual<__nv_bfloat16>(p, m0, n, slab0, lane);
+                    request_residual<__nv_bfloat16>(p, m0, n + 64, slab0 + SLAB, lane);
+                }
+            }
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = n + 4 * lane + j;
+                    if (c < p.N)
+                        bias[j] = p.io == CONVNN_F32 ? static_cast<const float*>(p.bias)[c]
+                                                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[c]);
+                }
+            }
             float acc[128];                                  // (pairs, as elsewhere, do not stay in registers here)
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) odd[j] = 0u;
             float last = 0.f;
+            float scale = scale_of(0);
+            bool ready = false;
 #pragma unroll 1
             for (int kb = 0; kb < p.blocks; ++kb) {
-                const int in_group = kb % SCALE_GROUP;
-                if (in_group == 0 && ok && !mbar_wait_warp(sfull0 + 8 * slot, sph, abort_flag)) { if (lane == 0) give_up(130); ok = false; }
-                float scale;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(sc0 + slot * SCALE_BYTES + in_group * (2 * BP * 4)) : "memory");
-                if (ok && !mbar_wait_warp(tfull0 + 8 * buf, tph, abort_flag)) { if (lane == 0) give_up(128); ok = false; }
+                if (!__all_sync(0xffffffffu, ready) && ok && !mbar_wait_warp(tfull0 + 8 * buf, tph, abort_flag)) {
+                    if (lane == 0) give_up(128);
+                    ok = false;
+                }
                 tc_fence_after_sync();
-                // sixteen columns are added up while the next are on their way, the last under the next block's first
+                // sixteen columns are added up while the next are on their way, the last under the next block's first; the next block's
+                // scale and barrier are asked for in between
                 const uint32_t from = taddr + buf * PAIR_N;
+                float next = 0.f;
                 tmem_ld_x16(from, even);
                 add_scaled(acc + 112, odd, last);
 #pragma unroll
@@ -703,76 +768,99 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                     tmem_ld_wait();
                     tmem_ld_x16(from + 16 * (c + 1), odd);
                     add_scaled(acc + 16 * c, even, scale);
+                    if (c == 0 && kb + 1 < p.blocks) next = scale_of(kb + 1);
+                    if (c == 4) {
+                        buf ^= 1u;
+                        if (buf == 0) tph ^= 1u;
+                        ready = mbar_test_a(tfull0 + 8 * buf, tph);
+                    }
                     tmem_ld_wait();
                     if (c == 6) break;
                     tmem_ld_x16(from + 16 * (c + 2), even);
                     add_scaled(acc + 16 * (c + 1), odd, scale);
                 }
                 last = scale;
+                scale = next;
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8 * buf);
-                buf ^= 1u;
-                if (buf == 0) tph ^= 1u;
-                if (in_group == SCALE_GROUP - 1 || kb == p.blocks - 1) {
-                    if (lane == 0) mbar_arrive(&sempty[slot]);
-                    if (++slot == SCALE_SLOTS) { slot = 0; sph ^= 1u; }
-                }
+                if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8 * (buf ^ 1u));
             }
+            if (lane == 0) mbar_arrive(&sempty[slot]);
+            if (++slot == SCALE_SLOTS) { slot = 0; sph ^= 1u; }
             add_scaled(acc + 112, odd, last);
-            const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
-            const int n = t % n_n * PAIR_N + half * KB;
             if (p.bias) {
-                if (p.io == CONVNN_F32) add_bias<float>(p, n, acc);
-                else add_bias<__nv_bfloat16>(p, n, acc);
+                sts128(bias0 + 16 * lane, make_uint4(__float_as_uint(bias[0]), __float_as_uint(bias[1]), __float_as_uint(bias[2]),
+                                                     __float_as_uint(bias[3])));
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 128; j += 4) add16(lds128(bias0 + 4 * j), acc + j, 0.f);
+                __syncwarp();
             }
             if (GELU && OUT == OUT_F32) {
 #pragma unroll
                 for (int j = 0; j < 128; ++j) acc[j] = gelu_erf(acc[j]);
             } else if (GELU) {
 #pragma unroll
-                for (int j = 0; j < 128; j += 2) unpack2(gelu_poly(pack2(acc[j], acc[j + 1])), acc[j], acc[j + 1]);
+                for (int j = 0; j < 128; j += 8) gelu_poly8(acc + j);
             }
             if (p.residual) {
+                residual_arrived();
                 if (p.io == CONVNN_F32) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) add_residual<float>(p, m0, n + 32 * q, slab, lane, acc + 32 * q);
+                    add_row<float>(slab0, lane, acc);
+                    add_row<float>(slab0 + SLAB, lane, acc + 32);
+                    __syncwarp();
+                    request_residual<float>(p, m0, n + 64, slab0, lane);
+                    request_residual<float>(p, m0, n + 96, slab0 + SLAB, lane);
+                    residual_arrived();
+                    add_row<float>(slab0, lane, acc + 64);
+                    add_row<float>(slab0 + SLAB, lane, acc + 96);
                 } else {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) add_residual<__nv_bfloat16>(p, m0, n + 64 * q, slab, lane, acc + 64 * q);
+                    add_row<__nv_bfloat16>(slab0, lane, acc);
+                    add_row<__nv_bfloat16>(slab0 + SLAB, lane, acc + 64);
                 }
             }
+            // (a lane writes the row of the slab that it has read)
             if (OUT == OUT_BF16) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    __syncwarp();                            // the slab has been read
+                    const uint32_t slab = slab0 + q * SLAB;
 #pragma unroll
                     for (int s = 0; s < 8; ++s) {
                         const float* v = acc + 64 * q + 8 * s;
                         const f32x2 four[4] = {pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
                         sts128(slab_at(slab, lane, s), f32x2_to_bf16x8(four));
                     }
-                    store_slab<__nv_bfloat16>(p, m0, n + 64 * q, slab, lane);
+                    store_slab<__nv_bfloat16>(p, &tmO, m0, n + 64 * q, slab, lane);
                 }
             } else if (OUT == OUT_F32) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    __syncwarp();
+                    const uint32_t slab = slab0 + (q & 1) * SLAB;
+                    if (q >= 2) {
+                        if (lane == 0) tma_store_wait_read<1>();
+                        __syncwarp();
+                    }
 #pragma unroll
                     for (int s = 0; s < 8; ++s) {
                         const float* f = acc + 32 * q + 4 * s;
                         sts128(slab_at(slab, lane, s), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
                                                                   __float_as_uint(f[3])));
                     }
-                    store_slab<float>(p, m0, n + 32 * q, slab, lane);
+                    store_slab<float>(p, &tmO, m0, n + 32 * q, slab, lane);
                 }
             } else {
-                uint32_t top = 0;
+                float most[4] = {0.f, 0.f, 0.f, 0.f};
+                if (n + KB <= p.N) {
 #pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    if (n + j < p.N) top = max(top, abs_bits(acc[j]));
-                const float scale = fp8_scale(top), inv = __frcp_rn(scale);
-                __syncwarp();
+                    for (int j = 0; j < 128; ++j) most[j & 3] = max_nan(most[j & 3], fabsf(acc[j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (n + j < p.N) most[j & 3] = max_nan(most[j & 3], fabsf(acc[j]));
+                }
+                const uint32_t top = abs_bits(max_nan(max_nan(most[0], most[1]), max_nan(most[2], most[3])));
+                const float to = fp8_scale(top), inv = __frcp_rn(to);
+                const uint32_t slab = slab0;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
                     uint32_t w[4];
@@ -783,10 +871,11 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                     }
                     sts128(slab_at(slab, lane, s), make_uint4(w[0], w[1], w[2], w[3]));
                 }
-                if (m0 + lane < p.M && n < p.N) p.so[(m0 + lane) * p.so_row + n / KB * p.so_block] = scale;
-                store_slab<uint8_t>(p, m0, n, slab, lane);
+                if (m0 + lane < p.M && n < p.N) p.so[(m0 + lane) * p.so_row + n / KB * p.so_block] = to;
+                store_slab<uint8_t>(p, &tmO, m0, n, slab, lane);
             }
         }
+        if (lane == 0) tma_store_wait<0>();
     }
     __syncwarp();
     tc_fence_before_sync();
@@ -797,7 +886,17 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 
 template <int OUT, bool GELU>
 int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8Params& p, cudaStream_t st) {
-    constexpr size_t smem = PAIR_STAGES * PAIR_STAGE + PAIR_WARPS * SLAB + SCALE_SLOTS * SCALE_BYTES + 1024;
+    CUtensorMap tmO = tmA;                                   // (unused where rows of the output start anywhere)
+    if (p.vec) {
+        const int elt = OUT == OUT_F32 ? 4 : OUT == OUT_BF16 ? 2 : 1;
+        const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.M}, strides[1] = {(uint64_t)p.ldo * elt};
+        const uint32_t box[2] = {(uint32_t)(128 / elt), 32};
+        const bool ok = OUT == OUT_F32    ? encode_tensor_map_f32(&tmO, p.out, 2, dims, strides, box, 128)
+                        : OUT == OUT_BF16 ? encode_tensor_map_bf16(&tmO, p.out, 2, dims, strides, box, 128)
+                                          : encode_tensor_map_u8(&tmO, p.out, 2, dims, strides, box, 128);
+        if (!ok) return CONVNN_E_CUDA;
+    }
+    constexpr size_t smem = PAIR_STAGES * PAIR_STAGE + 2 * PAIR_WARPS * SLAB + SCALE_SLOTS * SCALE_BYTES + PAIR_WARPS * 512 + 1024;
     const long long tiles = (long long)((p.M + 2 * BP - 1) / (2 * BP)) * ((p.N + PAIR_N - 1) / PAIR_N);
     if (tiles > 0x3fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %d x %d is too many tiles", p.M, p.N);
     auto kern = linear_fp8_pair_kernel<OUT, GELU>;
@@ -813,7 +912,7 @@ int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8
     if (const int rc = fit.query(reinterpret_cast<const void*>(kern), &cfg, &pairs)) return rc;
     cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs));
     attr[1] = chained_attribute(st); cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tmA, tmW, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tmA, tmW, tmO, p);
     if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "linear_fp8 pair launch: %s", cudaGetErrorString(e));
     CONVNN_CHECK_LAUNCH("linear_fp8_pair");
     return CONVNN_OK;

@@ -387,7 +387,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // encode call rejects the arguments.  dims / strides are innermost first; strides[0]
 // (the element stride) is implicit, strides_bytes has rank-1 entries.
 bool encode_tensor_map_f32(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                           const uint64_t* strides_bytes, const uint32_t* box);
+                           const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes = 0);
 bool encode_tensor_map_u8(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
                           const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes);
 bool encode_tensor_map_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,

@@ -70,10 +70,10 @@ bool encode_tensor_map_u8(CUtensorMap* out, const void* base, int rank, const ui
     return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box, swizzle_bytes);
 }
 
-// float32 elements, no swizzle (the row moments of the pre-norm fold)
+// float32 elements (without a swizzle: the row moments of the pre-norm fold)
 bool encode_tensor_map_f32(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                           const uint64_t* strides_bytes, const uint32_t* box) {
-    return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box, 0);
+                           const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes) {
+    return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box, swizzle_bytes);
 }
 
 }  // namespace convnn
