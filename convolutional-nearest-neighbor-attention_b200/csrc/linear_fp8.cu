@@ -422,7 +422,7 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 // the rows of w each, so that a CTA copies 32 KB for 512 cycles of products (a lone CTA's 128 x 256 tile: 48 KB).
 //   warp 0      TMA producer of its CTA's operands, credited to the even CTA's barriers
 //   warp 1      MMA issuer (even CTA), a block of k into one of two buffers of 256 columns
-//   warps 2, 3  scales: each the products of the rows' scales and that of one half of the columns, four blocks of k at a time
+//   warps 2, 3  the scales of four blocks of k at a time
 //   warps 4-11  epilogue: a warp has 32 rows and 128 columns, its sums in registers (128 of 224), and after the last block bias, GELU,
 //               residual, rounding; the results leave through its two slabs of shared memory, 32 rows of 128 bytes in the order
 //               of the 128-byte swizzle, by TMA where rows start on 16-byte boundaries.  Meanwhile the next tile's first two
@@ -434,8 +434,8 @@ constexpr int PAIR_WARPS = 8, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 constexpr int PAIR_N = 256;
 constexpr uint32_t PAIR_STAGE = 2 * BP * KB, SLAB = 4096;
 constexpr int PAIR_STAGES = 4;
-constexpr int SCALE_GROUP = 4, SCALE_SLOTS = 2;              // blocks of k whose scales come together, and how many times that is held
-constexpr uint32_t SCALE_BYTES = SCALE_GROUP * 2 * BP * 4;
+constexpr int SCALE_GROUP = 4, SCALE_SLOTS = 4;              // blocks of k whose scales come together, and how many times that is held
+constexpr uint32_t SCALE_BYTES = SCALE_GROUP * (BP + 2) * 4 + 96;        // the rows', the two column blocks'; a multiple of 128
 
 __device__ __forceinline__ void mma_e4m3_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                                  uint32_t accumulate) {
@@ -454,6 +454,10 @@ __device__ __forceinline__ void tma_store_2d_a(const CUtensorMap* m, uint32_t sr
 __device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&part)[16], float scale) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[j] = fmaf(__uint_as_float(part[j]), scale, acc[j]);
+}
+// Four bytes to shared memory; zero, and nothing read, where not `in`.
+__device__ __forceinline__ void copy4(uint32_t to, const float* base, const float* from, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(in ? from : base), "r"(in ? 4 : 0) : "memory");
 }
 // Whether a phase is over, without waiting for it.
 __device__ __forceinline__ bool mbar_test_a(uint32_t bar, uint32_t parity) {
@@ -565,7 +569,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* slabs = smem + PAIR_STAGES * PAIR_STAGE;         // two a warp
-    float* scales = reinterpret_cast<float*>(slabs + 2 * PAIR_WARPS * SLAB);       // [slot][block of the group][half of the columns][row]
+    float* scales = reinterpret_cast<float*>(slabs + 2 * PAIR_WARPS * SLAB);       // [slot]: [block of the group][row], [block][half of the columns]
     __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2], sfull[SCALE_SLOTS], sempty[SCALE_SLOTS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -576,7 +580,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     if (threadIdx.x == 0) {
         for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 2 * PAIR_WARPS); }
-        for (int b = 0; b < SCALE_SLOTS; ++b) { mbar_init(&sfull[b], 2); mbar_init(&sempty[b], PAIR_WARPS); }
+        for (int b = 0; b < SCALE_SLOTS; ++b) { mbar_init(&sfull[b], 64); mbar_init(&sempty[b], PAIR_WARPS); }
         abort_word = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmA);
@@ -656,41 +660,34 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 }
             }
         } else {
-            const int half = warp - 2;
+            // copied straight to shared memory, zeros where there is nothing; a warp has two blocks of a group
+            const int i0 = 2 * (warp - 2);
             const long long rows32 = 32 * p.sa_row;
             uint32_t slot = 0, ph = 0;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
-                const int m0 = t / n_n * 2 * BP + (int)rank * BP + lane, n = t % n_n * PAIR_N + half * KB;
-                const float* sa = p.sa + (long long)m0 * p.sa_row;
-                const float* sw = p.sw + (long long)(n / KB) * p.sw_row;
+                const int m0 = t / n_n * 2 * BP + (int)rank * BP + lane, n = t % n_n * PAIR_N + (lane & 1) * KB;
                 for (int kb0 = 0; kb0 < p.blocks; kb0 += SCALE_GROUP) {
-                    // (all requested before the first is used)
-                    float v[SCALE_GROUP][4], w[SCALE_GROUP];
+                    if (!mbar_wait_warp(smem_u32(&sempty[slot]), ph ^ 1u, abort_flag)) { if (lane == 0) give_up(129); ok = false; break; }
+                    const uint32_t to = smem_u32(scales) + slot * SCALE_BYTES;
 #pragma unroll
-                    for (int i = 0; i < SCALE_GROUP; ++i) {
-                        const bool in = kb0 + i < p.blocks && n < p.N;
-                        w[i] = 0.f;
-                        if (in) w[i] = sw[i * p.sw_block];
+                    for (int i = i0; i < i0 + 2; ++i) {
+                        const bool in = kb0 + i < p.blocks;
+                        const float* from = p.sa + (long long)m0 * p.sa_row + (kb0 + i) * p.sa_block;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            v[i][j] = 0.f;
-                            if (in && m0 + 32 * j < p.M) v[i][j] = sa[j * rows32 + i * p.sa_block];
+                            copy4(to + (i * BP + 32 * j + lane) * 4, p.sa, from, in && m0 + 32 * j < p.M);
+                            from += rows32;
                         }
+                        if (lane < 2)
+                            copy4(to + (SCALE_GROUP * BP + 2 * i + lane) * 4, p.sw, p.sw + (long long)(n / KB) * p.sw_row + (kb0 + i) * p.sw_block,
+                                  in && n < p.N);
                     }
-                    sa += SCALE_GROUP * p.sa_block;
-                    sw += SCALE_GROUP * p.sw_block;
-                    if (!mbar_wait_warp(smem_u32(&sempty[slot]), ph ^ 1u, abort_flag)) { if (lane == 0) give_up(129); ok = false; break; }
-                    float* to = scales + slot * (SCALE_BYTES / 4) + half * BP + lane;
-#pragma unroll
-                    for (int i = 0; i < SCALE_GROUP; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) to[i * 2 * BP + 32 * j] = v[i][j] * w[i];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sfull[slot]);
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sfull[slot])) : "memory");
                     if (++slot == SCALE_SLOTS) { slot = 0; ph ^= 1u; }
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -699,7 +696,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         const uint32_t bias0 = smem_u32(scales) + SCALE_SLOTS * SCALE_BYTES + (warp - 4) * 512;
         const uint32_t lead_tempty0 = map_to_cta(tempty0, 0);
         const uint32_t taddr = tmem_base + half * KB + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t sc0 = smem_u32(scales) + (half * BP + row) * 4, sfull0 = smem_u32(sfull);
+        const uint32_t sc0 = smem_u32(scales), sfull0 = smem_u32(sfull);
         uint32_t slot = 0, sph = 0, buf = 0, tph = 0;
         bool ok = true;
         uint32_t even[16], odd[16];
@@ -714,9 +711,10 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 }
                 if (ok && !mbar_wait_warp(sfull0 + 8 * slot, sph, abort_flag)) { if (lane == 0) give_up(130); ok = false; }
             }
-            float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sc0 + slot * SCALE_BYTES + i * (2 * BP * 4)) : "memory");
-            return v;
+            float a, w;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(sc0 + slot * SCALE_BYTES + (i * BP + row) * 4) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(sc0 + slot * SCALE_BYTES + (SCALE_GROUP * BP + 2 * i + half) * 4) : "memory");
+            return a * w;
         };
         for (int t = first; t < tiles; t += step) {
             const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
@@ -732,14 +730,29 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                     request_residual<__nv_bfloat16>(p, m0, n + 64, slab0 + SLAB, lane);
                 }
             }
-            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            // four columns' bias a lane, as they are stored
+            uint4 bias = make_uint4(0, 0, 0, 0);
             if (p.bias) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = n + 4 * lane + j;
-                    if (c < p.N)
-                        bias[j] = p.io == CONVNN_F32 ? static_cast<const float*>(p.bias)[c]
-                                                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[c]);
+                const int c = n + 4 * lane;
+                if (p.vec && c + 4 <= p.N) {
+                    if (p.io == CONVNN_F32) {
+                        bias = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.bias) + c);
+                    } else {
+                        const uint2 two = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.bias) + c);
+                        bias.x = two.x; bias.y = two.y;
+                    }
+                } else if (p.io == CONVNN_F32) {
+                    const uint32_t* from = static_cast<const uint32_t*>(p.bias) + c;
+                    if (c < p.N) bias.x = from[0];
+                    if (c + 1 < p.N) bias.y = from[1];
+                    if (c + 2 < p.N) bias.z = from[2];
+                    if (c + 3 < p.N) bias.w = from[3];
+                } else {
+                    const uint16_t* from = static_cast<const uint16_t*>(p.bias) + c;
+                    if (c < p.N) bias.x = from[0];
+                    if (c + 1 < p.N) bias.x |= (uint32_t)from[1] << 16;
+                    if (c + 2 < p.N) bias.y = from[2];
+                    if (c + 3 < p.N) bias.y |= (uint32_t)from[3] << 16;
                 }
             }
             float acc[128];                                  // (pairs, as elsewhere, do not stay in registers here)
@@ -789,8 +802,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
             if (++slot == SCALE_SLOTS) { slot = 0; sph ^= 1u; }
             add_scaled(acc + 112, odd, last);
             if (p.bias) {
-                sts128(bias0 + 16 * lane, make_uint4(__float_as_uint(bias[0]), __float_as_uint(bias[1]), __float_as_uint(bias[2]),
-                                                     __float_as_uint(bias[3])));
+                if (p.io != CONVNN_F32) bias = make_uint4(bias.x << 16, bias.x & 0xffff0000u, bias.y << 16, bias.y & 0xffff0000u);
+                sts128(bias0 + 16 * lane, bias);
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 128; j += 4) add16(lds128(bias0 + 4 * j), acc + j, 0.f);
