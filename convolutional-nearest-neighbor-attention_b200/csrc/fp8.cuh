@@ -13,6 +13,11 @@ constexpr int kFp8Block = 128;
 constexpr float kFp8Least = 1.17549435e-38f;               // 2^-126
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // The largest magnitude of a block as bits (so that NaN, above infinity, is kept) -> its scale.
 __device__ __forceinline__ float fp8_scale(uint32_t amax) {
     const float s = __uint_as_float(amax) * (1.0f / 448.0f);

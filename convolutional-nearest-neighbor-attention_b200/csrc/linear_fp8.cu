@@ -75,11 +75,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 
 // x * Phi(x), for results that stay in float32.
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 // The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 12 in a / 2.5 - 1
 // that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 6.4e-7; off by 8.5e-7 *
 // |x| at most as it is evaluated here).  Sixteen instructions instead of erff's ~30; single ones, whose constants are immediates, not

@@ -113,14 +113,25 @@ __device__ __forceinline__ void narrow(const f32x2 (&v)[4], Raw8<float>& r) {
     }
 }
 __device__ __forceinline__ uint32_t amax8(const f32x2 (&v)[4]) {
-    uint32_t m = 0;
+    float m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float a, b;
         unpack2(v[i], a, b);
-        m = max(m, max(abs_bits(a), abs_bits(b)));
+        m[i] = max_nan(fabsf(a), fabsf(b));
     }
-    return m;
+    return abs_bits(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])));
+}
+__device__ __forceinline__ uint32_t amax8(const Raw8<float>& r) {
+    f32x2 v[4];
+    widen(r, v);
+    return amax8(v);
+}
+// (the magnitudes of bfloat16 values order like their bits)
+__device__ __forceinline__ uint32_t amax8(const Raw8<__nv_bfloat16>& r) {
+    constexpr uint32_t MAG = 0x7fff7fffu;
+    const uint32_t m = __vmaxu2(__vmaxu2(r.v[0].x & MAG, r.v[0].y & MAG), __vmaxu2(r.v[0].z & MAG, r.v[0].w & MAG));
+    return max(m << 16, m & 0xffff0000u);
 }
 // Over the sixteen lanes of a block.
 __device__ __forceinline__ uint32_t block_max(uint32_t m) {
@@ -300,44 +311,36 @@ struct QuantParams {
     int D;
 };
 
-// A scale per row and block: a half-warp takes every other block of sixteen of the flattened (row, block) list.
-constexpr int kTasks = 8;
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantParams p) {
+// A scale per row and block: a half-warp takes G neighbouring blocks of R rows.
+template <typename T, bool VEC, int G, int R>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantParams p, int groups) {
     __shared__ __align__(16) T rooms[VEC ? 1 : kWarps][VEC ? 1 : 256];
     chain_begin();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = (lane & 15) * 8;
     T* room = rooms[VEC ? 0 : warp];
-    const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    const long long t0 = ((long long)blockIdx.x * kWarps + warp) * (2 * kTasks) + (lane >> 4);
-    const long long first = t0 / blocks;
-    const int b0 = (int)(t0 - first * blocks), at = (lane & 15) * 8;
-    auto on = [&](long long& row, int& b) {                  // two blocks on
-        b += 2;
-        if (b >= blocks) { b -= blocks; ++row; }
-        if (b >= blocks) { b -= blocks; ++row; }
-    };
-    Held<T, VEC> raw[kTasks];
-    long long row = first;
-    int b = b0;
+    const long long task = ((long long)blockIdx.x * kWarps + warp) * 2 + (lane >> 4), set = task / groups, row0 = set * R;
+    const int b0 = (int)(task - set * groups) * G, c0 = b0 * kFp8Block;
+    const T* x = static_cast<const T*>(p.x) + row0 * p.ldx;
+    Held<T, VEC> held[R][G];
 #pragma unroll
-    for (int t = 0; t < kTasks; ++t) {
-        raw[t] = fetch<T, VEC, 16>(static_cast<const T*>(p.x) + row * p.ldx, b * kFp8Block, lane, row < p.rows ? p.D : 0);
-        on(row, b);
-    }
-    row = first;
-    b = b0;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int t = 0; t < kTasks; ++t) {
-        const int c = b * kFp8Block + at;
-        f32x2 v[4];
-        widen(own8<T, VEC, 16>(raw[t], room, lane), v);
-        const float scale = fp8_scale(block_max(amax8(v)));
-        const int valid = row < p.rows ? p.D - c : 0;
-        store_e4m3<VEC>(p.q + row * p.ldq + c, valid, v, scale);
-        if (valid > 0 && at == 0) p.scales[row * p.scale_row + b * p.scale_block] = scale;
-        on(row, b);
-    }
+        for (int g = 0; g < G; ++g)
+            held[r][g] = fetch<T, VEC, 16>(x + r * p.ldx, c0 + g * kFp8Block, lane, row0 + r < p.rows ? p.D : 0);
+    uint8_t* q = p.q + row0 * p.ldq + c0 + at;
+    float* scales = p.scales + row0 * p.scale_row + b0 * p.scale_block;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const Raw8<T> raw = own8<T, VEC, 16>(held[r][g], room, lane);
+            const float scale = fp8_scale(block_max(amax8(raw)));
+            const int valid = row0 + r < p.rows ? p.D - c0 - g * kFp8Block - at : 0;
+            f32x2 v[4];
+            widen(raw, v);
+            store_e4m3<VEC>(q + r * p.ldq + g * kFp8Block, valid, v, scale);
+            if (valid > 0 && at == 0) scales[r * p.scale_row + g * p.scale_block] = scale;
+        }
 }
 
 // A scale per 128 x 128 block: a CTA holds the block in registers, eight rows a half-warp.
@@ -363,10 +366,8 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantPa
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        f32x2 v[4];
         raw[i] = own8<T, VEC, 16>(held[i], room, lane);
-        widen(raw[i], v);
-        m = max(m, amax8(v));
+        m = max(m, amax8(raw[i]));
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) top[warp] = m;
@@ -419,20 +420,32 @@ int norm_of(const NormParams& p, cudaStream_t st) {
     return CONVNN_OK;
 }
 
+template <typename T, int G, int R>
+int launch_quantize_rows(const QuantParams& p, bool vec, cudaStream_t st) {
+    const int groups = ((p.D + kFp8Block - 1) / kFp8Block + G - 1) / G;
+    const long long tasks = (p.rows + R - 1) / R * groups, grid = (tasks + 2 * kWarps - 1) / (2 * kWarps);
+    if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "quantize_fp8: %lld rows of %d", p.rows, p.D);
+    if (vec) launch_chained(quantize_rows_kernel<T, true, G, R>, (unsigned)grid, kThreads, 0, st, p, groups);
+    else launch_chained(quantize_rows_kernel<T, false, G, R>, (unsigned)grid, kThreads, 0, st, p, groups);
+    CONVNN_CHECK_LAUNCH("quantize_fp8");
+    return CONVNN_OK;
+}
+
 template <typename T>
 int quantize_of(const QuantParams& p, int block_rows, cudaStream_t st) {
     const bool vec = p.D % 8 == 0 && rows16<T>(p.x, p.ldx) && on_boundary(p.q, p.ldq, 8);
-    const long long blocks = (p.D + kFp8Block - 1) / kFp8Block;
-    const long long grid = block_rows == 1 ? (p.rows * blocks + 2 * kWarps * kTasks - 1) / (2 * kWarps * kTasks)
-                                           : (p.rows + kFp8Block - 1) / kFp8Block * blocks;
-    if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "quantize_fp8: %lld rows of %d", p.rows, p.D);
+    const int blocks = (p.D + kFp8Block - 1) / kFp8Block;
     if (block_rows == 1) {
-        if (vec) launch_chained(quantize_rows_kernel<T, true>, (unsigned)grid, kThreads, 0, st, p);
-        else launch_chained(quantize_rows_kernel<T, false>, (unsigned)grid, kThreads, 0, st, p);
-    } else {
-        if (vec) launch_chained(quantize_blocks_kernel<T, true>, (unsigned)grid, kThreads, 0, st, p);
-        else launch_chained(quantize_blocks_kernel<T, false>, (unsigned)grid, kThreads, 0, st, p);
+        // three or four blocks a half-warp, whichever leaves fewer out of the last one; rows of one or two blocks, several rows
+        if (blocks == 1) return launch_quantize_rows<T, 1, 4>(p, vec, st);
+        if (blocks == 2) return launch_quantize_rows<T, 2, 2>(p, vec, st);
+        if ((blocks + 2) / 3 * 3 < (blocks + 3) / 4 * 4) return launch_quantize_rows<T, 3, 1>(p, vec, st);
+        return launch_quantize_rows<T, 4, 1>(p, vec, st);
     }
+    const long long grid = (p.rows + kFp8Block - 1) / kFp8Block * blocks;
+    if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "quantize_fp8: %lld rows of %d", p.rows, p.D);
+    if (vec) launch_chained(quantize_blocks_kernel<T, true>, (unsigned)grid, kThreads, 0, st, p);
+    else launch_chained(quantize_blocks_kernel<T, false>, (unsigned)grid, kThreads, 0, st, p);
     CONVNN_CHECK_LAUNCH("quantize_fp8");
     return CONVNN_OK;
 }

@@ -532,11 +532,12 @@ def _device_of(like: torch.Tensor, *tensors) -> int:
     index = like.get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:
-            _require_cuda(like, *tensors)
-            raise RuntimeError(f"all tensors must be on one device, got {like.device} and {t.device}")
-    if index < 0:
-        _require_cuda(like)
-    return index
+            break
+    else:
+        if index >= 0:
+            return index
+    _require_cuda(like, *tensors)
+    raise RuntimeError(f"all tensors must be on one device, got {[str(t.device) for t in (like, *tensors) if t is not None]}")
 
 
 def _launch(index: int, fn, *args) -> None:
@@ -566,17 +567,20 @@ def _rows_of(t: torch.Tensor, shape) -> Tuple[torch.Tensor, int, int]:
     return t.contiguous(), rows, D
 
 
+_E4M3, _F32 = torch.float8_e4m3fn, torch.float32
+
+
 def _fp8_empty(shape, rows: int, device) -> Tuple[torch.Tensor, int, torch.Tensor]:
     """Room for 8-bit rows with a scale per row and block: values (rows on 16-byte boundaries, as ``linear_fp8`` reads them),
     their stride, scales (those of one block of channels side by side)."""
     D = shape[-1]
-    ld, blocks = -(-D // 16) * 16, -(-D // FP8_BLOCK)
+    ld, blocks = (D + 15) & -16, (D + 127) >> 7
     if len(shape) == 2:
-        lead = (1,)
-    else:
-        lead = tuple(math.prod(shape[i + 1:-1]) for i in range(len(shape) - 1))
-    values = torch.empty_strided(shape, (*[n * ld for n in lead], 1), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty_strided((*shape[:-1], blocks), (*lead, max(rows, 1)), dtype=torch.float32, device=device)
+        return (torch.empty_strided(shape, (ld, 1), dtype=_E4M3, device=device), ld,
+                torch.empty_strided((rows, blocks), (1, rows or 1), dtype=_F32, device=device))
+    lead = tuple(math.prod(shape[i + 1:-1]) for i in range(len(shape) - 1))
+    values = torch.empty_strided(shape, (*[n * ld for n in lead], 1), dtype=_E4M3, device=device)
+    scales = torch.empty_strided((*shape[:-1], blocks), (*lead, rows or 1), dtype=_F32, device=device)
     return values, ld, scales
 
 
@@ -680,9 +684,9 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
         _forward_only(bias, residual, sa, sw)
     index = _device_of(av, sa, wv, sw, bias, residual)
     io = _dtype_code(dtype)
-    if av.dtype != torch.float8_e4m3fn or wv.dtype != torch.float8_e4m3fn:
+    if av.dtype is not _E4M3 or wv.dtype is not _E4M3:
         raise TypeError(f"the values of a and w must be float8_e4m3fn, got {av.dtype} and {wv.dtype}")
-    if sa.dtype != torch.float32 or sw.dtype != torch.float32:
+    if sa.dtype is not _F32 or sw.dtype is not _F32:
         raise TypeError(f"the scales of a and w must be float32, got {sa.dtype} and {sw.dtype}")
     shape, wshape = av.shape, wv.shape
     K = _channels(shape, "linear_fp8")
