@@ -40,7 +40,8 @@ struct LinearFp8Params {
     int M, N, blocks;                     // blocks of k
     int out_kind, io, gelu;               // io: convnn_dtype of bias, residual (and out)
     int stages, splits;                   // CTAs of the cluster
-    bool vec;                             // bias and the rows of out and residual start on 16-byte boundaries
+    bool bias16, residual16, out16;       // their rows start on 16-byte boundaries
+    bool residual4, out4;                 // on 4-byte boundaries (and N is even: two bfloat16 values at a time)
 };
 
 __device__ __forceinline__ void fail(volatile int* abort_flag, int code) {
@@ -136,8 +137,8 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
     const int valid = row_valid ? p.N - n : 0;               // may be <= 0
     if (p.bias && valid > 0) {
         float b[8];
-        if (p.io == CONVNN_F32) load8<float>(p.bias, n, valid, p.vec, b);
-        else load8<__nv_bfloat16>(p.bias, n, valid, p.vec, b);
+        if (p.io == CONVNN_F32) load8<float>(p.bias, n, valid, p.bias16, b);
+        else load8<__nv_bfloat16>(p.bias, n, valid, p.bias16, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += b[j];
     }
@@ -149,8 +150,8 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
     }
     if (p.residual && valid > 0) {
         float r[8];
-        if (p.io == CONVNN_F32) load8<float>(p.residual, m * p.ldr + n, valid, p.vec, r);
-        else load8<__nv_bfloat16>(p.residual, m * p.ldr + n, valid, p.vec, r);
+        if (p.io == CONVNN_F32) load8<float>(p.residual, m * p.ldr + n, valid, p.residual16, r);
+        else load8<__nv_bfloat16>(p.residual, m * p.ldr + n, valid, p.residual16, r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += r[j];
     }
@@ -167,7 +168,7 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
             w.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
             w.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
             uint8_t* q = static_cast<uint8_t*>(p.out) + m * p.ldo + n;
-            if (p.vec && valid >= 8) *reinterpret_cast<uint2*>(q) = w;
+            if (p.out16 && valid >= 8) *reinterpret_cast<uint2*>(q) = w;
             else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -176,8 +177,8 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
             if (n % KB == 0) p.so[m * p.so_row + (n / KB) * p.so_block] = scale;
         }
     } else if (valid > 0) {
-        if (p.out_kind == OUT_F32) store8<float>(p.out, m * p.ldo + n, valid, p.vec, v);
-        else store8<__nv_bfloat16>(p.out, m * p.ldo + n, valid, p.vec, v);
+        if (p.out_kind == OUT_F32) store8<float>(p.out, m * p.ldo + n, valid, p.out16, v);
+        else store8<__nv_bfloat16>(p.out, m * p.ldo + n, valid, p.out16, v);
     }
 }
 
@@ -492,33 +493,79 @@ __device__ __forceinline__ void add16(const uint4& v, float* acc, float) {
     acc[0] += __uint_as_float(v.x); acc[1] += __uint_as_float(v.y);
     acc[2] += __uint_as_float(v.z); acc[3] += __uint_as_float(v.w);
 }
+// Rows that start anywhere: a row's 128 bytes from column n on as lanes side by side, B bytes each.  B is T's size, or 4 for pairs.
+template <typename T, int B> struct Bytes { using type = T; };
+template <> struct Bytes<__nv_bfloat16, 2> { using type = uint16_t; };
+template <> struct Bytes<__nv_bfloat16, 4> { using type = uint32_t; };
+template <typename T, int B>
+__device__ __forceinline__ void rows_to_slab(const T* base, long long ld, int M, int N, long long m0, int n, uint32_t slab, int lane) {
+    using E = typename Bytes<T, B>::type;
+    constexpr int U = 4 / B, AT_ONCE = 8 / U;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+        E v[AT_ONCE][U];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int col = n + (32 * u + lane) * B / (int)sizeof(T);
+                v[i][u] = E{};
+                if (m0 + r0 + i < M && col < N) v[i][u] = *reinterpret_cast<const E*>(base + (m0 + r0 + i) * ld + col);
+            }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int at = (32 * u + lane) * B;
+                const uint32_t to = slab_at(slab, r0 + i, at >> 4) + (at & 15);
+                if constexpr (B == 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(reinterpret_cast<const uint32_t&>(v[i][u])) : "memory");
+                else asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(reinterpret_cast<const uint16_t&>(v[i][u])) : "memory");
+            }
+    }
+}
+template <typename T, int B>
+__device__ __forceinline__ void slab_to_rows(T* base, long long ld, int M, int N, long long m0, int n, uint32_t slab, int lane) {
+    using E = typename Bytes<T, B>::type;
+    constexpr int U = 4 / B;
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = (32 * u + lane) * B, col = n + at / (int)sizeof(T);
+            const uint32_t from = slab_at(slab, r, at >> 4) + (at & 15);
+            E v;
+            if constexpr (B == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(reinterpret_cast<uint32_t&>(v)) : "r"(from) : "memory");
+            else if constexpr (B == 2) asm volatile("ld.shared.b16 %0, [%1];" : "=h"(reinterpret_cast<uint16_t&>(v)) : "r"(from) : "memory");
+            else {
+                uint32_t w;
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+                v = (E)w;
+            }
+            if (m0 + r < M && col < N) *reinterpret_cast<E*>(base + (m0 + r) * ld + col) = v;
+        }
+}
+
 // The residual of 32 rows and 128 bytes of columns from column n on into the slab: asked for here, there after residual_arrived().
 template <typename T>
 __device__ __forceinline__ void request_residual(const LinearFp8Params& p, long long m0, int n, uint32_t slab, int lane) {
-    constexpr int V = Values16<T>::N;
-    const int col = n + (lane & 7) * V, valid = p.N - col;
-    const T* from = static_cast<const T*>(p.residual) + (m0 + (lane >> 3)) * p.ldr + col;
+    const T* base = static_cast<const T*>(p.residual);
+    if (p.residual16) {
+        constexpr int V = Values16<T>::N;
+        const int col = n + (lane & 7) * V, valid = p.N - col;
+        const T* from = base + (m0 + (lane >> 3)) * p.ldr + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3);
-        const bool in = m0 + r < p.M && valid > 0;
-        const uint32_t to = slab_at(slab, r, lane & 7);
-        if (p.vec) {
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const bool in = m0 + r < p.M && valid > 0;
             const uint32_t bytes = in ? min(16u, (uint32_t)valid * (uint32_t)sizeof(T)) : 0u;      // the rest is filled with zeros
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? from : static_cast<const T*>(p.residual)),
-                         "r"(bytes)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slab_at(slab, r, lane & 7)), "l"(in ? from : base), "r"(bytes)
                          : "memory");
-        } else {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            T* e = reinterpret_cast<T*>(&v);
-            if (in) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (j < valid) e[j] = from[j];
-            }
-            sts128(to, v);
+            from += 4 * p.ldr;
         }
-        from += 4 * p.ldr;
+    } else if (sizeof(T) == 4 || !p.residual4) {
+        rows_to_slab<T, sizeof(T)>(base, p.ldr, p.M, p.N, m0, n, slab, lane);
+    } else {
+        rows_to_slab<T, 4>(base, p.ldr, p.M, p.N, m0, n, slab, lane);
     }
 }
 __device__ __forceinline__ void residual_arrived() {
@@ -534,9 +581,7 @@ __device__ __forceinline__ void add_row(uint32_t slab, int lane, float* acc) {
 // The slab's 32 rows of 128 bytes -> out, from column n on.
 template <typename T>
 __device__ __forceinline__ void store_slab(const LinearFp8Params& p, const CUtensorMap* tmO, long long m0, int n, uint32_t slab, int lane) {
-    constexpr int V = Values16<T>::N;
-    const int col = n + (lane & 7) * V;
-    if (p.vec) {
+    if (p.out16) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0 && m0 < p.M && n < p.N) tma_store_2d_a(tmO, slab, n, (int)m0);
@@ -544,16 +589,9 @@ __device__ __forceinline__ void store_slab(const LinearFp8Params& p, const CUten
         return;
     }
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3);
-        const uint4 v = lds128(slab_at(slab, r, lane & 7));
-        const T* e = reinterpret_cast<const T*>(&v);
-        T* to = static_cast<T*>(p.out) + (m0 + r) * p.ldo + col;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (m0 + r < p.M && col + j < p.N) to[j] = e[j];
-    }
+    T* out = static_cast<T*>(p.out);
+    if (sizeof(T) == 2 && p.out4) slab_to_rows<T, sizeof(T) == 2 ? 4 : sizeof(T)>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+    else slab_to_rows<T, sizeof(T)>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
     __syncwarp();
 }
 
@@ -729,7 +767,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
             uint4 bias = make_uint4(0, 0, 0, 0);
             if (p.bias) {
                 const int c = n + 4 * lane;
-                if (p.vec && c + 4 <= p.N) {
+                if (p.bias16 && c + 4 <= p.N) {
                     if (p.io == CONVNN_F32) {
                         bias = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.bias) + c);
                     } else {
@@ -895,7 +933,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 template <int OUT, bool GELU>
 int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8Params& p, cudaStream_t st) {
     CUtensorMap tmO = tmA;                                   // (unused where rows of the output start anywhere)
-    if (p.vec) {
+    if (p.out16) {
         const int elt = OUT == OUT_F32 ? 4 : OUT == OUT_BF16 ? 2 : 1;
         const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.M}, strides[1] = {(uint64_t)p.ldo * elt};
         const uint32_t box[2] = {(uint32_t)(128 / elt), 32};
@@ -947,10 +985,15 @@ int launch_linear_fp8(const void* a, long long lda, const float* sa, long long s
     p.io = io; p.gelu = gelu;
     p.out_kind = so ? OUT_E4M3 : io == CONVNN_F32 ? OUT_F32 : OUT_BF16;
     const long long per16 = io == CONVNN_F32 ? 4 : 8;
-    p.vec = (so ? ldo % 16 == 0 : ldo % per16 == 0) && aligned16(out) &&
-            (!bias || aligned16(bias)) && (!residual || (aligned16(residual) && ldr % per16 == 0));
+    const long long elt = io == CONVNN_F32 ? 4 : 2, out_elt = so ? 1 : elt;
+    auto on = [](const void* q, long long ld_bytes, int n) { return ((uintptr_t)ld_bytes | reinterpret_cast<uintptr_t>(q)) % n == 0; };
+    p.bias16 = on(bias, 0, 16);
+    p.residual16 = on(residual, ldr * elt, 16); p.residual4 = on(residual, ldr * elt, 4) && N % 2 == 0;
+    p.out16 = on(out, ldo * out_elt, 16); p.out4 = on(out, ldo * out_elt, 4) && N % 2 == 0;
     const long long pair_tiles = (long long)((M + 2 * BP - 1) / (2 * BP)) * ((N + PAIR_N - 1) / PAIR_N);
-    if (pair_tiles >= device_sms() / 2) {
+    // Pairs from a tile per five SMs on: 512 x 4096 x 4096 (32 tiles) 31.4 -> 24.2 us, 3152 x 768 x 768 (39) 10.9 -> 9.0; with fewer the
+    // clusters that share a tile's sum are faster (256 x 4096 x 4096, 16 tiles: 16.7 against 23.6).  Up to 128 rows half a tile is empty.
+    if (M > 128 && pair_tiles * 5 >= device_sms()) {
         CUtensorMap tmA, tmW;
         if (!encode_rows(&tmA, a, M, K, lda, BP) || !encode_rows(&tmW, w, N, K, ldw, BP)) return CONVNN_E_CUDA;
         if (p.out_kind == OUT_F32) return gelu ? launch_pairs<OUT_F32, true>(tmA, tmW, p, st) : launch_pairs<OUT_F32, false>(tmA, tmW, p, st);
