@@ -63,6 +63,47 @@ def stale() -> bool:
         return f.read().strip() != source_hash()
 
 
+# The host side of some calls as a Python extension module, against the headers of the torch that is installed.
+CALL_SRC = os.path.join(CSRC, "fp8_call.cpp")
+CALL_LIB = os.path.join(HERE, "_fp8_call.so")
+CALL_STAMP = CALL_LIB + ".srchash"
+
+
+def call_hash() -> str:
+    """Digest of the module's source and of what else its binary depends on."""
+    import hashlib
+    import torch
+    with open(CALL_SRC, "rb") as f:
+        return hashlib.sha256(f.read() + f"{sys.version_info[:2]} {torch.__version__}".encode()).hexdigest()
+
+
+def call_stale() -> bool:
+    if not os.path.exists(CALL_LIB) or not os.path.exists(CALL_STAMP):
+        return True
+    with open(CALL_STAMP) as f:
+        return f.read().strip() != call_hash()
+
+
+def build_call() -> str:
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [f"-isystem{i}" for i in include] + [CALL_SRC, "-o", CALL_LIB + ".tmp", "-L" + os.path.join(root, "lib")]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(CALL_SRC)}:\n{r.stderr[-8000:]}")
+    os.replace(CALL_LIB + ".tmp", CALL_LIB)
+    with open(CALL_STAMP, "w") as f:
+        f.write(call_hash())
+    return CALL_LIB
+
+
 def _nvcc() -> str:
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     if not os.path.exists(nvcc):
@@ -72,6 +113,8 @@ def _nvcc() -> str:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile what changed and link; return the library path."""
+    if force or call_stale():
+        build_call()
     if not force and not stale():
         return LIB
     nvcc = _nvcc()

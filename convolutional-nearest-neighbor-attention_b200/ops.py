@@ -6,13 +6,16 @@ back to torch ops.
 """
 from __future__ import annotations
 
+import ctypes
 import math
+import os
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _capi
+from . import build as _build
 
 
 @dataclass(frozen=True)
@@ -567,7 +570,28 @@ def _rows_of(t: torch.Tensor, shape) -> Tuple[torch.Tensor, int, int]:
     return t.contiguous(), rows, D
 
 
-_E4M3, _F32 = torch.float8_e4m3fn, torch.float32
+_E4M3, _F32, _BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
+
+
+def _ordinary_calls():
+    """The module that makes ordinary calls without Python in between (``csrc/fp8_call.cpp``), built if it is missing or was
+    built against another torch, and bound to the library."""
+    L = _capi.lib()
+    if os.environ.get("CONVNN_B200_NO_BUILD") != "1" and _build.call_stale():
+        _build.build_call()
+    from . import _fp8_call
+    names = ("rms_norm", "rms_norm_fp8", "quantize_fp8", "linear_fp8")
+    _fp8_call.bind(*(ctypes.cast(getattr(L, "convnn_b200_" + n), ctypes.c_void_p).value for n in names), Fp8Blocks, _capi.check)
+    return _fp8_call
+
+
+_calls = None
+
+
+def _bind_calls():
+    global _calls
+    _calls = _ordinary_calls()
+    return _calls
 
 
 def _fp8_empty(shape, rows: int, device) -> Tuple[torch.Tensor, int, torch.Tensor]:
@@ -595,6 +619,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``s * rsqrt(mean(s * s) + eps) * weight`` over the last dimension, ``s = x``, or with ``residual`` the sum ``x +
     residual`` rounded to ``x``'s type (float32 or bfloat16).  -> y, in ``x``'s type or with ``quantize`` as ``Fp8Blocks``
     (from the float32 values) for ``linear_fp8``; with ``residual`` -> (y, s)."""
+    done = (_calls or _bind_calls()).rms_norm(x, weight, eps, residual, quantize)
+    if done is not None:
+        return done
     if torch.is_grad_enabled():
         _forward_only(x, weight, residual)
     index = _device_of(x, weight, residual)
@@ -634,6 +661,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
     """``x`` (float32 or bfloat16) in 8 bits with a scale per row and 128 channels (``block_rows`` 1: activations (..., D)), or
     per 128 x 128 block (``block_rows`` 128: a weight (N, D)), for ``linear_fp8``."""
+    done = (_calls or _bind_calls()).quantize_fp8(x, block_rows)
+    if done is not None:
+        return done
     if torch.is_grad_enabled():
         _forward_only(x)
     index = _device_of(x)
@@ -679,6 +709,9 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     scales per 128 x 128 block), each an ``Fp8Blocks`` or such a pair.  bias (N) and residual (..., N) in ``dtype`` (float32 or
     bfloat16).  -> (..., N) in ``dtype``, summed in float32 and rounded once, or with ``quantize`` as ``Fp8Blocks`` for the
     next product."""
+    done = (_calls or _bind_calls()).linear_fp8(a, w, bias, gelu, residual, 1 if dtype is _BF16 else 0 if dtype is _F32 else -1, quantize)
+    if done is not None:
+        return done
     (av, sa), (wv, sw) = a, w
     if torch.is_grad_enabled():
         _forward_only(bias, residual, sa, sw)
