@@ -68,6 +68,11 @@ __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
                  : "r"(taddr)
                  : "memory");
 }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -99,86 +104,89 @@ __device__ __forceinline__ void gelu_poly8(float* x) {
     for (int j = 0; j < 8; ++j) x[j] = fmaf(-a[j], q[j], max_nan(x[j], 0.f));
 }
 
+// Eight values of a row from column n on: neighbours, 16 bytes at a time where `vec` and all are inside, or one by one, `step` apart.
+template <typename T> struct Eight { uint4 v[sizeof(T) / 2]; };
 template <typename T>
-__device__ __forceinline__ void load8(const void* base, long long at, int valid, bool vec, float (&v)[8]) {
+__device__ __forceinline__ Eight<T> load8(const void* base, long long at, int left, int step, bool vec) {
     const T* p = static_cast<const T*>(base) + at;
-    if (vec && valid >= 8) {
-        uint4 raw[sizeof(T) / 2];
+    Eight<T> r;
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
-        const T* e = reinterpret_cast<const T*>(raw);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = make_uint4(0, 0, 0, 0);
+    if (vec && left >= 8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
+        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < valid ? to_f32<T>(p[j]) : 0.f;
+        for (int j = 0; j < 8; ++j)
+            if (j * step < left) e[j] = p[j * step];
     }
+    return r;
 }
 template <typename T>
-__device__ __forceinline__ void store8(void* base, long long at, int valid, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* base, long long at, int left, int step, bool vec, const float (&v)[8]) {
     T* p = static_cast<T*>(base) + at;
-    if (vec && valid >= 8) {
-        uint4 raw[sizeof(T) / 2];
-        T* e = reinterpret_cast<T*>(raw);
+    if (vec && left >= 8) {
+        Eight<T> r;
+        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < valid) p[j] = from_f32<T>(v[j]);
+            if (j * step < left) p[j * step] = from_f32<T>(v[j]);
     }
 }
-
-// Eight neighbouring outputs of row m from column n on, from their sums.  Sixteen neighbouring lanes hold a row's block of 128
-// columns and come here together.
-__device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, int n, bool row_valid, float (&v)[8]) {
-    const int valid = row_valid ? p.N - n : 0;               // may be <= 0
-    if (p.bias && valid > 0) {
-        float b[8];
-        if (p.io == CONVNN_F32) load8<float>(p.bias, n, valid, p.bias16, b);
-        else load8<__nv_bfloat16>(p.bias, n, valid, p.bias16, b);
+template <typename T>
+__device__ __forceinline__ void add8(float (&v)[8], const Eight<T>& r) {
+    const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += b[j];
-    }
+    for (int j = 0; j < 8; ++j) v[j] += to_f32<T>(e[j]);
+}
+
+// Eight outputs of row m from column n on, `step` apart, `left` columns before the end (<= 0: none); `sum` gives their sums, which are
+// asked for after the bias and the residual.  Sixteen neighbouring lanes hold a row's block of 128 columns and come here together.
+template <typename IO, typename Sum>
+__device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, int n, int left, int step, const Sum& sum) {
+    Eight<IO> bias, residual;
+    const bool near = step == 1;
+    if (p.bias) bias = load8<IO>(p.bias, n, left, step, p.bias16 && near);
+    if (p.residual) residual = load8<IO>(p.residual, m * p.ldr + n, left, step, p.residual16 && near);
+    float v[8];
+    sum(v);
+    if (p.bias) add8<IO>(v, bias);
     if (p.gelu && p.out_kind == OUT_F32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = gelu_erf(v[j]);
     } else if (p.gelu) {
         gelu_poly8(v);
     }
-    if (p.residual && valid > 0) {
-        float r[8];
-        if (p.io == CONVNN_F32) load8<float>(p.residual, m * p.ldr + n, valid, p.residual16, r);
-        else load8<__nv_bfloat16>(p.residual, m * p.ldr + n, valid, p.residual16, r);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r[j];
-    }
+    if (p.residual) add8<IO>(v, residual);
     if (p.out_kind == OUT_E4M3) {
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < valid) top = max(top, abs_bits(v[j]));
+            if (j < left) top = max(top, abs_bits(v[j]));
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float scale = fp8_scale(top), inv = __frcp_rn(scale);
-        if (valid > 0) {
+        if (left > 0) {
             uint2 w;
             w.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
             w.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
             uint8_t* q = static_cast<uint8_t*>(p.out) + m * p.ldo + n;
-            if (p.out16 && valid >= 8) *reinterpret_cast<uint2*>(q) = w;
+            if (p.out16 && left >= 8) *reinterpret_cast<uint2*>(q) = w;
             else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (j < valid) q[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+                    if (j < left) q[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
             }
             if (n % KB == 0) p.so[m * p.so_row + (n / KB) * p.so_block] = scale;
         }
-    } else if (valid > 0) {
-        if (p.out_kind == OUT_F32) store8<float>(p.out, m * p.ldo + n, valid, p.out16, v);
-        else store8<__nv_bfloat16>(p.out, m * p.ldo + n, valid, p.out16, v);
+    } else if (left > 0) {
+        store8<IO>(p.out, m * p.ldo + n, left, step, p.out16 && near, v);
     }
 }
 
@@ -351,34 +359,60 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
     const int row_a = ROWS * rank / p.splits, row_b = ROWS * (rank + 1) / p.splits;
     constexpr int GROUPS = COLS / 8;                         // sixteen, in both forms
     static_assert(GROUPS == 16, "sixteen lanes hold a row");
-    const uint32_t tile0 = smem_u32(tile);
-    // (every warp goes round as often as the others: the lanes of a row exchange their largest values)
+    // A lane takes eight neighbouring columns of a row; sixteen apart where rows of the output start anywhere, so that the sixteen lanes
+    // of a row write side by side.  (Every warp goes round as often as the others: the lanes of a row exchange their largest values.)
+    const int step = p.out16 || p.out_kind == OUT_E4M3 ? 1 : GROUPS;
     for (int u = row_a * GROUPS + (int)threadIdx.x; u - lane < row_b * GROUPS; u += NTHREADS) {
-        const int r = u / GROUPS, g = u % GROUPS;
-        const bool inside = r < row_b;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        if (inside) {
-            const uint32_t off = tile0 + (r * PITCH + g * 8) * 4;
-            if (p.splits == 1) {
-                const float4 a = *reinterpret_cast<const float4*>(tile + r * PITCH + g * 8);
-                const float4 b = *reinterpret_cast<const float4*>(tile + r * PITCH + g * 8 + 4);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-            } else {
-                for (int c = 0; c < p.splits; ++c) {
-                    const uint32_t at = map_to_cta(off, c);
-                    const float4 a = ld_cluster_f32x4(at), b = ld_cluster_f32x4(at + 16);
-                    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-                    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-                }
-            }
-        }
+        const int r = u / GROUPS, g = u % GROUPS, c = step == 1 ? 8 * g : g;
         const long long m = (long long)(SWAP ? qt * BN : pt * BP) + r;
-        finish8(p, m, (SWAP ? pt * BP : qt * BN) + g * 8, inside && m < p.M, v);
+        const int n = (SWAP ? pt * BP : qt * BN) + c, left = r < row_b && m < p.M ? p.N - n : 0;
+        const float* from = tile + (r < row_b ? r : row_a) * PITCH + c;
+        auto sum = [&](float (&v)[8]) {
+            if (p.splits == 1) {
+                if (step == 1) {
+                    const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = from[GROUPS * j];
+                }
+                return;
+            }
+            // two CTAs' parts at once: what takes time is the way there
+            const uint32_t off = smem_u32(from);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+            for (int k = 0; k < p.splits; k += 2) {
+                const uint32_t at0 = map_to_cta(off, k), at1 = map_to_cta(off, k + 1);
+                float w0[8], w1[8];
+                if (step == 1) {
+                    const float4 a = ld_cluster_f32x4(at0), b = ld_cluster_f32x4(at0 + 16), c = ld_cluster_f32x4(at1),
+                                 d = ld_cluster_f32x4(at1 + 16);
+                    w0[0] = a.x; w0[1] = a.y; w0[2] = a.z; w0[3] = a.w; w0[4] = b.x; w0[5] = b.y; w0[6] = b.z; w0[7] = b.w;
+                    w1[0] = c.x; w1[1] = c.y; w1[2] = c.z; w1[3] = c.w; w1[4] = d.x; w1[5] = d.y; w1[6] = d.z; w1[7] = d.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w0[j] = ld_cluster_f32(at0 + 4 * GROUPS * j);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w1[j] = ld_cluster_f32(at1 + 4 * GROUPS * j);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (v[j] + w0[j]) + w1[j];
+            }
+        };
+        if (p.io == CONVNN_F32) finish8<float>(p, m, n, left, step, sum);
+        else finish8<__nv_bfloat16>(p, m, n, left, step, sum);
     }
     if (p.splits > 1) cluster_sync_all();                    // the others may still read this CTA's tile
+}
+
+// CTAs that share the blocks of k of a tile: as many as leave every CTA an SM and two blocks.  (Two CTAs per SM load no faster: 1 x 4096 x
+// 4096 7.6 -> 9.5 us with 256 CTAs instead of 128.  With fewer blocks the sum of the parts takes longer: 128 x 1024 x 1024 9.1 -> 10.8.)
+int splits_of(long long tiles, int blocks) {
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= device_sms() && blocks >= 4 * splits) splits *= 2;
+    return splits;
 }
 
 template <int BN, bool SWAP>
@@ -388,9 +422,7 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
     const long long tiles = SWAP ? (long long)((p.N + BP - 1) / BP) * ((p.M + BN - 1) / BN)
                                  : (long long)((p.M + BP - 1) / BP) * ((p.N + BN - 1) / BN);
     if (tiles * 8 > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "linear_fp8: %d x %d is too many tiles", p.M, p.N);
-    const int sms = device_sms();
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits * 2 <= sms && p.blocks >= 4 * p.splits) p.splits *= 2;
+    p.splits = splits_of(tiles, p.blocks);
     const int per = (p.blocks + p.splits - 1) / p.splits;
     p.stages = SWAP ? MAX_STAGES : 3;
     while (p.stages > per && p.stages > 2) --p.stages;
@@ -1000,7 +1032,11 @@ int launch_linear_fp8(const void* a, long long lda, const float* sa, long long s
         if (p.out_kind == OUT_BF16) return gelu ? launch_pairs<OUT_BF16, true>(tmA, tmW, p, st) : launch_pairs<OUT_BF16, false>(tmA, tmW, p, st);
         return gelu ? launch_pairs<OUT_E4M3, true>(tmA, tmW, p, st) : launch_pairs<OUT_E4M3, false>(tmA, tmW, p, st);
     }
-    const bool swap = M <= 64;
+    // The weights as the 128 rows of a tile, tokens as its columns: always up to 64 tokens; with more, 64 at a time, where that is at
+    // most one tile per SM and at most eight blocks of k per CTA: what takes time then is the output, of which a CTA has half
+    // as much (197 x 2304 x 768 8.6 -> 7.2 us, 582 x 1000 x 494 8.3 -> 6.8; 256 x 4096 x 4096, 32 blocks, 16.4 -> 20.1).
+    const long long small_tiles = (long long)((N + BP - 1) / BP) * ((M + 63) / 64);
+    const bool swap = M <= 64 || (small_tiles <= device_sms() && p.blocks <= 8 * splits_of(small_tiles, p.blocks));
     const int bn = !swap ? 128 : M <= 16 ? 16 : M <= 32 ? 32 : 64;
     CUtensorMap tmP, tmQ;
     if (!encode_rows(&tmP, swap ? w : a, swap ? N : M, K, swap ? ldw : lda, BP)) return CONVNN_E_CUDA;
