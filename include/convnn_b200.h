@@ -231,7 +231,8 @@ int convnn_b200_linear(int dtype, const void* a, int64_t lda, const void* w, con
 
 /* y = s * (mean(s^2) + eps)^-1/2 * weight over the last dimension, s = x or, with a residual, x +
  * residual rounded to dtype, which is then also written to `sum` (both or neither NULL).  rows x D,
- * strides in elements, statistics in fp32. */
+ * strides in elements, statistics in fp32.  `sum` may be x or the residual itself, y may be x
+ * itself (same pointer and stride); otherwise nothing that is written may overlap what is read. */
 int convnn_b200_rms_norm(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                          const void* weight, float eps, void* sum, int64_t lds, void* y, int64_t ldy,
                          int64_t rows, int32_t D, void* stream);

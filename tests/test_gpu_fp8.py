@@ -83,7 +83,7 @@ def check_blocks(got, want, err):
 # ---- the norm -------------------------------------------------------------------------------------------------------
 
 NORM_SHAPES = [(1, 1), (1, 768), (3, 5), (9, 127), (8, 128), (17, 129), (33, 192), (5, 256), (6, 260), (7, 512), (3, 514), (65, 768),
-               (2, 1001), (10, 1024), (4, 1028), (3, 4096), (2, 4099), (3, 8192), (2, 8196), (2, 20001), (1, 20480)]
+               (2, 1001), (10, 1024), (4, 1028), (30, 1002), (3, 2426), (70, 250), (3, 4096), (2, 4099), (3, 8192), (2, 8196), (2, 20001), (1, 20480)]
 
 
 def norm_exact(s, weight, eps):
@@ -161,7 +161,7 @@ def test_norm_zero_rows_infinities_and_nan(dtype):
 
 # ---- the quantisers -------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("rows,D", [(1, 1), (1, 4096), (2, 127), (3, 128), (127, 129), (128, 256), (129, 260), (200, 1001), (5, 20484)])
+@pytest.mark.parametrize("rows,D", [(1, 1), (1, 4096), (2, 127), (3, 128), (127, 129), (128, 256), (129, 260), (200, 1001), (5, 20484), (300, 384), (77, 386), (131, 130), (9, 640), (1000, 256)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_is_the_formula(rows, D, dtype, block_rows):
@@ -505,6 +505,102 @@ def test_beside_the_bfloat16_operators():
     got = ops.linear_fp8(ops.quantize_fp8(h), ops.quantize_fp8(w, 128))
     want = ops.linear(h, w)
     assert ((got - want).double().norm() / want.double().norm()) < 2 * 0.036   # two operands, each off by 0.036 in the mean square
+
+
+class _NoOrdinaryCalls:
+    """Stands in for the module that makes ordinary calls: every call goes the general way."""
+    rms_norm = quantize_fp8 = linear_fp8 = staticmethod(lambda *a: None)
+
+
+@pytest.mark.parametrize("shape", [(1, 768), (7, 200), (3, 5, 131), (2, 2, 3, 64), (64,)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_ordinary_and_general_calls_agree(monkeypatch, shape, dtype):
+    D, N = shape[-1], 150
+    x, res, w = randn(*shape, seed=1, dtype=dtype), randn(*shape, seed=2, dtype=dtype), randn(D, seed=3, dtype=dtype)
+    bias, out_res = randn(N, seed=4, dtype=dtype), randn(*shape[:-1], N, seed=5, dtype=dtype)
+    weight = randn(N, D, seed=6, dtype=dtype)
+
+    def everything():
+        found = [ops.rms_norm(x, w), ops.rms_norm(x, w, 1, residual=res), *ops.rms_norm(x, w, 1e-3, res),
+                 *ops.rms_norm(x, w, quantize=True)]
+        (q, s), t = ops.rms_norm(x, w, residual=res, quantize=True)
+        a, b = ops.quantize_fp8(x), ops.quantize_fp8(weight, 128)
+        found += [q, s, t, *a, *b, ops.linear_fp8(a, b), ops.linear_fp8(a, b, bias, True, out_res, dtype),
+                  *ops.linear_fp8(a, b, bias=bias, residual=out_res, dtype=dtype, quantize=True), ops.linear_fp8([q, s], list(b), dtype=F32)]
+        return [t for f in found for t in (f if isinstance(f, tuple) else (f,))]
+
+    want = everything()
+    monkeypatch.setattr(ops, "_calls", _NoOrdinaryCalls)
+    got = everything()
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert a.shape == b.shape and a.dtype == b.dtype and (a.stride() == b.stride() or 1 in a.shape)
+        assert torch.equal(a.float(), b.float())
+
+
+def test_ordinary_calls_raise_what_the_library_says():
+    with pytest.raises(ValueError, match="eps"):
+        ops.rms_norm(randn(2, 8), randn(8), -1.0)
+    x = randn(3, 64, dtype=BF16)
+    assert torch.equal(ops.rms_norm(x, randn(64, seed=1, dtype=BF16)), ops.rms_norm(x, randn(64, seed=1, dtype=BF16)))
+
+
+@pytest.mark.parametrize("rows,D", [(5, 192), (5, 130), (3, 131), (4, 1536), (4, 8200), (2, 9001)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_in_place(rows, D, dtype):
+    """The sum may take the place of x or of the residual, and y that of x."""
+    L, st, code = _capi.lib(), torch.cuda.current_stream().cuda_stream, _capi.BF16 if dtype == BF16 else _capi.F32
+    x, res, w = randn(rows, D, seed=1, dtype=dtype), randn(rows, D, seed=2, dtype=dtype), randn(D, seed=3, dtype=dtype)
+    y, s = ops.rms_norm(x, w, residual=res)
+    for into in (0, 1):
+        t = (x.clone(), res.clone())
+        out = torch.empty_like(x)
+        _capi.check(L.convnn_b200_rms_norm(code, t[0].data_ptr(), D, t[1].data_ptr(), D, w.data_ptr(), 1e-6, t[into].data_ptr(), D,
+                                           out.data_ptr(), D, rows, D, st))
+        assert torch.equal(t[into], s) and torch.equal(out, y)
+    t = x.clone()
+    _capi.check(L.convnn_b200_rms_norm(code, t.data_ptr(), D, None, 0, w.data_ptr(), 1e-6, None, 0, t.data_ptr(), D, rows, D, st))
+    assert torch.equal(t, ops.rms_norm(x, w))
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 200, 300), (100, 203, 300), (300, 512, 256), (4000, 1300, 400), (4000, 1301, 200)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_linear_in_the_place_of_its_residual(M, N, K, dtype):
+    a, w = operands(M, N, K, seed=4)
+    res = randn(M, N, seed=6, dtype=dtype)
+    want = ops.linear_fp8(a, w, residual=res, dtype=dtype)
+    code = _capi.BF16 if dtype == BF16 else _capi.F32
+    av, wv = a.values, w.values
+    _capi.check(_capi.lib().convnn_b200_linear_fp8(
+        av.data_ptr(), av.stride(0), a.scales.data_ptr(), *a.scales.stride(), wv.data_ptr(), wv.stride(0), w.scales.data_ptr(),
+        *w.scales.stride(), code, None, res.data_ptr(), N, res.data_ptr(), N, None, 0, 0, M, N, K, 0,
+        torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(res, want)
+
+
+def test_two_threads_at_once():
+    import threading
+    weights = mlp_weights(192, 768)
+    xs = [randn(100 + 50 * i, 192, seed=i, dtype=BF16) for i in range(2)]
+    want = [encoder_mlp(x, x, weights)[0] for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.no_grad(), torch.cuda.stream(st):
+            for _ in range(50):
+                got = encoder_mlp(xs[i], xs[i], weights)[0]
+            st.synchronize()
+            if not torch.equal(got, want[i]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 # ---- refusals -------------------------------------------------------------------------------------------------------
