@@ -792,9 +792,9 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         for (int t = first; t < tiles; t += step) {
             const long long m0 = (long long)(t / n_n) * 2 * BP + rank * BP + quarter * 32;      // of the warp
             const int n = t % n_n * PAIR_N + half * KB;
-            if (lane == 0) tma_store_wait_read<0>();         // the last tile's results have left the slabs
-            __syncwarp();
             if (p.residual) {
+                if (lane == 0) tma_store_wait_read<0>();     // the last tile's results have left the slabs
+                __syncwarp();
                 if (p.io == CONVNN_F32) {
                     request_residual<float>(p, m0, n, slab0, lane);
                     request_residual<float>(p, m0, n + 32, slab0 + SLAB, lane);
@@ -889,7 +889,10 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 #pragma unroll
                 for (int j = 0; j < 128; j += 8) gelu_poly8(acc + j);
             }
-            if (p.residual) {
+            if (!p.residual) {
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+            } else {
                 residual_arrived();
                 if (p.io == CONVNN_F32) {
                     add_row<float>(slab0, lane, acc);
