@@ -81,19 +81,20 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 
 // x * Phi(x), for results that stay in float32.
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-// The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 12 in a / 2.5 - 1
-// that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 6.4e-7; off by 8.5e-7 *
-// |x| at most as it is evaluated here).
+// The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 14 in a / 2.5 - 1
+// that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 1.1e-7; off by 3.5e-7 *
+// |x| at most as it is evaluated here; degree 12, 8.5e-7, moved twice as many 8-bit values to a neighbour as float32 sums do).
 // Four pairs side by side, in an order that the compiler keeps: it strings single instructions up value by value, each waiting for
-// the last (29.5 cycles a value and warp with two warps per scheduler, 17.0 so; 14 are the multiply-adds' own).
+// the last (29.5 cycles a value and warp with two warps per scheduler, 17.0 so, of which 14 are the multiply-adds' own, with degree 12).
 __device__ __forceinline__ f32x2 fma2_here(f32x2 a, f32x2 b, f32x2 c) {
     f32x2 r;
     asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
 __device__ __forceinline__ void gelu_poly8(float* x) {
-    constexpr float C[13] = {0.00621029362f, -0.0438225605f, 0.136878088f, -0.239581555f, 0.232788831f, -0.0657733977f, -0.131332964f,
-                             0.163930997f, -0.0241190977f, -0.0787944123f, 0.0401191078f, 0.0140417274f, -0.0105441259f};
+    constexpr float C[15] = {0.00620970316f, -0.0438223705f, 0.136935323f, -0.239579886f, 0.231888264f, -0.0658391565f, -0.126034617f,
+                             0.164323628f, -0.038938798f, -0.0797081888f, 0.0613802746f, 0.0149657773f, -0.0256648194f, -0.000339551596f,
+                             0.00422481867f};
     float a[8];
     f32x2 u[4], q[4];
 #pragma unroll
@@ -101,9 +102,9 @@ __device__ __forceinline__ void gelu_poly8(float* x) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) u[j] = fma2_here(pack2(a[2 * j], a[2 * j + 1]), pack2(0.4f, 0.4f), pack2(-1.0f, -1.0f));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = fma2_here(u[j], pack2(C[12], C[12]), pack2(C[11], C[11]));
+    for (int j = 0; j < 4; ++j) q[j] = fma2_here(u[j], pack2(C[14], C[14]), pack2(C[13], C[13]));
 #pragma unroll
-    for (int i = 10; i >= 0; --i)
+    for (int i = 12; i >= 0; --i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[j] = fma2_here(q[j], u[j], pack2(C[i], C[i]));
 #pragma unroll
@@ -466,8 +467,14 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 //               of the 128-byte swizzle, by TMA where rows start on 16-byte boundaries.  Meanwhile the next tile's first two
 //               blocks are multiplied.
 // Twelve warps are launched with 168 registers a thread; the first four keep 56, which leaves the others 224: 4 * 32 * 56 + 8 * 32 * 224
-// = 12 * 32 * 168.  (Sixteen epilogue warps of 64 columns took 1350 cycles a block of k, 720 of them for loads and sums, the rest around
-// barriers; the products take 512.)
+// = 12 * 32 * 168.
+// What bounds it: 16384 x 4096 x 4096 runs at 1.68 PFLOP/s under the 1000 W power cap (1.86 for ten launches), 1.2 times what a bfloat16
+// library product sustains there; a block of k takes about 1000 cycles, of them 512 to 600 the tensor cores', the rest the way from
+// the product to the sums and back with two buffers, and the sums' own reads of TMEM (128 columns of two warps per scheduler: 290
+// cycles at the port's rate).  Few blocks of k: the output, 18 operations a value for GELU (50432 x 768 x 192).
+// Slower, ten launches of 16384 x 4096 x 4096: sixteen epilogue warps of 64 columns 418 us, lone CTAs of 128 x 256 330, waits that spin
+// 309, where pairs took 296; halves of a tile one after the other with buffers of their own 292 -> 419 (50432 x 768 x 192 with
+// GELU 57.7 -> 62.4).  Sums as float32 pairs do not stay in registers; 48 columns in flight instead of 32 change nothing.
 constexpr int PAIR_WARPS = 8, PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 constexpr int PAIR_N = 256;
 constexpr uint32_t PAIR_STAGE = 2 * BP * KB, SLAB = 4096;

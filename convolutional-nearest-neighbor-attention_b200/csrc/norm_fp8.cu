@@ -5,7 +5,9 @@
 //   block's scale (a rounding to bfloat16 in between would move one value in 16 by a step of e4m3)
 // A lane reads eight neighbouring channels at once, sixteen lanes a block: its largest magnitude is four exchanges, its 8-bit
 // result one 128-byte store.  All kernels are bound by memory as long as their loads are all requested before the first is used (raw,
-// into registers: every input is read once) and their instructions stay under about 90 per 256 channels.
+// into registers: every input is read once) and their instructions stay under about 90 per 256 channels: 131072 x 768 bfloat16 with
+// residual and 8-bit result 106 us, 708 MB at 6.6 TB/s (79 % of the memory's cycles); the same with loads that branched and four
+// channels a lane 366.  Rows of one vector (50432 x 192: 15.3 us, 68 MB) start and end more often than they stream.
 #include "common.cuh"
 #include "f32x2.cuh"
 #include "fp8.cuh"
