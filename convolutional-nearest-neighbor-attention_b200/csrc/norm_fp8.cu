@@ -424,11 +424,12 @@ bool on_boundary(const void* p, long long ld_bytes, int bytes) {
 }
 template <typename T> bool rows_on(const void* p, long long ld, int bytes) { return on_boundary(p, ld * (long long)sizeof(T), bytes); }
 
-template <typename T, int NV, int R, int WPR>
+// EIGHT: for rows of a multiple of eight channels too.
+template <typename T, int NV, int R, int WPR, bool EIGHT = true>
 int launch_norm(const NormParams& p, int unit, cudaStream_t st) {
     const long long per = (long long)(kWarps / WPR) * R, grid = (p.rows + per - 1) / per;
     if (grid > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "rms_norm: %lld rows", p.rows);
-    if (unit == 8) launch_chained(rms_norm_kernel<T, NV, R, WPR, 8>, (unsigned)grid, kThreads, 0, st, p);
+    if (EIGHT && unit == 8) launch_chained(rms_norm_kernel<T, NV, R, WPR, EIGHT ? 8 : 1>, (unsigned)grid, kThreads, 0, st, p);
     else if (unit == 2) launch_chained(rms_norm_kernel<T, NV, R, WPR, 2>, (unsigned)grid, kThreads, 0, st, p);
     else launch_chained(rms_norm_kernel<T, NV, R, WPR, 1>, (unsigned)grid, kThreads, 0, st, p);
     CONVNN_CHECK_LAUNCH("rms_norm");
@@ -449,8 +450,23 @@ int norm_of(const NormParams& p, cudaStream_t st) {
     if (vectors <= 1) return sizeof(T) == 2 && unit == 8 ? launch_norm<T, 1, 4, 1>(p, unit, st) : launch_norm<T, 1, 2, 1>(p, unit, st);
     if (vectors <= 2) return launch_norm<T, 2, 1, 1>(p, unit, st);
     if (vectors <= 3) return launch_norm<T, 3, 1, 1>(p, unit, st);
-    if (vectors <= 4) return launch_norm<T, 4, 1, 1>(p, unit, st);
+    // As many warps a row as leave each a few vectors and none without: bfloat16 with residual and 8-bit result, 16001 rows of 1536
+    // channels 28 us in two warps, 31 in four, 38 in eight (49 in eight with room for two vectors each); of 2048 36 in four, 37 in two,
+    // 42 in eight; 10001 of 2560 31 in four, 36 in eight.  float32 keeps more registers a vector (1536: 54 in two, 48 in four, 49 in
+    // eight; 2048: 33 in four and eight), and rows of other channels more yet: 50001 of 1001 92 in two warps, 125 in one; 16001
+    // of 1501 61 in two, 54 in four, 52 in eight; 10001 of 2501 70 in four, 64 in eight.  The choice is one by width and type, not
+    // by where rows start, so that a view's results are those of its copy.
+    const bool whole = p.D % 8 == 0;
+    if (vectors <= 4) return whole ? launch_norm<T, 4, 1, 1>(p, unit, st) : launch_norm<T, 2, 1, 2, false>(p, unit, st);
+    if constexpr (sizeof(T) == 2) {
+        if (whole && vectors <= 6) return launch_norm<T, 3, 1, 2>(p, unit, st);
+        if (whole && vectors <= 8) return launch_norm<T, 2, 1, 4>(p, unit, st);
+        if (whole && vectors <= 12) return launch_norm<T, 3, 1, 4>(p, unit, st);
+    }
+    if (vectors <= 8) return launch_norm<T, 1, 1, 8, sizeof(T) == 4>(p, unit, st);
     if (vectors <= 16) return launch_norm<T, 2, 1, 8>(p, unit, st);
+    // (6001 of 6144: 40 with room for three vectors a warp, 47 for four)
+    if (vectors <= 24) return launch_norm<T, 3, 1, 8>(p, unit, st);
     if (vectors <= 32) return launch_norm<T, 4, 1, 8>(p, unit, st);
     if (p.rows > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "rms_norm: %lld rows", p.rows);
     if (unit == 8) launch_chained(rms_norm_wide_kernel<T, 8>, (unsigned)p.rows, kThreads, 0, st, p);

@@ -140,6 +140,21 @@ def test_norm_strided_weight_and_offset_storage():
     assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.clone(), w.contiguous()))
 
 
+# every share of a row among warps, full and with a rest, and rows that leave warps of the last CTA without one
+@pytest.mark.parametrize("rows,D", [(5, 1000), (6, 1018), (3, 1280), (5, 1281), (2, 1536), (5, 1544), (7, 2040), (1, 2048), (3, 2050), (3, 2568),
+                                    (5, 2560), (3, 2561), (9, 4088), (2, 4098), (3, 6144), (2, 6001), (2, 6152)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_rows_of_several_warps(rows, D, dtype):
+    for with_residual in (False, True):
+        test_norm(rows, D, dtype, with_residual)
+    x, w = randn(1 + rows * D, seed=7, dtype=dtype), randn(D, seed=8, dtype=dtype)
+    view, res = x[1:].view(rows, D), randn(rows, D, seed=9, dtype=dtype)       # (rows on two- or four-byte boundaries)
+    got, s = ops.rms_norm(view, w, residual=res, quantize=True)
+    want, t = ops.rms_norm(view.clone(), w, residual=res, quantize=True)
+    assert torch.equal(s, t) and same_bytes(got.values, want.values) and torch.equal(got.scales, want.scales)
+    assert torch.equal(ops.rms_norm(view, w), ops.rms_norm(view.clone(), w))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_norm_zero_rows_infinities_and_nan(dtype):
     x = randn(5, 300, seed=1, dtype=dtype)
