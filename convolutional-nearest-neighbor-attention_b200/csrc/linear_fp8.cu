@@ -81,36 +81,70 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 
 // x * Phi(x), for results that stay in float32.
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-// The same for results of 8 or 16 bits: max(x, 0) - a * q(a) with a = min(|x|, 5) and q the polynomial of degree 14 in a / 2.5 - 1
-// that comes nearest to 1 - Phi on [0, 5] in the maximum norm (fitted by weighted least squares against erfc, 1.1e-7; off by 3.5e-7 *
-// |x| at most as it is evaluated here; degree 12, 8.5e-7, moved twice as many 8-bit values to a neighbour as float32 sums do).
+// The same for results of 8 or 16 bits: max(x, 0) - a Q(a) with a = |x| and Q = 1 - Phi = exp(-a^2 / 2) R(a), R the polynomial of degree 7
+// in t = 1 / (1 + 0.35 a) that comes nearest to erfcx(a / sqrt 2) / 2 on [0, 13.5] relative to it (Hastings' form, fitted by
+// weighted least squares: 3.1e-7).  Q is off by 2^-19 + a^2 2^-24 of itself at most as it is evaluated here, so that a block of 128
+// channels that lies wholly in the tail has its own scale and values (an approximation near in absolute terms does not: a polynomial of
+// degree 14 within 1.1e-7 of Q was 3 % off at -4.5 and constant below -5).  Below -13.2 the result is zero; -inf gives NaN as the
+// formula does, since the positive part is made as x / 2 + |x| / 2.
 // Four pairs side by side, in an order that the compiler keeps: it strings single instructions up value by value, each waiting for
-// the last (29.5 cycles a value and warp with two warps per scheduler, 17.0 so, of which 14 are the multiply-adds' own, with degree 12).
+// the last.  A value's two approximations (16 cycles of a warp's scheduler) run beside its 14 multiply-adds: 50432 x 768 x 192 into 8 bits
+// 52.0 us, 51.4 with that polynomial; one reciprocal for two values 53.5.
 __device__ __forceinline__ f32x2 fma2_here(f32x2 a, f32x2 b, f32x2 c) {
     f32x2 r;
     asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-__device__ __forceinline__ void gelu_poly8(float* x) {
-    constexpr float C[15] = {0.00620970316f, -0.0438223705f, 0.136935323f, -0.239579886f, 0.231888264f, -0.0658391565f, -0.126034617f,
-                             0.164323628f, -0.038938798f, -0.0797081888f, 0.0613802746f, 0.0149657773f, -0.0256648194f, -0.000339551596f,
-                             0.00422481867f};
-    float a[8];
-    f32x2 u[4], q[4];
+__device__ __forceinline__ f32x2 mul2_here(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm volatile("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float rcp_here(float x) {
+    float r;
+    asm volatile("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float ex2_here(float x) {
+    float r;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void gelu8(float* x) {
+    constexpr float C[8] = {2.73154092e-05f, -0.140270337f, -0.133355111f, -0.155961424f, 0.0170232989f,
+                            -0.240640655f, 0.202119172f, -0.0489424132f};
+    f32x2 a[4], t[4], e[4], q[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = fminf(fabsf(x[j]), 5.0f);
+    for (int j = 0; j < 4; ++j) a[j] = pack2(fminf(fabsf(x[2 * j]), 14.0f), fminf(fabsf(x[2 * j + 1]), 14.0f));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = fma2_here(pack2(a[2 * j], a[2 * j + 1]), pack2(0.4f, 0.4f), pack2(-1.0f, -1.0f));
+    for (int j = 0; j < 4; ++j) t[j] = fma2_here(a[j], pack2(0.35f, 0.35f), pack2(1.0f, 1.0f));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = fma2_here(u[j], pack2(C[14], C[14]), pack2(C[13], C[13]));
+    for (int j = 0; j < 4; ++j) e[j] = mul2_here(mul2(a[j], pack2(-0.72134752f, -0.72134752f)), a[j]);
 #pragma unroll
-    for (int i = 12; i >= 0; --i)
+    for (int j = 0; j < 4; ++j) {
+        float u, v;
+        unpack2(t[j], u, v);
+        t[j] = pack2(rcp_here(u), rcp_here(v));
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = fma2_here(q[j], u[j], pack2(C[i], C[i]));
+    for (int j = 0; j < 4; ++j) q[j] = fma2_here(t[j], pack2(C[7], C[7]), pack2(C[6], C[6]));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        unpack2(fma2_here(pack2(-a[2 * j], -a[2 * j + 1]), q[j], pack2(max_nan(x[2 * j], 0.f), max_nan(x[2 * j + 1], 0.f))), x[2 * j],
-                x[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) {
+        float u, v;
+        unpack2(e[j], u, v);
+        e[j] = pack2(ex2_here(u), ex2_here(v));
+    }
+#pragma unroll
+    for (int i = 5; i >= 0; --i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = fma2_here(q[j], t[j], pack2(C[i], C[i]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = mul2_here(q[j], e[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float u = 0.5f * x[2 * j], v = 0.5f * x[2 * j + 1];
+        unpack2(fma2_here(a[j], q[j], pack2(u + fabsf(u), v + fabsf(v))), x[2 * j], x[2 * j + 1]);
+    }
 }
 
 // Eight values of a row from column n on: neighbours, 16 bytes at a time where `vec` and all are inside, or one by one, `step` apart.
@@ -170,7 +204,7 @@ __device__ __forceinline__ void finish8(const LinearFp8Params& p, long long m, i
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = gelu_erf(v[j]);
     } else if (p.gelu) {
-        gelu_poly8(v);
+        gelu8(v);
     }
     if (p.residual) add8<IO>(v, residual);
     if (p.out_kind == OUT_E4M3) {
@@ -471,7 +505,7 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 // What bounds it: 16384 x 4096 x 4096 runs at 1.68 PFLOP/s under the 1000 W power cap (1.86 for ten launches), 1.2 times what a bfloat16
 // library product sustains there; a block of k takes about 1000 cycles, of them 512 to 600 the tensor cores', the rest the way from
 // the product to the sums and back with two buffers, and the sums' own reads of TMEM (128 columns of two warps per scheduler: 290
-// cycles at the port's rate).  Few blocks of k: the output, 18 operations a value for GELU (50432 x 768 x 192).
+// cycles at the port's rate).  Few blocks of k: the output, GELU's 14 multiply-adds a value (50432 x 768 x 192).
 // Slower, ten launches of 16384 x 4096 x 4096: sixteen epilogue warps of 64 columns 418 us, lone CTAs of 128 x 256 330, waits that spin
 // 309, where pairs took 296; halves of a tile one after the other with buffers of their own 292 -> 419 (50432 x 768 x 192 with
 // GELU 57.7 -> 62.4).  Sums as float32 pairs do not stay in registers; 48 columns in flight instead of 32 change nothing.
@@ -896,7 +930,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 for (int j = 0; j < 128; ++j) acc[j] = gelu_erf(acc[j]);
             } else if (GELU) {
 #pragma unroll
-                for (int j = 0; j < 128; j += 8) gelu_poly8(acc + j);
+                for (int j = 0; j < 128; j += 8) gelu8(acc + j);
             }
             if (!p.residual) {
                 if (lane == 0) tma_store_wait_read<0>();
