@@ -59,6 +59,7 @@ SIGNATURES = {
     "convnn_b200_forwards_in_flight": (ctypes.c_int, [ctypes.c_int32]),
     "convnn_b200_device_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "convnn_b200_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_uint32, c_void, c_void, c_void]),
+    "convnn_b200_selftest_pair_drain": (ctypes.c_int, [c_i32, c_i32, c_void, c_void, c_void, c_void]),
     "convnn_b200_head_channels": (ctypes.c_int, [ctypes.POINTER(ConvnnDesc)]),
     "convnn_b200_workspace_bytes": (c_size, [ctypes.POINTER(ConvnnDesc)]),
     "convnn_b200_stage_scratch_bytes": (c_size, [ctypes.POINTER(ConvnnDesc)]),

@@ -258,6 +258,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
     float* tile = reinterpret_cast<float*>(smem);            // in the place of the ring, once that is read
     __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[NBUF], tempty[NBUF];
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t counts[2];                           // blocks of k asked for, and multiplied
     __shared__ int abort_word;
     __shared__ __align__(16) float col_scale[SWAP ? 8 : 1][2][SWAP ? 32 : 1];
     volatile int* abort_flag = &abort_word;
@@ -296,14 +297,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
                 tma_load_2d(sQ + s * Q_BYTES, &tmQ, &full[s], kb * KB, qt * BN);
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
             }
-            if (kb < kb1) {                                  // gave up: what is on its way lands before the CTA leaves
-                int never = 0;
-                for (uint32_t i = 0; i < STAGES && kb > kb0; ++i, --kb) {
-                    if (s == 0) { s = STAGES; ph ^= 1u; }
-                    --s;
-                    mbar_wait(&full[s], ph, &never);
-                }
-            }
+            counts[0] = (uint32_t)(kb - kb0);
         }
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_e4m3_f32(BP, BN);
@@ -311,7 +305,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
         const uint32_t full0 = smem_u32(full), tempty0 = smem_u32(tempty), empty0 = smem_u32(empty), tfull0 = smem_u32(tfull);
         const uint32_t sP0 = smem_u32(sP), sQ0 = smem_u32(sQ);
         uint32_t s = 0, ph = 0, buf = 0, tph = 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        int kb = kb0;
+        for (; kb < kb1; ++kb) {
             if (!mbar_wait_warp(tempty0 + 8 * buf, tph ^ 1u, abort_flag)) { if (lane == 0) fail(abort_flag, 122); break; }
             if (!mbar_wait_warp(full0 + 8 * s, ph, abort_flag)) { if (lane == 0) fail(abort_flag, 123); break; }
             tc_fence_after_sync();
@@ -328,6 +323,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
             if (++s == STAGES) { s = 0; ph ^= 1u; }
             if (++buf == NBUF) { buf = 0; tph ^= 1u; }
         }
+        if (lane == 0) counts[1] = (uint32_t)(kb - kb0);
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;   // (a warp reads the TMEM lanes of its number mod 4)
         const int c0 = half * CW, row = quarter * 32 + lane;
@@ -397,6 +393,17 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant
     tc_fence_before_sync();
     if (p.splits > 1) cluster_sync_all();
     else __syncthreads();
+    if (*abort_flag && warp == 1) {
+        // A wait gave up: what was asked for lands and what was issued ends before the CTA leaves and its tensor memory is another's.
+        int never = 0;
+        for (uint32_t f = counts[0] > STAGES ? counts[0] - STAGES : 0; f < counts[0]; ++f)
+            mbar_wait_warp(smem_u32(&full[f % STAGES]), (f / STAGES) & 1u, &never);
+        if (counts[1] > 0) {
+            const uint32_t last = counts[1] - 1;
+            mbar_wait_warp(smem_u32(&empty[last % STAGES]), (last / STAGES) & 1u, &never);
+            mbar_wait_warp(smem_u32(&tfull[last % NBUF]), (last / NBUF) & 1u, &never);
+        }
+    }
     if (warp == 1) tmem_dealloc(tmem_base, TCOLS);
     // After a wait that gave up, the tiles of the cluster are not whole, and what is written is undefined.
     const int row_a = ROWS * rank / p.splits, row_b = ROWS * (rank + 1) / p.splits;
@@ -688,6 +695,7 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     float* scales = reinterpret_cast<float*>(slabs + 2 * PAIR_WARPS * SLAB);       // [slot]: [block of the group][row], [block][half of the columns]
     __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], tfull[2], tempty[2], sfull[SCALE_SLOTS], sempty[SCALE_SLOTS];
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t counts[3];                           // fills by the even and by the odd CTA, blocks of k multiplied
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
 
@@ -714,6 +722,12 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     auto give_up = [&](int code) {
         st_cluster_u32(peer_abort, 1u);
         fail(abort_flag, code);
+    };
+    auto tell = [&](uint32_t i, uint32_t n) {                // both CTAs
+        if (lane == 0) {
+            counts[i] = n;
+            st_cluster_u32(map_to_cta(smem_u32(&counts[i]), rank ^ 1u), n);
+        }
     };
     chain_begin();
 
@@ -748,11 +762,12 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                 --s;
                 ok = mbar_wait_warp(empty0 + 8 * s, ph, abort_flag);
             }
+            tell(rank, fills);
         } else if (warp == 1) {
             if (rank == 0) {
                 constexpr uint32_t idesc = idesc_e4m3_f32(2 * BP, PAIR_N);
                 const uint64_t hi = kmajor_desc_hi(KB);
-                uint32_t s = 0, ph = 0, buf = 0, tph = 0;
+                uint32_t s = 0, ph = 0, buf = 0, tph = 0, issued = 0;
                 bool ok = true;
                 for (int t = first; t < tiles && ok; t += step) {
                     for (int kb = 0; kb < p.blocks; ++kb) {
@@ -772,8 +787,10 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
                         if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
                         buf ^= 1u;
                         if (buf == 0) tph ^= 1u;
+                        ++issued;
                     }
                 }
+                tell(2, issued);
             }
         } else {
             // copied straight to shared memory, zeros where there is nothing; a warp has two blocks of a group
@@ -1013,6 +1030,21 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();                                      // the peer no longer signals or reads this CTA
+    if (*abort_flag) {
+        // A wait gave up (in both CTAs, give_up() has seen to that): what was asked for lands and what was issued ends before
+        // either of them leaves.
+        if (warp == 0 && lane == 0) {
+            int never = 0;
+            if (rank == 0) drain_pair_ring(full0, PAIR_STAGES, PAIR_STAGE, counts[0], counts[1]);
+            if (counts[2] > 0) {
+                const uint32_t last = counts[2] - 1;
+                mbar_wait_a(empty0 + 8 * (last % PAIR_STAGES), (last / PAIR_STAGES) & 1u, &never);
+                mbar_wait_a(tfull0 + 8 * (last & 1u), (last >> 1) & 1u, &never);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
     if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 

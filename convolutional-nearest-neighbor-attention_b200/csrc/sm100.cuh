@@ -329,6 +329,27 @@ __device__ __forceinline__ void mma_bf16_ts_pair(uint32_t tmem_d, uint32_t tmem_
         ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Bytes that were expected on a barrier and will not come count as having come.
+__device__ __forceinline__ void mbar_complete_tx_a(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// After a wait that gave up, one thread of the even CTA, once neither CTA asks for more: waits until what either has asked for has
+// landed.  Fill f of the ring's `stages` is `bytes` from each CTA on full barrier f % stages of the even CTA, which arrives and expects
+// both with its own fill; `own` and `peer` are how often the even and the odd CTA filled.  A fill waits for the products of the one
+// before it in its stage, and those for both CTAs' copies, so that the counts differ by `stages` at most and only each stage's
+// last fill can be on its way.  Returns whether all ended in time.
+__device__ __forceinline__ bool drain_pair_ring(uint32_t full0, uint32_t stages, uint32_t bytes, uint32_t own, uint32_t peer) {
+    const uint32_t fills = own > peer ? own : peer;
+    int never = 0;
+    bool landed = true;
+    for (uint32_t f = fills > stages ? fills - stages : 0; f < fills; ++f) {
+        const uint32_t bar = full0 + 8 * (f % stages);
+        if (f >= peer) mbar_complete_tx_a(bar, bytes);       // never asked for by the odd CTA
+        else if (f >= own) mbar_expect_tx_a(bar, bytes);     // asked for by the odd CTA alone
+        landed = mbar_wait_a(bar, (f / stages) & 1u, &never) && landed;
+    }
+    return landed;
+}
 // One arrival on the barrier at `bar_cluster` (own or peer CTA) when every MMA this thread
 // has issued so far has completed in both CTAs.
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar_cluster) {

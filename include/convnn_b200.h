@@ -120,6 +120,13 @@ int convnn_b200_device_status(int* code);
  * neither traps nor touches the error latch; the context stays usable. */
 int convnn_b200_selftest_wait_timeout(uint32_t budget_us, int* status_dev, uint64_t* waited_ns_dev,
                                       void* stream);
+/* No reference counterpart: the way out that a CTA pair of the 8-bit product takes after a wait that gave up, without any MMA and
+ * without a wait that gives up.  Two CTAs ask for `fills_even` and `fills_odd` (0 .. 8, at most 4 apart) copies of 2 KB each from src
+ * (32 KB; copy f of the even / odd CTA is row 2 f / 2 f + 1 of its sixteen 2 KB rows) into rings of four stages, then wait for what is on
+ * its way as the product does.  dst (16 KB): the stages of the even, then of the odd CTA, zeros where nothing was asked for.
+ * *status: 0, or 1 where a copy did not land in time.  All DEVICE pointers. */
+int convnn_b200_selftest_pair_drain(int32_t fills_even, int32_t fills_odd, const void* src_dev, void* dst_dev,
+                                    int* status_dev, void* stream);
 
 /* Channels per head as stored in q/k/v (Cp above). Negative status on a bad descriptor. */
 int convnn_b200_head_channels(const convnn_desc* d);
