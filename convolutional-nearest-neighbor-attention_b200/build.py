@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -112,9 +113,18 @@ def _nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile what changed and link; return the library path."""
-    if force or call_stale():
-        build_call()
+    """Compile what changed and link; return the library's path.  The host side of some calls is built after it; without
+    that module the calls go through Python."""
+    path = build_library(force, verbose)
+    try:
+        if force or call_stale():
+            build_call()
+    except (RuntimeError, ImportError, OSError) as e:        # the compiler, torch, a folder
+        warnings.warn(f"the host side of the 8-bit calls is not built, they go through Python: {e}", RuntimeWarning)
+    return path
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and not stale():
         return LIB
     nvcc = _nvcc()

@@ -1,0 +1,60 @@
+"""The build's host side: what one part's failure means for the other, and builders that come at the same time.  Compilers are stood in
+for: nothing is compiled here."""
+import os
+import subprocess
+import types
+
+import pytest
+
+from convnn_b200 import build as B
+
+
+def output_of(cmd):
+    return cmd[cmd.index("-o") + 1]
+
+
+@pytest.fixture
+def elsewhere(monkeypatch, tmp_path):
+    """The build's products in a folder of their own, all of them missing."""
+    for name in ("LIB", "STAMP", "CALL_LIB", "CALL_STAMP"):
+        monkeypatch.setattr(B, name, str(tmp_path / os.path.basename(getattr(B, name))))
+    monkeypatch.setattr(B, "OBJ", str(tmp_path / "build"))
+    return tmp_path
+
+
+def compilers(monkeypatch, gpp_works):
+    ran = []
+
+    def run(cmd, **kw):
+        tool = os.path.basename(cmd[0])
+        ran.append(tool)
+        if tool == "g++" and gpp_works is None:
+            raise FileNotFoundError(2, "Python.h: no such file, nor a compiler")
+        if tool == "g++" and not gpp_works:
+            return types.SimpleNamespace(returncode=1, stdout="", stderr="Python.h: no such file")
+        with open(output_of(cmd), "w") as f:
+            f.write(tool)
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    return ran
+
+
+@pytest.mark.parametrize("force", [False, True])
+@pytest.mark.parametrize("gpp_works", [False, None])
+def test_the_library_is_built_where_the_host_module_cannot_be(elsewhere, monkeypatch, force, gpp_works):
+    ran = compilers(monkeypatch, gpp_works)
+    with pytest.warns(RuntimeWarning, match="Python.h"):
+        assert B.build(force=force) == B.LIB
+    assert os.path.exists(B.LIB) and not B.stale() and not os.path.exists(B.CALL_LIB) and B.call_stale()
+    assert "nvcc" in ran
+
+
+def test_both_are_built(elsewhere, monkeypatch, recwarn):
+    ran = compilers(monkeypatch, gpp_works=True)
+    B.build()
+    assert os.path.exists(B.LIB) and os.path.exists(B.CALL_LIB) and not B.stale() and not B.call_stale()
+    assert not [w for w in recwarn if issubclass(w.category, RuntimeWarning)]
+    del ran[:]
+    B.build()
+    assert not ran
