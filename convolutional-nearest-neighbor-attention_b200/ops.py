@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import warnings
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
@@ -573,13 +574,24 @@ def _rows_of(t: torch.Tensor, shape) -> Tuple[torch.Tensor, int, int]:
 _E4M3, _F32, _BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
 
 
+class _GeneralCalls:
+    """Stands in for the module of ordinary calls where it cannot be had: every call goes the general way."""
+    rms_norm = quantize_fp8 = linear_fp8 = staticmethod(lambda *args: None)
+
+
 def _ordinary_calls():
     """The module that makes ordinary calls without Python in between (``csrc/fp8_call.cpp``), built if it is missing or was
-    built against another torch, and bound to the library."""
+    built against another torch, and bound to the library.  Without it calls take the time of their Python form."""
     L = _capi.lib()
-    if os.environ.get("CONVNN_B200_NO_BUILD") != "1" and _build.call_stale():
-        _build.build_call()
-    from . import _fp8_call
+    try:
+        if _build.call_stale():
+            if os.environ.get("CONVNN_B200_NO_BUILD") == "1":
+                raise RuntimeError("_fp8_call.so is missing or out of date")
+            _build.build_call()
+        from . import _fp8_call
+    except (RuntimeError, ImportError, OSError) as e:
+        warnings.warn(f"8-bit calls go through Python: {e}", RuntimeWarning)
+        return _GeneralCalls
     names = ("rms_norm", "rms_norm_fp8", "quantize_fp8", "linear_fp8")
     _fp8_call.bind(*(ctypes.cast(getattr(L, "convnn_b200_" + n), ctypes.c_void_p).value for n in names), Fp8Blocks, _capi.check)
     return _fp8_call

@@ -3,8 +3,10 @@ for: nothing is compiled here."""
 import os
 import subprocess
 import types
+import warnings
 
 import pytest
+import torch
 
 from convnn_b200 import build as B
 
@@ -58,3 +60,37 @@ def test_both_are_built(elsewhere, monkeypatch, recwarn):
     del ran[:]
     B.build()
     assert not ran
+
+
+@pytest.fixture
+def no_calls(monkeypatch):
+    """ops as it is before its first 8-bit call."""
+    from convnn_b200 import ops
+    monkeypatch.setattr(ops, "_calls", None)
+    return ops
+
+
+def test_calls_go_through_python_where_the_module_cannot_be_built(no_calls, monkeypatch):
+    def build_call():
+        raise RuntimeError("g++ failed")
+
+    monkeypatch.delenv("CONVNN_B200_NO_BUILD", raising=False)
+    monkeypatch.setattr(B, "call_stale", lambda: True)
+    monkeypatch.setattr(B, "build_call", build_call)
+    x, w = torch.zeros(2, 8), torch.zeros(8)
+    with torch.no_grad():
+        with pytest.warns(RuntimeWarning, match="through Python"), pytest.raises(RuntimeError, match="no CPU path"):
+            no_calls.rms_norm(x, w)
+        with warnings.catch_warnings(), pytest.raises(RuntimeError, match="no CPU path"):
+            warnings.simplefilter("error")                   # (once is enough)
+            no_calls.quantize_fp8(x)
+
+
+def test_a_module_of_another_source_is_not_loaded(no_calls, monkeypatch):
+    """Where nothing may be built: its signatures need not be the library's."""
+    monkeypatch.setenv("CONVNN_B200_NO_BUILD", "1")
+    monkeypatch.setattr(B, "call_stale", lambda: True)
+    monkeypatch.setattr(B, "build_call", lambda: pytest.fail("built"))
+    with torch.no_grad(), pytest.warns(RuntimeWarning, match="out of date"), pytest.raises(RuntimeError, match="no CPU path"):
+        no_calls.rms_norm(torch.zeros(2, 8), torch.zeros(8))
+    assert not hasattr(no_calls._calls, "bind")
