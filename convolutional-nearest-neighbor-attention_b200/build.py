@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import threading
 import warnings
 from concurrent.futures import ThreadPoolExecutor
 
@@ -94,14 +95,20 @@ def build_call() -> str:
                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    cmd += [f"-isystem{i}" for i in include] + [CALL_SRC, "-o", CALL_LIB + ".tmp", "-L" + os.path.join(root, "lib")]
+    tmp = f"{CALL_LIB}.{os.getpid()}.{threading.get_ident()}.tmp"        # (ranks and threads may build at the same time)
+    cmd += [f"-isystem{i}" for i in include] + [CALL_SRC, "-o", tmp, "-L" + os.path.join(root, "lib")]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {os.path.basename(CALL_SRC)}:\n{r.stderr[-8000:]}")
-    os.replace(CALL_LIB + ".tmp", CALL_LIB)
-    with open(CALL_STAMP, "w") as f:
-        f.write(call_hash())
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on {os.path.basename(CALL_SRC)}:\n{r.stderr[-8000:]}")
+        os.replace(tmp, CALL_LIB)
+        with open(tmp, "w") as f:
+            f.write(call_hash())
+        os.replace(tmp, CALL_STAMP)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
     return CALL_LIB
 
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import threading
 import warnings
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
@@ -598,12 +599,15 @@ def _ordinary_calls():
 
 
 _calls = None
+_calls_lock = threading.Lock()
 
 
 def _bind_calls():
     global _calls
-    _calls = _ordinary_calls()
-    return _calls
+    with _calls_lock:
+        if _calls is None:
+            _calls = _ordinary_calls()
+        return _calls
 
 
 def _fp8_empty(shape, rows: int, device) -> Tuple[torch.Tensor, int, torch.Tensor]:

@@ -2,6 +2,8 @@
 for: nothing is compiled here."""
 import os
 import subprocess
+import threading
+import time
 import types
 import warnings
 
@@ -94,3 +96,65 @@ def test_a_module_of_another_source_is_not_loaded(no_calls, monkeypatch):
     with torch.no_grad(), pytest.warns(RuntimeWarning, match="out of date"), pytest.raises(RuntimeError, match="no CPU path"):
         no_calls.rms_norm(torch.zeros(2, 8), torch.zeros(8))
     assert not hasattr(no_calls._calls, "bind")
+
+
+def test_builders_at_the_same_time_do_not_share_a_file(elsewhere, monkeypatch):
+    """Ranks that come first together: each puts a whole file in place."""
+    both = threading.Barrier(2)
+
+    def run(cmd, **kw):
+        with open(output_of(cmd), "w") as f:
+            f.write("first half")
+            f.flush()
+            both.wait(10)
+            f.write(", second half")
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    failed = []
+
+    def build():
+        try:
+            B.build_call()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=build) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    with open(B.CALL_LIB) as f:
+        assert f.read() == "first half, second half"
+    assert not B.call_stale()
+    assert sorted(os.listdir(elsewhere)) == sorted(os.path.basename(p) for p in (B.CALL_LIB, B.CALL_STAMP))
+
+
+def test_a_failed_build_leaves_nothing_behind(elsewhere, monkeypatch):
+    def run(cmd, **kw):
+        open(output_of(cmd), "w").close()
+        return types.SimpleNamespace(returncode=1, stdout="", stderr="no space left")
+
+    monkeypatch.setattr(subprocess, "run", run)
+    with pytest.raises(RuntimeError, match="no space left"):
+        B.build_call()
+    assert os.listdir(elsewhere) == []
+
+
+def test_threads_that_come_first_together_bind_once(no_calls, monkeypatch):
+    bound, calls = [], no_calls._GeneralCalls
+
+    def ordinary():
+        bound.append(threading.get_ident())
+        time.sleep(0.2)
+        return calls
+
+    monkeypatch.setattr(no_calls, "_ordinary_calls", ordinary)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(no_calls._calls or no_calls._bind_calls())) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(bound) == 1 and got == [calls] * 4
