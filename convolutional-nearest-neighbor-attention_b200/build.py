@@ -72,11 +72,15 @@ CALL_STAMP = CALL_LIB + ".srchash"
 
 
 def call_hash() -> str:
-    """Digest of the module's source and of what else its binary depends on."""
+    """Digest of the module's source, of the library's header, whose signatures it calls, and of what else its binary
+    depends on."""
     import hashlib
     import torch
-    with open(CALL_SRC, "rb") as f:
-        return hashlib.sha256(f.read() + f"{sys.version_info[:2]} {torch.__version__}".encode()).hexdigest()
+    h = hashlib.sha256(f"{sys.version_info[:2]} {torch.__version__}".encode())
+    for name in (CALL_SRC, os.path.join(INCLUDE, "convnn_b200.h")):
+        with open(name, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
 
 
 def call_stale() -> bool:
@@ -96,7 +100,7 @@ def build_call() -> str:
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     tmp = f"{CALL_LIB}.{os.getpid()}.{threading.get_ident()}.tmp"        # (ranks and threads may build at the same time)
-    cmd += [f"-isystem{i}" for i in include] + [CALL_SRC, "-o", tmp, "-L" + os.path.join(root, "lib")]
+    cmd += [f"-isystem{i}" for i in include] + ["-I" + INCLUDE, CALL_SRC, "-o", tmp, "-L" + os.path.join(root, "lib")]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     try:
         r = subprocess.run(cmd, capture_output=True, text=True)

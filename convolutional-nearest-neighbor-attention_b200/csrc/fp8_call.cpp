@@ -11,24 +11,17 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include "convnn_b200.h"
+
 namespace {
 
-enum { F32 = 0, BF16 = 1 };                                  // convnn_dtype
 constexpr int64_t BLOCK = 128;
 
-// The C entry points (declared in convnn_b200.h), and the class of a pair of values and scales: given by bind().
-using NormFn = int (*)(int, const void*, int64_t, const void*, int64_t, const void*, float, void*, int64_t, void*, int64_t, int64_t,
-                       int32_t, void*);
-using NormFp8Fn = int (*)(int, const void*, int64_t, const void*, int64_t, const void*, float, void*, int64_t, void*, int64_t, float*,
-                          int64_t, int64_t, int64_t, int32_t, void*);
-using QuantizeFn = int (*)(int, const void*, int64_t, int32_t, void*, int64_t, float*, int64_t, int64_t, int64_t, int32_t, void*);
-using LinearFn = int (*)(const void*, int64_t, const float*, int64_t, int64_t, const void*, int64_t, const float*, int64_t, int64_t,
-                         int, const void*, const void*, int64_t, void*, int64_t, float*, int64_t, int64_t, int64_t, int32_t, int32_t,
-                         int32_t, void*);
-NormFn norm_fn = nullptr;
-NormFp8Fn norm_fp8_fn = nullptr;
-QuantizeFn quantize_fn = nullptr;
-LinearFn linear_fn = nullptr;
+// The C entry points, and the class of a pair of values and scales: given by bind().
+decltype(&convnn_b200_rms_norm) norm_fn = nullptr;
+decltype(&convnn_b200_rms_norm_fp8) norm_fp8_fn = nullptr;
+decltype(&convnn_b200_quantize_fp8) quantize_fn = nullptr;
+decltype(&convnn_b200_linear_fp8) linear_fn = nullptr;
 PyObject *blocks_class = nullptr, *check_fn = nullptr;
 
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -41,10 +34,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
         at[i] = PyLong_AsVoidPtr(args[i]);
         if (PyErr_Occurred()) return nullptr;
     }
-    norm_fn = reinterpret_cast<NormFn>(at[0]);
-    norm_fp8_fn = reinterpret_cast<NormFp8Fn>(at[1]);
-    quantize_fn = reinterpret_cast<QuantizeFn>(at[2]);
-    linear_fn = reinterpret_cast<LinearFn>(at[3]);
+    norm_fn = reinterpret_cast<decltype(norm_fn)>(at[0]);
+    norm_fp8_fn = reinterpret_cast<decltype(norm_fp8_fn)>(at[1]);
+    quantize_fn = reinterpret_cast<decltype(quantize_fn)>(at[2]);
+    linear_fn = reinterpret_cast<decltype(linear_fn)>(at[3]);
     Py_INCREF(args[4]);
     Py_INCREF(args[5]);
     blocks_class = args[4];
@@ -60,7 +53,7 @@ const at::Tensor* plain(PyObject* o, int& device, bool grad) {
     if (device < 0) device = t.get_device();
     return t.get_device() == device ? &t : nullptr;
 }
-int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? BF16 : t == at::kFloat ? F32 : -1; }
+int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? CONVNN_BF16 : t == at::kFloat ? CONVNN_F32 : -1; }
 
 // Rows of the last dimension with one stride between them.
 bool rows_of(const at::Tensor& t, int64_t& rows, int64_t& ld) {
@@ -212,11 +205,11 @@ PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* bias = with_bias ? plain(args[2], device, grad) : nullptr;
     const at::Tensor* res = with_residual ? plain(args[4], device, grad) : nullptr;
     OR_NONE((bias || !with_bias) && (res || !with_residual));
-    const auto type = io == BF16 ? at::kBFloat16 : at::kFloat;
-    // (two dimensions: the scales of more need not be evenly strided)
-    OR_NONE((io == F32 || io == BF16) && a->scalar_type() == at::kFloat8_e4m3fn && w->scalar_type() == at::kFloat8_e4m3fn &&
-            sa->scalar_type() == at::kFloat && sw->scalar_type() == at::kFloat && a->dim() == 2 && w->dim() == 2 && sa->dim() == 2 &&
-            sw->dim() == 2);
+    const auto type = io == CONVNN_BF16 ? at::kBFloat16 : at::kFloat;
+    // (values of more dimensions go through Python, which looks at how their scales are strided)
+    OR_NONE((io == CONVNN_F32 || io == CONVNN_BF16) && a->scalar_type() == at::kFloat8_e4m3fn &&
+            w->scalar_type() == at::kFloat8_e4m3fn && sa->scalar_type() == at::kFloat && sw->scalar_type() == at::kFloat &&
+            a->dim() == 2 && w->dim() == 2 && sa->dim() == 2 && sw->dim() == 2);
     int64_t M, N, lda, ldw, ldr = 0, res_rows;
     OR_NONE(rows_of(*a, M, lda) && rows_of(*w, N, ldw));
     const int64_t K = a->size(1), blocks = (K + BLOCK - 1) / BLOCK;

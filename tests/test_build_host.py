@@ -158,3 +158,25 @@ def test_threads_that_come_first_together_bind_once(no_calls, monkeypatch):
     for t in threads:
         t.join()
     assert len(bound) == 1 and got == [calls] * 4
+
+
+def test_a_changed_header_rebuilds_the_host_module(elsewhere, monkeypatch):
+    """The module calls the library by address with the signatures of the header."""
+    compilers(monkeypatch, True)
+    header = elsewhere / "include" / "convnn_b200.h"
+    header.parent.mkdir()
+    with open(os.path.join(B.INCLUDE, header.name)) as f:
+        header.write_text(f.read())
+    monkeypatch.setattr(B, "INCLUDE", str(header.parent))
+    B.build_call()
+    assert not B.call_stale()
+    header.write_text(header.read_text() + "/* another signature */")
+    assert B.call_stale()
+
+
+def test_the_host_module_takes_the_signatures_from_the_header():
+    """A signature that is written down twice can differ."""
+    with open(B.CALL_SRC) as f:
+        source = f.read()
+    for name in ("rms_norm", "rms_norm_fp8", "quantize_fp8", "linear_fp8"):
+        assert f"decltype(&convnn_b200_{name})" in source
