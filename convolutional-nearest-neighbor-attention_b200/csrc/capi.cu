@@ -2,6 +2,7 @@
 // chaining of the stage kernels on the caller's stream.
 #include <atomic>
 #include <mutex>
+#include <numeric>
 #include <stdarg.h>
 #include <stdlib.h>
 #include <string.h>
@@ -549,11 +550,22 @@ int convnn_b200_linear(int dtype, const void* a, int64_t lda, const void* w, con
 
 // ---- 8-bit values with a scale per block of 128 ---------------------------------------------------
 
-// Strides of (rows, blocks) float32 scales, in elements; written scales may not share an address.
-static int scales_ok(const char* what, const float* s, int64_t row, int64_t block, bool written) {
+// Strides of float32 scales that are read, in elements.
+static int scales_ok(const char* what, const float* s, int64_t row, int64_t block) {
     if (reinterpret_cast<uintptr_t>(s) & 3u) return set_error(CONVNN_E_ALIGN, "%s: scales must be 4-byte aligned", what);
-    if (row < (written ? 1 : 0) || block < (written ? 1 : 0))
+    if (row < 0 || block < 0)
         return set_error(CONVNN_E_INVALID, "%s: strides %lld, %lld of the scales", what, (long long)row, (long long)block);
+    return CONVNN_OK;
+}
+// Of rows x blocks scales that are written: no two at one address.  The nearest two that could meet are block / g rows and row / g
+// blocks apart, g the strides' greatest common divisor.
+static int written_scales_ok(const char* what, const float* s, int64_t row, int64_t block, int64_t rows, int64_t blocks) {
+    const int rc = scales_ok(what, s, row, block);
+    if (rc) return rc;
+    const int64_t g = row < 1 || block < 1 ? 0 : std::gcd(row, block);
+    if (g == 0 || (block / g < rows && row / g < blocks))
+        return set_error(CONVNN_E_INVALID, "%s: strides %lld, %lld of %lld x %lld scales that are written", what, (long long)row,
+                         (long long)block, (long long)rows, (long long)blocks);
     return CONVNN_OK;
 }
 
@@ -571,7 +583,7 @@ static int rms_norm_impl(const char* what, int dtype, const void* x, int64_t ldx
          reinterpret_cast<uintptr_t>(sum) | reinterpret_cast<uintptr_t>(y)) & elt)
         return set_error(CONVNN_E_ALIGN, "%s: a pointer is not aligned to its type", what);
     int rc;
-    if (q && (rc = scales_ok(what, scales, scale_row, scale_block, true))) return rc;
+    if (q && (rc = written_scales_ok(what, scales, scale_row, scale_block, rows, (D + 127) / 128))) return rc;
     if ((rc = check_device())) return rc;
     if (rows == 0) return CONVNN_OK;
     return launch_rms_norm(dtype, x, ldx, residual, ldr, weight, eps, sum, lds, y, q, ldy, scales, scale_row, scale_block, rows, D,
@@ -601,7 +613,8 @@ int convnn_b200_quantize_fp8(int dtype, const void* x, int64_t ldx, int32_t bloc
         return set_error(CONVNN_E_INVALID, "quantize_fp8: a scale belongs to 1 or 128 rows, not %d", block_rows);
     if (reinterpret_cast<uintptr_t>(x) & (dtype == CONVNN_F32 ? 3u : 1u))
         return set_error(CONVNN_E_ALIGN, "quantize_fp8: x is not aligned to its type");
-    int rc = scales_ok("quantize_fp8", scales, scale_row, scale_block, true);
+    int rc = written_scales_ok("quantize_fp8", scales, scale_row, scale_block, block_rows == 1 ? rows : rows / 128 + (rows % 128 != 0),
+                               (D + 127) / 128);
     if (rc || (rc = check_device())) return rc;
     if (rows == 0) return CONVNN_OK;
     return launch_quantize_fp8(dtype, x, ldx, block_rows, q, ldq, scales, scale_row, scale_block, rows, D,
@@ -625,9 +638,9 @@ int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, in
          (out_scales ? (uintptr_t)0 : reinterpret_cast<uintptr_t>(out))) & elt)
         return set_error(CONVNN_E_ALIGN, "linear_fp8: a pointer is not aligned to its type");
     int rc;
-    if ((rc = scales_ok("linear_fp8: a", a_scales, a_scale_row, a_scale_block, false)) ||
-        (rc = scales_ok("linear_fp8: w", w_scales, w_scale_row, w_scale_block, false)) ||
-        (out_scales && (rc = scales_ok("linear_fp8: out", out_scales, out_scale_row, out_scale_block, true))))
+    if ((rc = scales_ok("linear_fp8: a", a_scales, a_scale_row, a_scale_block)) ||
+        (rc = scales_ok("linear_fp8: w", w_scales, w_scale_row, w_scale_block)) ||
+        (out_scales && (rc = written_scales_ok("linear_fp8: out", out_scales, out_scale_row, out_scale_block, M, (N + 127) / 128))))
         return rc;
     if ((rc = check_device())) return rc;
     if (M == 0) return CONVNN_OK;

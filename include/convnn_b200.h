@@ -232,9 +232,9 @@ int convnn_b200_linear(int dtype, const void* a, int64_t lda, const void* w, con
  * stored as q and means q * scale, with scale = max(amax|block| / 448, 2^-126), q = e4m3(v / scale)
  * (rounded to nearest even).  A block is 128 neighbouring channels (the last one of a row may be
  * shorter) of one row, or of 128 rows in a weight.  scales[row_block * *_scale_row + channel_block *
- * *_scale_block]: strides in elements, any order; the kernels read and write them fastest where
- * the scales of neighbouring rows lie side by side.  A block that holds a NaN or an infinity means
- * NaN throughout.  Row counts may be 0. */
+ * *_scale_block]: strides in elements, any order (written ones: no two at one address); the
+ * kernels read and write them fastest where the scales of neighbouring rows lie side by side.  A
+ * block that holds a NaN or an infinity means NaN throughout.  Row counts may be 0. */
 
 /* y = s * (mean(s^2) + eps)^-1/2 * weight over the last dimension, s = x or, with a residual, x +
  * residual rounded to dtype, which is then also written to `sum` (both or neither NULL).  rows x D,
