@@ -624,9 +624,14 @@ def _fp8_empty(shape, rows: int, device) -> Tuple[torch.Tensor, int, torch.Tenso
     return values, ld, scales
 
 
+MOST_CHANNELS = 1 << 30                          # (the kernels count channels in 32 bits, rows in 64)
+
+
 def _channels(shape, what: str) -> int:
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"{what} needs a last dimension of at least one channel, got shape {tuple(shape)}")
+    if shape[-1] > MOST_CHANNELS:
+        raise ValueError(f"{what} takes up to 2^30 channels, got shape {tuple(shape)}")
     return shape[-1]
 
 
@@ -741,6 +746,8 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     K = _channels(shape, "linear_fp8")
     if len(wshape) != 2 or wshape[1] != K or wshape[0] < 1:
         raise ValueError(f"w must be (N, {K}), got {tuple(wshape)}")
+    if wshape[0] > MOST_CHANNELS:
+        raise ValueError(f"linear_fp8 takes up to 2^30 output channels, got {tuple(wshape)}")
     N, blocks, lead = wshape[0], -(-K // FP8_BLOCK), shape[:-1]
     if sa.shape != (*lead, blocks):
         raise ValueError(f"the scales of a must have shape {(*lead, blocks)}, got {tuple(sa.shape)}")
