@@ -735,7 +735,7 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
         return done
     (av, sa), (wv, sw) = a, w
     if torch.is_grad_enabled():
-        _forward_only(bias, residual, sa, sw)
+        _forward_only(av, sa, wv, sw, bias, residual)
     index = _device_of(av, sa, wv, sw, bias, residual)
     io = _dtype_code(dtype)
     if av.dtype is not _E4M3 or wv.dtype is not _E4M3:

@@ -62,3 +62,18 @@ def test_widths_that_no_32_bit_argument_holds(on_any_device, over):
         ops.rms_norm(meta(2, 1 << 30), meta(1 << 30))
         ops.quantize_fp8(meta(1 << 33, 8))                   # (rows are counted in 64 bits)
     assert len(on_any_device) == 2
+
+
+@pytest.mark.parametrize("which", ["a", "a scales", "w", "w scales", "bias", "residual"])
+def test_a_product_of_what_wants_a_gradient(which):
+    t = {"a": torch.zeros(2, 16).to(torch.float8_e4m3fn), "a scales": torch.ones(2, 1), "w": torch.zeros(8, 16).to(torch.float8_e4m3fn),
+         "w scales": torch.ones(1, 1), "bias": torch.zeros(8), "residual": torch.zeros(2, 8)}
+    t[which].requires_grad_()
+
+    def call():
+        return ops.linear_fp8((t["a"], t["a scales"]), (t["w"], t["w scales"]), bias=t["bias"], residual=t["residual"], dtype=torch.float32)
+
+    with pytest.raises(RuntimeError, match="forward-only"):
+        call()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        call()
