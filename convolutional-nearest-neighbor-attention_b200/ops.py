@@ -729,7 +729,7 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     """``[GELU](a @ w.T + bias) [+ residual]`` of 8-bit tensors: ``a`` (values (..., K), scales per row) and ``w`` (values (N, K),
     scales per 128 x 128 block), each an ``Fp8Blocks`` or such a pair.  bias (N) and residual (..., N) in ``dtype`` (float32 or
     bfloat16).  -> (..., N) in ``dtype``, summed in float32 and rounded once, or with ``quantize`` as ``Fp8Blocks`` for the
-    next product."""
+    next product.  The product of a block's two scales has to be a normal float32 or zero."""
     done = (_calls or _bind_calls()).linear_fp8(a, w, bias, gelu, residual, 1 if dtype is _BF16 else 0 if dtype is _F32 else -1, quantize)
     if done is not None:
         return done

@@ -259,6 +259,8 @@ int convnn_b200_quantize_fp8(int dtype, const void* x, int64_t ldx, int32_t bloc
  * float32, one rounding at the store.  bias (N) and residual (M, N) in dtype, or NULL.  out (M, N) in
  * dtype or, where out_scales is given, in 8 bits with a scale per row and 128 columns (the next
  * product's a).  Rows of a and w must start on 16-byte boundaries (lda, ldw multiples of 16).
+ * A block's sum is multiplied by its two scales' product, which has to be a normal float32 or zero: a
+ * larger one makes the block infinite (NaN where its sum is zero), a smaller one loses bits.
  * out may be the residual itself, nothing else of the inputs. */
 int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, int64_t a_scale_row,
                            int64_t a_scale_block, const void* w, int64_t ldw, const float* w_scales,
