@@ -41,7 +41,8 @@ struct LinearFp8Params {
     int out_kind, io, gelu;               // io: convnn_dtype of bias, residual (and out)
     int stages, splits;                   // CTAs of the cluster
     bool bias16, residual16, out16;       // their rows start on 16-byte boundaries
-    bool residual4, out4;                 // on 4-byte boundaries (and N is even: two bfloat16 values at a time)
+    bool out_tma;                         // and those of out end on one: a copy by TMA writes on to it, over what lies behind the last column
+    bool residual4, out4;                 // on 4-byte boundaries (residual: and N is even, two bfloat16 values at a time)
 };
 
 __device__ __forceinline__ void fail(volatile int* abort_flag, int code) {
@@ -505,7 +506,7 @@ int launch_tiles(const CUtensorMap& tmP, const CUtensorMap& tmQ, LinearFp8Params
 //   warps 2, 3  the scales of four blocks of k at a time
 //   warps 4-11  epilogue: a warp has 32 rows and 128 columns, its sums in registers (128 of 224), and after the last block bias, GELU,
 //               residual, rounding; the results leave through its two slabs of shared memory, 32 rows of 128 bytes in the order
-//               of the 128-byte swizzle, by TMA where rows start on 16-byte boundaries.  Meanwhile the next tile's first two
+//               of the 128-byte swizzle, by TMA where rows start and end on 16-byte boundaries.  Meanwhile the next tile's first two
 //               blocks are multiplied.
 // Twelve warps are launched with 168 registers a thread; the first four keep 56, which leaves the others 224: 4 * 32 * 56 + 8 * 32 * 224
 // = 12 * 32 * 168.
@@ -613,15 +614,15 @@ __device__ __forceinline__ void rows_to_slab(const T* base, long long ld, int M,
             }
     }
 }
-template <typename T, int B>
+template <typename T>
 __device__ __forceinline__ void slab_to_rows(T* base, long long ld, int M, int N, long long m0, int n, uint32_t slab, int lane) {
-    using E = typename Bytes<T, B>::type;
-    constexpr int U = 4 / B;
+    using E = typename Bytes<T, sizeof(T)>::type;
+    constexpr int B = sizeof(T), U = 4 / B;
 #pragma unroll 4
     for (int r = 0; r < 32; ++r)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int at = (32 * u + lane) * B, col = n + at / (int)sizeof(T);
+            const int at = (32 * u + lane) * B, col = n + 32 * u + lane;
             const uint32_t from = slab_at(slab, r, at >> 4) + (at & 15);
             E v;
             if constexpr (B == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(reinterpret_cast<uint32_t&>(v)) : "r"(from) : "memory");
@@ -633,6 +634,40 @@ __device__ __forceinline__ void slab_to_rows(T* base, long long ld, int M, int N
             }
             if (m0 + r < M && col < N) *reinterpret_cast<E*>(base + (m0 + r) * ld + col) = v;
         }
+}
+// The same for rows on 4-byte boundaries: two bfloat16 values a lane, or the last of a row.
+__device__ __forceinline__ void slab_to_rows4(__nv_bfloat16* base, long long ld, int M, int N, long long m0, int n, uint32_t slab, int lane) {
+    const int col = n + 2 * lane;
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(slab_at(slab, r, lane >> 2) + ((4 * lane) & 15)) : "memory");
+        __nv_bfloat16* to = base + (m0 + r) * ld + col;
+        if (m0 + r >= M || col >= N) continue;
+        if (col + 1 < N) *reinterpret_cast<uint32_t*>(to) = v;
+        else *reinterpret_cast<uint16_t*>(to) = (uint16_t)v;
+    }
+}
+// 8-bit rows on 16-byte boundaries: sixteen a lane, the last of a row in smaller pieces.  (50432 x 1000 x 768 into 8 bits 72 us, four a lane 82;
+// by TMA, over what lies behind, 63.  The whole slabs of a row by TMA and this for its last: 70, but 28.7 instead of 27.9 for 768 columns.)
+__device__ __forceinline__ void slab_to_rows16(uint8_t* base, long long ld, int M, int N, long long m0, int n, uint32_t slab, int lane) {
+    const int left = N - n - 16 * (lane & 7);
+    uint8_t* to = base + (m0 + (lane >> 3)) * ld + n + 16 * (lane & 7);
+#pragma unroll 2
+    for (int r = lane >> 3; r < 32; r += 4, to += 4 * ld) {
+        const uint4 v = lds128(slab_at(slab, r, lane & 7));
+        if (m0 + r >= M || left <= 0) continue;
+        if (left >= 16) {
+            *reinterpret_cast<uint4*>(to) = v;
+        } else {
+            uint32_t w[3] = {v.x, v.y, v.z};
+            uint8_t* p = to;
+            if (left & 8) { *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]); w[0] = w[2]; w[1] = v.w; p += 8; }
+            if (left & 4) { *reinterpret_cast<uint32_t*>(p) = w[0]; w[0] = w[1]; p += 4; }
+            if (left & 2) { *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0]; w[0] >>= 16; p += 2; }
+            if (left & 1) *p = (uint8_t)w[0];
+        }
+    }
 }
 
 // The residual of 32 rows and 128 bytes of columns from column n on into the slab: asked for here, there after residual_arrived().
@@ -671,7 +706,7 @@ __device__ __forceinline__ void add_row(uint32_t slab, int lane, float* acc) {
 // The slab's 32 rows of 128 bytes -> out, from column n on.
 template <typename T>
 __device__ __forceinline__ void store_slab(const LinearFp8Params& p, const CUtensorMap* tmO, long long m0, int n, uint32_t slab, int lane) {
-    if (p.out16) {
+    if (p.out_tma) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0 && m0 < p.M && n < p.N) tma_store_2d_a(tmO, slab, n, (int)m0);
@@ -680,8 +715,15 @@ __device__ __forceinline__ void store_slab(const LinearFp8Params& p, const CUten
     }
     __syncwarp();
     T* out = static_cast<T*>(p.out);
-    if (sizeof(T) == 2 && p.out4) slab_to_rows<T, sizeof(T) == 2 ? 4 : sizeof(T)>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
-    else slab_to_rows<T, sizeof(T)>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+    if constexpr (sizeof(T) == 1) {
+        if (p.out16) slab_to_rows16(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+        else slab_to_rows<T>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+    } else if constexpr (sizeof(T) == 2) {
+        if (p.out4) slab_to_rows4(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+        else slab_to_rows<T>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+    } else {
+        slab_to_rows<T>(out, p.ldo, p.M, p.N, m0, n, slab, lane);
+    }
     __syncwarp();
 }
 
@@ -1050,8 +1092,8 @@ linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 
 template <int OUT, bool GELU>
 int launch_pairs(const CUtensorMap& tmA, const CUtensorMap& tmW, const LinearFp8Params& p, cudaStream_t st) {
-    CUtensorMap tmO = tmA;                                   // (unused where rows of the output start anywhere)
-    if (p.out16) {
+    CUtensorMap tmO = tmA;                                   // (unused where rows of the output start or end anywhere)
+    if (p.out_tma) {
         const int elt = OUT == OUT_F32 ? 4 : OUT == OUT_BF16 ? 2 : 1;
         const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.M}, strides[1] = {(uint64_t)p.ldo * elt};
         const uint32_t box[2] = {(uint32_t)(128 / elt), 32};
@@ -1107,7 +1149,7 @@ int launch_linear_fp8(const void* a, long long lda, const float* sa, long long s
     auto on = [](const void* q, long long ld_bytes, int n) { return ((uintptr_t)ld_bytes | reinterpret_cast<uintptr_t>(q)) % n == 0; };
     p.bias16 = on(bias, 0, 16);
     p.residual16 = on(residual, ldr * elt, 16); p.residual4 = on(residual, ldr * elt, 4) && N % 2 == 0;
-    p.out16 = on(out, ldo * out_elt, 16); p.out4 = on(out, ldo * out_elt, 4) && N % 2 == 0;
+    p.out16 = on(out, ldo * out_elt, 16); p.out_tma = p.out16 && N * out_elt % 16 == 0; p.out4 = on(out, ldo * out_elt, 4);
     const long long pair_tiles = (long long)((M + 2 * BP - 1) / (2 * BP)) * ((N + PAIR_N - 1) / PAIR_N);
     // Pairs from a tile per five SMs on: 512 x 4096 x 4096 (32 tiles) 31.4 -> 24.2 us, 3152 x 768 x 768 (39) 10.9 -> 9.0; with fewer the
     // clusters that share a tile's sum are faster (256 x 4096 x 4096, 16 tiles: 16.7 against 23.6).  Up to 128 rows half a tile is empty.
