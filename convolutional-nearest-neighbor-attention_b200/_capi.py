@@ -50,6 +50,28 @@ class ConvnnModel(ctypes.Structure):
                                        "pixel_inv_std", "head_w", "head_b")])
 
 
+class ConvnnHeads(ctypes.Structure):
+    """Mirror of ``struct convnn_heads``."""
+    _fields_ = ([(n, c_i32) for n in ("dtype", "B", "T", "Hq", "Hk", "D", "rotary", "interleaved", "rope_rows")] +
+                [("eps", ctypes.c_float)] + [(n, c_void) for n in ("q", "k", "v")] +
+                [(n, c_i64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("q_weight", c_void), ("k_weight", c_void),
+                 ("rope", c_void), ("rope_stride", c_i64), ("positions", c_void), ("position_stride", c_i64 * 2),
+                 ("q_out", c_void), ("k_out", c_void), ("q_out_stride", c_i64 * 3), ("k_out_stride", c_i64 * 3)])
+
+
+class ConvnnCache(ctypes.Structure):
+    """Mirror of ``struct convnn_cache``."""
+    _fields_ = [("k", c_void), ("v", c_void), ("k_stride", c_i64 * 3), ("v_stride", c_i64 * 3), ("table", c_void),
+                ("table_stride", c_i64), ("pages", c_i32), ("page_size", c_i32), ("width", c_i32)]
+
+
+class ConvnnTreeAttention(ctypes.Structure):
+    """Mirror of ``struct convnn_tree_attention``."""
+    _fields_ = ([(n, c_i32) for n in ("dtype", "B", "T", "Hq", "Hk", "D")] +
+                [("scale", ctypes.c_float), ("q", c_void), ("q_stride", c_i64 * 3), ("lengths", c_void), ("counts", c_void),
+                 ("tree", c_void), ("tree_stride", c_i64 * 2), ("out", c_void), ("out_stride", c_i64 * 3)])
+
+
 # name -> (restype, argtypes); must list every symbol the header declares
 SIGNATURES = {
     "convnn_b200_abi_version": (ctypes.c_int, []),
@@ -89,6 +111,11 @@ SIGNATURES = {
     "convnn_b200_linear_fp8": (ctypes.c_int, [c_void, c_i64, c_void, c_i64, c_i64, c_void, c_i64, c_void, c_i64, c_i64,
                                               ctypes.c_int, c_void, c_void, c_i64, c_void, c_i64, c_void, c_i64, c_i64, c_i64,
                                               c_i32, c_i32, c_i32, c_void]),
+    "convnn_b200_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(ConvnnHeads), c_void]),
+    "convnn_b200_append_kv": (ctypes.c_int, [ctypes.POINTER(ConvnnHeads), ctypes.POINTER(ConvnnCache), c_void, c_void, c_void]),
+    "convnn_b200_tree_attention_workspace_bytes": (c_size, [ctypes.c_int, c_i32, c_i32, c_i32, c_i32]),
+    "convnn_b200_tree_attention": (ctypes.c_int, [ctypes.POINTER(ConvnnTreeAttention), ctypes.POINTER(ConvnnCache), c_void, c_size,
+                                                  c_void]),
     "convnn_b200_patchify": (ctypes.c_int, [ctypes.c_int, c_void, c_void, c_i32, c_i32, c_i32, c_i32, c_i32, c_void]),
     "convnn_b200_patchify_u8": (ctypes.c_int, [ctypes.c_int, c_void, c_void, c_void, c_void, c_i32, c_i32, c_i32, c_i32,
                                                c_i32, c_void]),

@@ -1,6 +1,7 @@
 // extern "C" surface of libconvnn_b200: argument validation, workspace carving and the
 // chaining of the stage kernels on the caller's stream.
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <numeric>
 #include <stdarg.h>
@@ -647,6 +648,108 @@ int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, in
     return launch_linear_fp8(a, lda, a_scales, a_scale_row, a_scale_block, w, ldw, w_scales, w_scale_row, w_scale_block, bias,
                              residual, ldr, dtype, out, ldo, out_scales, out_scale_row, out_scale_block, (int)M, N, K, gelu,
                              static_cast<cudaStream_t>(stream));
+}
+
+// ---- heads, a paged cache, and attention over it ----------------------------------------------------
+
+constexpr int kMostHeadChannels = 256;
+
+static int cache_ok(const char* what, const convnn_cache* c, uintptr_t elt) {
+    if (!c) return set_error(CONVNN_E_NULL, "%s: argument 'cache' is NULL", what);
+    if (!c->k || !c->v || (!c->table && c->width)) return set_error(CONVNN_E_NULL, "%s: a required pointer is NULL", what);
+    if (c->pages < 1 || c->page_size < 1 || c->width < 0 || c->table_stride < 0)
+        return set_error(CONVNN_E_INVALID, "%s: %d pages of %d entries, %d a sequence", what, c->pages, c->page_size, c->width);
+    if ((int64_t)c->width * c->page_size > (1 << 30))
+        return set_error(CONVNN_E_UNSUPPORTED, "%s: more than 2^30 entries a sequence", what);
+    for (int i = 0; i < 3; ++i)
+        if (c->k_stride[i] < 0 || c->v_stride[i] < 0) return set_error(CONVNN_E_INVALID, "%s: negative strides", what);
+    if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & (elt - 1)) ||
+        (reinterpret_cast<uintptr_t>(c->table) & 3u))
+        return set_error(CONVNN_E_ALIGN, "%s: a pointer is not aligned to its type", what);
+    return CONVNN_OK;
+}
+
+static int heads_ok(const char* what, const convnn_heads* h) {
+    if (!h) return set_error(CONVNN_E_NULL, "%s: argument 'heads' is NULL", what);
+    if (h->dtype != CONVNN_F32 && h->dtype != CONVNN_BF16) return set_error(CONVNN_E_INVALID, "unknown dtype %d", h->dtype);
+    if (h->B < 0 || h->T < 0 || h->D < 1 || (h->q && h->Hq < 1) || (h->k && h->Hk < 1))
+        return set_error(CONVNN_E_INVALID, "%s: bad shape", what);
+    if (h->D > kMostHeadChannels)
+        return set_error(CONVNN_E_UNSUPPORTED, "%s: %d channels a head, up to %d are", what, h->D, kMostHeadChannels);
+    if ((int64_t)h->B * h->T > (1ll << 30)) return set_error(CONVNN_E_UNSUPPORTED, "%s: more than 2^30 tokens", what);
+    if ((h->q ? h->Hq : 0) > (1 << 20) || (h->k ? h->Hk : 0) > (1 << 20))
+        return set_error(CONVNN_E_UNSUPPORTED, "%s: more than 2^20 heads", what);
+    if (!(h->eps >= 0.f)) return set_error(CONVNN_E_INVALID, "%s: eps must not be negative", what);
+    if (h->rope && (h->rotary < 2 || h->rotary % 2 || h->rotary > h->D || h->rope_rows < 0 || h->rope_stride < h->rotary))
+        return set_error(CONVNN_E_INVALID, "%s: %d channels of %d turned by a table of %d rows", what, h->rotary, h->D, h->rope_rows);
+    if (h->position_stride[0] < 0 || h->position_stride[1] < 0) return set_error(CONVNN_E_INVALID, "%s: negative strides", what);
+    const uintptr_t elt = h->dtype == CONVNN_F32 ? 3u : 1u;
+    if (((reinterpret_cast<uintptr_t>(h->q) | reinterpret_cast<uintptr_t>(h->k) | reinterpret_cast<uintptr_t>(h->v) |
+          reinterpret_cast<uintptr_t>(h->q_weight) | reinterpret_cast<uintptr_t>(h->k_weight) |
+          reinterpret_cast<uintptr_t>(h->q_out) | reinterpret_cast<uintptr_t>(h->k_out)) & elt) ||
+        ((reinterpret_cast<uintptr_t>(h->rope) | reinterpret_cast<uintptr_t>(h->positions)) & 3u))
+        return set_error(CONVNN_E_ALIGN, "%s: a pointer is not aligned to its type", what);
+    return CONVNN_OK;
+}
+
+int convnn_b200_qk_norm_rope(const convnn_heads* heads, void* stream) {
+    int rc = heads_ok("qk_norm_rope", heads);
+    if (rc) return rc;
+    if ((!heads->q && !heads->k) || !heads->q != !heads->q_out || !heads->k != !heads->k_out)
+        return set_error(CONVNN_E_NULL, "qk_norm_rope: queries or keys, each with room for its result");
+    if ((rc = check_device())) return rc;
+    if (heads->B == 0 || heads->T == 0) return CONVNN_OK;
+    return launch_heads(heads, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int convnn_b200_append_kv(const convnn_heads* heads, const convnn_cache* cache, const int32_t* lengths, const int32_t* counts,
+                          void* stream) {
+    int rc = heads_ok("append_kv", heads);
+    if (rc || (rc = cache_ok("append_kv", cache, heads->dtype == CONVNN_F32 ? 4u : 2u))) return rc;
+    REQUIRE_PTR(lengths);
+    if (!heads->k || !heads->v || !heads->q != !heads->q_out)
+        return set_error(CONVNN_E_NULL, "append_kv: keys, values, and queries with room for their result");
+    if ((reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(counts)) & 3u)
+        return set_error(CONVNN_E_ALIGN, "append_kv: lengths and counts are int32");
+    if ((rc = check_device())) return rc;
+    if (heads->B == 0 || heads->T == 0) return CONVNN_OK;
+    return launch_heads(heads, cache, lengths, counts, static_cast<cudaStream_t>(stream));
+}
+
+size_t convnn_b200_tree_attention_workspace_bytes(int dtype, int32_t T, int32_t Hq, int32_t Hk, int32_t D) {
+    if (T < 1 || T > 64 || Hk < 1 || Hq < Hk || Hq % Hk || D < 1 || D > kMostHeadChannels) return 0;
+    return tree_attention_workspace(dtype, T, Hq / Hk, D);
+}
+
+int convnn_b200_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    REQUIRE_PTR(a);
+    if (a->dtype != CONVNN_F32 && a->dtype != CONVNN_BF16) return set_error(CONVNN_E_INVALID, "unknown dtype %d", a->dtype);
+    const int V = a->dtype == CONVNN_F32 ? 4 : 8;                  // values in 16 bytes
+    int rc = cache_ok("tree_attention", cache, 16);
+    if (rc) return rc;
+    if (!a->q || !a->out || !a->lengths) return set_error(CONVNN_E_NULL, "tree_attention: a required pointer is NULL");
+    if (a->B < 0 || a->T < 0 || a->Hk < 1 || a->Hq < 1 || a->Hq % a->Hk || a->D < 1)
+        return set_error(CONVNN_E_INVALID, "tree_attention: %d query heads over %d key heads of %d channels", a->Hq, a->Hk, a->D);
+    if (a->T > 64) return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %d drafted tokens, up to 64 are", a->T);
+    if (a->D > kMostHeadChannels)
+        return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %d channels a head, up to %d are", a->D, kMostHeadChannels);
+    if (!std::isfinite(a->scale)) return set_error(CONVNN_E_INVALID, "tree_attention: the scale is not finite");
+    if (a->Hq > (1 << 20)) return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: more than 2^20 heads");
+    bool rows = a->D % V == 0 && aligned16(a->q) && aligned16(a->out);
+    for (int i = 0; i < 3; ++i) {
+        rows = rows && a->q_stride[i] % V == 0 && a->out_stride[i] % V == 0 && cache->k_stride[i] % V == 0 && cache->v_stride[i] % V == 0;
+        if (a->q_stride[i] < 0 || a->out_stride[i] < 0) return set_error(CONVNN_E_INVALID, "tree_attention: negative strides");
+    }
+    if (!rows) return set_error(CONVNN_E_ALIGN, "tree_attention: rows of q, out and the cache must start on 16-byte boundaries");
+    if (a->tree_stride[0] < 0 || a->tree_stride[1] < 0) return set_error(CONVNN_E_INVALID, "tree_attention: negative strides");
+    if (((reinterpret_cast<uintptr_t>(a->lengths) | reinterpret_cast<uintptr_t>(a->counts)) & 3u) ||
+        (reinterpret_cast<uintptr_t>(a->tree) & 7u) || !aligned16(workspace))
+        return set_error(CONVNN_E_ALIGN, "tree_attention: a pointer is not aligned to its type");
+    if ((rc = check_device())) return rc;
+    if (a->B == 0 || a->T == 0) return CONVNN_OK;
+    REQUIRE_PTR(workspace);
+    return launch_tree_attention(a, cache, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 // ---- LayerNorm folded into the GEMM that consumes it ----------------------------------------------

@@ -326,6 +326,11 @@ int launch_linear_fp8(const void* a, long long lda, const float* sa, long long s
                       long long ldr, int io, void* out, long long ldo, float* so, long long so_row, long long so_block, int M, int N,
                       int K, int gelu, cudaStream_t st);
 int read_linear_fp8_status(int* out);
+// Heads normed and turned (qk_norm_rope.cu), with a cache into its pages.
+int launch_heads(const convnn_heads* h, const convnn_cache* cache, const int32_t* lengths, const int32_t* counts, cudaStream_t st);
+size_t tree_attention_workspace(int dtype, int T, int G, int D);
+int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace, size_t workspace_bytes,
+                          cudaStream_t st);
 int launch_row_moments(const void* x, long long ldx, long long rows, int D, float* moments, cudaStream_t st);
 int launch_fold_layernorm(const void* w, const void* bias, const void* gamma, const void* beta, int N, int K,
                           void* w_folded, void* w_extra, cudaStream_t st);

@@ -1,0 +1,160 @@
+// What the kernels of attention over a paged cache share: the call's parameters, the work's division among CTAs and the places of what
+// they hand on to one another.
+//
+// A unit is a tile of query rows (row = token * group + head of the group) of one sequence and key head; its keys come in tiles.  Tiles of
+// all units, in order, are divided evenly among the CTAs, whatever the sequences' lengths: they are on the device, and the host never
+// learns them.  A unit whose tiles belong to several CTAs is joined from their unnormalised sums by a second kernel, which also writes the
+// rows that no unit has (tokens behind a sequence's count, nothing to attend to).  The order of every sum is the division's, so that
+// results do not change from run to run.
+#pragma once
+
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace convnn {
+namespace paged {
+
+struct Params {
+    const void *q, *k, *v;
+    void* out;
+    long long qs[3], os[3];                      // batch, token, head
+    long long ks[3], vs[3];                      // page, head, row
+    const int32_t *table, *lengths, *counts;
+    const long long* tree;                       // (B, T) masks, nullptr: a chain
+    long long table_stride, tree_stride[2];
+    int B, T, Hk, G, D, pages, page_size, width;
+    int row_tiles, rows_per_tile, tile;          // of T * G rows; keys per tile
+    float scale_log2;                            // scale * log2(e)
+    float* partial;                              // [2 * CTAs][rows_per_tile * (D + 2) + 4]
+    long long slot;                              // floats of one of them
+    int ctas;
+};
+
+// One sequence.
+struct Sequence {
+    int length, count, total;                    // cached entries, drafted tokens, both (as far as the table goes)
+    int tiles, row_tiles;                        // of keys; of rows that are there
+    __device__ __forceinline__ int work() const { return tiles * row_tiles; }
+};
+__device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
+    Sequence s;
+    const int room = p.width * p.page_size;      // (at most 2^30)
+    s.length = min(max(p.lengths[b], 0), room);
+    s.count = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    s.total = s.count ? min(s.length + s.count, room) : 0;
+    s.tiles = (s.total + p.tile - 1) / p.tile;
+    s.row_tiles = (s.count * p.G + p.rows_per_tile - 1) / p.rows_per_tile;
+    return s;
+}
+// Whole warp: tiles of all units, and of the sequences before b.
+__device__ __forceinline__ long long total_work(const Params& p, int b, long long& before) {
+    const int lane = threadIdx.x & 31;
+    long long all = 0, first = 0;
+    for (int i = lane; i < p.B; i += 32) {
+        const long long w = (long long)sequence_of(p, i).work() * p.Hk;
+        all += w;
+        if (i < b) first += w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        first += __shfl_xor_sync(0xffffffffu, first, o);
+    }
+    before = first;
+    return all;
+}
+// CTAs that get tiles, one at least each.
+__device__ __forceinline__ int busy_ctas(long long work, int ctas) { return work < ctas ? (int)work : ctas; }
+__device__ __forceinline__ long long first_tile(long long work, int cta, int ctas) { return work * cta / ctas; }
+// The CTA that has tile `at`.
+__device__ __forceinline__ int cta_of(long long work, long long at, int ctas) { return (int)(((at + 1) * ctas - 1) / work); }
+
+// A CTA's way through its tiles.
+struct Cursor {
+    Sequence s;
+    int b, h, rt, tile;
+    long long left;                              // tiles that are still to come, this one included
+
+    // Whole warp; the same in all lanes.
+    __device__ __forceinline__ void start(const Params& p, int cta, int ctas) {
+        const int lane = threadIdx.x & 31;
+        long long none;
+        const long long work = total_work(p, 0, none);
+        ctas = busy_ctas(work, ctas);
+        b = h = rt = tile = 0;
+        left = 0;
+        if (cta >= ctas) return;
+        const long long begin = first_tile(work, cta, ctas);
+        left = first_tile(work, cta + 1, ctas) - begin;
+        long long before = 0;
+        for (int b0 = 0;; b0 += 32) {
+            long long w = 0;
+            if (b0 + lane < p.B) w = (long long)sequence_of(p, b0 + lane).work() * p.Hk;
+            long long sum = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned found = __ballot_sync(0xffffffffu, before + sum > begin);
+            if (found) {
+                const int at = __ffs(found) - 1;
+                b = b0 + at;
+                before += __shfl_sync(0xffffffffu, sum - w, at);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        s = sequence_of(p, b);
+        const int rest = (int)(begin - before);          // (of one sequence: its heads' tiles fit 31 bits)
+        h = rest / s.work();
+        const int in_head = rest - h * s.work();
+        rt = in_head / s.tiles;
+        tile = in_head - rt * s.tiles;
+    }
+    __device__ __forceinline__ void next(const Params& p) {
+        if (--left == 0) return;
+        if (++tile < s.tiles) return;
+        tile = 0;
+        if (++rt < s.row_tiles) return;
+        rt = 0;
+        if (++h < p.Hk) return;
+        h = 0;
+        do s = sequence_of(p, ++b);
+        while (s.work() == 0);
+    }
+    __device__ __forceinline__ bool last_of_unit() const { return left == 1 || tile + 1 == s.tiles; }
+};
+
+// Mask of the drafted tokens that row r sees; rows that are not there see none.
+__device__ __forceinline__ unsigned long long seen_by(const Params& p, const Sequence& s, int b, int row) {
+    const int t = row / p.G;
+    if (t >= s.count) return 0;
+    if (!p.tree) return ~0ull >> (63 - t);
+    return (unsigned long long)p.tree[b * p.tree_stride[0] + t * p.tree_stride[1]];
+}
+
+// Values that are not finite do not stay in a product with zero: those of drafted tokens, which some rows see and others do not, are
+// taken out before it (a zero in their place) and added to the rows that see them here, at the end.
+template <typename T>
+__device__ __forceinline__ float not_finite_seen(const Params& p, const Sequence& s, int b, int h, unsigned long long mask, int c) {
+    float add = 0.f;
+    for (int j = 0; j < s.total - s.length; ++j) {
+        const int entry = s.length + j, slot = entry / p.page_size;
+        const int page = p.table[b * p.table_stride + slot];
+        if (!(mask >> j & 1) || (unsigned)page >= (unsigned)p.pages) continue;
+        const float v = to_f32(static_cast<const T*>(p.v)[page * p.vs[0] + h * p.vs[1] + (entry - slot * p.page_size) * p.vs[2] + c]);
+        if (!isfinite(v)) add += v;
+    }
+    return add;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace paged
+}  // namespace convnn

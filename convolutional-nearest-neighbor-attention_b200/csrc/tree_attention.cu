@@ -1,0 +1,692 @@
+// Attention of a tree of drafted tokens over a paged cache (one token per sequence: ordinary decoding).
+//   s_ij = scale * q_i . k_j over the cached entries j < length and those drafted tokens whose bit is set in i's mask
+//   out_i = sum_j 2^(s_ij log2(e) - m_i) v_j / sum_j 2^(s_ij log2(e) - m_i);  nothing to attend to: zeros
+// One pass over the keys with a running maximum and sum in float32.  The query heads that share a key head, for all of a sequence's
+// tokens, are the rows of one product, so that keys and values are read once.  With few rows reading them is all that takes time.
+//
+// rows_kernel (bfloat16): 16 rows on mma.sync.  Each of four warps walks every fourth slice of 16 keys by itself, copies of its next
+// slices in flight, and the four join at the unit's end: no barrier between slices.
+// scalar_kernel (float32): 16 rows, four to a warp, products on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA.
+// join_kernel: units that several CTAs had, and rows without anything.
+#include "paged_attention.cuh"
+
+namespace convnn {
+namespace {
+
+using namespace paged;
+
+constexpr int ROWS = 16, kThreads = 128, kWarps = 4;
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes, zeros where there is nothing to copy.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two values >= 0 as the next bfloat16 below them, and what is left as bfloat16: off by 2^-15 of the value (a step is 2^-7, half a step of
+// the rest 2^-8 of it).  Below, not nearest: neither part of a value above zero is zero or negative, so that an infinite value in the
+// product stays what it is.
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& rest) {
+    const uint32_t hx = max(__float_as_uint(x), 1u) - 1u, hy = max(__float_as_uint(y), 1u) - 1u;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x - __uint_as_float(hx & 0xffff0000u), y - __uint_as_float(hy & 0xffff0000u));
+    rest = *reinterpret_cast<const uint32_t*>(&lo);
+    return __byte_perm(hx, hy, 0x7632);
+}
+
+// The page that holds entry `entry` of sequence b, -1: none.
+__device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& row) {
+    const int slot = entry / p.page_size;
+    row = entry - slot * p.page_size;
+    const int page = p.table[b * p.table_stride + slot];
+    return (unsigned)page < (unsigned)p.pages ? page : -1;
+}
+
+// The partial sums of a CTA's unit: slot 0 if the CTA's first tile is in it, else 1.
+__device__ __forceinline__ float* slot_of(const Params& p, int cta, bool first) { return p.partial + (2ll * cta + !first) * p.slot; }
+
+// ---- bfloat16: 16 rows a tile on mma.sync ---------------------------------------------------------------------------------------
+
+// DS steps of 16 channels (D rounded up; the channels behind D are zeros), STAGES slices in flight per warp.
+template <int DS, int STAGES>
+__global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
+    constexpr int DP = 16 * DS, CH = DP / 8, PITCH = (CH | 1) * 16;      // an odd number of 16-byte columns: no bank conflicts
+    constexpr int SLICE = 16 * PITCH, STAGE = 2 * SLICE, OP = DP + 8;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* sQ = smem;                                                  // [16][PITCH]
+    float* sO = reinterpret_cast<float*>(sQ + SLICE);                    // [16][OP]: one warp's sums on their way to the next
+    float* sM = sO + ROWS * OP;                                          // [4][16] maxima
+    float* sL = sM + kWarps * ROWS;                                      // [16] sums
+    int* sBad = reinterpret_cast<int*>(sL + ROWS);
+    uint8_t* ring = reinterpret_cast<uint8_t*>(sBad + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t own = smem_at(ring) + warp * (STAGES * STAGE);
+
+    for (int i = threadIdx.x; i < (SLICE + kWarps * STAGES * STAGE) / 16; i += kThreads) {
+        uint8_t* at = i < SLICE / 16 ? sQ + 16 * i : ring + 16 * (i - SLICE / 16);
+        *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    chain_begin();
+
+    Cursor at;
+    at.start(p, blockIdx.x, p.ctas);
+    if (at.left == 0) return;                                            // (the whole CTA)
+    Cursor ahead = at;
+    const int chunks = p.D / 8;
+    const bool one_page = p.page_size % 16 == 0;                         // a slice lies in one page
+
+    // this warp's slice of ahead's tile into `stage`
+    auto fetch = [&](int stage) {
+        const int first = ahead.tile * 64 + warp * 16;
+        if (first < ahead.s.total) {
+            const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k) + ahead.h * p.ks[1];
+            const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v) + ahead.h * p.vs[1];
+            const uint32_t dst = own + stage * STAGE;
+            const int lr = lane & 15;
+            int row = 0, page = -1;
+            if (one_page || first + lr < ahead.s.total) page = page_of(p, ahead.b, one_page ? first : first + lr, row);
+            const bool there = page >= 0 && first + lr < ahead.s.total;
+            const long long kr = there ? page * p.ks[0] + (row + (one_page ? lr : 0)) * p.ks[2] : 0;
+            const long long vr = there ? page * p.vs[0] + (row + (one_page ? lr : 0)) * p.vs[2] : 0;
+#pragma unroll
+            for (int i = 0; i < DS; ++i) {
+                const int c = i * 32 + lane, r = c / CH, col = c - r * CH;
+                const long long ko = __shfl_sync(0xffffffffu, kr, r), vo = __shfl_sync(0xffffffffu, vr, r);
+                const bool copied = __shfl_sync(0xffffffffu, (int)there, r);
+                if (col < chunks) {
+                    copy16(dst + r * PITCH + col * 16, k + ko + col * 8, copied);
+                    copy16(dst + SLICE + r * PITCH + col * 16, v + vo + col * 8, copied);
+                }
+            }
+        }
+        copies_end();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (ahead.left > 0) { fetch(i); ahead.next(p); }
+        else copies_end();
+    }
+
+    const uint32_t q_at = smem_at(sQ) + (lane & 15) * PITCH + (lane >> 4) * 16;
+    const uint32_t k_lane = ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
+    const uint32_t v_lane = ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
+    int stage = 0;
+    bool first_unit = true;
+    while (at.left > 0) {
+        // ---- a unit: its rows
+        const Sequence s = at.s;
+        const int b = at.b, h = at.h, row0 = at.rt * ROWS, tile0 = at.tile;
+        for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
+            const int r = i / chunks, col = i - r * chunks, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (t < s.count)
+                v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + b * p.qs[0] + t * p.qs[1] +
+                                                    (h * p.G + g) * p.qs[2] + col * 8);
+            *reinterpret_cast<uint4*>(sQ + r * PITCH + col * 16) = v;
+        }
+        if (threadIdx.x == 0) *sBad = 0;
+        const unsigned long long mask0 = seen_by(p, s, b, row0 + lane / 4), mask1 = seen_by(p, s, b, row0 + lane / 4 + 8);
+        __syncthreads();
+        float o[2 * DS][4], m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2 * DS; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+        bool bad = false, end, at_end;
+        do {
+            // ---- a tile: this warp's slice of it
+            if (ahead.left > 0) {
+                fetch(stage == 0 ? STAGES - 1 : stage - 1);
+                ahead.next(p);
+            } else {
+                copies_end();
+            }
+            copies_wait<STAGES - 1>();
+            __syncwarp();
+            const int first = at.tile * 64 + warp * 16;
+            if (first < s.total) {
+                const uint32_t sk = own + stage * STAGE + k_lane, sv = own + stage * STAGE + SLICE + v_lane;
+                float c[2][4] = {};
+#pragma unroll
+                for (int d = 0; d < DS; ++d) {
+                    uint32_t qa[4], kb[4];
+                    ldsm4(qa, q_at + d * 32);
+                    ldsm4(kb, sk + d * 32);
+                    mma(c[0], qa, kb[0], kb[1]);
+                    mma(c[1], qa, kb[2], kb[3]);
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[n][e] *= p.scale_log2;
+                if (first + 16 > s.length) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = first + n * 8 + (lane & 3) * 2 + (e & 1) - s.length;
+                            const bool seen = j < 0 || (j < s.total - s.length && ((e < 2 ? mask0 : mask1) >> j & 1));
+                            if (!seen) c[n][e] = -CUDART_INF_F;
+                        }
+                    // what is not finite among the drafted tokens' values: a zero in its place, for now
+                    const int lr = lane & 15;
+                    if (first + lr >= s.length) {
+                        uint8_t* row = ring + warp * (STAGES * STAGE) + stage * STAGE + SLICE + lr * PITCH;
+                        for (int col = lane >> 4; col < chunks; col += 2) {
+                            uint4* w = reinterpret_cast<uint4*>(row + col * 16);
+                            uint32_t x[4] = {w->x, w->y, w->z, w->w};
+                            bool hit = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if ((x[e] & 0x7f80u) == 0x7f80u) { x[e] &= 0xffff0000u; hit = true; }
+                                if ((x[e] & 0x7f800000u) == 0x7f800000u) { x[e] &= 0xffffu; hit = true; }
+                            }
+                            if (hit) {
+                                *w = make_uint4(x[0], x[1], x[2], x[3]);
+                                bad = true;
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+                float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+#pragma unroll
+                for (int w = 1; w <= 2; w <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, w));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, w));
+                }
+                if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                    const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
+                    m0 = n0; m1 = n1;
+                    l0 *= f0; l1 *= f1;
+#pragma unroll
+                    for (int n = 0; n < 2 * DS; ++n) {
+                        o[n][0] *= f0; o[n][1] *= f0;
+                        o[n][2] *= f1; o[n][3] *= f1;
+                    }
+                }
+                const float z0 = m0 == -CUDART_INF_F ? 0.f : m0, z1 = m1 == -CUDART_INF_F ? 0.f : m1;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    c[n][0] = ex2(c[n][0] - z0); c[n][1] = ex2(c[n][1] - z0);
+                    c[n][2] = ex2(c[n][2] - z1); c[n][3] = ex2(c[n][3] - z1);
+                    l0 += c[n][0] + c[n][1];
+                    l1 += c[n][2] + c[n][3];
+                }
+                // The weights as the sum of two bfloat16: a rounding to one would cost as much as the result's own, and the second
+                // product is free while memory is what is waited for.
+                uint32_t pa[4], pr[4];
+                pa[0] = split2(c[0][0], c[0][1], pr[0]);
+                pa[1] = split2(c[0][2], c[0][3], pr[1]);
+                pa[2] = split2(c[1][0], c[1][1], pr[2]);
+                pa[3] = split2(c[1][2], c[1][3], pr[3]);
+#pragma unroll
+                for (int d = 0; d < DS; ++d) {
+                    uint32_t vb[4];
+                    ldsm4_t(vb, sv + d * 32);
+                    mma(o[2 * d], pa, vb[0], vb[1]);
+                    mma(o[2 * d + 1], pa, vb[2], vb[3]);
+                    mma(o[2 * d], pr, vb[0], vb[1]);
+                    mma(o[2 * d + 1], pr, vb[2], vb[3]);
+                }
+                __syncwarp();                                            // (the stage is filled again)
+            }
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            end = at.last_of_unit();
+            at_end = at.tile + 1 == s.tiles;
+            at.next(p);
+        } while (!end);
+
+        // ---- the four warps' sums: maxima first, then one after the other
+        if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(sBad, 1);
+#pragma unroll
+        for (int w = 1; w <= 2; w <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+        }
+        const int r0 = lane / 4, r1 = r0 + 8;
+        if ((lane & 3) == 0) {
+            sM[warp * ROWS + r0] = m0;
+            sM[warp * ROWS + r1] = m1;
+        }
+        __syncthreads();
+        float t0 = sM[r0], t1 = sM[r1];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            t0 = fmaxf(t0, sM[w * ROWS + r0]);
+            t1 = fmaxf(t1, sM[w * ROWS + r1]);
+        }
+        const float f0 = m0 == -CUDART_INF_F ? 0.f : ex2(m0 - t0), f1 = m1 == -CUDART_INF_F ? 0.f : ex2(m1 - t1);
+        l0 *= f0; l1 *= f1;
+#pragma unroll 1
+        for (int w = kWarps - 1; w >= 0; --w) {
+            if (warp == w) {
+#pragma unroll
+                for (int n = 0; n < 2 * DS; ++n) {
+                    float2* y0 = reinterpret_cast<float2*>(sO + r0 * OP + n * 8 + (lane & 3) * 2);
+                    float2* y1 = reinterpret_cast<float2*>(sO + r1 * OP + n * 8 + (lane & 3) * 2);
+                    // (what no key of this warp went into is zero times a factor of zero)
+                    float2 a = make_float2(o[n][0] * f0, o[n][1] * f0), c = make_float2(o[n][2] * f1, o[n][3] * f1);
+                    if (w != kWarps - 1) {
+                        const float2 u = *y0, v = *y1;
+                        a.x += u.x; a.y += u.y;
+                        c.x += v.x; c.y += v.y;
+                    }
+                    *y0 = a;
+                    *y1 = c;
+                }
+                if ((lane & 3) == 0) {
+                    sL[r0] = w == kWarps - 1 ? l0 : sL[r0] + l0;
+                    sL[r1] = w == kWarps - 1 ? l1 : sL[r1] + l1;
+                }
+            }
+            __syncthreads();
+        }
+        // ---- handed on, or the result
+        const bool whole = tile0 == 0 && at_end;
+        float* slot = slot_of(p, blockIdx.x, first_unit);
+        const bool any_bad = *sBad;
+        for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
+            const int r = i / chunks, col = i - r * chunks;
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = sO[r * OP + col * 8 + e];
+            if (whole) {
+                const int t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+                if (t >= s.count) continue;
+                const float inv = sL[r] == 0.f ? 0.f : 1.0f / sL[r];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] *= inv;
+                if (any_bad) {
+                    const unsigned long long mask = seen_by(p, s, b, row0 + r);
+                    for (int e = 0; e < 8; ++e) y[e] += not_finite_seen<__nv_bfloat16>(p, s, b, h, mask, col * 8 + e);
+                }
+                __nv_bfloat162 w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] +
+                                          col * 8) = *reinterpret_cast<uint4*>(w);
+            } else {
+                float4* dst = reinterpret_cast<float4*>(slot + r * p.D + col * 8);
+                dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+                dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+            }
+        }
+        if (!whole) {
+            float* tail = slot + ROWS * p.D;
+            if (threadIdx.x < ROWS) {
+                const int r = threadIdx.x;
+                tail[r] = fmaxf(fmaxf(sM[r], sM[ROWS + r]), fmaxf(sM[2 * ROWS + r], sM[3 * ROWS + r]));
+                tail[ROWS + r] = sL[r];
+            }
+            if (threadIdx.x == 0) tail[2 * ROWS] = any_bad ? 1.f : 0.f;
+        }
+        first_unit = false;
+        __syncthreads();                                                 // (sQ, sO, sM, sL of the next unit)
+    }
+    copies_wait<0>();
+}
+
+// ---- float32: 16 rows a tile on the fp32 pipes ----------------------------------------------------------------------------------
+
+// A warp owns four rows: a lane's key of the tile for the scores, its four (or twice four) neighbouring channels for the sums.
+template <int STAGES>
+__global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
+    constexpr int TILE = 32;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int pitch = p.D + 4;                                           // floats (rows start on 16-byte boundaries: D is a multiple of 4)
+    const int pieces = p.D / 4;
+    float* sQ = reinterpret_cast<float*>(smem);                          // [16][pitch]
+    float* sP = sQ + ROWS * pitch;                                       // [16][32]
+    float* ring = sP + ROWS * TILE;
+    const int stage_floats = 2 * TILE * pitch;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    chain_begin();
+
+    Cursor at;
+    at.start(p, blockIdx.x, p.ctas);
+    if (at.left == 0) return;
+    Cursor ahead = at;
+    auto fetch = [&](int stage) {
+        float* dst = ring + stage * stage_floats;
+        const float* k = static_cast<const float*>(p.k) + ahead.h * p.ks[1];
+        const float* v = static_cast<const float*>(p.v) + ahead.h * p.vs[1];
+        // four threads a row
+        const int r = threadIdx.x >> 2, entry = ahead.tile * TILE + r;
+        int row = 0, page = -1;
+        if (entry < ahead.s.total) page = page_of(p, ahead.b, entry, row);
+        const long long ko = page < 0 ? 0 : page * p.ks[0] + row * p.ks[2], vo = page < 0 ? 0 : page * p.vs[0] + row * p.vs[2];
+        for (int c = threadIdx.x & 3; c < pieces; c += 4) {
+            copy16(smem_at(dst + r * pitch + 4 * c), k + ko + 4 * c, page >= 0);
+            copy16(smem_at(dst + (TILE + r) * pitch + 4 * c), v + vo + 4 * c, page >= 0);
+        }
+        copies_end();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (ahead.left > 0) { fetch(i); ahead.next(p); }
+        else copies_end();
+    }
+    int stage = 0;
+    bool first_unit = true;
+    while (at.left > 0) {
+        const Sequence s = at.s;
+        const int b = at.b, h = at.h, row0 = at.rt * ROWS, tile0 = at.tile;
+        for (int i = threadIdx.x; i < ROWS * pieces; i += kThreads) {
+            const int r = i / pieces, col = i - r * pieces, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (t < s.count)
+                v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + b * p.qs[0] + t * p.qs[1] +
+                                                     (h * p.G + g) * p.qs[2] + col * 4);
+            *reinterpret_cast<float4*>(sQ + r * pitch + col * 4) = v;
+        }
+        const bool busy = row0 + 4 * warp < s.count * p.G;               // (any of this warp's rows)
+        unsigned long long mask[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mask[i] = seen_by(p, s, b, row0 + 4 * warp + i);
+        float m[4], l[4];
+        float4 o[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = -CUDART_INF_F;
+            l[i] = 0.f;
+            o[i][0] = o[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        bool end, at_end;
+        do {
+            copies_wait<STAGES - 2>();
+            __syncthreads();                                             // the tile is there, and the one before it read
+            if (ahead.left > 0) {
+                fetch(stage == 0 ? STAGES - 1 : stage - 1);
+                ahead.next(p);
+            } else {
+                copies_end();
+            }
+            if (busy) {
+                const float* sk = ring + stage * stage_floats + lane * pitch;
+                const float* sv = ring + stage * stage_floats + TILE * pitch;
+                const float* sq = sQ + 4 * warp * pitch;
+                float c[4] = {};
+#pragma unroll 4
+                for (int d = 0; d < pieces; ++d) {
+                    const float4 kk = *reinterpret_cast<const float4*>(sk + 4 * d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 qq = *reinterpret_cast<const float4*>(sq + i * pitch + 4 * d);
+                        c[i] = fmaf(qq.x, kk.x, c[i]);
+                        c[i] = fmaf(qq.y, kk.y, c[i]);
+                        c[i] = fmaf(qq.z, kk.z, c[i]);
+                        c[i] = fmaf(qq.w, kk.w, c[i]);
+                    }
+                }
+                const int j = at.tile * TILE + lane - s.length;
+                const bool drafts = at.tile * TILE + TILE > s.length;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = c[i] * p.scale_log2;
+                    if (drafts && j >= 0 && !(j < s.total - s.length && (mask[i] >> j & 1))) x = -CUDART_INF_F;
+                    float top = x;
+#pragma unroll
+                    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    const float n = fmaxf(m[i], top), f = m[i] == n ? 1.f : ex2(m[i] - n);
+                    m[i] = n;
+                    const float w = ex2(x - (n == -CUDART_INF_F ? 0.f : n));
+                    l[i] = fmaf(l[i], f, w);
+                    sP[(4 * warp + i) * TILE + lane] = w;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        o[i][u].x *= f; o[i][u].y *= f; o[i][u].z *= f; o[i][u].w *= f;
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int col = lane + 32 * u;
+                    if (col >= pieces) continue;
+#pragma unroll 2
+                    for (int e = 0; e < TILE; e += 4) {
+                        float4 w[4], v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(sP + (4 * warp + i) * TILE + e);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const float4*>(sv + (e + x) * pitch + 4 * col);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if (drafts && ws[x] == 0.f) continue;    // (what a row does not see need not be finite)
+                                o[i][u].x = fmaf(ws[x], v[x].x, o[i][u].x);
+                                o[i][u].y = fmaf(ws[x], v[x].y, o[i][u].y);
+                                o[i][u].z = fmaf(ws[x], v[x].z, o[i][u].z);
+                                o[i][u].w = fmaf(ws[x], v[x].w, o[i][u].w);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            end = at.last_of_unit();
+            at_end = at.tile + 1 == s.tiles;
+            at.next(p);
+        } while (!end);
+        const bool whole = tile0 == 0 && at_end;
+        float* slot = slot_of(p, blockIdx.x, first_unit);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * warp + i, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+            const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int col = lane + 32 * u;
+                if (col >= pieces) continue;
+                float4 y = o[i][u];
+                if (whole) {
+                    if (t >= s.count) continue;
+                    y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] +
+                                               4 * col) = y;
+                } else {
+                    *reinterpret_cast<float4*>(slot + r * p.D + 4 * col) = y;
+                }
+            }
+            if (!whole && lane == 0) {
+                slot[ROWS * p.D + r] = m[i];
+                slot[ROWS * p.D + ROWS + r] = l[i];
+            }
+        }
+        if (!whole && threadIdx.x == 0) slot[ROWS * p.D + 2 * ROWS] = 0.f;
+        first_unit = false;
+        __syncthreads();                                                 // (sQ)
+    }
+    copies_wait<0>();
+}
+
+// ---- units that several CTAs had ------------------------------------------------------------------------------------------------
+
+// A warp per row of a unit: the pieces' maxima, then their sums, in the order of the keys.
+constexpr int JOIN_ROWS = 4;
+template <typename T>
+__global__ void __launch_bounds__(32 * JOIN_ROWS) join_kernel(const Params p) {
+    chain_begin();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int unit = blockIdx.x, b = unit / (p.Hk * p.row_tiles), rest = unit - b * p.Hk * p.row_tiles;
+    const int h = rest / p.row_tiles, rt = rest - h * p.row_tiles;
+    const int r = blockIdx.y * JOIN_ROWS + warp, row = rt * p.rows_per_tile + r, t = row / p.G, g = row - t * p.G;
+    if (r >= p.rows_per_tile || t >= p.T) return;                        // (a whole warp)
+    const Sequence s = sequence_of(p, b);
+    T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2];
+    if (t >= s.count || s.total == 0) {                                  // nothing is there, or nothing to attend to
+        for (int c = lane; c < p.D; c += 32) out[c] = from_f32<T>(0.f);
+        return;
+    }
+    long long before;
+    const long long work = total_work(p, b, before), begin = before + ((long long)h * s.row_tiles + rt) * s.tiles;
+    const int ctas = busy_ctas(work, p.ctas);
+    const int c0 = cta_of(work, begin, ctas), c1 = cta_of(work, begin + s.tiles - 1, ctas);
+    if (c0 == c1) return;                                                // (written by its CTA)
+    float top = -CUDART_INF_F;
+    bool bad = false;
+    const long long tail = (long long)p.rows_per_tile * p.D;
+    for (int c = c0 + lane; c <= c1; c += 32) {
+        const float* slot = slot_of(p, c, first_tile(work, c, ctas) >= begin);
+        top = fmaxf(top, slot[tail + r]);
+        bad |= slot[tail + 2 * p.rows_per_tile] != 0.f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bad = __any_sync(0xffffffffu, bad);
+    if (top == -CUDART_INF_F) top = 0.f;
+    float sum = 0.f;
+    float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+        const float* slot = slot_of(p, c, first_tile(work, c, ctas) >= begin);
+        const float f = ex2(slot[tail + r] - top);
+        sum = fmaf(slot[tail + p.rows_per_tile + r], f, sum);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int col = 4 * (lane + 32 * u);
+            if (col >= p.D) continue;
+            const float4 x = *reinterpret_cast<const float4*>(slot + (long long)r * p.D + col);
+            y[u].x = fmaf(x.x, f, y[u].x); y[u].y = fmaf(x.y, f, y[u].y);
+            y[u].z = fmaf(x.z, f, y[u].z); y[u].w = fmaf(x.w, f, y[u].w);
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const unsigned long long mask = seen_by(p, s, b, row);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int col = 4 * (lane + 32 * u);
+        if (col >= p.D) continue;
+        float x[4] = {y[u].x * inv, y[u].y * inv, y[u].z * inv, y[u].w * inv};
+        if (bad)
+            for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[col + e] = from_f32<T>(x[e]);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------
+
+struct Plan {
+    int rows_per_tile, tile, stages, ctas_per_sm;
+    size_t smem;
+};
+
+constexpr int kStepsBuilt[] = {4, 5, 6, 8, 12, 16};
+int steps_of(int D) {
+    for (int s : kStepsBuilt)
+        if (16 * s >= D) return s;
+    return 0;
+}
+
+Plan plan_of(int dtype, int rows, int D) {
+    Plan g{};
+    g.rows_per_tile = ROWS;
+    if (dtype == CONVNN_F32) {
+        g.tile = 32;
+        g.stages = D <= 128 ? 3 : 2;
+        g.smem = 4 * ((size_t)ROWS * (D + 4) + ROWS * 32 + (size_t)g.stages * 64 * (D + 4));
+        g.ctas_per_sm = g.smem <= 74 * 1024 ? 3 : g.smem <= 112 * 1024 ? 2 : 1;
+    } else {
+        const int DP = 16 * steps_of(D), pitch = ((DP / 8) | 1) * 16;
+        g.tile = 64;
+        g.stages = DP <= 64 ? 4 : DP <= 96 ? 3 : 2;
+        g.smem = (size_t)16 * pitch + 4 * (ROWS * (DP + 8) + 5 * ROWS + 4) + (size_t)kWarps * g.stages * 32 * pitch;
+        g.ctas_per_sm = g.smem <= 112 * 1024 ? 2 : 1;
+    }
+    return g;
+}
+
+long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
+
+template <int DS, int STAGES>
+int launch_rows(const Params& p, size_t smem, cudaStream_t st) {
+    CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES>), smem);
+    launch_chained(rows_kernel<DS, STAGES>, p.ctas, kThreads, smem, st, p);
+    CONVNN_CHECK_LAUNCH("tree_attention");
+    return CONVNN_OK;
+}
+template <int STAGES>
+int launch_scalar(const Params& p, size_t smem, cudaStream_t st) {
+    CONVNN_ENSURE_SMEM(scalar_kernel<STAGES>, smem);
+    launch_chained(scalar_kernel<STAGES>, p.ctas, kThreads, smem, st, p);
+    CONVNN_CHECK_LAUNCH("tree_attention");
+    return CONVNN_OK;
+}
+
+}  // namespace
+
+size_t tree_attention_workspace(int dtype, int T, int G, int D) {
+    const Plan g = plan_of(dtype, T * G, D);
+    return (size_t)device_sms() * g.ctas_per_sm * 2 * slot_floats(g, D) * 4;
+}
+
+int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace, size_t workspace_bytes,
+                          cudaStream_t st) {
+    const Plan g = plan_of(a->dtype, a->T * (a->Hq / a->Hk), a->D);
+    Params p{};
+    p.q = a->q; p.k = cache->k; p.v = cache->v; p.out = a->out;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_stride[i]; p.os[i] = a->out_stride[i];
+        p.ks[i] = cache->k_stride[i]; p.vs[i] = cache->v_stride[i];
+    }
+    p.table = cache->table; p.table_stride = cache->table_stride;
+    p.lengths = a->lengths; p.counts = a->counts;
+    p.tree = reinterpret_cast<const long long*>(a->tree);
+    p.tree_stride[0] = a->tree_stride[0]; p.tree_stride[1] = a->tree_stride[1];
+    p.B = a->B; p.T = a->T; p.Hk = a->Hk; p.G = a->Hq / a->Hk; p.D = a->D;
+    p.pages = cache->pages; p.page_size = cache->page_size; p.width = cache->width;
+    p.rows_per_tile = g.rows_per_tile; p.tile = g.tile;
+    p.row_tiles = (p.T * p.G + g.rows_per_tile - 1) / g.rows_per_tile;
+    p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
+    p.partial = static_cast<float*>(workspace);
+    p.slot = slot_floats(g, p.D);
+    p.ctas = device_sms() * g.ctas_per_sm;
+    const long long units = (long long)p.B * p.Hk * p.row_tiles, keys = (long long)p.width * p.page_size;
+    if (units > 0x7fffffffll || (keys + p.tile - 1) / p.tile * p.row_tiles * p.Hk > 0x7fffffffll)
+        return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %lld units of up to %lld keys", units, keys);
+    if (workspace_bytes < (size_t)p.ctas * 2 * p.slot * 4)
+        return set_error(CONVNN_E_WORKSPACE, "tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
+                         (size_t)p.ctas * 2 * p.slot * 4);
+    int rc;
+    if (a->dtype == CONVNN_F32) {
+        rc = g.stages == 3 ? launch_scalar<3>(p, g.smem, st) : launch_scalar<2>(p, g.smem, st);
+    } else {
+        switch (steps_of(p.D)) {
+            case 4: rc = launch_rows<4, 4>(p, g.smem, st); break;
+            case 5: rc = launch_rows<5, 3>(p, g.smem, st); break;
+            case 6: rc = launch_rows<6, 3>(p, g.smem, st); break;
+            case 8: rc = launch_rows<8, 2>(p, g.smem, st); break;
+            case 12: rc = launch_rows<12, 2>(p, g.smem, st); break;
+            default: rc = launch_rows<16, 2>(p, g.smem, st); break;
+        }
+    }
+    if (rc) return rc;
+    const dim3 grid((unsigned)units, (g.rows_per_tile + JOIN_ROWS - 1) / JOIN_ROWS);
+    if (a->dtype == CONVNN_F32) launch_chained(join_kernel<float>, grid, 32 * JOIN_ROWS, 0, st, p);
+    else launch_chained(join_kernel<__nv_bfloat16>, grid, 32 * JOIN_ROWS, 0, st, p);
+    CONVNN_CHECK_LAUNCH("tree_attention");
+    return CONVNN_OK;
+}
+
+}  // namespace convnn

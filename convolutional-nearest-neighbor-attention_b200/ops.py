@@ -785,6 +785,257 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     return Fp8Blocks(out, out_scales) if quantize else out
 
 
+# ---- heads, a paged cache, and attention over it --------------------------------------------------------------------
+
+MOST_HEAD_CHANNELS, MOST_DRAFTED = 256, 64
+
+
+class PagedCache(NamedTuple):
+    """Keys and values of several sequences, in pages: ``k`` and ``v`` (pages, heads, page_size, channels) in float32 or bfloat16,
+    and ``table`` (sequences, width) int32, the pages of each sequence's entries in order: entry ``j`` is row ``j % page_size`` of
+    page ``table[b, j // page_size]``.  A page number outside ``0 .. pages - 1`` keeps nothing and reads as zeros."""
+    k: torch.Tensor
+    v: torch.Tensor
+    table: torch.Tensor
+
+
+def _as_heads(t: torch.Tensor, lead, what: str, H: Optional[int] = None, D: Optional[int] = None) -> torch.Tensor:
+    """(..., H, D) -> (B, T, H, D) with channels side by side."""
+    shape = t.shape
+    if len(shape) < 2 or shape[:-2] != lead or shape[-2] < 1 or not 1 <= shape[-1] <= MOST_HEAD_CHANNELS:
+        raise ValueError(f"{what} must be {(*lead, 'heads', 'channels')} with up to {MOST_HEAD_CHANNELS} channels, got {tuple(shape)}")
+    if (H is not None and shape[-2] != H) or (D is not None and shape[-1] != D):
+        raise ValueError(f"{what} must have {H or 'any number of'} heads of {D} channels, got {tuple(shape)}")
+    if len(shape) != 4:
+        T = lead[-1] if lead else 1
+        t = t.reshape(math.prod(lead[:-1]), T, shape[-2], shape[-1])
+    if (t.stride(3) != 1 and shape[-1] > 1) or min(t.stride()) < 0:
+        t = t.contiguous()
+    return t
+
+
+def _index_arg(t: Optional[torch.Tensor], shape, what: str, dtype: torch.dtype = torch.int32) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        try:
+            return t.expand(shape)
+        except RuntimeError:
+            raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}") from None
+    return t
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _cache_arg(cache, B: int, Hk: int, D: int, dtype: torch.dtype, written: bool):
+    """-> (the struct, what it points to)"""
+    k, v, table = cache
+    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != Hk or k.shape[3] != D or min(k.shape) < 1:
+        raise ValueError(f"a cache's keys and values must be (pages, {Hk}, page_size, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"the cache must be {dtype}, got {k.dtype} and {v.dtype}")
+    if table.dtype != torch.int32:
+        raise TypeError(f"the cache's table must be int32, got {table.dtype}")
+    if table.dim() != 2 or table.shape[0] != B:
+        raise ValueError(f"the cache's table must be ({B}, pages of a sequence), got {tuple(table.shape)}")
+    if table.shape[1] * k.shape[2] > MOST_CHANNELS or max(k.shape) > MOST_CHANNELS:
+        raise ValueError(f"a cache takes up to 2^30 entries a sequence, got {table.shape[1]} pages of {k.shape[2]}")
+    for t in (k, v):
+        if t.stride(3) != 1 and D > 1:
+            raise ValueError("the channels of a cache must lie side by side")
+        if written:
+            room = D
+            for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(3) if t.shape[i] > 1):
+                if stride < room:
+                    raise ValueError(f"entries of the cache overlap: strides {tuple(t.stride())} of {tuple(t.shape)}")
+                room = stride * size
+    table = _dense(table)
+    c = _capi.ConvnnCache(k.data_ptr(), v.data_ptr(), k.stride()[:3], v.stride()[:3], table.data_ptr(), table.shape[1],
+                          k.shape[0], k.shape[2], table.shape[1])
+    return c, (k, v, table)
+
+
+def _heads_arg(q, k, v, q_weight, k_weight, rope, positions, eps, interleaved, lead):
+    """-> (the struct without its results, what it points to)"""
+    a = _capi.ConvnnHeads()
+    like = q if q is not None else k
+    D, dtype = like.shape[-1], like.dtype
+    a.dtype, a.D, a.eps, a.interleaved = _dtype_code(dtype), D, eps, bool(interleaved)
+    a.B, a.T = (math.prod(lead[:-1]), lead[-1]) if lead else (1, 1)
+    kept = []
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"heads must be of one type, got {dtype} and {t.dtype}")
+        t = _as_heads(t, lead, name, None if name == "q" or t is k else k.shape[-2], D)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_stride", t.stride()[:3])
+        kept.append(t)
+    a.Hq, a.Hk = q.shape[-2] if q is not None else 0, k.shape[-2] if k is not None else 0
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if w.dtype != dtype:
+            raise TypeError(f"{name} must have the heads' type, {dtype}")
+        if w.shape != (D,):
+            raise ValueError(f"{name} must have shape ({D},), got {tuple(w.shape)}")
+        w = _dense(w)
+        setattr(a, name, w.data_ptr())
+        kept.append(w)
+    if rope is not None:
+        if rope.dtype != _F32:
+            raise TypeError(f"rope must be float32, got {rope.dtype}")
+        if rope.dim() != 2 or rope.shape[1] < 2 or rope.shape[1] % 2 or rope.shape[1] > D or rope.shape[0] >= 1 << 31:
+            raise ValueError(f"rope must be (positions, turned channels), an even number up to {D} of them, got {tuple(rope.shape)}")
+        if rope.stride(1) != 1 or rope.stride(0) < rope.shape[1]:
+            rope = rope.contiguous()
+        a.rope, a.rope_stride, (a.rope_rows, a.rotary) = rope.data_ptr(), rope.stride(0), rope.shape
+        kept.append(rope)
+    if positions is not None:
+        positions = _index_arg(positions, lead, "positions").reshape(a.B, a.T)
+        a.positions, a.position_stride = positions.data_ptr(), positions.stride()
+        kept.append(positions)
+    return a, kept
+
+
+def _heads_out(out: Optional[torch.Tensor], like: torch.Tensor, what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"{what} must be {tuple(like.shape)} in {like.dtype}, got {tuple(out.shape)} in {out.dtype}")
+    room = 1
+    for stride, size in sorted((out.stride(i), out.shape[i]) for i in range(out.dim()) if out.shape[i] > 1):
+        if stride < room:
+            raise ValueError(f"values of {what} overlap: strides {tuple(out.stride())} of {tuple(out.shape)}")
+        room = stride * size
+    if (out.stride(-1) != 1 and out.shape[-1] > 1) or (out.dim() > 4 and not out.is_contiguous()):
+        raise ValueError(f"the channels of {what} must lie side by side, got strides {tuple(out.stride())}")
+    return out
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False, out=None):
+    """Norm of every query and key head over its channels, and rotation by its token's position, in one pass: ``q`` (..., tokens,
+    heads, channels) and ``k`` (the same tokens, its own heads; or None), any strides with channels side by side, as a packed
+    projection leaves them.  A head is ``x * rsqrt(mean(x * x) + eps) * weight`` (``x`` without a weight); then the pairs ``(i, i +
+    R / 2)``, with ``interleaved`` ``(2 i, 2 i + 1)``, of its first ``R`` channels are turned by the angle whose cosine and sine are in
+    ``rope`` (positions, R) float32, cosines first, at row ``positions`` (..., tokens) int32, by default the token's index.  A
+    position outside ``rope`` makes NaN of the turned channels.  -> (q, k), rounded once; ``out`` a pair to write to, which may be
+    ``q`` and ``k``."""
+    if torch.is_grad_enabled():
+        _forward_only(q, k, q_weight, k_weight, rope)
+    like = q if q is not None else k
+    if like is None:
+        raise ValueError("qk_norm_rope needs queries or keys")
+    into = (None, None) if out is None else out
+    index = _device_of(like, q, k, q_weight, k_weight, rope, positions, *into)
+    if like.dim() < 2:
+        raise ValueError(f"heads must be (..., tokens, heads, channels), got {tuple(like.shape)}")
+    lead = like.shape[:-2]
+    a, kept = _heads_arg(q, k, None, q_weight, k_weight, rope, positions, eps, interleaved, lead)
+    results = []
+    for name, t, o in (("q", q, into[0]), ("k", k, into[1])):
+        if t is None:
+            results.append(None)
+            continue
+        o = _heads_out(o, t, name + "'s result")
+        four = o if o.dim() == 4 else o.view(a.B, a.T, *o.shape[-2:]) if o.dim() > 4 else o.reshape(a.B, a.T, *o.shape[-2:])
+        setattr(a, name + "_out", four.data_ptr())
+        setattr(a, name + "_out_stride", four.stride()[:3])
+        results.append(o)
+    if a.B and a.T:
+        _launch(index, _capi.lib().convnn_b200_qk_norm_rope, ctypes.byref(a))
+    return tuple(results)
+
+
+def append_kv(cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, q: Optional[torch.Tensor] = None,
+              q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
+              positions: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              interleaved: bool = False) -> Optional[torch.Tensor]:
+    """Appends the keys and values (B, T, heads, channels) of new tokens to ``cache`` (a ``PagedCache``, in place), the keys normed
+    and turned on the way as ``qk_norm_rope`` does: token ``t`` of sequence ``b`` becomes entry ``lengths[b] + t``, of which the first
+    ``counts[b]`` (default: all) are there; entries that its table has no page for are dropped.  ``lengths``, ``counts`` (B) and
+    ``positions`` (B, T; default: the entry) int32.  ``q`` (B, T, query heads, channels) is normed and turned in the same launch.
+    -> its result (zeros for tokens that are not there), or None."""
+    if torch.is_grad_enabled():
+        _forward_only(q, k, v, q_weight, k_weight, rope, cache[0], cache[1])
+    index = _device_of(k, v, lengths, q, q_weight, k_weight, rope, positions, counts, *cache)
+    if k.dim() != 4:
+        raise ValueError(f"keys must be (sequences, tokens, heads, channels), got {tuple(k.shape)}")
+    lead = k.shape[:2]
+    a, kept = _heads_arg(q, k, v, q_weight, k_weight, rope, positions, eps, interleaved, lead)
+    c, kept_too = _cache_arg(cache, a.B, a.Hk, a.D, k.dtype, True)
+    lengths, counts = _dense(_index_arg(lengths, lead[:1], "lengths")), _dense(_index_arg(counts, lead[:1], "counts"))
+    result = None
+    if q is not None:
+        result = torch.empty_like(q, memory_format=torch.contiguous_format)
+        a.q_out, a.q_out_stride = result.data_ptr(), result.stride()[:3]
+    if a.B and a.T:
+        _launch(index, _capi.lib().convnn_b200_append_kv, ctypes.byref(a), ctypes.byref(c), lengths.data_ptr(),
+                None if counts is None else counts.data_ptr())
+    return result
+
+
+def _on_16_bytes(t: torch.Tensor) -> bool:
+    unit = 16 // t.element_size()
+    return t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1])
+
+
+def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional[torch.Tensor] = None,
+                   counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``softmax(scale * q k^T) v`` of up to 64 drafted tokens of each sequence, ``q`` (B, T, heads, channels), over a
+    ``PagedCache`` to which their keys and values are already appended: token ``t`` attends to the ``lengths[b]`` entries before
+    them and to drafted token ``j`` where bit ``j`` of ``tree[b, t]`` (int64) is set, of which there are ``counts[b]`` (default:
+    T); without ``tree`` to every ``j <= t``, so that one token is ordinary decoding.  The heads of ``q`` share the cache's evenly,
+    neighbours the same; ``scale`` is by default ``channels ** -0.5``.  Zeros for tokens that are not there or have nothing to attend
+    to; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels, float32 of 4, rows of the
+    cache on 16-byte boundaries.  -> (B, T, heads, channels) in ``q``'s type, or ``out``."""
+    if torch.is_grad_enabled():
+        _forward_only(q, cache[0], cache[1])
+    index = _device_of(q, lengths, tree, counts, out, *cache)
+    if q.dim() != 4:
+        raise ValueError(f"queries must be (sequences, tokens, heads, channels), got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    q = _as_heads(q, q.shape[:2], "q")
+    dt = _dtype_code(q.dtype)
+    if T > MOST_DRAFTED:
+        raise ValueError(f"tree_attention takes up to {MOST_DRAFTED} drafted tokens, got {T}")
+    Hk = cache[0].shape[1] if cache[0].dim() == 4 else 0
+    if Hk < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads do not share a cache of shape {tuple(cache[0].shape)} evenly")
+    unit = 16 // q.element_size()
+    if D % unit or not (_on_16_bytes(cache[0]) and _on_16_bytes(cache[1])):
+        raise ValueError(f"heads must be a multiple of {unit} channels and the cache's rows on 16-byte boundaries, got {D} channels")
+    c, kept = _cache_arg(cache, B, Hk, D, q.dtype, False)
+    lengths, counts = _dense(_index_arg(lengths, q.shape[:1], "lengths")), _dense(_index_arg(counts, q.shape[:1], "counts"))
+    tree = _index_arg(tree, q.shape[:2], "tree", torch.int64)
+    if not _on_16_bytes(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    result = _heads_out(out, q, "out")
+    room = result if _on_16_bytes(result) else torch.empty_like(q, memory_format=torch.contiguous_format)
+    a = _capi.ConvnnTreeAttention(dt, B, T, Hq, Hk, D, D ** -0.5 if scale is None else scale, q.data_ptr(), q.stride()[:3],
+                                  lengths.data_ptr(), None if counts is None else counts.data_ptr())
+    if tree is not None:
+        a.tree, a.tree_stride = tree.data_ptr(), tree.stride()
+    a.out, a.out_stride = room.data_ptr(), room.stride()[:3]
+    if B and T:
+        L = _capi.lib()
+        with torch.cuda.device(index):
+            need = L.convnn_b200_tree_attention_workspace_bytes(dt, T, Hq, Hk, D)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _launch(index, L.convnn_b200_tree_attention, ctypes.byref(a), ctypes.byref(c), workspace.data_ptr(), need)
+    if room is not result:
+        result.copy_(room)
+    return result
+
+
 def patch_embed(images: torch.Tensor, conv_weight: torch.Tensor, conv_bias: torch.Tensor, norm_weight, norm_bias,
                 cls: torch.Tensor, pe: torch.Tensor, patch: int, eps: float = 1e-5,
                 pixel_mean: Optional[torch.Tensor] = None, pixel_inv_std: Optional[torch.Tensor] = None,

@@ -269,6 +269,76 @@ int convnn_b200_linear_fp8(const void* a, int64_t lda, const float* a_scales, in
                            int64_t out_scale_row, int64_t out_scale_block, int64_t M, int32_t N, int32_t K,
                            int32_t gelu, void* stream);
 
+/* ---- heads, a paged cache, and attention over it ---------------------------------------------
+ * No reference counterpart: what lies between the packed q, k, v projection and the output projection
+ * when a model answers token by token.  Strides are in elements; the channels of a head lie side by
+ * side.  Up to 256 channels a head. */
+
+/* Query and key heads (B, T, H, D), strides (batch, token, head), and what happens to each of them:
+ *   n = x * (mean(x^2) + eps)^-1/2 * weight, or x where the weight is NULL;
+ *   with `rope`, the pairs (i, i + rotary / 2), or interleaved (2i, 2i + 1), i < rotary / 2, turned:
+ *   (n_a, n_b) -> (n_a cos_i - n_b sin_i, n_b cos_i + n_a sin_i).  Row `position` of rope (rope_rows,
+ *   rotary) float32, row stride rope_stride, holds the cosines and behind them the sines.
+ * Computed in float32 and rounded once.  positions (B, T) int32, strides position_stride; NULL: the
+ * token's index, in a cache its entry.  A position outside the table turns its channels into NaN. */
+typedef struct convnn_heads {
+    int32_t dtype, B, T, Hq, Hk, D;
+    int32_t rotary, interleaved, rope_rows;
+    float eps;
+    const void *q, *k, *v;                    /* v: append_kv only */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const void *q_weight, *k_weight;          /* (D) in dtype, or NULL */
+    const float* rope;                        /* or NULL: no rotation */
+    int64_t rope_stride;
+    const int32_t* positions;
+    int64_t position_stride[2];
+    void *q_out, *k_out;                      /* may be q and k themselves; k_out: qk_norm_rope only */
+    int64_t q_out_stride[3], k_out_stride[3];
+} convnn_heads;
+
+/* Keys and values in pages (pages, Hk, page_size, D), strides (page, head, row), and for every sequence
+ * the pages of its entries in order: table (B, width) int32, row stride table_stride, entry j in row
+ * j % page_size of page table[b][j / page_size].  Sequences may share pages that nothing is appended to.
+ * A page number outside 0 .. pages - 1 stands for zeros: it keeps nothing and reads as zeros. */
+typedef struct convnn_cache {
+    void *k, *v;
+    int64_t k_stride[3], v_stride[3];
+    const int32_t* table;
+    int64_t table_stride;
+    int32_t pages, page_size, width;
+} convnn_cache;
+
+/* q and k (either may be NULL) -> q_out, k_out. */
+int convnn_b200_qk_norm_rope(const convnn_heads* heads, void* stream);
+
+/* Token t of sequence b, t < counts[b] (NULL: T), becomes entry lengths[b] + t of its cache: the key normed
+ * and turned, the value as it is; entries behind the table's end are dropped.  q (or NULL) goes to q_out on the
+ * way, zeros behind counts[b].  lengths, counts (B) int32.  No two tokens may go to one place. */
+int convnn_b200_append_kv(const convnn_heads* heads, const convnn_cache* cache, const int32_t* lengths,
+                          const int32_t* counts, void* stream);
+
+/* softmax(scale * q k^T) v of T <= 64 drafted tokens of each sequence, already appended behind its
+ * lengths[b] entries.  Token t attends to all entries before them and to drafted token j where bit j of
+ * tree[b][t] (int64, strides tree_stride) is set, of the first counts[b]; tree NULL: to j <= t.  Query head h
+ * reads key head h / (Hq / Hk).  out (B, T, Hq, D): zeros for tokens from counts[b] on and for those that
+ * have nothing to attend to.  What a token does not see may hold anything, infinities and NaN included.
+ * Rows of q, out and the cache start on 16-byte boundaries (D a multiple of 8, in float32 of 4). */
+typedef struct convnn_tree_attention {
+    int32_t dtype, B, T, Hq, Hk, D;
+    float scale;
+    const void* q;
+    int64_t q_stride[3];
+    const int32_t *lengths, *counts;
+    const int64_t* tree;
+    int64_t tree_stride[2];
+    void* out;
+    int64_t out_stride[3];
+} convnn_tree_attention;
+/* On the current device; of the arguments' types and sizes only. */
+size_t convnn_b200_tree_attention_workspace_bytes(int dtype, int32_t T, int32_t Hq, int32_t Hk, int32_t D);
+int convnn_b200_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 /* Unfold non-overlapping P x P patches: img (B, C, Hh, Ww) -> out (B * Hh/P * Ww/P, C*P*P),
  * the im2col of Conv2d(kernel = stride = P) (vit.py:99, 105-107). */
 int convnn_b200_patchify(int dtype, const void* img, void* out, int32_t B, int32_t C, int32_t Hh,
