@@ -1,8 +1,8 @@
-// Host side of the 8-bit operators' ordinary calls (Python module _fp8_call): checks the tensors, allocates the results and makes
-// the library call.  Where anything is out of the ordinary (a wrong type or shape, other strides, another device than the current
+// Host side of the ordinary calls of the 8-bit operators and of those around a paged cache (Python module _fp8_call): checks the
+// tensors, allocates the results and makes the library call.  Where anything is out of the ordinary (a wrong type or shape, other strides, another device than the current
 // one, a tensor subclass, no rows) a function returns None, and the Python form in ops.py does the same with the messages.
-// rms_norm with a residual and an 8-bit result takes 14 us of host time through Python, linear_fp8 12; their kernels for a few
-// rows take less.
+// rms_norm with a residual and an 8-bit result takes 14 us of host time through Python, linear_fp8 12, qk_norm_rope 20, append_kv 32 and
+// tree_attention 30; their kernels for a few rows take less.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -10,6 +10,8 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
+
+#include <cmath>
 
 #include "convnn_b200.h"
 
@@ -42,6 +44,28 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_INCREF(args[5]);
     blocks_class = args[4];
     check_fn = args[5];
+    Py_RETURN_NONE;
+}
+
+decltype(&convnn_b200_qk_norm_rope) heads_fn = nullptr;
+decltype(&convnn_b200_append_kv) append_fn = nullptr;
+decltype(&convnn_b200_tree_attention) attention_fn = nullptr;
+decltype(&convnn_b200_tree_attention_workspace_bytes) attention_room_fn = nullptr;
+
+PyObject* bind_heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 4) {
+        PyErr_SetString(PyExc_TypeError, "bind_heads takes four addresses");
+        return nullptr;
+    }
+    void* at[4];
+    for (int i = 0; i < 4; ++i) {
+        at[i] = PyLong_AsVoidPtr(args[i]);
+        if (PyErr_Occurred()) return nullptr;
+    }
+    heads_fn = reinterpret_cast<decltype(heads_fn)>(at[0]);
+    append_fn = reinterpret_cast<decltype(append_fn)>(at[1]);
+    attention_fn = reinterpret_cast<decltype(attention_fn)>(at[2]);
+    attention_room_fn = reinterpret_cast<decltype(attention_room_fn)>(at[3]);
     Py_RETURN_NONE;
 }
 
@@ -233,9 +257,217 @@ PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- heads, a paged cache, and attention over it ------------------------------------------------------------------
+
+constexpr int64_t MOST_CHANNELS = 256, MOST_DRAFTED = 64, MOST = 1 << 30;
+
+// None, or a plain tensor.
+bool maybe(PyObject* o, const at::Tensor*& t, int& device, bool grad) {
+    t = o == Py_None ? nullptr : plain(o, device, grad);
+    return t || o == Py_None;
+}
+// (B, T, H, D) or (T, H, D), channels side by side.
+bool heads_of(const at::Tensor& t, int64_t B, int64_t T, int64_t D, at::ScalarType type, int32_t& H, int64_t (&stride)[3]) {
+    const int64_t dim = t.dim(), f = dim - 3;
+    if ((dim != 3 && dim != 4) || t.scalar_type() != type || (f && t.size(0) != B) || (!f && B != 1) || t.size(f) != T || t.size(f + 2) != D ||
+        t.size(f + 1) < 1 || t.size(f + 1) > (1 << 20) || (t.stride(f + 2) != 1 && D > 1))
+        return false;
+    H = (int32_t)t.size(f + 1);
+    stride[0] = f ? t.stride(0) : 0;
+    stride[1] = t.stride(f);
+    stride[2] = t.stride(f + 1);
+    return true;
+}
+bool weight_of(const at::Tensor* w, int64_t D, at::ScalarType type) {
+    return !w || (w->scalar_type() == type && w->dim() == 1 && w->size(0) == D && w->is_contiguous());
+}
+bool rope_of(const at::Tensor* rope, int64_t D, convnn_heads& a) {
+    if (!rope) return true;
+    if (rope->scalar_type() != at::kFloat || rope->dim() != 2 || rope->size(1) < 2 || rope->size(1) % 2 || rope->size(1) > D ||
+        rope->size(0) > MOST || rope->stride(1) != 1 || rope->stride(0) < rope->size(1))
+        return false;
+    a.rope = static_cast<const float*>(rope->data_ptr());
+    a.rope_stride = rope->stride(0);
+    a.rope_rows = (int32_t)rope->size(0);
+    a.rotary = (int32_t)rope->size(1);
+    return true;
+}
+bool ints_of(const at::Tensor* t, int64_t n) {
+    return !t || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && (t->stride(0) == 1 || n == 1));
+}
+bool cache_of(PyObject* o, int& device, bool grad, int64_t B, int64_t H, int64_t D, at::ScalarType type, bool written, convnn_cache& c) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 3) return false;
+    const at::Tensor* k = plain(PyTuple_GET_ITEM(o, 0), device, grad);
+    const at::Tensor* v = k ? plain(PyTuple_GET_ITEM(o, 1), device, grad) : nullptr;
+    const at::Tensor* table = v ? plain(PyTuple_GET_ITEM(o, 2), device, grad) : nullptr;
+    if (!table || k->scalar_type() != type || v->scalar_type() != type || table->scalar_type() != at::kInt || k->dim() != 4 ||
+        v->sizes() != k->sizes() || k->size(1) != H || k->size(3) != D || k->size(0) < 1 || k->size(2) < 1 || k->size(0) > MOST ||
+        k->size(2) > MOST || table->dim() != 2 || table->size(0) != B || table->size(1) > MOST || table->size(1) * k->size(2) > MOST ||
+        !table->is_contiguous())
+        return false;
+    // (pages that were strided otherwise may overlap, which Python looks at)
+    if (written ? !k->is_contiguous() || !v->is_contiguous() : (k->stride(3) != 1 || v->stride(3) != 1) && D > 1) return false;
+    c.k = k->data_ptr();
+    c.v = v->data_ptr();
+    for (int i = 0; i < 3; ++i) {
+        c.k_stride[i] = k->stride(i);
+        c.v_stride[i] = v->stride(i);
+    }
+    c.table = static_cast<const int32_t*>(table->data_ptr());
+    c.table_stride = table->size(1);
+    c.pages = (int32_t)k->size(0);
+    c.page_size = (int32_t)k->size(2);
+    c.width = (int32_t)table->size(1);
+    return true;
+}
+bool positions_of(const at::Tensor* t, int64_t B, int64_t T, int64_t dims, convnn_heads& a) {
+    if (!t) return true;
+    if (t->scalar_type() != at::kInt || t->dim() != dims || t->size(dims - 1) != T || (dims == 2 && t->size(0) != B)) return false;
+    a.positions = static_cast<const int32_t*>(t->data_ptr());
+    a.position_stride[0] = dims == 2 ? t->stride(0) : 0;
+    a.position_stride[1] = t->stride(dims - 1);
+    return true;
+}
+void dense_strides(int64_t (&stride)[3], int64_t T, int64_t H, int64_t D) {
+    stride[0] = T * H * D;
+    stride[1] = H * D;
+    stride[2] = D;
+}
+
+// qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved, out)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    OR_NONE(n == 9 && heads_fn && PyFloat_CheckExact(args[6]) && PyBool_Check(args[7]) && args[8] == Py_None);
+    const bool grad = c10::GradMode::is_enabled();
+    int device = -1;
+    const at::Tensor *q = plain(args[0], device, grad), *k, *wq, *wk, *rope, *at_;
+    OR_NONE(q && maybe(args[1], k, device, grad) && maybe(args[2], wq, device, grad) && maybe(args[3], wk, device, grad) &&
+            maybe(args[4], rope, device, grad) && maybe(args[5], at_, device, grad) && device == c10::cuda::current_device());
+    convnn_heads a{};
+    const auto type = q->scalar_type();
+    const int64_t dim = q->dim();
+    OR_NONE((dim == 3 || dim == 4) && dtype_code(type) >= 0);
+    const int64_t D = q->size(dim - 1), T = q->size(dim - 3), B = dim == 4 ? q->size(0) : 1;
+    OR_NONE(B >= 1 && T >= 1 && B <= MOST && T <= MOST && D >= 1 && D <= MOST_CHANNELS);
+    a.dtype = dtype_code(type); a.B = (int32_t)B; a.T = (int32_t)T; a.D = (int32_t)D;
+    a.eps = (float)PyFloat_AS_DOUBLE(args[6]);
+    a.interleaved = args[7] == Py_True;
+    OR_NONE(heads_of(*q, B, T, D, type, a.Hq, a.q_stride) && (!k || (k->dim() == dim && heads_of(*k, B, T, D, type, a.Hk, a.k_stride))) &&
+            weight_of(wq, D, type) && weight_of(wk, D, type) && rope_of(rope, D, a) && positions_of(at_, B, T, dim - 2, a));
+    a.q = q->data_ptr();
+    a.q_weight = wq ? wq->data_ptr() : nullptr;
+    a.k_weight = wk ? wk->data_ptr() : nullptr;
+    at::Tensor yq = at::empty(q->sizes(), at::TensorOptions().device(q->device()).dtype(type)), yk;
+    a.q_out = yq.data_ptr();
+    dense_strides(a.q_out_stride, T, a.Hq, D);
+    if (k) {
+        yk = at::empty(k->sizes(), at::TensorOptions().device(q->device()).dtype(type));
+        a.k = k->data_ptr();
+        a.k_out = yk.data_ptr();
+        dense_strides(a.k_out_stride, T, a.Hk, D);
+    }
+    if (!ok(heads_fn(&a, c10::cuda::getCurrentCUDAStream(device).stream()))) return nullptr;
+    PyObject* first = THPVariable_Wrap(yq);
+    PyObject* second = first ? (k ? THPVariable_Wrap(yk) : Py_NewRef(Py_None)) : nullptr;
+    PyObject* both = second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// append_kv(cache, k, v, lengths, q, q_weight, k_weight, rope, positions, counts, eps, interleaved); False: done, and no queries
+PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    OR_NONE(n == 12 && append_fn && PyFloat_CheckExact(args[10]) && PyBool_Check(args[11]));
+    const bool grad = c10::GradMode::is_enabled();
+    int device = -1;
+    const at::Tensor *k = plain(args[1], device, grad), *v = k ? plain(args[2], device, grad) : nullptr;
+    const at::Tensor *lengths = v ? plain(args[3], device, grad) : nullptr, *q, *wq, *wk, *rope, *at_, *counts;
+    OR_NONE(lengths && maybe(args[4], q, device, grad) && maybe(args[5], wq, device, grad) && maybe(args[6], wk, device, grad) &&
+            maybe(args[7], rope, device, grad) && maybe(args[8], at_, device, grad) && maybe(args[9], counts, device, grad) &&
+            device == c10::cuda::current_device());
+    convnn_heads a{};
+    convnn_cache c{};
+    const auto type = k->scalar_type();
+    OR_NONE(k->dim() == 4 && v->dim() == 4 && (!q || q->dim() == 4) && dtype_code(type) >= 0);
+    const int64_t D = k->size(3), T = k->size(1), B = k->size(0);
+    OR_NONE(B >= 1 && T >= 1 && B <= MOST && T <= MOST && D >= 1 && D <= MOST_CHANNELS);
+    a.dtype = dtype_code(type); a.B = (int32_t)B; a.T = (int32_t)T; a.D = (int32_t)D;
+    a.eps = (float)PyFloat_AS_DOUBLE(args[10]);
+    a.interleaved = args[11] == Py_True;
+    int32_t Hv = 0;
+    OR_NONE(heads_of(*k, B, T, D, type, a.Hk, a.k_stride) && heads_of(*v, B, T, D, type, Hv, a.v_stride) && Hv == a.Hk &&
+            (!q || heads_of(*q, B, T, D, type, a.Hq, a.q_stride)) && weight_of(wq, D, type) && weight_of(wk, D, type) &&
+            rope_of(rope, D, a) && positions_of(at_, B, T, 2, a) && ints_of(lengths, B) && ints_of(counts, B) &&
+            cache_of(args[0], device, grad, B, a.Hk, D, type, true, c));
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.q_weight = wq ? wq->data_ptr() : nullptr;
+    a.k_weight = wk ? wk->data_ptr() : nullptr;
+    at::Tensor y;
+    if (q) {
+        y = at::empty(q->sizes(), at::TensorOptions().device(k->device()).dtype(type));
+        a.q = q->data_ptr();
+        a.q_out = y.data_ptr();
+        dense_strides(a.q_out_stride, T, a.Hq, D);
+    }
+    if (!ok(append_fn(&a, &c, static_cast<const int32_t*>(lengths->data_ptr()),
+                      counts ? static_cast<const int32_t*>(counts->data_ptr()) : nullptr, c10::cuda::getCurrentCUDAStream(device).stream())))
+        return nullptr;
+    if (!q) Py_RETURN_FALSE;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// tree_attention(q, cache, lengths, tree, counts, scale, out)
+PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    OR_NONE(n == 7 && attention_fn && (args[5] == Py_None || PyFloat_CheckExact(args[5])) && args[6] == Py_None);
+    const bool grad = c10::GradMode::is_enabled();
+    int device = -1;
+    const at::Tensor *q = plain(args[0], device, grad), *lengths = q ? plain(args[2], device, grad) : nullptr, *tree, *counts;
+    OR_NONE(lengths && maybe(args[3], tree, device, grad) && maybe(args[4], counts, device, grad) && device == c10::cuda::current_device());
+    convnn_tree_attention a{};
+    convnn_cache c{};
+    const auto type = q->scalar_type();
+    const int dt = dtype_code(type);
+    OR_NONE(q->dim() == 4 && dt >= 0 && PyTuple_Check(args[1]) && PyTuple_GET_SIZE(args[1]) == 3);
+    const at::Tensor* pages = plain(PyTuple_GET_ITEM(args[1], 0), device, grad);
+    OR_NONE(pages && pages->dim() == 4);
+    const int64_t B = q->size(0), T = q->size(1), D = q->size(3), H = pages->size(1), unit = dt == CONVNN_F32 ? 4 : 8;
+    OR_NONE(B >= 1 && B <= MOST && T >= 1 && T <= MOST_DRAFTED && D >= 1 && D <= MOST_CHANNELS && D % unit == 0 && H >= 1 && H <= (1 << 20));
+    a.dtype = dt; a.B = (int32_t)B; a.T = (int32_t)T; a.D = (int32_t)D; a.Hk = (int32_t)H;
+    OR_NONE(heads_of(*q, B, T, D, type, a.Hq, a.q_stride) && a.Hq % H == 0 && ints_of(lengths, B) && ints_of(counts, B) &&
+            cache_of(args[1], device, grad, B, H, D, type, false, c));
+    if (tree) {
+        OR_NONE(tree->scalar_type() == at::kLong && tree->dim() == 2 && tree->size(0) == B && tree->size(1) == T);
+        a.tree = static_cast<const int64_t*>(tree->data_ptr());
+        a.tree_stride[0] = tree->stride(0);
+        a.tree_stride[1] = tree->stride(1);
+    }
+    bool rows = (reinterpret_cast<uintptr_t>(q->data_ptr()) | reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 == 0;
+    for (int i = 0; i < 3; ++i) rows = rows && a.q_stride[i] % unit == 0 && c.k_stride[i] % unit == 0 && c.v_stride[i] % unit == 0;
+    OR_NONE(rows);
+    a.scale = args[5] == Py_None ? (float)std::pow((double)D, -0.5) : (float)PyFloat_AS_DOUBLE(args[5]);
+    a.q = q->data_ptr();
+    a.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+    a.counts = counts ? static_cast<const int32_t*>(counts->data_ptr()) : nullptr;
+    const auto options = at::TensorOptions().device(q->device());
+    at::Tensor out = at::empty(q->sizes(), options.dtype(type));
+    a.out = out.data_ptr();
+    dense_strides(a.out_stride, T, a.Hq, D);
+    const size_t need = attention_room_fn(dt, a.T, a.Hq, a.Hk, a.D);
+    at::Tensor room = at::empty({(int64_t)need}, options.dtype(at::kByte));
+    if (!ok(attention_fn(&a, &c, room.data_ptr(), need, c10::cuda::getCurrentCUDAStream(device).stream()))) return nullptr;
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"bind", FAST(bind)}, {"rms_norm", FAST(rms_norm)}, {"quantize_fp8", FAST(quantize_fp8)},
-                         {"linear_fp8", FAST(linear_fp8)}, {nullptr, nullptr, 0, nullptr}};
+                         {"linear_fp8", FAST(linear_fp8)}, {"bind_heads", FAST(bind_heads)}, {"qk_norm_rope", FAST(qk_norm_rope)},
+                         {"append_kv", FAST(append_kv)}, {"tree_attention", FAST(tree_attention)}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp8_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -577,7 +577,7 @@ _E4M3, _F32, _BF16 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
 
 class _GeneralCalls:
     """Stands in for the module of ordinary calls where it cannot be had: every call goes the general way."""
-    rms_norm = quantize_fp8 = linear_fp8 = staticmethod(lambda *args: None)
+    rms_norm = quantize_fp8 = linear_fp8 = qk_norm_rope = append_kv = tree_attention = staticmethod(lambda *args: None)
 
 
 def _ordinary_calls():
@@ -591,10 +591,14 @@ def _ordinary_calls():
             _build.build_call()
         from . import _fp8_call
     except (RuntimeError, ImportError, OSError) as e:
-        warnings.warn(f"8-bit calls go through Python: {e}", RuntimeWarning)
+        warnings.warn(f"calls of 8-bit operators and paged caches go through Python: {e}", RuntimeWarning)
         return _GeneralCalls
-    names = ("rms_norm", "rms_norm_fp8", "quantize_fp8", "linear_fp8")
-    _fp8_call.bind(*(ctypes.cast(getattr(L, "convnn_b200_" + n), ctypes.c_void_p).value for n in names), Fp8Blocks, _capi.check)
+
+    def addresses(*names):
+        return (ctypes.cast(getattr(L, "convnn_b200_" + n), ctypes.c_void_p).value for n in names)
+
+    _fp8_call.bind(*addresses("rms_norm", "rms_norm_fp8", "quantize_fp8", "linear_fp8"), Fp8Blocks, _capi.check)
+    _fp8_call.bind_heads(*addresses("qk_norm_rope", "append_kv", "tree_attention", "tree_attention_workspace_bytes"))
     return _fp8_call
 
 
@@ -928,6 +932,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     ``rope`` (positions, R) float32, cosines first, at row ``positions`` (..., tokens) int32, by default the token's index.  A
     position outside ``rope`` makes NaN of the turned channels.  -> (q, k), rounded once; ``out`` a pair to write to, which may be
     ``q`` and ``k``."""
+    done = (_calls or _bind_calls()).qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved, out)
+    if done is not None:
+        return done
     if torch.is_grad_enabled():
         _forward_only(q, k, q_weight, k_weight, rope)
     like = q if q is not None else k
@@ -963,6 +970,9 @@ def append_kv(cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, q:
     ``counts[b]`` (default: all) are there; entries that its table has no page for are dropped.  ``lengths``, ``counts`` (B) and
     ``positions`` (B, T; default: the entry) int32.  ``q`` (B, T, query heads, channels) is normed and turned in the same launch.
     -> its result (zeros for tokens that are not there), or None."""
+    done = (_calls or _bind_calls()).append_kv(cache, k, v, lengths, q, q_weight, k_weight, rope, positions, counts, eps, interleaved)
+    if done is not None:
+        return None if done is False else done
     if torch.is_grad_enabled():
         _forward_only(q, k, v, q_weight, k_weight, rope, cache[0], cache[1])
     index = _device_of(k, v, lengths, q, q_weight, k_weight, rope, positions, counts, *cache)
@@ -997,6 +1007,9 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     neighbours the same; ``scale`` is by default ``channels ** -0.5``.  Zeros for tokens that are not there or have nothing to attend
     to; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels, float32 of 4, rows of the
     cache on 16-byte boundaries.  -> (B, T, heads, channels) in ``q``'s type, or ``out``."""
+    done = (_calls or _bind_calls()).tree_attention(q, cache, lengths, tree, counts, scale, out)
+    if done is not None:
+        return done
     if torch.is_grad_enabled():
         _forward_only(q, cache[0], cache[1])
     index = _device_of(q, lengths, tree, counts, out, *cache)
