@@ -245,6 +245,7 @@ int convnn_b200_device_status(int* code) {
     if (!c && (rc = read_conv_std_status(&c))) return rc;
     if (!c && (rc = read_conv1d_tc_status(&c))) return rc;
     if (!c && (rc = read_linear_fp8_status(&c))) return rc;
+    if (!c && (rc = read_tree_attention_status(&c))) return rc;
     *code = a ? a : (b ? b : c);
     return CONVNN_OK;
 }

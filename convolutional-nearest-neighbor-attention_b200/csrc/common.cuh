@@ -331,6 +331,7 @@ int launch_heads(const convnn_heads* h, const convnn_cache* cache, const int32_t
 size_t tree_attention_workspace(int dtype, int T, int G, int D);
 int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace, size_t workspace_bytes,
                           cudaStream_t st);
+int read_tree_attention_status(int* out);
 int launch_row_moments(const void* x, long long ldx, long long rows, int D, float* moments, cudaStream_t st);
 int launch_fold_layernorm(const void* w, const void* bias, const void* gamma, const void* beta, int N, int K,
                           void* w_folded, void* w_extra, cudaStream_t st);

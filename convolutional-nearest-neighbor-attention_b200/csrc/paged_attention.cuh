@@ -15,6 +15,8 @@
 namespace convnn {
 namespace paged {
 
+constexpr int kTileKeys = 128;                   // keys of a tile on the tensor cores
+
 struct Params {
     const void *q, *k, *v;
     void* out;
@@ -124,6 +126,13 @@ struct Cursor {
         do s = sequence_of(p, ++b);
         while (s.work() == 0);
     }
+    // Tiles of the unit that belong to this CTA, and the next unit.
+    __device__ __forceinline__ int run() const { return left < s.tiles - tile ? (int)left : s.tiles - tile; }
+    __device__ __forceinline__ void skip(const Params& p, int n) {
+        tile += n - 1;
+        left -= n - 1;
+        next(p);
+    }
     __device__ __forceinline__ bool last_of_unit() const { return left == 1 || tile + 1 == s.tiles; }
 };
 
@@ -156,5 +165,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The partial sums of a CTA's unit: slot 0 if the CTA's first tile is in it, else 1.
+__device__ __forceinline__ float* slot_of(const Params& p, int cta, bool first) { return p.partial + (2ll * cta + !first) * p.slot; }
+
 }  // namespace paged
+
+// 128 rows a tile on the tensor cores (tree_attention_tc.cu): bfloat16, up to 128 channels, pages of a multiple of 16 entries.
+bool tree_tiles_supported(const convnn_tree_attention* a, const convnn_cache* cache);
+int launch_tree_tiles(const paged::Params& p, cudaStream_t st);
 }  // namespace convnn

@@ -223,6 +223,13 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                  : "memory");
 }
 
+// Constant upper part of the descriptor of an operand whose 128-byte rows run along M or N (64 elements of 16 bits) and follow one another
+// along K, in groups of 8 rows, 128-byte swizzled: leading byte offset = distance between two such columns of 64, stride byte
+// offset = between groups of 8 rows along K.  The instruction descriptor says which operand is stored so (bit 15: A, 16: B).
+__device__ __forceinline__ uint64_t mnmajor_desc_hi(uint32_t column_bytes) {
+    return ((uint64_t)(column_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t kIdescBAlongN = 1u << 16;
 // Constant upper part of a K-major descriptor (everything except the start address).
 __device__ __forceinline__ uint64_t kmajor_desc_hi(uint32_t pitch) {
     const uint64_t layout = pitch == 128 ? 2 : (pitch == 64 ? 4 : 6);
@@ -326,6 +333,15 @@ __device__ __forceinline__ void mma_bf16_ts_pair(uint32_t tmem_d, uint32_t tmem_
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// The same on one CTA.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }

@@ -54,9 +54,6 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& r
     return (unsigned)page < (unsigned)p.pages ? page : -1;
 }
 
-// The partial sums of a CTA's unit: slot 0 if the CTA's first tile is in it, else 1.
-__device__ __forceinline__ float* slot_of(const Params& p, int cta, bool first) { return p.partial + (2ll * cta + !first) * p.slot; }
-
 // ---- bfloat16: 16 rows a tile on mma.sync ---------------------------------------------------------------------------------------
 
 // DS steps of 16 channels (D rounded up; the channels behind D are zeros), STAGES slices in flight per warp.
@@ -588,6 +585,7 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) join_kernel(const Params p) {
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 
 struct Plan {
+    bool tiles;                          // on the tensor cores, 128 rows a tile
     int rows_per_tile, tile, stages, ctas_per_sm;
     size_t smem;
 };
@@ -599,8 +597,14 @@ int steps_of(int D) {
     return 0;
 }
 
-Plan plan_of(int dtype, int rows, int D) {
+Plan plan_of(int dtype, int rows, int D, bool tiles) {
     Plan g{};
+    if (tiles) {
+        g.tiles = true;
+        g.rows_per_tile = g.tile = 128;
+        g.ctas_per_sm = 1;
+        return g;
+    }
     g.rows_per_tile = ROWS;
     if (dtype == CONVNN_F32) {
         g.tile = 32;
@@ -616,6 +620,9 @@ Plan plan_of(int dtype, int rows, int D) {
     }
     return g;
 }
+
+// More than one tile of 16 rows: keys and values would be read more than once.
+bool tiles_wanted(int dtype, int rows, int D) { return dtype == CONVNN_BF16 && rows > ROWS && D <= 128; }
 
 long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
 
@@ -637,13 +644,15 @@ int launch_scalar(const Params& p, size_t smem, cudaStream_t st) {
 }  // namespace
 
 size_t tree_attention_workspace(int dtype, int T, int G, int D) {
-    const Plan g = plan_of(dtype, T * G, D);
-    return (size_t)device_sms() * g.ctas_per_sm * 2 * slot_floats(g, D) * 4;
+    const Plan scalar = plan_of(dtype, T * G, D, false), tiles = plan_of(dtype, T * G, D, true);
+    const size_t a = (size_t)scalar.ctas_per_sm * slot_floats(scalar, D), b = (size_t)tiles.ctas_per_sm * slot_floats(tiles, D);
+    return (size_t)device_sms() * 2 * 4 * (tiles_wanted(dtype, T * G, D) && b > a ? b : a);
 }
 
 int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* cache, void* workspace, size_t workspace_bytes,
                           cudaStream_t st) {
-    const Plan g = plan_of(a->dtype, a->T * (a->Hq / a->Hk), a->D);
+    const int rows = a->T * (a->Hq / a->Hk);
+    const Plan g = plan_of(a->dtype, rows, a->D, tiles_wanted(a->dtype, rows, a->D) && tree_tiles_supported(a, cache));
     Params p{};
     p.q = a->q; p.k = cache->k; p.v = cache->v; p.out = a->out;
     for (int i = 0; i < 3; ++i) {
@@ -669,7 +678,9 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
         return set_error(CONVNN_E_WORKSPACE, "tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
                          (size_t)p.ctas * 2 * p.slot * 4);
     int rc;
-    if (a->dtype == CONVNN_F32) {
+    if (g.tiles) {
+        rc = launch_tree_tiles(p, st);
+    } else if (a->dtype == CONVNN_F32) {
         rc = g.stages == 3 ? launch_scalar<3>(p, g.smem, st) : launch_scalar<2>(p, g.smem, st);
     } else {
         switch (steps_of(p.D)) {
@@ -682,7 +693,8 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
         }
     }
     if (rc) return rc;
-    const dim3 grid((unsigned)units, (g.rows_per_tile + JOIN_ROWS - 1) / JOIN_ROWS);
+    const int joined = rows < g.rows_per_tile ? rows : g.rows_per_tile;
+    const dim3 grid((unsigned)units, (joined + JOIN_ROWS - 1) / JOIN_ROWS);
     if (a->dtype == CONVNN_F32) launch_chained(join_kernel<float>, grid, 32 * JOIN_ROWS, 0, st, p);
     else launch_chained(join_kernel<__nv_bfloat16>, grid, 32 * JOIN_ROWS, 0, st, p);
     CONVNN_CHECK_LAUNCH("tree_attention");

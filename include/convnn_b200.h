@@ -108,8 +108,8 @@ int convnn_b200_forwards_in_flight(int32_t n);
 /* No reference counterpart: reads the device-side error latch (synchronises the device).
  * 0 = no kernel gave up; otherwise the code of the first bounded wait that expired inside
  * a tensor-core kernel (similarity: 1 producer, 2/3 MMA issuer, 4 epilogue; GEMM: 11-16; pair
- * similarity: 21-26; streaming depthwise conv: 31; 8-bit product: 121-130).  A wait gives up after 250 ms.  Results of
- * a call that latched a code are undefined. */
+ * similarity: 21-26; streaming depthwise conv: 31; 8-bit product: 121-130; attention over a cache: 141-149).  A wait gives up after 250 ms.
+ * Results of a call that latched a code are undefined. */
 int convnn_b200_device_status(int* code);
 
 /* No reference counterpart: exercises the bounded wait every tensor-core kernel of this
