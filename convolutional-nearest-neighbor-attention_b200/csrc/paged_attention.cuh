@@ -31,6 +31,12 @@ struct Params {
     float* partial;                              // [2 * CTAs][rows_per_tile * (D + 2) + 4]
     long long slot;                              // floats of one of them
     int ctas;
+
+    // entry / page_size of an entry below 2^31: the product with 2^slot_shift / page_size, rounded up to 32 bits, is off by less than
+    // entry * page_size < 2^slot_shift
+    uint32_t slot_factor;
+    int slot_shift;
+    __device__ __forceinline__ int slot_at(int entry) const { return (int)(((unsigned long long)(unsigned)entry * slot_factor) >> slot_shift); }
 };
 
 // One sequence.
@@ -49,54 +55,58 @@ __device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
     s.row_tiles = (s.count * p.G + p.rows_per_tile - 1) / p.rows_per_tile;
     return s;
 }
-// Whole warp: tiles of all units, and of the sequences before b.
-__device__ __forceinline__ long long total_work(const Params& p, int b, long long& before) {
+// Whole warp: tiles of all units (fewer than 2^31), and of the sequences before b.
+__device__ __forceinline__ int total_work(const Params& p, int b, int& before) {
     const int lane = threadIdx.x & 31;
-    long long all = 0, first = 0;
+    int all = 0, first = 0;
     for (int i = lane; i < p.B; i += 32) {
-        const long long w = (long long)sequence_of(p, i).work() * p.Hk;
+        const int w = sequence_of(p, i).work() * p.Hk;
         all += w;
         if (i < b) first += w;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-        first += __shfl_xor_sync(0xffffffffu, first, o);
-    }
-    before = first;
-    return all;
+    before = (int)__reduce_add_sync(0xffffffffu, (unsigned)first);
+    return (int)__reduce_add_sync(0xffffffffu, (unsigned)all);
 }
-// CTAs that get tiles, one at least each.
-__device__ __forceinline__ int busy_ctas(long long work, int ctas) { return work < ctas ? (int)work : ctas; }
-__device__ __forceinline__ long long first_tile(long long work, int cta, int ctas) { return work * cta / ctas; }
-// The CTA that has tile `at`.
-__device__ __forceinline__ int cta_of(long long work, long long at, int ctas) { return (int)(((at + 1) * ctas - 1) / work); }
+// How the tiles are divided: `ctas` CTAs get some, the first `more` of them one more than the others.
+struct Division {
+    int ctas, each, more;
+    __device__ __forceinline__ Division(int work, int most) {
+        ctas = min(work, most);
+        each = ctas ? work / ctas : 0;
+        more = work - each * ctas;
+    }
+    __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, more); }
+    __device__ __forceinline__ int cta_of(int at) const {
+        const int rich = more * (each + 1);
+        return at < rich ? at / (each + 1) : more + (at - rich) / each;
+    }
+};
 
 // A CTA's way through its tiles.
 struct Cursor {
     Sequence s;
     int b, h, rt, tile;
-    long long left;                              // tiles that are still to come, this one included
+    int left;                                    // tiles that are still to come, this one included
 
     // Whole warp; the same in all lanes.
-    __device__ __forceinline__ void start(const Params& p, int cta, int ctas) {
+    __device__ __forceinline__ void start(const Params& p, int cta) {
+        int none;
+        const Division d(total_work(p, 0, none), p.ctas);
+        b = h = rt = tile = left = 0;
+        if (cta < d.ctas) find(p, d.first(cta), d.first(cta + 1) - d.first(cta));
+    }
+    // `count` tiles from `begin` on.
+    __device__ __forceinline__ void find(const Params& p, int begin, int count) {
         const int lane = threadIdx.x & 31;
-        long long none;
-        const long long work = total_work(p, 0, none);
-        ctas = busy_ctas(work, ctas);
-        b = h = rt = tile = 0;
-        left = 0;
-        if (cta >= ctas) return;
-        const long long begin = first_tile(work, cta, ctas);
-        left = first_tile(work, cta + 1, ctas) - begin;
-        long long before = 0;
+        left = count;
+        int before = 0;
         for (int b0 = 0;; b0 += 32) {
-            long long w = 0;
-            if (b0 + lane < p.B) w = (long long)sequence_of(p, b0 + lane).work() * p.Hk;
-            long long sum = w;
+            int w = 0;
+            if (b0 + lane < p.B) w = sequence_of(p, b0 + lane).work() * p.Hk;
+            int sum = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+                const int x = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += x;
             }
             const unsigned found = __ballot_sync(0xffffffffu, before + sum > begin);
@@ -109,7 +119,7 @@ struct Cursor {
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         s = sequence_of(p, b);
-        const int rest = (int)(begin - before);          // (of one sequence: its heads' tiles fit 31 bits)
+        const int rest = begin - before;
         h = rest / s.work();
         const int in_head = rest - h * s.work();
         rt = in_head / s.tiles;
@@ -127,7 +137,7 @@ struct Cursor {
         while (s.work() == 0);
     }
     // Tiles of the unit that belong to this CTA, and the next unit.
-    __device__ __forceinline__ int run() const { return left < s.tiles - tile ? (int)left : s.tiles - tile; }
+    __device__ __forceinline__ int run() const { return min(left, s.tiles - tile); }
     __device__ __forceinline__ void skip(const Params& p, int n) {
         tile += n - 1;
         left -= n - 1;
@@ -150,7 +160,7 @@ template <typename T>
 __device__ __forceinline__ float not_finite_seen(const Params& p, const Sequence& s, int b, int h, unsigned long long mask, int c) {
     float add = 0.f;
     for (int j = 0; j < s.total - s.length; ++j) {
-        const int entry = s.length + j, slot = entry / p.page_size;
+        const int entry = s.length + j, slot = p.slot_at(entry);
         const int page = p.table[b * p.table_stride + slot];
         if (!(mask >> j & 1) || (unsigned)page >= (unsigned)p.pages) continue;
         const float v = to_f32(static_cast<const T*>(p.v)[page * p.vs[0] + h * p.vs[1] + (entry - slot * p.page_size) * p.vs[2] + c]);

@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& rest) {
 
 // The page that holds entry `entry` of sequence b, -1: none.
 __device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& row) {
-    const int slot = entry / p.page_size;
+    const int slot = p.slot_at(entry);
     row = entry - slot * p.page_size;
     const int page = p.table[b * p.table_stride + slot];
     return (unsigned)page < (unsigned)p.pages ? page : -1;
@@ -71,15 +71,17 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t own = smem_at(ring) + warp * (STAGES * STAGE);
 
-    for (int i = threadIdx.x; i < (SLICE + kWarps * STAGES * STAGE) / 16; i += kThreads) {
-        uint8_t* at = i < SLICE / 16 ? sQ + 16 * i : ring + 16 * (i - SLICE / 16);
-        *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+    if (p.D != DP) {                                                     // channels behind D are zeros
+        for (int i = threadIdx.x; i < (SLICE + kWarps * STAGES * STAGE) / 16; i += kThreads) {
+            uint8_t* at = i < SLICE / 16 ? sQ + 16 * i : ring + 16 * (i - SLICE / 16);
+            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     chain_begin();
 
     Cursor at;
-    at.start(p, blockIdx.x, p.ctas);
+    at.start(p, blockIdx.x);
     if (at.left == 0) return;                                            // (the whole CTA)
     Cursor ahead = at;
     const int chunks = p.D / 8;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
     chain_begin();
 
     Cursor at;
-    at.start(p, blockIdx.x, p.ctas);
+    at.start(p, blockIdx.x);
     if (at.left == 0) return;
     Cursor ahead = at;
     auto fetch = [&](int stage) {
@@ -519,66 +521,130 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
 
 // ---- units that several CTAs had ------------------------------------------------------------------------------------------------
 
-// A warp per row of a unit: the pieces' maxima, then their sums, in the order of the keys.
-constexpr int JOIN_ROWS = 4;
-template <typename T>
-__global__ void __launch_bounds__(32 * JOIN_ROWS) join_kernel(const Params p) {
-    chain_begin();
+// The pieces' maxima, then their sums, in the order of the keys.  WARPS of a block's four warps share the pieces of a row: all four where
+// units have several pieces each (a block per unit and row), else a warp goes through every fourth row of 16 of one unit (a block per
+// boundary between two CTAs' tiles, and the unit that is cut there first belongs to it).
+// What says which pieces there are is read while the kernel before is still at work: it does not write that.
+constexpr int JOIN_ROWS = 16;
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
+    __shared__ float4 sY[WARPS == 4 ? 4 : 1][2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x, b = unit / (p.Hk * p.row_tiles), rest = unit - b * p.Hk * p.row_tiles;
-    const int h = rest / p.row_tiles, rt = rest - h * p.row_tiles;
-    const int r = blockIdx.y * JOIN_ROWS + warp, row = rt * p.rows_per_tile + r, t = row / p.G, g = row - t * p.G;
-    if (r >= p.rows_per_tile || t >= p.T) return;                        // (a whole warp)
-    const Sequence s = sequence_of(p, b);
-    T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2];
-    if (t >= s.count || s.total == 0) {                                  // nothing is there, or nothing to attend to
-        for (int c = lane; c < p.D; c += 32) out[c] = from_f32<T>(0.f);
-        return;
+    Sequence s{};
+    int b = 0, h = 0, rt = 0, c0 = 0, c1 = 0;
+    bool second = false;                         // the first piece is its CTA's last unit
+    {
+        int before;
+        if (WARPS == 4) {
+            const int unit = blockIdx.x, rest = unit % (p.Hk * p.row_tiles);
+            b = unit / (p.Hk * p.row_tiles);
+            h = rest / p.row_tiles;
+            rt = rest - h * p.row_tiles;
+            s = sequence_of(p, b);
+            const Division d(total_work(p, b, before), p.ctas);
+            if (rt < s.row_tiles && s.tiles) {
+                const int begin = before + (h * s.row_tiles + rt) * s.tiles;
+                c0 = d.cta_of(begin);
+                c1 = d.cta_of(begin + s.tiles - 1);
+                second = d.first(c0) < begin;
+            }
+        } else {
+            const Division d(total_work(p, 0, before), p.ctas);
+            const int c = blockIdx.x;
+            if (c > 0 && c < d.ctas) {
+                Cursor at;
+                at.find(p, d.first(c), 1);
+                const int begin = d.first(c) - at.tile;
+                if (at.tile && d.cta_of(begin) == c - 1) {
+                    b = at.b; h = at.h; rt = at.rt;
+                    s = at.s;
+                    c0 = c - 1;
+                    c1 = d.cta_of(begin + s.tiles - 1);
+                    second = d.first(c0) < begin;
+                }
+            }
+        }
     }
-    long long before;
-    const long long work = total_work(p, b, before), begin = before + ((long long)h * s.row_tiles + rt) * s.tiles;
-    const int ctas = busy_ctas(work, p.ctas);
-    const int c0 = cta_of(work, begin, ctas), c1 = cta_of(work, begin + s.tiles - 1, ctas);
-    if (c0 == c1) return;                                                // (written by its CTA)
-    float top = -CUDART_INF_F;
-    bool bad = false;
+    chain_begin();
+    // rows without anything, of all sequences
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * kWarps + warp; i < p.B * p.T; i += gridDim.x * gridDim.y * kWarps) {
+        const int zb = i / p.T, t = i - zb * p.T;
+        const Sequence z = sequence_of(p, zb);
+        if (t < z.count && z.total) continue;
+        T* out = static_cast<T*>(p.out) + zb * p.os[0] + t * p.os[1];
+        for (int hh = 0; hh < p.Hk * p.G; ++hh)
+            for (int c = lane; c < p.D; c += 32) out[hh * p.os[2] + c] = from_f32<T>(0.f);
+    }
+    if (c0 == c1) return;                        // (written by its CTA, or not this block's)
     const long long tail = (long long)p.rows_per_tile * p.D;
-    for (int c = c0 + lane; c <= c1; c += 32) {
-        const float* slot = slot_of(p, c, first_tile(work, c, ctas) >= begin);
-        top = fmaxf(top, slot[tail + r]);
-        bad |= slot[tail + 2 * p.rows_per_tile] != 0.f;
-    }
+    auto piece = [&](int c) { return slot_of(p, c, c > c0 || !second); };
+#pragma unroll 1
+    for (int i = 0; i < (WARPS == 4 ? 1 : JOIN_ROWS / kWarps); ++i) {
+        const int r = WARPS == 4 ? blockIdx.y : blockIdx.y * JOIN_ROWS + i * kWarps + warp;
+        const int row = rt * p.rows_per_tile + r, t = row / p.G, g = row - t * p.G;
+        if (r >= p.rows_per_tile || t >= s.count) return;                // (the whole block, or a warp that meets no other)
+        float top = -CUDART_INF_F, sum = 0.f;
+        bool bad = false;
+        for (int c = c0 + lane; c <= c1; c += 32) {
+            const float* from = piece(c) + tail;
+            top = fmaxf(top, from[r]);
+            bad |= from[2 * p.rows_per_tile] != 0.f;
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    bad = __any_sync(0xffffffffu, bad);
-    if (top == -CUDART_INF_F) top = 0.f;
-    float sum = 0.f;
-    float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-        const float* slot = slot_of(p, c, first_tile(work, c, ctas) >= begin);
-        const float f = ex2(slot[tail + r] - top);
-        sum = fmaf(slot[tail + p.rows_per_tile + r], f, sum);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bad = __any_sync(0xffffffffu, bad);
+        if (top == -CUDART_INF_F) top = 0.f;
+        for (int c = c0 + lane; c <= c1; c += 32) {
+            const float* from = piece(c) + tail;
+            sum = fmaf(from[p.rows_per_tile + r], ex2(from[r] - top), sum);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 8
+        for (int c = c0 + (WARPS == 4 ? warp : 0); c <= c1; c += WARPS) {
+            const float* from = piece(c);
+            const float f = ex2(from[tail + r] - top);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int col = 4 * (lane + 32 * u);
+                if (col >= p.D) continue;
+                const float4 x = *reinterpret_cast<const float4*>(from + (long long)r * p.D + col);
+                y[u].x = fmaf(x.x, f, y[u].x); y[u].y = fmaf(x.y, f, y[u].y);
+                y[u].z = fmaf(x.z, f, y[u].z); y[u].w = fmaf(x.w, f, y[u].w);
+            }
+        }
+        if (WARPS == 4) {
+            sY[warp][0][lane] = y[0];
+            sY[warp][1][lane] = y[1];
+            __syncthreads();
+            if (warp) return;
+#pragma unroll
+            for (int w = 1; w < 4; ++w)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float4 x = sY[w % WARPS][u][lane];
+                    y[u].x += x.x; y[u].y += x.y; y[u].z += x.z; y[u].w += x.w;
+                }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int col = 4 * (lane + 32 * u);
             if (col >= p.D) continue;
-            const float4 x = *reinterpret_cast<const float4*>(slot + (long long)r * p.D + col);
-            y[u].x = fmaf(x.x, f, y[u].x); y[u].y = fmaf(x.y, f, y[u].y);
-            y[u].z = fmaf(x.z, f, y[u].z); y[u].w = fmaf(x.w, f, y[u].w);
+            float x[4] = {y[u].x * inv, y[u].y * inv, y[u].z * inv, y[u].w * inv};
+            if (bad) {
+                const unsigned long long mask = seen_by(p, s, b, row);
+                for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
+            }
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4*>(out + col) = make_float4(x[0], x[1], x[2], x[3]);
+            } else {
+                __nv_bfloat162 w[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+                *reinterpret_cast<uint2*>(out + col) = *reinterpret_cast<uint2*>(w);
+            }
         }
-    }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const unsigned long long mask = seen_by(p, s, b, row);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int col = 4 * (lane + 32 * u);
-        if (col >= p.D) continue;
-        float x[4] = {y[u].x * inv, y[u].y * inv, y[u].z * inv, y[u].w * inv};
-        if (bad)
-            for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[col + e] = from_f32<T>(x[e]);
     }
 }
 
@@ -671,8 +737,12 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     p.partial = static_cast<float*>(workspace);
     p.slot = slot_floats(g, p.D);
     p.ctas = device_sms() * g.ctas_per_sm;
+    int bits = 0;
+    while ((1ll << bits) < p.page_size) ++bits;
+    p.slot_shift = 31 + bits;
+    p.slot_factor = (uint32_t)(((1ull << p.slot_shift) + p.page_size - 1) / p.page_size);
     const long long units = (long long)p.B * p.Hk * p.row_tiles, keys = (long long)p.width * p.page_size;
-    if (units > 0x7fffffffll || (keys + p.tile - 1) / p.tile * p.row_tiles * p.Hk > 0x7fffffffll)
+    if (units > 0x7fffffffll || (double)units * (double)((keys + p.tile - 1) / p.tile) > 2147483647.0)
         return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %lld units of up to %lld keys", units, keys);
     if (workspace_bytes < (size_t)p.ctas * 2 * p.slot * 4)
         return set_error(CONVNN_E_WORKSPACE, "tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
@@ -694,9 +764,15 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     }
     if (rc) return rc;
     const int joined = rows < g.rows_per_tile ? rows : g.rows_per_tile;
-    const dim3 grid((unsigned)units, (joined + JOIN_ROWS - 1) / JOIN_ROWS);
-    if (a->dtype == CONVNN_F32) launch_chained(join_kernel<float>, grid, 32 * JOIN_ROWS, 0, st, p);
-    else launch_chained(join_kernel<__nv_bfloat16>, grid, 32 * JOIN_ROWS, 0, st, p);
+    const bool many = units * 4 <= p.ctas;                   // pieces a unit
+    const dim3 grid = many ? dim3((unsigned)units, joined) : dim3(p.ctas, (joined + JOIN_ROWS - 1) / JOIN_ROWS);
+    if (a->dtype == CONVNN_F32) {
+        if (many) launch_chained(join_kernel<float, 4>, grid, kThreads, 0, st, p);
+        else launch_chained(join_kernel<float, 1>, grid, kThreads, 0, st, p);
+    } else {
+        if (many) launch_chained(join_kernel<__nv_bfloat16, 4>, grid, kThreads, 0, st, p);
+        else launch_chained(join_kernel<__nv_bfloat16, 1>, grid, kThreads, 0, st, p);
+    }
     CONVNN_CHECK_LAUNCH("tree_attention");
     return CONVNN_OK;
 }

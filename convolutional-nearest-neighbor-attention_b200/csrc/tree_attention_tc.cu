@@ -98,8 +98,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    // (what q's rows leave open stays zero: channels behind D)
-    for (uint32_t i = threadIdx.x; i < kTileBytes / 16; i += kTileThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+    // (channels behind D, which q's rows leave open, stay zeros)
+    if (p.D % 16)
+      for (uint32_t i = threadIdx.x; i < kTileBytes / 16; i += kTileThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -108,7 +109,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 
     const int steps = (p.D + 15) / 16;                       // of 16 channels
     Cursor at;
-    at.start(p, blockIdx.x, p.ctas);
+    at.start(p, blockIdx.x);
     uint32_t it = 0;                                         // tiles so far
 
     if (warp == 0) {
@@ -119,7 +120,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             const int n = at.run();
             for (int j = 0; j < n; ++j, ++it) {
                 const uint32_t stage = it % STAGES, ph = (it / STAGES) & 1u;
-                const int entry = (at.tile + j) * kKeys + lane * tm.box, slot = entry / p.page_size, row = entry - slot * p.page_size;
+                const int entry = (at.tile + j) * kKeys + lane * tm.box, slot = p.slot_at(entry), row = entry - slot * p.page_size;
                 int page = -1;
                 if (lane < tm.boxes && entry < at.s.total) page = p.table[at.b * p.table_stride + slot];
                 if ((unsigned)page >= (unsigned)p.pages) page = p.pages;      // outside the map: zeros
