@@ -4,8 +4,9 @@
 //   (n_a, n_b) -> (n_a cos_i - n_b sin_i, n_b cos_i + n_a sin_i)   on the pairs (i, i + R/2), or neighbours (2i, 2i + 1), i < R/2
 // rounded once, to the storage type.  Values are copied as they are.
 // A group of lanes owns a head: each lane two vectors of V channels, those of a pair where pairs lie R/2 apart, so that the rotation
-// needs no exchange and the norm's sum log2(lanes) of them.  A group keeps its token: cosines, sines and weights are loaded once and
-// serve all of its heads, U of which are requested before the first is used.
+// needs no exchange and the norm's sum log2(lanes) of them.  A group keeps its U heads, all queries', all keys' or all values', and goes
+// from token to token with their weight in registers; cosines and sines serve the U heads, whose values are requested before the first is
+// used.  Groups that share a token are neighbours: a warp reads its heads as one stretch.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -24,8 +25,9 @@ struct HeadsParams {
     const int32_t *positions, *table, *lengths, *counts;
     long long rope_stride, pos_stride[2], table_stride;
     int rope_rows, pages, page_size, width;
-    unsigned tokens, parts;                              // B * T; groups that share a token's heads
-    int T, Hq, Hk, heads, D, half, interleaved;          // heads: with the values'; half = R / 2
+    unsigned tokens, parts, abreast;                     // B * T; groups that share a token's heads; tokens at a time
+    int parts_q, parts_k;
+    int T, Hq, Hk, D, half, interleaved;                 // half = R / 2
     float eps, inv_d;
 };
 
@@ -72,174 +74,170 @@ __device__ __forceinline__ typename Vec<T, V>::type narrow(const float (&x)[V]) 
 
 // LPH lanes a head, N pairs of vectors a lane (several only where V = 1), U heads at once.
 template <typename T, int V, int LPH, int N, int U>
-__global__ void __launch_bounds__(kThreads) heads_kernel(const HeadsParams p) {
+__global__ void __launch_bounds__(kThreads, 2) heads_kernel(const HeadsParams p) {
     using Raw = typename Vec<T, V>::type;
     chain_begin();
-    const unsigned unit = blockIdx.x * (unsigned)(kThreads / LPH) + threadIdx.x / LPH;
-    const unsigned token = unit / p.parts;
-    if (token >= p.tokens) return;                       // (a whole group, and no exchange leaves its group)
-    const int part = (int)(unit - token * p.parts), lane = threadIdx.x % LPH;
+    const unsigned unit = blockIdx.x * (unsigned)(kThreads / LPH) + threadIdx.x / LPH, first = unit / p.parts;
+    if (first >= p.abreast) return;                      // (a whole group, and no exchange leaves its group)
+    const int part = (int)(unit - first * p.parts), lane = threadIdx.x % LPH;
     const unsigned group_mask = LPH == 32 ? 0xffffffffu : ((1u << (LPH % 32)) - 1u) << ((threadIdx.x & 31u) / LPH * LPH);
-    const int b = (int)(token / (unsigned)p.T), t = (int)(token - (unsigned)b * (unsigned)p.T);
 
-    // where the token is, and where it goes
-    long long position = t;
-    bool live = true;
-    long long dst_page = 0, dst_row = 0;
-    bool stored = true;
-    if (p.table) {
-        live = !p.counts || t < p.counts[b];
-        const long long length = p.lengths[b], entry = (length > 0 ? length : 0) + t, slot = entry / p.page_size;
-        position = entry;
-        int page = -1;
-        if (live && slot < p.width) page = p.table[b * p.table_stride + slot];
-        stored = (unsigned)page < (unsigned)p.pages;     // (a page that is not there keeps nothing)
-        dst_page = page;
-        dst_row = entry - slot * p.page_size;
-    }
-    if (p.positions) position = p.positions[b * p.pos_stride[0] + t * p.pos_stride[1]];
+    // the group's heads
+    const bool is_q = part < p.parts_q, is_v = part >= p.parts_q + p.parts_k;
+    const int h0 = (is_q ? part : part - p.parts_q - (is_v ? p.parts_k : 0)) * U, count = min(U, (is_q ? p.Hq : p.Hk) - h0);
+    const long long *ss = is_q ? p.qs : is_v ? p.vs : p.ks, *ds = is_q ? p.qo : is_v ? p.vo : p.ko;
+    const long long s0 = ss[0], s1 = ss[1], s2 = ss[2], d0 = ds[0], d1 = ds[1], d2 = ds[2];
+    const T* from = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + h0 * s2;
+    T* to = static_cast<T*>(is_q ? p.q_out : is_v ? p.v_out : p.k_out) + h0 * d2;
+    const T* weight = static_cast<const T*>(is_q ? p.wq : is_v ? nullptr : p.wk);
+    const bool normed = weight != nullptr, turn = !is_v && p.half, paged = p.table != nullptr && !is_q;
 
-    // the lane's channels: two vectors each, their cosines and sines
-    int c0[N], c1[N];
-    float cs[N][V], sn[N][V];
+    // the lane's channels: two vectors each, and their place in the table of cosines and sines
+    int c0[N], c1[N], place[N];
+    Raw w0[N], w1[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int pair = lane + n * LPH;                 // of vectors
         const int turned = p.half / V;                   // pairs of vectors that are rotated
-        int at = -1;                                     // their place in the table
+        place[n] = -1;
         if (p.interleaved) {
             c0[n] = 2 * V * pair;
             c1[n] = c0[n] + V;
-            if (pair < turned) at = V * pair;
+            if (pair < turned) place[n] = V * pair;
         } else if (pair < turned) {
             c0[n] = V * pair;
             c1[n] = c0[n] + p.half;
-            at = c0[n];
+            place[n] = c0[n];
         } else {
             c0[n] = 2 * p.half + 2 * V * (pair - turned);
             c1[n] = c0[n] + V;
         }
-        if (at >= 0 && (unsigned long long)position < (unsigned long long)p.rope_rows) {
-            const float* row = p.rope + position * p.rope_stride + at;
-            if constexpr (V % 4 == 0) {
-#pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    *reinterpret_cast<float4*>(&cs[n][e]) = *reinterpret_cast<const float4*>(row + e);
-                    *reinterpret_cast<float4*>(&sn[n][e]) = *reinterpret_cast<const float4*>(row + p.half + e);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    cs[n][e] = row[e];
-                    sn[n][e] = row[p.half + e];
-                }
-            }
-        } else {                                         // not rotated; or no such position, which shows
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                cs[n][e] = at >= 0 ? CUDART_NAN_F : 1.f;
-                sn[n][e] = at >= 0 ? CUDART_NAN_F : 0.f;
-            }
-        }
+        w0[n] = w1[n] = Raw{};
+        if (normed && c0[n] < p.D) w0[n] = *reinterpret_cast<const Raw*>(weight + c0[n]);
+        if (normed && c1[n] < p.D) w1[n] = *reinterpret_cast<const Raw*>(weight + c1[n]);
     }
-    Raw wq0[N], wq1[N], wk0[N], wk1[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        wq0[n] = wq1[n] = wk0[n] = wk1[n] = Raw{};
-        if (p.wq && c0[n] < p.D) wq0[n] = *reinterpret_cast<const Raw*>(static_cast<const T*>(p.wq) + c0[n]);
-        if (p.wq && c1[n] < p.D) wq1[n] = *reinterpret_cast<const Raw*>(static_cast<const T*>(p.wq) + c1[n]);
-        if (p.wk && c0[n] < p.D) wk0[n] = *reinterpret_cast<const Raw*>(static_cast<const T*>(p.wk) + c0[n]);
-        if (p.wk && c1[n] < p.D) wk1[n] = *reinterpret_cast<const Raw*>(static_cast<const T*>(p.wk) + c1[n]);
-    }
-
-    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + t * p.qs[1];
-    const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + t * p.ks[1];
-    const T* v = static_cast<const T*>(p.v) + b * p.vs[0] + t * p.vs[1];
-    T* qo = static_cast<T*>(p.q_out) + b * p.qo[0] + t * p.qo[1];
-    T* ko = static_cast<T*>(p.k_out) + (p.table ? dst_page : b) * p.ko[0] + (p.table ? dst_row : t) * p.ko[1];
-    T* vo = static_cast<T*>(p.v_out) + dst_page * p.vo[0] + dst_row * p.vo[1];
-    const int keys = p.Hq + p.Hk;
 
 #pragma unroll 1
-    for (int h0 = part * U; h0 < p.heads; h0 += (int)p.parts * U) {
+    for (unsigned token = first; token < p.tokens; token += p.abreast) {
+        const int b = (int)(token / (unsigned)p.T), t = (int)(token - (unsigned)b * (unsigned)p.T);
+        const T* src = from + b * s0 + t * s1;
         Raw x0[U][N], x1[U][N];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + u;
-            const T* src = h < p.Hq ? q + h * p.qs[2] : h < keys ? k + (h - p.Hq) * p.ks[2] : v + (h - keys) * p.vs[2];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 x0[u][n] = x1[u][n] = Raw{};
-                if (h < p.heads && c0[n] < p.D) x0[u][n] = *reinterpret_cast<const Raw*>(src + c0[n]);
-                if (h < p.heads && c1[n] < p.D) x1[u][n] = *reinterpret_cast<const Raw*>(src + c1[n]);
+                if (u < count && c0[n] < p.D) x0[u][n] = *reinterpret_cast<const Raw*>(src + u * s2 + c0[n]);
+                if (u < count && c1[n] < p.D) x1[u][n] = *reinterpret_cast<const Raw*>(src + u * s2 + c1[n]);
+            }
+        // where the token is, and where it goes
+        long long position = t;
+        bool live = true, stored = true;
+        T* dst = to + b * d0 + t * d1;
+        if (p.table) {
+            live = !p.counts || t < p.counts[b];
+            const unsigned entry = (unsigned)max(p.lengths[b], 0) + (unsigned)t, slot = entry / (unsigned)p.page_size;   // (below 2^32)
+            position = entry;
+            if (paged) {
+                int page = -1;
+                if (live && slot < (unsigned)p.width) page = p.table[b * p.table_stride + slot];
+                stored = (unsigned)page < (unsigned)p.pages;                 // (a page that is not there keeps nothing)
+                dst = to + page * d0 + (long long)(entry - slot * p.page_size) * d1;
+            }
+        }
+        float cs[N][V], sn[N][V];
+        if (turn) {
+            if (p.positions) position = p.positions[b * p.pos_stride[0] + t * p.pos_stride[1]];
+            const bool there = (unsigned long long)position < (unsigned long long)p.rope_rows;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const float* row = p.rope + position * p.rope_stride + place[n];
+                if (place[n] >= 0 && there) {
+                    if constexpr (V % 4 == 0) {
+#pragma unroll
+                        for (int e = 0; e < V; e += 4) {
+                            *reinterpret_cast<float4*>(&cs[n][e]) = *reinterpret_cast<const float4*>(row + e);
+                            *reinterpret_cast<float4*>(&sn[n][e]) = *reinterpret_cast<const float4*>(row + p.half + e);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            cs[n][e] = row[e];
+                            sn[n][e] = row[p.half + e];
+                        }
+                    }
+                } else {                                 // not rotated; or no such position, which shows
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        cs[n][e] = place[n] >= 0 ? CUDART_NAN_F : 1.f;
+                        sn[n][e] = place[n] >= 0 ? CUDART_NAN_F : 0.f;
+                    }
+                }
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = h0 + u;
-            if (h >= p.heads) break;                     // (the same for the whole group)
-            const bool is_q = h < p.Hq, is_v = h >= keys;
-            T* dst = is_q ? qo + h * p.qo[2] : is_v ? vo + (h - keys) * p.vo[2] : ko + (h - p.Hq) * p.ko[2];
-            const bool normed = is_q ? p.wq != nullptr : !is_v && p.wk != nullptr;
-            const bool store = is_q || stored;
-            float a[N][V], c[N][V];
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                widen<T, V>(a[n], x0[u][n]);
-                widen<T, V>(c[n], x1[u][n]);
-            }
-            if (normed) {
-                float sum = 0.f;
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) sum = fmaf(a[n][e], a[n][e], fmaf(c[n][e], c[n][e], sum));
-#pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
-                const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+            if (u >= count) break;                   // (the same for the whole group)
+            if (normed || turn) {
+                float a[N][V], c[N][V];
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    float w0[V], w1[V];
-                    widen<T, V>(w0, is_q ? wq0[n] : wk0[n]);
-                    widen<T, V>(w1, is_q ? wq1[n] : wk1[n]);
+                    widen<T, V>(a[n], x0[u][n]);
+                    widen<T, V>(c[n], x1[u][n]);
+                }
+                if (normed) {
+                    float sum = 0.f;
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        a[n][e] *= r * w0[e];
-                        c[n][e] *= r * w1[e];
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) sum = fmaf(a[n][e], a[n][e], fmaf(c[n][e], c[n][e], sum));
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
+                    const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        float g0[V], g1[V];
+                        widen<T, V>(g0, w0[n]);
+                        widen<T, V>(g1, w1[n]);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            a[n][e] *= r * g0[e];
+                            c[n][e] *= r * g1[e];
+                        }
                     }
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    if (turn) {
+                        if (!p.interleaved || V == 1) {
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                const float y = a[n][e] * cs[n][e] - c[n][e] * sn[n][e];
+                                c[n][e] = c[n][e] * cs[n][e] + a[n][e] * sn[n][e];
+                                a[n][e] = y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; e += 2) {
+                                const int i = e / 2, j = V / 2 + e / 2, e1 = (e + 1) % V;
+                                const float y = a[n][e] * cs[n][i] - a[n][e1] * sn[n][i];
+                                a[n][e1] = a[n][e1] * cs[n][i] + a[n][e] * sn[n][i];
+                                a[n][e] = y;
+                                const float z = c[n][e] * cs[n][j] - c[n][e1] * sn[n][j];
+                                c[n][e1] = c[n][e1] * cs[n][j] + c[n][e] * sn[n][j];
+                                c[n][e] = z;
+                            }
+                        }
+                    }
+                    x0[u][n] = narrow<T, V>(a[n]);
+                    x1[u][n] = narrow<T, V>(c[n]);
                 }
             }
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                if (!is_v && p.half) {
-                    if (!p.interleaved || V == 1) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float y = a[n][e] * cs[n][e] - c[n][e] * sn[n][e];
-                            c[n][e] = c[n][e] * cs[n][e] + a[n][e] * sn[n][e];
-                            a[n][e] = y;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < V; e += 2) {
-                            const int i = e / 2, j = V / 2 + e / 2, e1 = (e + 1) % V;
-                            const float y = a[n][e] * cs[n][i] - a[n][e1] * sn[n][i];
-                            a[n][e1] = a[n][e1] * cs[n][i] + a[n][e] * sn[n][i];
-                            a[n][e] = y;
-                            const float z = c[n][e] * cs[n][j] - c[n][e1] * sn[n][j];
-                            c[n][e1] = c[n][e1] * cs[n][j] + c[n][e] * sn[n][j];
-                            c[n][e] = z;
-                        }
-                    }
-                }
-                Raw y0 = x0[u][n], y1 = x1[u][n];
-                if (!is_v && (normed || p.half)) {
-                    y0 = narrow<T, V>(a[n]);
-                    y1 = narrow<T, V>(c[n]);
-                }
-                if (is_q && !live) y0 = y1 = Raw{};
-                if (store && c0[n] < p.D) *reinterpret_cast<Raw*>(dst + c0[n]) = y0;
-                if (store && c1[n] < p.D) *reinterpret_cast<Raw*>(dst + c1[n]) = y1;
+                if (is_q && !live) x0[u][n] = x1[u][n] = Raw{};
+                if (stored && c0[n] < p.D) *reinterpret_cast<Raw*>(dst + u * d2 + c0[n]) = x0[u][n];
+                if (stored && c1[n] < p.D) *reinterpret_cast<Raw*>(dst + u * d2 + c1[n]) = x1[u][n];
             }
         }
     }
@@ -247,14 +245,15 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(const HeadsParams p) {
 
 template <typename T, int V, int LPH, int N, int U>
 int launch_group(HeadsParams& p, cudaStream_t st) {
-    // as few groups to a token as still fill the device: a group's set-up costs as much as two heads
-    const unsigned most = (unsigned)((p.heads + U - 1) / U);
-    const long long wanted = (long long)device_sms() * 2 * kThreads / LPH;
-    long long parts = (wanted + p.tokens - 1) / p.tokens;
-    p.parts = parts < 1 ? 1u : parts > most ? most : (unsigned)parts;
-    const long long groups = (long long)p.tokens * p.parts, grid = (groups * LPH + kThreads - 1) / kThreads;
-    if (groups > 0x7fffffffll) return set_error(CONVNN_E_UNSUPPORTED, "qk_norm_rope: %lld groups of heads", groups);
-    launch_chained(heads_kernel<T, V, LPH, N, U>, (unsigned)grid, kThreads, 0, st, p);
+    p.parts_q = (p.Hq + U - 1) / U;
+    p.parts_k = (p.Hk + U - 1) / U;
+    p.parts = (unsigned)(p.parts_q + p.parts_k * (p.v ? 2 : 1));
+    // as many groups as are resident at once, two CTAs an SM: each has its set-up behind it after one token
+    const long long resident = (long long)device_sms() * 2 * (kThreads / LPH);
+    const long long abreast = resident / p.parts < 1 ? 1 : resident / p.parts;
+    p.abreast = abreast < p.tokens ? (unsigned)abreast : p.tokens;
+    const unsigned grid = (unsigned)(((long long)p.abreast * p.parts + kThreads / LPH - 1) / (kThreads / LPH));
+    launch_chained(heads_kernel<T, V, LPH, N, U>, grid, kThreads, 0, st, p);
     CONVNN_CHECK_LAUNCH("qk_norm_rope");
     return CONVNN_OK;
 }
@@ -315,7 +314,6 @@ int launch_heads(const convnn_heads* h, const convnn_cache* cache, const int32_t
     p.pos_stride[0] = h->position_stride[0]; p.pos_stride[1] = h->position_stride[1];
     p.T = h->T; p.tokens = (unsigned)h->B * (unsigned)h->T;
     p.Hq = h->q ? h->Hq : 0; p.Hk = h->k ? h->Hk : 0;
-    p.heads = p.Hq + p.Hk + (cache ? p.Hk : 0);
     p.D = h->D; p.half = h->rope ? h->rotary / 2 : 0; p.interleaved = h->interleaved;
     p.eps = h->eps; p.inv_d = 1.0f / (float)h->D;
     return h->dtype == CONVNN_F32 ? launch_of<float>(p, st) : launch_of<__nv_bfloat16>(p, st);
