@@ -667,7 +667,8 @@ Plan plan_of(int dtype, int rows, int D, bool tiles) {
     Plan g{};
     if (tiles) {
         g.tiles = true;
-        g.rows_per_tile = g.tile = 128;
+        g.rows_per_tile = rows > 128 ? 256 : 128;
+        g.tile = 128;
         g.ctas_per_sm = 1;
         return g;
     }

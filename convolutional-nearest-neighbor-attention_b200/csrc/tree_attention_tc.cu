@@ -1,13 +1,14 @@
 // Attention of drafted tokens over a paged cache on the tensor cores: a tile of 128 query rows of one sequence and key head against
 // tiles of 128 keys (tree_attention.cu has the formulas, the division of the work and the join).
+// A unit's work is two streams, each with scores, weights and an accumulator of its own in tensor memory, so that one's exponentials run
+// while the other's products do: with up to 128 rows the even and the odd tiles of keys, whose accumulators are added at the unit's end,
+// with more two tiles of rows, which share every tile of keys and values.
 //   warp 0     copies: the pages that hold a tile's keys and values, a box per page (or part of one) and 64 channels, 128-byte
 //              swizzled; pages that are not there by a coordinate outside the map, which fills zeros
 //   warp 1     products.  S = Q K^T (both from shared memory, K-major) and O += P V (P from tensor memory, V as it lies in its pages:
 //              channels side by side are rows along N).  Neither the scores nor their weights leave the SM's tensor memory.
-//   warps 2-9  softmax, in two groups of four: a thread owns a row, the groups take the unit's tiles in turn, each with a maximum, a
-//              sum and an accumulator of its own, so that one group's exponentials run while the other's products do.  A maximum is
-//              replaced, and the accumulator multiplied, only when a tile exceeds it by 2^8 (float32 holds what that leaves).
-// At the unit's end the two accumulators are added, each group writing half of the channels.
+//   warps 4-11 softmax, a group of four for each stream: a thread owns a row, with a maximum and a sum.  The maximum is replaced, and
+//              the accumulator multiplied, only when a tile exceeds it by 2^8 (float32 holds what that leaves).
 // A weight is rounded to one bfloat16 for its product (a second part would cost half the tensor cores' time); its sum is of the
 // unrounded ones.
 #include "f32x2.cuh"
@@ -23,7 +24,7 @@ namespace {
 using namespace sm100;
 using namespace paged;
 
-constexpr int kRows = 128, kKeys = kTileKeys, kTileThreads = 320;
+constexpr int kRows = 128, kKeys = kTileKeys, kTileThreads = 384;
 constexpr uint32_t kChunk = 128 * 128;        // 128 rows of 64 channels
 
 struct TileMaps {
@@ -54,20 +55,25 @@ __device__ __forceinline__ void tie16(uint32_t (&r)[16]) {
 // The two softmax groups.
 __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// DC columns of 64 channels, STAGES tiles of keys and of values in flight.
-template <int DC, int STAGES>
+// Registers move from the warps that copy and multiply to those that hold a row of scores: 56 + 2 * 216 of the 3 * 168 a thread that the
+// block starts with.
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// DC columns of 64 channels, KS tiles of keys and VS of values in flight; TWO: tiles of rows, else tiles of keys as the two streams.
+template <int DC, int KS, int VS, bool TWO>
 __global__ void __launch_bounds__(kTileThreads, 1)
 tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p, const TileMaps tm) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     constexpr uint32_t kTileBytes = DC * kChunk;
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + kTileBytes;
-    uint8_t* sV = sK + STAGES * kTileBytes;
-    float2* sScale = reinterpret_cast<float2*>(sV + STAGES * kTileBytes);    // [128]
+    uint8_t* sK = sQ + (TWO ? 2 : 1) * kTileBytes;
+    uint8_t* sV = sK + KS * kTileBytes;
+    float2* sScale = reinterpret_cast<float2*>(sV + VS * kTileBytes);        // [128]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kRows);
-    uint64_t *k_full = bars, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
-    uint64_t *s_full = v_empty + STAGES, *p_ready = s_full + 2, *o_done = p_ready + 2, *q_ready = o_done + 2, *drained = q_ready + 1;
+    uint64_t *k_full = bars, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
+    uint64_t *s_full = v_empty + VS, *p_ready = s_full + 2, *o_done = p_ready + 2, *q_ready = o_done + 2, *drained = q_ready + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* sBad = reinterpret_cast<int*>(tmem_slot + 2);
@@ -75,9 +81,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
+        for (int i = 0; i < KS; ++i) {
             mbar_init(k_full + i, 1);
             mbar_init(k_empty + i, 1);
+        }
+        for (int i = 0; i < VS; ++i) {
             mbar_init(v_full + i, 1);
             mbar_init(v_empty + i, 1);
         }
@@ -100,7 +108,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     }
     // (channels behind D, which q's rows leave open, stay zeros)
     if (p.D % 16)
-      for (uint32_t i = threadIdx.x; i < kTileBytes / 16; i += kTileThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+        for (uint32_t i = threadIdx.x; i < (TWO ? 2 : 1) * kTileBytes / 16; i += kTileThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -110,76 +118,77 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     const int steps = (p.D + 15) / 16;                       // of 16 channels
     Cursor at;
     at.start(p, blockIdx.x);
-    uint32_t it = 0;                                         // tiles so far
+    uint32_t it = 0;                                         // tiles of keys so far
 
-    if (warp == 0) {
+    if (warp < 4) {
+      registers_down<56>();
+      if (warp == 0) {
         // ---- copies
         const uint32_t k0 = smem_u32(sK), v0 = smem_u32(sV);
+        uint32_t keys = 0;                                   // tiles of keys asked for (of values: it)
         bool ok = true;
         while (at.left > 0 && ok) {
             const int n = at.run();
             for (int j = 0; j < n; ++j, ++it) {
-                const uint32_t stage = it % STAGES, ph = (it / STAGES) & 1u;
+                const uint32_t ks = it % KS, vs = it % VS;
                 const int entry = (at.tile + j) * kKeys + lane * tm.box, slot = p.slot_at(entry), row = entry - slot * p.page_size;
                 int page = -1;
                 if (lane < tm.boxes && entry < at.s.total) page = p.table[at.b * p.table_stride + slot];
                 if ((unsigned)page >= (unsigned)p.pages) page = p.pages;      // outside the map: zeros
-                const uint32_t dst = stage * kTileBytes + lane * (tm.box * 128);
-                if (!mbar_wait_warp(smem_u32(k_empty + stage), ph ^ 1u, abort_flag)) { fail(abort_flag, 141); ok = false; break; }
-                if (lane == 0) mbar_expect_tx(k_full + stage, kTileBytes);
+                const uint32_t off = lane * (tm.box * 128);
+                if (!mbar_wait_warp(smem_u32(k_empty + ks), ((it / KS) & 1u) ^ 1u, abort_flag)) { fail(abort_flag, 141); ok = false; break; }
+                if (lane == 0) mbar_expect_tx(k_full + ks, kTileBytes);
                 __syncwarp();
                 if (lane < tm.boxes)
                     for (int c = 0; c < DC; ++c)
-                        tma_load_4d_a(k0 + dst + c * kChunk, &tmK, smem_u32(k_full + stage), c * 64, row, at.h, page);
-                if (!mbar_wait_warp(smem_u32(v_empty + stage), ph ^ 1u, abort_flag)) { fail(abort_flag, 142); ok = false; break; }
-                if (lane == 0) mbar_expect_tx(v_full + stage, kTileBytes);
+                        tma_load_4d_a(k0 + ks * kTileBytes + off + c * kChunk, &tmK, smem_u32(k_full + ks), c * 64, row, at.h, page);
+                keys = it + 1;
+                if (!mbar_wait_warp(smem_u32(v_empty + vs), ((it / VS) & 1u) ^ 1u, abort_flag)) { fail(abort_flag, 142); ok = false; break; }
+                if (lane == 0) mbar_expect_tx(v_full + vs, kTileBytes);
                 __syncwarp();
                 if (lane < tm.boxes)
                     for (int c = 0; c < DC; ++c)
-                        tma_load_4d_a(v0 + dst + c * kChunk, &tmV, smem_u32(v_full + stage), c * 64, row, at.h, page);
+                        tma_load_4d_a(v0 + vs * kTileBytes + off + c * kChunk, &tmV, smem_u32(v_full + vs), c * 64, row, at.h, page);
             }
             if (ok) at.skip(p, n);
         }
-        if (!ok && lane == 0) {
-            // what was asked for lands before the block leaves (it: the tile whose keys, and perhaps values, were not)
+        if (!ok && lane == 0) {                              // what was asked for lands before the block leaves
             int never = 0;
-            for (uint32_t f = it >= STAGES ? it - STAGES : 0; f < it; ++f) {
-                mbar_wait(k_full + f % STAGES, (f / STAGES) & 1u, &never);
-                mbar_wait(v_full + f % STAGES, (f / STAGES) & 1u, &never);
-            }
-            if (mbar_try_wait(k_empty + it % STAGES, ((it / STAGES) & 1u) ^ 1u)) mbar_wait(k_full + it % STAGES, (it / STAGES) & 1u, &never);
+            for (uint32_t f = keys > KS ? keys - KS : 0; f < keys; ++f) mbar_wait(k_full + f % KS, (f / KS) & 1u, &never);
+            for (uint32_t f = it > VS ? it - VS : 0; f < it; ++f) mbar_wait(v_full + f % VS, (f / VS) & 1u, &never);
         }
-    } else if (warp == 1) {
+      } else if (warp == 1) {
         // ---- products
         const uint32_t idesc_s = make_idesc_bf16_f32(kRows, kKeys), idesc_o = make_idesc_bf16_f32(kRows, 16 * steps) | kIdescBAlongN;
         const uint64_t kd = kmajor_desc_hi(128), nd = mnmajor_desc_hi(kChunk);
         const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
-        uint32_t units = 0, made[2] = {0, 0}, scored = 0;
+        uint32_t units = 0, made[2] = {0, 0};
         bool ok = true;
-        auto scores = [&](int j) -> bool {                   // tile j of the unit, the it + (j - done)-th of the CTA
-            const uint32_t stage = scored % STAGES, ph = (scored / STAGES) & 1u;
+        // step i of a unit: stream i & 1 with tile i (TWO: i / 2) of its keys
+        auto scores = [&](int i) -> bool {
+            const uint32_t kt = it + (TWO ? i >> 1 : i), stage = kt % KS, ph = (kt / KS) & 1u, s = i & 1;
             if (!mbar_wait_warp(smem_u32(k_full + stage), ph, abort_flag)) { fail(abort_flag, 143); return false; }
             tc_fence_after_sync();
             if (elect_one()) {
-                const uint64_t ad = kd | (uint64_t)((q0 & 0x3FFFFu) >> 4), bd = kd | (uint64_t)(((k0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
+                const uint64_t ad = kd | (uint64_t)(((q0 + (TWO ? s * kTileBytes : 0)) & 0x3FFFFu) >> 4);
+                const uint64_t bd = kd | (uint64_t)(((k0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
                 for (int k = 0; k < steps; ++k) {
                     const uint32_t off = (k >> 2) * (kChunk >> 4) + (k & 3) * 2;
-                    mma_bf16_ss(tmem + (j & 1) * kKeys, ad + off, bd + off, idesc_s, k != 0);
+                    mma_bf16_ss(tmem + s * kKeys, ad + off, bd + off, idesc_s, k != 0);
                 }
-                mma_commit(k_empty + stage);
-                mma_commit(s_full + (j & 1));
+                if (!TWO || s) mma_commit(k_empty + stage);
+                mma_commit(s_full + s);
             }
-            ++scored;
             return true;
         };
         while (at.left > 0 && ok) {
-            const int n = at.run();
+            const int n = at.run(), last = TWO ? 2 * n : n;
             if (!mbar_wait_warp(smem_u32(q_ready), units & 1u, abort_flag)) { fail(abort_flag, 144); ok = false; break; }
             ++units;
             tc_fence_after_sync();
-            ok = scores(0) && (n < 2 || scores(1));
-            for (int j = 0; j < n && ok; ++j, ++it) {
-                const uint32_t stage = it % STAGES, ph = (it / STAGES) & 1u, s = j & 1;
+            ok = scores(0) && (last < 2 || scores(1));
+            for (int i = 0; i < last && ok; ++i) {
+                const uint32_t vt = it + (TWO ? i >> 1 : i), stage = vt % VS, ph = (vt / VS) & 1u, s = i & 1;
                 if (!mbar_wait_warp(smem_u32(p_ready + s), made[s] & 1u, abort_flag)) { fail(abort_flag, 145); ok = false; break; }
                 ++made[s];
                 if (!mbar_wait_warp(smem_u32(v_full + stage), ph, abort_flag)) { fail(abort_flag, 146); ok = false; break; }
@@ -187,21 +196,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 if (elect_one()) {
                     const uint64_t bd = nd | (uint64_t)(((v0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
                     for (int k = 0; k < kKeys / 16; ++k)
-                        mma_bf16_ts(tmem + 2 * kKeys + s * 128, tmem + s * kKeys + k * 8, bd + k * (2048 >> 4), idesc_o, j >= 2 || k != 0);
-                    mma_commit(v_empty + stage);
+                        mma_bf16_ts(tmem + 2 * kKeys + s * 128, tmem + s * kKeys + k * 8, bd + k * (2048 >> 4), idesc_o, i >= 2 || k != 0);
+                    if (!TWO || s) mma_commit(v_empty + stage);
                     mma_commit(o_done + s);
                 }
-                if (j + 2 < n) ok = scores(j + 2);
+                if (i + 2 < last) ok = scores(i + 2);
             }
+            it += n;
             if (ok) at.skip(p, n);
         }
         // none is in flight when the tensor memory is given back, however the loop ended
         int never = 0;
         if (elect_one()) mma_commit(drained);
         mbar_wait_warp(smem_u32(drained), 0, &never);
+      }
     } else {
         // ---- softmax
-        const int group = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+        registers_up<216>();
+        const int group = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t tS = tmem + group * kKeys + lanes, tO = tmem + 2 * kKeys + group * 128 + lanes, tO0 = tmem + 2 * kKeys + lanes;
         const int chunks = p.D / 8;
@@ -211,16 +223,17 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             bool ok = true;
             const int n = at.run(), tile0 = at.tile;
             const Sequence s = at.s;
-            const int b = at.b, h = at.h, row0 = at.rt * kRows;
+            const int b = at.b, h = at.h, unit0 = at.rt * (TWO ? 2 : 1) * kRows, row0 = unit0 + (TWO ? group * kRows : 0);
+            const int last = TWO ? 2 * n : n;
             // the unit's rows of q, by all eight warps
-            for (int i = threadIdx.x - 64; i < kRows * chunks; i += 256) {
-                const int rr = i / chunks, col = i - rr * chunks, t = (row0 + rr) / p.G, g = row0 + rr - t * p.G;
+            for (int i = threadIdx.x - 128; i < (TWO ? 2 : 1) * kRows * chunks; i += 256) {
+                const int rr = i / chunks, col = i - rr * chunks, t = (unit0 + rr) / p.G, g = unit0 + rr - t * p.G;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (t < s.count && tm.sign != 0.f)
                     v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + b * p.qs[0] + t * p.qs[1] +
                                                         (h * p.G + g) * p.qs[2] + col * 8);
                 if (tm.sign < 0.f) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-                *reinterpret_cast<uint4*>(sQ + (col >> 3) * kChunk + rr * 128 + (((col & 7) ^ (rr & 7)) << 4)) = v;
+                *reinterpret_cast<uint4*>(sQ + (rr >> 7) * kTileBytes + (col >> 3) * kChunk + (rr & 127) * 128 + (((col & 7) ^ (rr & 7)) << 4)) = v;
             }
             fence_proxy_async();
             tc_fence_before_sync();
@@ -232,7 +245,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             const bool busy = row0 + quad * 32 < s.count * p.G;               // (any row of this warp)
             float m = -CUDART_INF_F, l = 0.f;
             bool bad = false;
-            for (int j = group; j < n; j += 2, ++seen) {
+            for (int i = group; i < last; i += 2, ++seen) {
+                const int j = TWO ? i >> 1 : i;
                 const uint32_t tile_at = it + j;
                 if (!__all_sync(0xffffffffu, mbar_wait(s_full + group, seen & 1u, abort_flag))) { if (lane == 0) fail(abort_flag, 147); ok = false; break; }
                 tc_fence_after_sync();
@@ -271,7 +285,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                         const float f = grows ? ex2((m - now) * tm.factor) : 1.f;
                         m = now;
                         l *= f;
-                        if (j >= 2) {
+                        if (i >= 2) {
                             if (!__all_sync(0xffffffffu, mbar_wait(o_done + group, (seen - 1) & 1u, abort_flag))) {
                                 if (lane == 0) fail(abort_flag, 148);
                                 ok = false;
@@ -315,8 +329,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 }
                 if (masked) {
                     // values of entries that are not there: zeros; of drafted tokens that are not finite: zeros for now
-                    const uint32_t stage = tile_at % STAGES;
-                    if (!__all_sync(0xffffffffu, mbar_wait(v_full + stage, (tile_at / STAGES) & 1u, abort_flag))) { if (lane == 0) fail(abort_flag, 149); ok = false; break; }
+                    const uint32_t stage = tile_at % VS;
+                    if (!__all_sync(0xffffffffu, mbar_wait(v_full + stage, (tile_at / VS) & 1u, abort_flag))) { if (lane == 0) fail(abort_flag, 149); ok = false; break; }
                     const int entry = key0 + r;
                     if (entry >= s.length) {
                         for (int col = 0; col < chunks; ++col) {
@@ -347,56 +361,57 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             }
             // ---- the unit's end: both groups' sums.  A warp that gave up comes here too, and all eight leave together (a barrier has no limit)
             if (bad) atomicOr(sBad, 1);
-            if (ok && n > group && !__all_sync(0xffffffffu, mbar_wait(o_done + group, (seen - 1) & 1u, abort_flag)) && lane == 0)
+            if (ok && last > group && !__all_sync(0xffffffffu, mbar_wait(o_done + group, (seen - 1) & 1u, abort_flag)) && lane == 0)
                 fail(abort_flag, 148);
-            if (group == 1) sScale[r] = make_float2(m, l);
+            if (!TWO && group == 1) sScale[r] = make_float2(m, l);
             tc_fence_before_sync();
             groups_sync();
             tc_fence_after_sync();
-            if (threadIdx.x == 64) *sStop = *abort_flag;
+            if (threadIdx.x == 128) *sStop = *abort_flag;
             const bool any_bad = *reinterpret_cast<volatile int*>(sBad) != 0;
             const bool whole = tile0 == 0 && n == s.tiles;
             float* slot = slot_of(p, blockIdx.x, first_unit);
-            if (group == 0) {
-                const float2 other = sScale[r];
+            float2 f = make_float2(1.f, 0.f);                // what this stream's and, of the same rows, the other's sums are multiplied by
+            if (TWO || group == 0) {
+                const float2 other = TWO ? make_float2(-CUDART_INF_F, 0.f) : sScale[r];
                 const float top = fmaxf(m, other.x);
-                float f0 = m == -CUDART_INF_F ? 0.f : ex2((m - top) * tm.factor);
-                float f1 = other.x == -CUDART_INF_F ? 0.f : ex2((other.x - top) * tm.factor);
-                const float sum = l * f0 + other.y * f1;
+                f.x = m == -CUDART_INF_F ? 0.f : ex2((m - top) * tm.factor);
+                f.y = other.x == -CUDART_INF_F ? 0.f : ex2((other.x - top) * tm.factor);
+                const float sum = l * f.x + other.y * f.y;
                 if (whole) {
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                    f0 *= inv;
-                    f1 *= inv;
+                    f.x *= inv;
+                    f.y *= inv;
                 } else {
-                    float* tail = slot + (long long)kRows * p.D;
-                    tail[r] = top * tm.factor;
-                    tail[kRows + r] = sum;
-                    if (r == 0) tail[2 * kRows] = any_bad ? 1.f : 0.f;
+                    float* tail = slot + (long long)p.rows_per_tile * p.D;
+                    tail[row0 - unit0 + r] = top * tm.factor;
+                    tail[p.rows_per_tile + row0 - unit0 + r] = sum;
+                    if (threadIdx.x == 128) tail[2 * p.rows_per_tile] = any_bad ? 1.f : 0.f;
                 }
-                sScale[r] = make_float2(f0, f1);
+                if (!TWO) sScale[r] = f;
             }
             groups_sync();
             if (*sStop) break;
-            if (threadIdx.x == 64) *sBad = 0;
+            if (threadIdx.x == 128) *sBad = 0;
             if (busy) {
-                const float2 f = sScale[r];
+                if (!TWO) f = sScale[r];
                 const int t = (row0 + r) / p.G, g = row0 + r - t * p.G;
                 const bool there = t < s.count;
-                const int half = (steps + 1) / 2;
+                const int half = (steps + 1) / 2;            // (TWO: each group writes its own rows, else half of the channels of all)
 #pragma unroll 1
-                for (int c = group ? half : 0; c < (group ? steps : half); ++c) {
+                for (int c = !TWO && group ? half : 0; c < (TWO || group ? steps : half); ++c) {
                     uint32_t o[16], o1[16];
                     __syncwarp();
-                    tmem_ld_x16(tO0 + 16 * c, o);
-                    if (n > 1) tmem_ld_x16(tO0 + 128 + 16 * c, o1);
+                    tmem_ld_x16((TWO ? tO : tO0) + 16 * c, o);
+                    if (!TWO && n > 1) tmem_ld_x16(tO0 + 128 + 16 * c, o1);
                     tmem_ld_wait();
                     tie16(o);
-                    if (n > 1) tie16(o1);
+                    if (!TWO && n > 1) tie16(o1);
                     float y[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         y[e] = __uint_as_float(o[e]) * f.x;
-                        if (n > 1) y[e] = fmaf(__uint_as_float(o1[e]), f.y, y[e]);
+                        if (!TWO && n > 1) y[e] = fmaf(__uint_as_float(o1[e]), f.y, y[e]);
                     }
                     if (!there) continue;
                     if (whole) {
@@ -413,7 +428,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                             *reinterpret_cast<uint4*>(out + 8 * u) = *reinterpret_cast<uint4*>(w);
                         }
                     } else {
-                        float* dst = slot + (long long)r * p.D + 16 * c;
+                        float* dst = slot + (long long)(row0 - unit0 + r) * p.D + 16 * c;
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             if (16 * c + 4 * u < p.D)
@@ -435,11 +450,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     }
 }
 
-template <int DC, int STAGES>
+template <int DC, int KS, int VS, bool TWO>
 int launch_tiles(const CUtensorMap& k, const CUtensorMap& v, const Params& p, const TileMaps& tm, cudaStream_t st) {
-    const size_t smem = 1024 + (size_t)(1 + 2 * STAGES) * DC * kChunk + kRows * sizeof(float2) + 8 * (4 * STAGES + 8) + 16;
-    CONVNN_ENSURE_SMEM((tiles_kernel<DC, STAGES>), smem);
-    launch_chained(tiles_kernel<DC, STAGES>, p.ctas, kTileThreads, smem, st, k, v, p, tm);
+    const size_t smem = 1024 + (size_t)((TWO ? 2 : 1) + KS + VS) * DC * kChunk + kRows * sizeof(float2) + 8 * (2 * KS + 2 * VS + 8) + 16;
+    CONVNN_ENSURE_SMEM((tiles_kernel<DC, KS, VS, TWO>), smem);
+    launch_chained(tiles_kernel<DC, KS, VS, TWO>, p.ctas, kTileThreads, smem, st, k, v, p, tm);
     CONVNN_CHECK_LAUNCH("tree_attention");
     return CONVNN_OK;
 }
@@ -472,7 +487,9 @@ int launch_tree_tiles(const Params& p, cudaStream_t st) {
     tm.sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;
     CUtensorMap k, v;
     if (!map_of(&k, p.k, p, p.ks, tm.box) || !map_of(&v, p.v, p, p.vs, tm.box)) return CONVNN_E_CUDA;
-    return p.D <= 64 ? launch_tiles<1, 6>(k, v, p, tm, st) : launch_tiles<2, 3>(k, v, p, tm, st);
+    if (p.rows_per_tile > kRows)
+        return p.D <= 64 ? launch_tiles<1, 6, 5, true>(k, v, p, tm, st) : launch_tiles<2, 3, 2, true>(k, v, p, tm, st);
+    return p.D <= 64 ? launch_tiles<1, 6, 6, false>(k, v, p, tm, st) : launch_tiles<2, 3, 3, false>(k, v, p, tm, st);
 }
 
 int read_tree_attention_status(int* out) {

@@ -344,3 +344,93 @@ def test_a_step_of_decoding():
         off = (y[:, t].double() - single[i].double()).norm() / single[i].double().norm()
         assert off < 2.0 ** -4
     check_heads(tree_cache.k[int(cache.table[0, 100 // P]), :, 100 % P][None, None], rows[:1, :1, H:H + Hk], wk, rope[None, 100:101], 1e-6, False)
+
+
+# ---- many rows --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,G", [(17, 1), (32, 4), (43, 3), (64, 4), (33, 8), (64, 8)])
+@pytest.mark.parametrize("D", [8, 40, 64, 72, 80, 104, 128])
+def test_tiles_of_rows(T, G, D):
+    B, H, P = 3, 2, 16
+    cache = cache_of(B, H, P, D, 400 + T)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16)
+    lengths, counts, tree = ints(400, 129, 0), ints(T, (T + 1) // 2, 1), trees(B, T)
+    check_attention(ops.tree_attention(q, cache, lengths, tree, counts), q, cache, lengths, tree, counts)
+
+
+@pytest.mark.parametrize("P", [1, 8, 16, 20, 48, 64, 96, 128, 256, 512])
+@pytest.mark.parametrize("T,G", [(20, 1), (50, 4)])
+@pytest.mark.parametrize("rows_first", [False, True])
+def test_tiles_of_rows_and_pages(P, T, G, rows_first):
+    B, H, D = 3, 2, 64
+    cache = cache_of(B, H, P, D, 700 + T, rows_first=rows_first)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16)
+    lengths = ints(700, 127, 128)
+    check_attention(ops.tree_attention(q, cache, lengths), q, cache, lengths)
+
+
+@pytest.mark.parametrize("G", [2, 8])
+def test_tiles_of_rows_at_every_length(G):
+    lengths = [0, 1, 63, 64, 65, 107, 108, 109, 127, 128, 129, 235, 236, 237, 255, 256, 257, 383, 384, 511, 512, 513]
+    B, H, D, T = len(lengths), 1, 64, 20
+    cache = cache_of(B, H, 32, D, 540)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16)
+    at, tree = ints(*lengths), trees(B, T)
+    check_attention(ops.tree_attention(q, cache, at, tree), q, cache, at, tree)
+
+
+@pytest.mark.parametrize("G", [2, 8])
+@pytest.mark.parametrize("growth", [0.02, 1.0])
+def test_maxima_that_grow(G, growth):
+    """Scores that rise along the keys, a little or by far more than 2^8 a tile; and fall."""
+    B, H, D, T, n = 2, 1, 64, 20, 1500
+    cache = cache_of(B, H, 16, D, n + T)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16).abs()
+    for b, order in ((0, 1), (1, -1)):
+        for j in range(n):
+            e = j if order == 1 else n - 1 - j
+            cache.k[int(cache.table[b, e // 16]), 0, e % 16] = growth * j / 10
+    lengths = ints(n, n)
+    check_attention(ops.tree_attention(q, cache, lengths, scale=1 / 64), q, cache, lengths, scale=1 / 64)
+
+
+@pytest.mark.parametrize("T,G", [(30, 2), (40, 4), (64, 8)])
+def test_tiles_of_rows_of_several_ctas(T, G):
+    B, H, D = 3, 2, 128
+    cache = cache_of(B, H, 64, D, 5000 + T)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16)
+    lengths, counts, tree = ints(5000, 0, 3333), ints(T - 1, T, T // 2), trees(B, T)
+    got = ops.tree_attention(q, cache, lengths, tree, counts)
+    check_attention(got, q, cache, lengths, tree, counts)
+    assert torch.equal(got, ops.tree_attention(q, cache, lengths, tree, counts))
+
+
+@pytest.mark.parametrize("T,G", [(20, 2), (40, 4)])
+@pytest.mark.parametrize("length", [40, 3000])
+def test_tiles_of_rows_and_what_is_not_seen(T, G, length):
+    """Nothing in the pages behind the last entry, and values of other branches that are not finite."""
+    B, H, D, P = 1, 2, 128, 64
+    cache = cache_of(B, H, P, D, length + T + 200)
+    q = randn(B, T, H * G, D, seed=9, dtype=BF16)
+    lengths, tree = ints(length), trees(B, T, seed=3)
+    tree[0] &= ~2
+    tree[0, 2] |= 2
+    want = ops.tree_attention(q, cache, lengths, tree)
+    check_attention(want, q, cache, lengths, tree)
+    for e in range(length + T, length + T + 200):
+        for c in (cache.k, cache.v):
+            c[int(cache.table[0, e // P]), :, e % P] = float("nan")
+    e = length + 1
+    cache.v[int(cache.table[0, e // P]), 1, e % P, 70] = float("inf")
+    got = ops.tree_attention(q, cache, lengths, tree)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, 2, G:, 70] = True
+    assert torch.equal(got[~hit], want[~hit]) and torch.isinf(got[hit]).all()
+
+
+@pytest.mark.parametrize("T,G", [(20, 2), (40, 4)])
+@pytest.mark.parametrize("scale", [1.0, 0.0, -0.2])
+def test_tiles_of_rows_and_scales(T, G, scale):
+    cache = cache_of(1, 2, 16, 64, 400)
+    q = randn(1, T, 2 * G, 64, seed=9, dtype=BF16)
+    check_attention(ops.tree_attention(q, cache, ints(300), scale=scale), q, cache, ints(300), scale=scale)
