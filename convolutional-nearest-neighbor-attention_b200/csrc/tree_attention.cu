@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
         for (int c = c0 + lane; c <= c1; c += 32) {
             const float* from = piece(c) + tail;
             top = fmaxf(top, from[r]);
-            bad |= from[2 * p.rows_per_tile] != 0.f;
+            bad |= from[2 * p.rows_per_tile + (r >> 7)] != 0.f;          // (a word for every 128 rows)
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
             for (int u = 0; u < 2; ++u) {
                 const int col = 4 * (lane + 32 * u);
                 if (col >= p.D) continue;
-                const float4 x = *reinterpret_cast<const float4*>(from + (long long)r * p.D + col);
+                const float4 x = reinterpret_cast<const float4*>(from)[(long long)r * p.slot_row + (lane + 32 * u) * p.slot_col];
                 y[u].x = fmaf(x.x, f, y[u].x); y[u].y = fmaf(x.y, f, y[u].y);
                 y[u].z = fmaf(x.z, f, y[u].z); y[u].w = fmaf(x.w, f, y[u].w);
             }
@@ -737,6 +737,8 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
     p.partial = static_cast<float*>(workspace);
     p.slot = slot_floats(g, p.D);
+    p.slot_row = g.tiles ? 1 : p.D / 4;
+    p.slot_col = g.tiles ? g.rows_per_tile : 1;
     p.ctas = device_sms() * g.ctas_per_sm;
     int bits = 0;
     while ((1ll << bits) < p.page_size) ++bits;

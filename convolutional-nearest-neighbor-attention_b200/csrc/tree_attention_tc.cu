@@ -52,8 +52,11 @@ __device__ __forceinline__ void tie16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
-// The two softmax groups.
-__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The softmax warps: with TWO each group for itself.
+template <bool TWO> __device__ __forceinline__ void groups_sync(int group) {
+    if (TWO) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+    else asm volatile("bar.sync 1, 256;" ::: "memory");
+}
 
 // Registers move from the warps that copy and multiply to those that hold a row of scores: 56 + 2 * 216 of the 3 * 168 a thread that the
 // block starts with.
@@ -73,11 +76,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     float2* sScale = reinterpret_cast<float2*>(sV + VS * kTileBytes);        // [128]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + kRows);
     uint64_t *k_full = bars, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
-    uint64_t *s_full = v_empty + VS, *p_ready = s_full + 2, *o_done = p_ready + 2, *q_ready = o_done + 2, *drained = q_ready + 1;
+    uint64_t *s_full = v_empty + VS, *p_ready = s_full + 2, *o_done = p_ready + 2, *q_ready = o_done + 2, *drained = q_ready + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* sBad = reinterpret_cast<int*>(tmem_slot + 2);
-    volatile int* sStop = reinterpret_cast<volatile int*>(tmem_slot + 3);
+    volatile int* sStop = reinterpret_cast<volatile int*>(tmem_slot + 2);    // [2]: a group's
+    int* sBad = reinterpret_cast<int*>(tmem_slot + 4);                       // [4]: a unit's, in turn
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -94,10 +97,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             mbar_init(p_ready + i, 4);
             mbar_init(o_done + i, 1);
         }
-        mbar_init(q_ready, 8);
+        mbar_init(q_ready, TWO ? 4 : 8);
+        mbar_init(q_ready + 1, 4);
         mbar_init(drained, 1);
         *abort_flag = 0;
-        *sBad = 0;
+        sBad[0] = sBad[1] = sBad[2] = sBad[3] = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
@@ -167,6 +171,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         // step i of a unit: stream i & 1 with tile i (TWO: i / 2) of its keys
         auto scores = [&](int i) -> bool {
             const uint32_t kt = it + (TWO ? i >> 1 : i), stage = kt % KS, ph = (kt / KS) & 1u, s = i & 1;
+            if (i < (TWO ? 2 : 1) && !mbar_wait_warp(smem_u32(q_ready + i), units & 1u, abort_flag)) { fail(abort_flag, 144); return false; }
             if (!mbar_wait_warp(smem_u32(k_full + stage), ph, abort_flag)) { fail(abort_flag, 143); return false; }
             tc_fence_after_sync();
             if (elect_one()) {
@@ -183,9 +188,6 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         };
         while (at.left > 0 && ok) {
             const int n = at.run(), last = TWO ? 2 * n : n;
-            if (!mbar_wait_warp(smem_u32(q_ready), units & 1u, abort_flag)) { fail(abort_flag, 144); ok = false; break; }
-            ++units;
-            tc_fence_after_sync();
             ok = scores(0) && (last < 2 || scores(1));
             for (int i = 0; i < last && ok; ++i) {
                 const uint32_t vt = it + (TWO ? i >> 1 : i), stage = vt % VS, ph = (vt / VS) & 1u, s = i & 1;
@@ -203,6 +205,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 if (i + 2 < last) ok = scores(i + 2);
             }
             it += n;
+            ++units;
             if (ok) at.skip(p, n);
         }
         // none is in flight when the tensor memory is given back, however the loop ended
@@ -217,34 +220,52 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t tS = tmem + group * kKeys + lanes, tO = tmem + 2 * kKeys + group * 128 + lanes, tO0 = tmem + 2 * kKeys + lanes;
         const int chunks = p.D / 8;
-        uint32_t seen = 0;                                   // tiles of this group so far
+        // Rows of q of the unit at c, this warp's share of them: TWO, 32 of its group's tile; else 16 of the one tile.
+        auto load_rows = [&](const Cursor& c) {
+            constexpr int CPR = DC * 8, ITEMS = (TWO ? 32 : 16) * CPR / 32, BATCH = ITEMS < 8 ? ITEMS : 8;
+            const int row_first = TWO ? group * kRows + quad * 32 : (warp - 4) * 16, tile_row = c.rt * (TWO ? 2 : 1) * kRows;
+#pragma unroll 1
+            for (int i0 = 0; i0 < ITEMS; i0 += BATCH) {
+                uint4 v[BATCH];
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    const int item = (i0 + e) * 32 + lane, col = item % CPR, row = tile_row + row_first + item / CPR, t = row / p.G;
+                    v[e] = make_uint4(0, 0, 0, 0);
+                    if (t < c.s.count && col < chunks && tm.sign != 0.f)
+                        v[e] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + c.b * p.qs[0] + t * p.qs[1] +
+                                                               (c.h * p.G + row - t * p.G) * p.qs[2] + col * 8);
+                }
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    const int item = (i0 + e) * 32 + lane, col = item % CPR, rr = row_first + item / CPR;
+                    if (tm.sign < 0.f) { v[e].x ^= 0x80008000u; v[e].y ^= 0x80008000u; v[e].z ^= 0x80008000u; v[e].w ^= 0x80008000u; }
+                    if (col < chunks)
+                        *reinterpret_cast<uint4*>(sQ + (rr >> 7) * kTileBytes + (col >> 3) * kChunk + (rr & 127) * 128 +
+                                                  (((col & 7) ^ (rr & 7)) << 4)) = v[e];
+                }
+            }
+            fence_proxy_async();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready + (TWO ? group : 0));
+        };
+        uint32_t seen = 0, units = 0;                        // tiles of this group, units so far
         bool first_unit = true;
+        if (TWO && at.left > 0) load_rows(at);
         while (at.left > 0) {
             bool ok = true;
             const int n = at.run(), tile0 = at.tile;
             const Sequence s = at.s;
             const int b = at.b, h = at.h, unit0 = at.rt * (TWO ? 2 : 1) * kRows, row0 = unit0 + (TWO ? group * kRows : 0);
             const int last = TWO ? 2 * n : n;
-            // the unit's rows of q, by all eight warps
-            for (int i = threadIdx.x - 128; i < (TWO ? 2 : 1) * kRows * chunks; i += 256) {
-                const int rr = i / chunks, col = i - rr * chunks, t = (unit0 + rr) / p.G, g = unit0 + rr - t * p.G;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (t < s.count && tm.sign != 0.f)
-                    v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + b * p.qs[0] + t * p.qs[1] +
-                                                        (h * p.G + g) * p.qs[2] + col * 8);
-                if (tm.sign < 0.f) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-                *reinterpret_cast<uint4*>(sQ + (rr >> 7) * kTileBytes + (col >> 3) * kChunk + (rr & 127) * 128 + (((col & 7) ^ (rr & 7)) << 4)) = v;
-            }
-            fence_proxy_async();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_ready);
+            int* unit_bad = sBad + (units & 3);
+            if (threadIdx.x == 128) sBad[(units + 2) & 3] = 0;               // (the groups are less than a unit apart)
+            if (!TWO) load_rows(at);
 
             const unsigned long long drafts = s.total - s.length >= 64 ? ~0ull : (1ull << (s.total - s.length)) - 1;
             const unsigned long long mask = seen_by(p, s, b, row0 + r) & drafts;
             const bool busy = row0 + quad * 32 < s.count * p.G;               // (any row of this warp)
             float m = -CUDART_INF_F, l = 0.f;
-            bool bad = false;
             for (int i = group; i < last; i += 2, ++seen) {
                 const int j = TWO ? i >> 1 : i;
                 const uint32_t tile_at = it + j;
@@ -347,9 +368,10 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                                 if ((w[e] & 0x7f80u) == 0x7f80u) { w[e] &= 0xffff0000u; hit = true; }
                                 if ((w[e] & 0x7f800000u) == 0x7f800000u) { w[e] &= 0xffffu; hit = true; }
                             }
-                            if (hit) {
+                            if (hit) {                       // (first the word of it: with TWO the other group may come second)
+                                atomicOr(unit_bad, 1);
+                                __threadfence_block();
                                 *at16 = make_uint4(w[0], w[1], w[2], w[3]);
-                                bad = true;
                             }
                         }
                     }
@@ -359,16 +381,20 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready + group);
             }
-            // ---- the unit's end: both groups' sums.  A warp that gave up comes here too, and all eight leave together (a barrier has no limit)
-            if (bad) atomicOr(sBad, 1);
+            // ---- the unit's end.  A warp that gave up comes here too, and the warps of a barrier, which has no limit, leave together
+            if (TWO && ok && at.left > n) {                  // the stream's scores are done, and the next unit's may begin
+                Cursor ahead = at;
+                ahead.skip(p, n);
+                load_rows(ahead);
+            }
             if (ok && last > group && !__all_sync(0xffffffffu, mbar_wait(o_done + group, (seen - 1) & 1u, abort_flag)) && lane == 0)
                 fail(abort_flag, 148);
             if (!TWO && group == 1) sScale[r] = make_float2(m, l);
             tc_fence_before_sync();
-            groups_sync();
+            groups_sync<TWO>(group);
             tc_fence_after_sync();
-            if (threadIdx.x == 128) *sStop = *abort_flag;
-            const bool any_bad = *reinterpret_cast<volatile int*>(sBad) != 0;
+            if (threadIdx.x == 128 || (TWO && threadIdx.x == 256)) sStop[group] = *abort_flag;
+            const bool any_bad = *reinterpret_cast<volatile int*>(unit_bad) != 0;
             const bool whole = tile0 == 0 && n == s.tiles;
             float* slot = slot_of(p, blockIdx.x, first_unit);
             float2 f = make_float2(1.f, 0.f);                // what this stream's and, of the same rows, the other's sums are multiplied by
@@ -386,13 +412,12 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                     float* tail = slot + (long long)p.rows_per_tile * p.D;
                     tail[row0 - unit0 + r] = top * tm.factor;
                     tail[p.rows_per_tile + row0 - unit0 + r] = sum;
-                    if (threadIdx.x == 128) tail[2 * p.rows_per_tile] = any_bad ? 1.f : 0.f;
+                    if (r == 0) tail[2 * p.rows_per_tile + (TWO ? group : 0)] = any_bad ? 1.f : 0.f;
                 }
                 if (!TWO) sScale[r] = f;
             }
-            groups_sync();
-            if (*sStop) break;
-            if (threadIdx.x == 128) *sBad = 0;
+            groups_sync<TWO>(group);
+            if (sStop[TWO ? group : 0]) break;
             if (busy) {
                 if (!TWO) f = sScale[r];
                 const int t = (row0 + r) / p.G, g = row0 + r - t * p.G;
@@ -428,17 +453,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                             *reinterpret_cast<uint4*>(out + 8 * u) = *reinterpret_cast<uint4*>(w);
                         }
                     } else {
-                        float* dst = slot + (long long)(row0 - unit0 + r) * p.D + 16 * c;
+                        // (four channels of a warp's rows side by side)
+                        float4* dst = reinterpret_cast<float4*>(slot) + (long long)(4 * c) * p.rows_per_tile + row0 - unit0 + r;
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
                             if (16 * c + 4 * u < p.D)
-                                *reinterpret_cast<float4*>(dst + 4 * u) = make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
+                                dst[u * p.rows_per_tile] = make_float4(y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]);
                     }
                 }
             }
             first_unit = false;
+            ++units;
             it += n;
             at.skip(p, n);
+            if (!TWO) {                                      // both accumulators are read by both groups
+                tc_fence_before_sync();
+                groups_sync<TWO>(group);
+                tc_fence_after_sync();
+            }
         }
     }
 
@@ -452,7 +484,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 
 template <int DC, int KS, int VS, bool TWO>
 int launch_tiles(const CUtensorMap& k, const CUtensorMap& v, const Params& p, const TileMaps& tm, cudaStream_t st) {
-    const size_t smem = 1024 + (size_t)((TWO ? 2 : 1) + KS + VS) * DC * kChunk + kRows * sizeof(float2) + 8 * (2 * KS + 2 * VS + 8) + 16;
+    const size_t smem = 1024 + (size_t)((TWO ? 2 : 1) + KS + VS) * DC * kChunk + kRows * sizeof(float2) + 8 * (2 * KS + 2 * VS + 9) + 32;
     CONVNN_ENSURE_SMEM((tiles_kernel<DC, KS, VS, TWO>), smem);
     launch_chained(tiles_kernel<DC, KS, VS, TWO>, p.ctas, kTileThreads, smem, st, k, v, p, tm);
     CONVNN_CHECK_LAUNCH("tree_attention");
