@@ -52,6 +52,18 @@ __device__ __forceinline__ void tie16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
+// A wait of a converged warp for as many barriers as its lanes name (0: none), which costs what one does.
+__device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, volatile int* abort) {
+    bool done = bar == 0 || mbar_try_wait_a(bar, parity);
+    if (__all_sync(0xffffffffu, done)) return true;
+    const unsigned long long t0 = global_timer_ns();
+    for (uint32_t i = 0; i < kStartPollLimit; ++i) {
+        if (!done) done = mbar_try_wait_a(bar, parity);
+        if (__all_sync(0xffffffffu, done)) return true;
+        if ((i & 255u) == 255u && __any_sync(0xffffffffu, *abort || global_timer_ns() - t0 > kWaitBudgetNs)) return false;
+    }
+    return false;
+}
 // The softmax warps: with TWO each group for itself.
 template <bool TWO> __device__ __forceinline__ void groups_sync(int group) {
     if (TWO) asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
@@ -168,41 +180,57 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
         uint32_t units = 0, made[2] = {0, 0};
         bool ok = true;
-        // step i of a unit: stream i & 1 with tile i (TWO: i / 2) of its keys
-        auto scores = [&](int i) -> bool {
-            const uint32_t kt = it + (TWO ? i >> 1 : i), stage = kt % KS, ph = (kt / KS) & 1u, s = i & 1;
-            if (i < (TWO ? 2 : 1) && !mbar_wait_warp(smem_u32(q_ready + i), units & 1u, abort_flag)) { fail(abort_flag, 144); return false; }
-            if (!mbar_wait_warp(smem_u32(k_full + stage), ph, abort_flag)) { fail(abort_flag, 143); return false; }
-            tc_fence_after_sync();
-            if (elect_one()) {
-                const uint64_t ad = kd | (uint64_t)(((q0 + (TWO ? s * kTileBytes : 0)) & 0x3FFFFu) >> 4);
-                const uint64_t bd = kd | (uint64_t)(((k0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
+        // Step i of a unit: stream i & 1 with tile i (TWO: i / 2) of its keys.  The warp waits once a step, for the weights and values of
+        // one product and the keys of the next scores.
+        auto tile_of = [&](int i) { return it + (uint32_t)(TWO ? i >> 1 : i); };
+        auto scores = [&](int i) {                           // (one lane)
+            const uint32_t stage = tile_of(i) % KS, s = i & 1;
+            const uint64_t ad = kd | (uint64_t)(((q0 + (TWO ? s * kTileBytes : 0)) & 0x3FFFFu) >> 4);
+            const uint64_t bd = kd | (uint64_t)(((k0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
+            const uint32_t d = tmem + s * kKeys;
+            if (steps == 4 * DC) {
+#pragma unroll
+                for (int k = 0; k < 4 * DC; ++k) {
+                    const uint32_t off = (k >> 2) * (kChunk >> 4) + (k & 3) * 2;
+                    mma_bf16_ss(d, ad + off, bd + off, idesc_s, k != 0);
+                }
+            } else {
                 for (int k = 0; k < steps; ++k) {
                     const uint32_t off = (k >> 2) * (kChunk >> 4) + (k & 3) * 2;
-                    mma_bf16_ss(tmem + s * kKeys, ad + off, bd + off, idesc_s, k != 0);
+                    mma_bf16_ss(d, ad + off, bd + off, idesc_s, k != 0);
                 }
-                if (!TWO || s) mma_commit(k_empty + stage);
-                mma_commit(s_full + s);
             }
-            return true;
+            if (!TWO || s) mma_commit(k_empty + stage);
+            mma_commit(s_full + s);
         };
         while (at.left > 0 && ok) {
             const int n = at.run(), last = TWO ? 2 * n : n;
-            ok = scores(0) && (last < 2 || scores(1));
+            for (int i = 0; i < 2 && i < last && ok; ++i) {
+                uint32_t bar = 0, parity = 0;
+                if (lane == 0) { bar = smem_u32(k_full + tile_of(i) % KS); parity = (tile_of(i) / KS) & 1u; }
+                if (lane == 1 && (TWO || i == 0)) { bar = smem_u32(q_ready + i); parity = units & 1u; }
+                if (!mbar_wait_lanes(bar, parity, abort_flag)) { fail(abort_flag, 143); ok = false; break; }
+                tc_fence_after_sync();
+                if (elect_one()) scores(i);
+            }
             for (int i = 0; i < last && ok; ++i) {
-                const uint32_t vt = it + (TWO ? i >> 1 : i), stage = vt % VS, ph = (vt / VS) & 1u, s = i & 1;
-                if (!mbar_wait_warp(smem_u32(p_ready + s), made[s] & 1u, abort_flag)) { fail(abort_flag, 145); ok = false; break; }
+                const uint32_t stage = tile_of(i) % VS, s = i & 1;
+                uint32_t bar = 0, parity = 0;
+                if (lane == 0) { bar = smem_u32(p_ready + s); parity = made[s] & 1u; }
+                if (lane == 1) { bar = smem_u32(v_full + stage); parity = (tile_of(i) / VS) & 1u; }
+                if (lane == 2 && i + 2 < last) { bar = smem_u32(k_full + tile_of(i + 2) % KS); parity = (tile_of(i + 2) / KS) & 1u; }
+                if (!mbar_wait_lanes(bar, parity, abort_flag)) { fail(abort_flag, 145); ok = false; break; }
                 ++made[s];
-                if (!mbar_wait_warp(smem_u32(v_full + stage), ph, abort_flag)) { fail(abort_flag, 146); ok = false; break; }
                 tc_fence_after_sync();
                 if (elect_one()) {
                     const uint64_t bd = nd | (uint64_t)(((v0 + stage * kTileBytes) & 0x3FFFFu) >> 4);
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        mma_bf16_ts(tmem + 2 * kKeys + s * 128, tmem + s * kKeys + k * 8, bd + k * (2048 >> 4), idesc_o, i >= 2 || k != 0);
+                    const uint32_t d = tmem + 2 * kKeys + s * 128, a = tmem + s * kKeys;
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k) mma_bf16_ts(d, a + k * 8, bd + k * (2048 >> 4), idesc_o, i >= 2 || k != 0);
                     if (!TWO || s) mma_commit(v_empty + stage);
                     mma_commit(o_done + s);
+                    if (i + 2 < last) scores(i + 2);
                 }
-                if (i + 2 < last) ok = scores(i + 2);
             }
             it += n;
             ++units;
