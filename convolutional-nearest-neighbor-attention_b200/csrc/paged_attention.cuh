@@ -30,7 +30,6 @@ struct Params {
     float scale_log2;                            // scale * log2(e)
     float* partial;                              // [2 * CTAs][rows_per_tile * (D + 2) + 4]: sums, maxima, sums of weights, what was not finite
     long long slot;                              // floats of one of them
-    int slot_row, slot_col;                      // its sums: four channels of one row; distance of rows, of neighbouring fours
     int ctas;
 
     // entry / page_size of an entry below 2^31: the product with 2^slot_shift / page_size, rounded up to 32 bits, is off by less than

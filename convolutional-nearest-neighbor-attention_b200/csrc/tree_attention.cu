@@ -521,80 +521,109 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
 
 // ---- units that several CTAs had ------------------------------------------------------------------------------------------------
 
-// The pieces' maxima, then their sums, in the order of the keys.  WARPS of a block's four warps share the pieces of a row: all four where
-// units have several pieces each (a block per unit and row), else a warp goes through every fourth row of 16 of one unit (a block per
-// boundary between two CTAs' tiles, and the unit that is cut there first belongs to it).
-// What says which pieces there are is read while the kernel before is still at work: it does not write that.
+// The pieces' maxima, then their sums, in the order of the keys.  What says which pieces there are is read while the kernel before is
+// still at work: it does not write that.
+
+// The unit that is cut for the first time where CTA `cta`'s tiles begin: its pieces are c0 .. c1 (c0 == c1: there is none).
+struct Cut {
+    Sequence s;
+    int b, h, rt, c0, c1;
+    bool second;                                 // the first piece is its CTA's last unit
+};
+__device__ __forceinline__ Cut cut_at(const Params& p, int cta) {
+    Cut u{};
+    int none;
+    const Division d(total_work(p, 0, none), p.ctas);
+    if (cta < 1 || cta >= d.ctas) return u;
+    Cursor at;
+    at.find(p, d.first(cta), 1);
+    const int begin = d.first(cta) - at.tile;
+    if (!at.tile || d.cta_of(begin) != cta - 1) return u;
+    u.s = at.s;
+    u.b = at.b; u.h = at.h; u.rt = at.rt;
+    u.c0 = cta - 1;
+    u.c1 = d.cta_of(begin + at.s.tiles - 1);
+    u.second = d.first(u.c0) < begin;
+    return u;
+}
+// Rows without anything, of all sequences: zeros, by all warps of the grid.
+template <typename T>
+__device__ __forceinline__ void write_zeros(const Params& p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, blocks = gridDim.x * gridDim.y * gridDim.z;
+    for (int i = block * kWarps + warp; i < p.B * p.T; i += blocks * kWarps) {
+        const int b = i / p.T, t = i - b * p.T;
+        const Sequence s = sequence_of(p, b);
+        if (t < s.count && s.total) continue;
+        T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1];
+        for (int h = 0; h < p.Hk * p.G; ++h)
+            for (int c = lane; c < p.D; c += 32) out[h * p.os[2] + c] = from_f32<T>(0.f);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void write_four(const Params& p, const Sequence& s, int b, int h, int row, int col, const float4& sum, float inv,
+                                           bool bad) {
+    const int t = row / p.G, g = row - t * p.G;
+    float x[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+    if (bad) {
+        const unsigned long long mask = seen_by(p, s, b, row);
+        for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
+    }
+    T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] + col;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        __nv_bfloat162 w[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(w);
+    }
+}
+
+// Tiles of 16 rows.  WARPS of a block's four warps share the pieces of a row: all four where units have several pieces each (a block per
+// unit and row), else a warp goes through every fourth row of 16 of one unit (a block per boundary between two CTAs' tiles).
 constexpr int JOIN_ROWS = 16;
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
     __shared__ float4 sY[WARPS == 4 ? 4 : 1][2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Sequence s{};
-    int b = 0, h = 0, rt = 0, c0 = 0, c1 = 0;
-    bool second = false;                         // the first piece is its CTA's last unit
-    {
+    Cut u{};
+    if (WARPS == 4) {
         int before;
-        if (WARPS == 4) {
-            const int unit = blockIdx.x, rest = unit % (p.Hk * p.row_tiles);
-            b = unit / (p.Hk * p.row_tiles);
-            h = rest / p.row_tiles;
-            rt = rest - h * p.row_tiles;
-            s = sequence_of(p, b);
-            const Division d(total_work(p, b, before), p.ctas);
-            if (rt < s.row_tiles && s.tiles) {
-                const int begin = before + (h * s.row_tiles + rt) * s.tiles;
-                c0 = d.cta_of(begin);
-                c1 = d.cta_of(begin + s.tiles - 1);
-                second = d.first(c0) < begin;
-            }
-        } else {
-            const Division d(total_work(p, 0, before), p.ctas);
-            const int c = blockIdx.x;
-            if (c > 0 && c < d.ctas) {
-                Cursor at;
-                at.find(p, d.first(c), 1);
-                const int begin = d.first(c) - at.tile;
-                if (at.tile && d.cta_of(begin) == c - 1) {
-                    b = at.b; h = at.h; rt = at.rt;
-                    s = at.s;
-                    c0 = c - 1;
-                    c1 = d.cta_of(begin + s.tiles - 1);
-                    second = d.first(c0) < begin;
-                }
-            }
+        const int unit = blockIdx.x, rest = unit % (p.Hk * p.row_tiles);
+        u.b = unit / (p.Hk * p.row_tiles);
+        u.h = rest / p.row_tiles;
+        u.rt = rest - u.h * p.row_tiles;
+        u.s = sequence_of(p, u.b);
+        const Division d(total_work(p, u.b, before), p.ctas);
+        if (u.rt < u.s.row_tiles && u.s.tiles) {
+            const int begin = before + (u.h * u.s.row_tiles + u.rt) * u.s.tiles;
+            u.c0 = d.cta_of(begin);
+            u.c1 = d.cta_of(begin + u.s.tiles - 1);
+            u.second = d.first(u.c0) < begin;
         }
+    } else {
+        u = cut_at(p, blockIdx.x);
     }
     chain_begin();
-    // rows without anything, of all sequences
-    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * kWarps + warp; i < p.B * p.T; i += gridDim.x * gridDim.y * kWarps) {
-        const int zb = i / p.T, t = i - zb * p.T;
-        const Sequence z = sequence_of(p, zb);
-        if (t < z.count && z.total) continue;
-        T* out = static_cast<T*>(p.out) + zb * p.os[0] + t * p.os[1];
-        for (int hh = 0; hh < p.Hk * p.G; ++hh)
-            for (int c = lane; c < p.D; c += 32) out[hh * p.os[2] + c] = from_f32<T>(0.f);
-    }
-    if (c0 == c1) return;                        // (written by its CTA, or not this block's)
+    write_zeros<T>(p);
+    if (u.c0 == u.c1) return;                    // (written by its CTA, or not this block's)
     const long long tail = (long long)p.rows_per_tile * p.D;
-    auto piece = [&](int c) { return slot_of(p, c, c > c0 || !second); };
+    auto piece = [&](int c) { return slot_of(p, c, c > u.c0 || !u.second); };
 #pragma unroll 1
     for (int i = 0; i < (WARPS == 4 ? 1 : JOIN_ROWS / kWarps); ++i) {
-        const int r = WARPS == 4 ? blockIdx.y : blockIdx.y * JOIN_ROWS + i * kWarps + warp;
-        const int row = rt * p.rows_per_tile + r, t = row / p.G, g = row - t * p.G;
-        if (r >= p.rows_per_tile || t >= s.count) return;                // (the whole block, or a warp that meets no other)
+        const int r = WARPS == 4 ? blockIdx.y : blockIdx.y * JOIN_ROWS + i * kWarps + warp, row = u.rt * p.rows_per_tile + r;
+        if (r >= p.rows_per_tile || row >= u.s.count * p.G) return;          // (the whole block, or a warp that meets no other)
         float top = -CUDART_INF_F, sum = 0.f;
         bool bad = false;
-        for (int c = c0 + lane; c <= c1; c += 32) {
+        for (int c = u.c0 + lane; c <= u.c1; c += 32) {
             const float* from = piece(c) + tail;
             top = fmaxf(top, from[r]);
-            bad |= from[2 * p.rows_per_tile + (r >> 7)] != 0.f;          // (a word for every 128 rows)
+            bad |= from[2 * p.rows_per_tile] != 0.f;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         bad = __any_sync(0xffffffffu, bad);
         if (top == -CUDART_INF_F) top = 0.f;
-        for (int c = c0 + lane; c <= c1; c += 32) {
+        for (int c = u.c0 + lane; c <= u.c1; c += 32) {
             const float* from = piece(c) + tail;
             sum = fmaf(from[p.rows_per_tile + r], ex2(from[r] - top), sum);
         }
@@ -602,16 +631,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 8
-        for (int c = c0 + (WARPS == 4 ? warp : 0); c <= c1; c += WARPS) {
+        for (int c = u.c0 + (WARPS == 4 ? warp : 0); c <= u.c1; c += WARPS) {
             const float* from = piece(c);
             const float f = ex2(from[tail + r] - top);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int col = 4 * (lane + 32 * u);
+            for (int v = 0; v < 2; ++v) {
+                const int col = 4 * (lane + 32 * v);
                 if (col >= p.D) continue;
-                const float4 x = reinterpret_cast<const float4*>(from)[(long long)r * p.slot_row + (lane + 32 * u) * p.slot_col];
-                y[u].x = fmaf(x.x, f, y[u].x); y[u].y = fmaf(x.y, f, y[u].y);
-                y[u].z = fmaf(x.z, f, y[u].z); y[u].w = fmaf(x.w, f, y[u].w);
+                const float4 x = *reinterpret_cast<const float4*>(from + r * p.D + col);
+                y[v].x = fmaf(x.x, f, y[v].x); y[v].y = fmaf(x.y, f, y[v].y);
+                y[v].z = fmaf(x.z, f, y[v].z); y[v].w = fmaf(x.w, f, y[v].w);
             }
         }
         if (WARPS == 4) {
@@ -622,29 +651,59 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
 #pragma unroll
             for (int w = 1; w < 4; ++w)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float4 x = sY[w % WARPS][u][lane];
-                    y[u].x += x.x; y[u].y += x.y; y[u].z += x.z; y[u].w += x.w;
+                for (int v = 0; v < 2; ++v) {
+                    const float4 x = sY[w % WARPS][v][lane];
+                    y[v].x += x.x; y[v].y += x.y; y[v].z += x.z; y[v].w += x.w;
                 }
         }
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int col = 4 * (lane + 32 * u);
-            if (col >= p.D) continue;
-            float x[4] = {y[u].x * inv, y[u].y * inv, y[u].z * inv, y[u].w * inv};
-            if (bad) {
-                const unsigned long long mask = seen_by(p, s, b, row);
-                for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
-            }
-            if constexpr (sizeof(T) == 4) {
-                *reinterpret_cast<float4*>(out + col) = make_float4(x[0], x[1], x[2], x[3]);
-            } else {
-                __nv_bfloat162 w[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
-                *reinterpret_cast<uint2*>(out + col) = *reinterpret_cast<uint2*>(w);
-            }
+        for (int v = 0; v < 2; ++v) {
+            const int col = 4 * (lane + 32 * v);
+            if (col < p.D) write_four<T>(p, u.s, u.b, u.h, row, col, y[v], inv, bad);
         }
+    }
+}
+
+// Tiles of 128 rows and more: a block per boundary, 128 rows and 32 channels, a thread a row (its neighbours' sums lie beside its own).
+__global__ void __launch_bounds__(kThreads) join_tiles_kernel(const Params p) {
+    const Cut u = cut_at(p, blockIdx.x);
+    chain_begin();
+    write_zeros<__nv_bfloat16>(p);
+    const int r = blockIdx.y * 128 + threadIdx.x, row = u.rt * p.rows_per_tile + r;
+    if (u.c0 == u.c1 || row >= u.s.count * p.G) return;
+    const long long tail = (long long)p.rows_per_tile * p.D;
+    auto piece = [&](int c) { return slot_of(p, c, c > u.c0 || !u.second); };
+    float top = -CUDART_INF_F, sum = 0.f;
+    bool bad = false;
+    for (int c = u.c0; c <= u.c1; ++c) {
+        const float* from = piece(c) + tail;
+        top = fmaxf(top, from[r]);
+        bad |= from[2 * p.rows_per_tile + (r >> 7)] != 0.f;                  // (a word for every 128 rows)
+    }
+    if (top == -CUDART_INF_F) top = 0.f;
+    float4 y[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v) y[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int c = u.c0; c <= u.c1; ++c) {
+        const float* from = piece(c);
+        const float f = ex2(from[tail + r] - top);
+        sum = fmaf(from[tail + p.rows_per_tile + r], f, sum);
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+            const int four = blockIdx.z * 8 + v;
+            if (4 * four >= p.D) continue;
+            const float4 x = reinterpret_cast<const float4*>(from)[four * p.rows_per_tile + r];
+            y[v].x = fmaf(x.x, f, y[v].x); y[v].y = fmaf(x.y, f, y[v].y);
+            y[v].z = fmaf(x.z, f, y[v].z); y[v].w = fmaf(x.w, f, y[v].w);
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+        const int col = (blockIdx.z * 8 + v) * 4;
+        if (col < p.D) write_four<__nv_bfloat16>(p, u.s, u.b, u.h, row, col, y[v], inv, bad);
     }
 }
 
@@ -737,8 +796,6 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
     p.partial = static_cast<float*>(workspace);
     p.slot = slot_floats(g, p.D);
-    p.slot_row = g.tiles ? 1 : p.D / 4;
-    p.slot_col = g.tiles ? g.rows_per_tile : 1;
     p.ctas = device_sms() * g.ctas_per_sm;
     int bits = 0;
     while ((1ll << bits) < p.page_size) ++bits;
@@ -766,7 +823,12 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
         }
     }
     if (rc) return rc;
-    const int joined = rows < g.rows_per_tile ? rows : g.rows_per_tile;
+    if (g.tiles) {
+        launch_chained(join_tiles_kernel, dim3(p.ctas, g.rows_per_tile / 128, (p.D + 31) / 32), kThreads, 0, st, p);
+        CONVNN_CHECK_LAUNCH("tree_attention");
+        return CONVNN_OK;
+    }
+    const int joined = rows < ROWS ? rows : ROWS;
     const bool many = units * 4 <= p.ctas;                   // pieces a unit
     const dim3 grid = many ? dim3((unsigned)units, joined) : dim3(p.ctas, (joined + JOIN_ROWS - 1) / JOIN_ROWS);
     if (a->dtype == CONVNN_F32) {
