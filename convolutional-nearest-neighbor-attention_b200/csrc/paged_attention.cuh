@@ -31,6 +31,7 @@ struct Params {
     float* partial;                              // [2 * CTAs][rows_per_tile * (D + 2) + 4]: sums, maxima, sums of weights, what was not finite
     long long slot;                              // floats of one of them
     int ctas;
+    int split;                                   // CTAs of a cluster that share a unit, each an even part of its tiles; 0: division over all
 
     // entry / page_size of an entry below 2^31: the product with 2^slot_shift / page_size, rounded up to 32 bits, is off by less than
     // entry * page_size < 2^slot_shift
@@ -94,6 +95,16 @@ struct Cursor {
         const Division d(total_work(p, 0, none), p.ctas);
         b = h = rt = tile = left = 0;
         if (cta < d.ctas) find(p, d.first(cta), d.first(cta + 1) - d.first(cta));
+    }
+    // A unit of its own for every `split` CTAs, a part of its tiles each; whatever is not there has none.
+    __device__ __forceinline__ void start_part(const Params& p, int cta) {
+        const int unit = cta / p.split, part = cta - unit * p.split, rest = unit % (p.Hk * p.row_tiles);
+        b = unit / (p.Hk * p.row_tiles);
+        h = rest / p.row_tiles;
+        rt = rest - h * p.row_tiles;
+        s = sequence_of(p, b);
+        tile = s.tiles * part / p.split;
+        left = rt < s.row_tiles ? s.tiles * (part + 1) / p.split - tile : 0;
     }
     // `count` tiles from `begin` on.
     __device__ __forceinline__ void find(const Params& p, int begin, int count) {

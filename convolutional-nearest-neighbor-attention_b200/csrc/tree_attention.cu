@@ -8,7 +8,10 @@
 // slices in flight, and the four join at the unit's end: no barrier between slices.
 // scalar_kernel (float32): 16 rows, four to a warp, products on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA.
 // join_kernel: units that several CTAs had, and rows without anything.
+// Where the cache is short, a second kernel would cost more than the even division gains: a cluster of up to sixteen CTAs has a unit, and
+// they join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels).
 #include "paged_attention.cuh"
+#include "sm100.cuh"
 
 namespace convnn {
 namespace {
@@ -54,10 +57,84 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& r
     return (unsigned)page < (unsigned)p.pages ? page : -1;
 }
 
+__device__ __forceinline__ float4 load_cluster4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_cluster(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void write_four(const Params& p, const Sequence& s, int b, int h, int row, int col, const float4& sum, float inv,
+                                           bool bad) {
+    const int t = row / p.G, g = row - t * p.G;
+    float x[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+    if (bad) {
+        const unsigned long long mask = seen_by(p, s, b, row);
+        for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
+    }
+    T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] + col;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        __nv_bfloat162 w[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(w);
+    }
+}
+constexpr int MOST_PARTS = 16;
+// The whole cluster, when each CTA has its part's sums (16 rows, `pitch` floats apart), maxima and sums of weights in shared memory: writes
+// the unit's rows, four channels a thread, those that are not there or attend to nothing as zeros.
+template <typename T>
+__device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s, int b, int h, int rt, const float* sums, int pitch,
+                                             const float* tops, const float* weights, const int* bads) {
+    sm100::cluster_sync_all();
+    const int part = blockIdx.x % p.split, fours = p.D / 4, rows = min(ROWS, p.T * p.G - rt * ROWS);
+    const uint32_t sums_at = smem_at(sums), tops_at = smem_at(tops), weights_at = smem_at(weights), bads_at = smem_at(bads);
+    for (int i = part * kThreads + threadIdx.x; i < rows * fours; i += p.split * kThreads) {
+        const int r = i / fours, four = i - r * fours, row = rt * ROWS + r;
+        float top = -CUDART_INF_F, sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        bool bad = false;
+        if (row < s.count * p.G) {
+            // (all of them asked for before the first is used)
+            float m[MOST_PARTS], l[MOST_PARTS];
+            float4 x[MOST_PARTS];
+            uint32_t not_finite[MOST_PARTS];
+#pragma unroll
+            for (int c = 0; c < MOST_PARTS; ++c) {
+                m[c] = -CUDART_INF_F;
+                l[c] = 0.f;
+                not_finite[c] = 0;
+                if (c >= p.split) continue;
+                m[c] = load_cluster(sm100::map_to_cta(tops_at, c) + 4 * r);
+                l[c] = load_cluster(sm100::map_to_cta(weights_at, c) + 4 * r);
+                x[c] = load_cluster4(sm100::map_to_cta(sums_at, c) + 4 * (r * pitch + 4 * four));
+                not_finite[c] = __float_as_uint(load_cluster(sm100::map_to_cta(bads_at, c)));
+            }
+#pragma unroll
+            for (int c = 0; c < MOST_PARTS; ++c) top = fmaxf(top, m[c]);
+#pragma unroll
+            for (int c = 0; c < MOST_PARTS; ++c) {
+                if (c >= p.split || (m[c] == -CUDART_INF_F && l[c] == 0.f)) continue;    // a part without keys
+                const float f = m[c] == top ? 1.f : ex2(m[c] - top);
+                sum = fmaf(l[c], f, sum);
+                y.x = fmaf(x[c].x, f, y.x); y.y = fmaf(x[c].y, f, y.y);
+                y.z = fmaf(x[c].z, f, y.z); y.w = fmaf(x[c].w, f, y.w);
+                bad |= not_finite[c] != 0;
+            }
+        }
+        write_four<T>(p, s, b, h, row, 4 * four, y, sum == 0.f ? 0.f : 1.0f / sum, bad);
+    }
+    sm100::cluster_sync_all();                                       // (no CTA leaves while others read its memory)
+}
+
 // ---- bfloat16: 16 rows a tile on mma.sync ---------------------------------------------------------------------------------------
 
 // DS steps of 16 channels (D rounded up; the channels behind D are zeros), STAGES slices in flight per warp.
-template <int DS, int STAGES>
+template <int DS, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     constexpr int DP = 16 * DS, CH = DP / 8, PITCH = (CH | 1) * 16;      // an odd number of 16-byte columns: no bank conflicts
     constexpr int SLICE = 16 * PITCH, STAGE = 2 * SLICE, OP = DP + 8;
@@ -81,8 +158,18 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     chain_begin();
 
     Cursor at;
-    at.start(p, blockIdx.x);
-    if (at.left == 0) return;                                            // (the whole CTA)
+    if (SPLIT) at.start_part(p, blockIdx.x);
+    else at.start(p, blockIdx.x);
+    if (at.left == 0) {
+        if (!SPLIT) return;                                              // (the whole CTA)
+        if (threadIdx.x < ROWS) {
+            sM[threadIdx.x] = -CUDART_INF_F;
+            sL[threadIdx.x] = 0.f;
+        }
+        if (threadIdx.x == 0) *sBad = 0;
+        join_cluster<__nv_bfloat16>(p, at.s, at.b, at.h, at.rt, sO, OP, sM, sL, sBad);
+        return;
+    }
     Cursor ahead = at;
     const int chunks = p.D / 8;
     const bool one_page = p.page_size % 16 == 0;                         // a slice lies in one page
@@ -297,6 +384,12 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
             __syncthreads();
         }
         // ---- handed on, or the result
+        if (SPLIT) {
+            if (threadIdx.x < ROWS)
+                sM[threadIdx.x] = fmaxf(fmaxf(sM[threadIdx.x], sM[ROWS + threadIdx.x]), fmaxf(sM[2 * ROWS + threadIdx.x], sM[3 * ROWS + threadIdx.x]));
+            join_cluster<__nv_bfloat16>(p, s, b, h, row0 / ROWS, sO, OP, sM, sL, sBad);
+            break;
+        }
         const bool whole = tile0 == 0 && at_end;
         float* slot = slot_of(p, blockIdx.x, first_unit);
         const bool any_bad = *sBad;
@@ -344,7 +437,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
 // ---- float32: 16 rows a tile on the fp32 pipes ----------------------------------------------------------------------------------
 
 // A warp owns four rows: a lane's key of the tile for the scores, its four (or twice four) neighbouring channels for the sums.
-template <int STAGES>
+template <int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
     constexpr int TILE = 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -357,9 +450,22 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     chain_begin();
 
+    // what a cluster's CTAs read from one another: the sums, where the ring was, and beside the queries
+    float *sTop = sP, *sSum = sP + ROWS;
+    int* sBad = reinterpret_cast<int*>(sP + 2 * ROWS);
     Cursor at;
-    at.start(p, blockIdx.x);
-    if (at.left == 0) return;
+    if (SPLIT) at.start_part(p, blockIdx.x);
+    else at.start(p, blockIdx.x);
+    if (at.left == 0) {
+        if (!SPLIT) return;
+        if (threadIdx.x < ROWS) {
+            sTop[threadIdx.x] = -CUDART_INF_F;
+            sSum[threadIdx.x] = 0.f;
+        }
+        if (threadIdx.x == 0) *sBad = 0;
+        join_cluster<float>(p, at.s, at.b, at.h, at.rt, ring, pitch, sTop, sSum, sBad);
+        return;
+    }
     Cursor ahead = at;
     auto fetch = [&](int stage) {
         float* dst = ring + stage * stage_floats;
@@ -485,6 +591,26 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
             at_end = at.tile + 1 == s.tiles;
             at.next(p);
         } while (!end);
+        if (SPLIT) {
+            copies_wait<0>();
+            __syncthreads();                                             // (the ring and the weights are read)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * warp + i;
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (lane + 32 * u < pieces) *reinterpret_cast<float4*>(ring + r * pitch + 4 * (lane + 32 * u)) = o[i][u];
+                if (lane == 0) {
+                    sTop[r] = m[i];
+                    sSum[r] = l[i];
+                }
+            }
+            if (threadIdx.x == 0) *sBad = 0;
+            join_cluster<float>(p, s, b, h, row0 / ROWS, ring, pitch, sTop, sSum, sBad);
+            break;
+        }
         const bool whole = tile0 == 0 && at_end;
         float* slot = slot_of(p, blockIdx.x, first_unit);
 #pragma unroll
@@ -560,24 +686,6 @@ __device__ __forceinline__ void write_zeros(const Params& p) {
             for (int c = lane; c < p.D; c += 32) out[h * p.os[2] + c] = from_f32<T>(0.f);
     }
 }
-template <typename T>
-__device__ __forceinline__ void write_four(const Params& p, const Sequence& s, int b, int h, int row, int col, const float4& sum, float inv,
-                                           bool bad) {
-    const int t = row / p.G, g = row - t * p.G;
-    float x[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
-    if (bad) {
-        const unsigned long long mask = seen_by(p, s, b, row);
-        for (int e = 0; e < 4; ++e) x[e] += not_finite_seen<T>(p, s, b, h, mask, col + e);
-    }
-    T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] + col;
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-        __nv_bfloat162 w[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
-        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(w);
-    }
-}
-
 // Tiles of 16 rows.  WARPS of a block's four warps share the pieces of a row: all four where units have several pieces each (a block per
 // unit and row), else a warp goes through every fourth row of 16 of one unit (a block per boundary between two CTAs' tiles).
 constexpr int JOIN_ROWS = 16;
@@ -752,17 +860,53 @@ bool tiles_wanted(int dtype, int rows, int D) { return dtype == CONVNN_BF16 && r
 
 long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
 
+int launch_clusters(void (*kern)(Params), const Params& p, unsigned grid, size_t smem, cudaStream_t st) {
+    // (more than eight CTAs are not every device's: this one's are)
+    static std::atomic<const void*> allowed[16];
+    const void* const me = reinterpret_cast<const void*>(kern);
+    bool seen = false;
+    for (auto& k : allowed) seen = seen || k.load(std::memory_order_relaxed) == me;
+    if (!seen) {
+        const cudaError_t e = cudaFuncSetAttribute(me, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "tree_attention: %s", cudaGetErrorString(e));
+        for (auto& k : allowed) {
+            const void* none = nullptr;
+            if (k.compare_exchange_strong(none, me)) break;
+        }
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2] = {chained_attribute(st), {}};
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid; cfg.blockDim = kThreads; cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, p);               // an error stays the thread's last error (CONVNN_CHECK_LAUNCH)
+    return CONVNN_OK;
+}
 template <int DS, int STAGES>
-int launch_rows(const Params& p, size_t smem, cudaStream_t st) {
-    CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES>), smem);
-    launch_chained(rows_kernel<DS, STAGES>, p.ctas, kThreads, smem, st, p);
+int launch_rows(const Params& p, unsigned units, size_t smem, cudaStream_t st) {
+    if (p.split) {
+        CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, true>), smem);
+        const int rc = launch_clusters(rows_kernel<DS, STAGES, true>, p, units * p.split, smem, st);
+        if (rc) return rc;
+    } else {
+        CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, false>), smem);
+        launch_chained(rows_kernel<DS, STAGES, false>, p.ctas, kThreads, smem, st, p);
+    }
     CONVNN_CHECK_LAUNCH("tree_attention");
     return CONVNN_OK;
 }
 template <int STAGES>
-int launch_scalar(const Params& p, size_t smem, cudaStream_t st) {
-    CONVNN_ENSURE_SMEM(scalar_kernel<STAGES>, smem);
-    launch_chained(scalar_kernel<STAGES>, p.ctas, kThreads, smem, st, p);
+int launch_scalar(const Params& p, unsigned units, size_t smem, cudaStream_t st) {
+    if (p.split) {
+        CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, true>), smem);
+        const int rc = launch_clusters(scalar_kernel<STAGES, true>, p, units * p.split, smem, st);
+        if (rc) return rc;
+    } else {
+        CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, false>), smem);
+        launch_chained(scalar_kernel<STAGES, false>, p.ctas, kThreads, smem, st, p);
+    }
     CONVNN_CHECK_LAUNCH("tree_attention");
     return CONVNN_OK;
 }
@@ -807,22 +951,27 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     if (workspace_bytes < (size_t)p.ctas * 2 * p.slot * 4)
         return set_error(CONVNN_E_WORKSPACE, "tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
                          (size_t)p.ctas * 2 * p.slot * 4);
+    // A unit to a cluster where all tiles that there may be are few for each CTA that runs at once: as many CTAs as run at once, up to
+    // sixteen a unit.
+    const long long unit_tiles = (keys + p.tile - 1) / p.tile;
+    if (!g.tiles && units * unit_tiles <= 16ll * p.ctas)
+        for (p.split = 1; p.split < MOST_PARTS && p.split < unit_tiles && units * p.split * 2 <= p.ctas;) p.split *= 2;
     int rc;
     if (g.tiles) {
         rc = launch_tree_tiles(p, st);
     } else if (a->dtype == CONVNN_F32) {
-        rc = g.stages == 3 ? launch_scalar<3>(p, g.smem, st) : launch_scalar<2>(p, g.smem, st);
+        rc = g.stages == 3 ? launch_scalar<3>(p, (unsigned)units, g.smem, st) : launch_scalar<2>(p, (unsigned)units, g.smem, st);
     } else {
         switch (steps_of(p.D)) {
-            case 4: rc = launch_rows<4, 4>(p, g.smem, st); break;
-            case 5: rc = launch_rows<5, 3>(p, g.smem, st); break;
-            case 6: rc = launch_rows<6, 3>(p, g.smem, st); break;
-            case 8: rc = launch_rows<8, 2>(p, g.smem, st); break;
-            case 12: rc = launch_rows<12, 2>(p, g.smem, st); break;
-            default: rc = launch_rows<16, 2>(p, g.smem, st); break;
+            case 4: rc = launch_rows<4, 4>(p, (unsigned)units, g.smem, st); break;
+            case 5: rc = launch_rows<5, 3>(p, (unsigned)units, g.smem, st); break;
+            case 6: rc = launch_rows<6, 3>(p, (unsigned)units, g.smem, st); break;
+            case 8: rc = launch_rows<8, 2>(p, (unsigned)units, g.smem, st); break;
+            case 12: rc = launch_rows<12, 2>(p, (unsigned)units, g.smem, st); break;
+            default: rc = launch_rows<16, 2>(p, (unsigned)units, g.smem, st); break;
         }
     }
-    if (rc) return rc;
+    if (rc || p.split) return rc;
     if (g.tiles) {
         launch_chained(join_tiles_kernel, dim3(p.ctas, g.rows_per_tile / 128, (p.D + 31) / 32), kThreads, 0, st, p);
         CONVNN_CHECK_LAUNCH("tree_attention");

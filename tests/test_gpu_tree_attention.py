@@ -434,3 +434,78 @@ def test_tiles_of_rows_and_scales(T, G, scale):
     cache = cache_of(1, 2, 16, 64, 400)
     q = randn(1, T, 2 * G, 64, seed=9, dtype=BF16)
     check_attention(ops.tree_attention(q, cache, ints(300), scale=scale), q, cache, ints(300), scale=scale)
+
+
+# ---- the even division ------------------------------------------------------------------------------------------------
+
+def widened(cache, entries=1 << 20):
+    """The same cache with room in its tables for far more entries than there are: the work is divided over all CTAs, and joined by a second
+    kernel, by what the tables could hold."""
+    more = entries // cache.k.shape[2]
+    return cache._replace(table=torch.cat([cache.table, torch.full((cache.table.shape[0], more), -1, dtype=torch.int32, device="cuda")], 1))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [8, 40, 64, 80, 96, 128, 136, 256])
+@pytest.mark.parametrize("T,G", [(1, 1), (1, 8), (3, 3)])
+def test_division_widths(dtype, D, T, G):
+    cache = widened(cache_of(2, 3, 16, D, 900 + T, dtype))
+    q = randn(2, T, 3 * G, D, seed=9, dtype=dtype)
+    lengths = ints(900, 444)
+    got = ops.tree_attention(q, cache, lengths)
+    check_attention(got, q, cache, lengths)
+    assert torch.equal(got, ops.tree_attention(q, cache, lengths))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,G", [(1, 4), (6, 3)])
+def test_division_lengths(dtype, T, G):
+    lengths = [0, 1, 31, 32, 33, 63, 64, 65, 0, 127, 128, 129, 1000, 257, 2, 511, 513, 0, 0, 1023, 1025, 7, 64, 64, 64, 64, 1, 1, 1, 1, 1, 1, 1, 3000, 0, 1]
+    B, H, D = len(lengths), 2, 64
+    cache = widened(cache_of(B, H, 16, D, 3010, dtype))
+    q = randn(B, T, H * G, D, seed=9, dtype=dtype)
+    at, counts, tree = ints(*lengths), ints(*[(b * 5) % (T + 1) for b in range(B)]), trees(B, T)
+    check_attention(ops.tree_attention(q, cache, at), q, cache, at)
+    check_attention(ops.tree_attention(q, cache, at, tree, counts), q, cache, at, tree, counts)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [4, 20])
+def test_division_of_nothing(dtype, T):
+    cache = widened(cache_of(3, 2, 16, 64, 60, dtype))
+    q = randn(3, T, 4, 64, seed=9, dtype=dtype)
+    nobody = torch.zeros(3, T, dtype=torch.int64, device="cuda")
+    for lengths, counts in ((ints(0, 0, 0), ints(0, 0, 0)), (ints(9, 9, 9), ints(0, -1, 0)), (ints(0, 0, 0), ints(T, T, T))):
+        got = ops.tree_attention(q, cache, lengths, nobody, counts, out=torch.full_like(q, 7.0))
+        assert not got.any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("length", [5, 3000])
+def test_division_and_what_is_not_seen(dtype, wide, length):
+    B, H, D, P, T = 1, 2, 64, 16, 6
+    cache = cache_of(B, H, P, D, length + T, dtype)
+    cache = widened(cache) if wide else cache
+    q = randn(B, T, 4, D, seed=9, dtype=dtype)
+    lengths, tree = ints(length), trees(B, T, seed=3)
+    tree[0] &= ~2
+    tree[0, 2] |= 2
+    want = ops.tree_attention(q, cache, lengths, tree)
+    check_attention(want, q, cache, lengths, tree)
+    e = length + 1
+    cache.v[int(cache.table[0, e // P]), 1, e % P, 7] = -float("inf")
+    got = ops.tree_attention(q, cache, lengths, tree)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, 2, 2:, 7] = True
+    assert torch.equal(got[~hit], want[~hit]) and (got[hit] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,T,H,G,D,length", [(1, 1, 8, 4, 128, 20000), (3, 1, 40, 1, 64, 900), (100, 1, 3, 2, 64, 300), (2, 5, 2, 3, 192, 3001)])
+def test_division_and_clusters_agree(dtype, B, T, H, G, D, length):
+    cache = cache_of(B, H, 64, D, length + T, dtype)
+    q = randn(B, T, H * G, D, seed=9, dtype=dtype)
+    lengths = ints(*[length - (b * 37) % length for b in range(B)])
+    for c in (cache, widened(cache)):
+        check_attention(ops.tree_attention(q, c, lengths), q, c, lengths)
