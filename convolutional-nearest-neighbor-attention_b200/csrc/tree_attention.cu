@@ -57,16 +57,14 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& r
     return (unsigned)page < (unsigned)p.pages ? page : -1;
 }
 
-__device__ __forceinline__ float4 load_cluster4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void push4(uint32_t at, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-__device__ __forceinline__ float load_cluster(uint32_t at) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void push2(uint32_t at, float x, float y) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 template <typename T>
 __device__ __forceinline__ void write_four(const Params& p, const Sequence& s, int b, int h, int row, int col, const float4& sum, float inv,
                                            bool bad) {
@@ -85,51 +83,62 @@ __device__ __forceinline__ void write_four(const Params& p, const Sequence& s, i
     }
 }
 constexpr int MOST_PARTS = 16;
-// The whole cluster, when each CTA has its part's sums (16 rows, `pitch` floats apart), maxima and sums of weights in shared memory: writes
-// the unit's rows, four channels a thread, those that are not there or attend to nothing as zeros.
-template <typename T>
-__device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s, int b, int h, int rt, const float* sums, int pitch,
-                                             const float* tops, const float* weights, const int* bads) {
-    sm100::cluster_sync_all();
-    const int part = blockIdx.x % p.split, fours = p.D / 4, rows = min(ROWS, p.T * p.G - rt * ROWS);
-    const uint32_t sums_at = smem_at(sums), tops_at = smem_at(tops), weights_at = smem_at(weights), bads_at = smem_at(bads);
-    for (int i = part * kThreads + threadIdx.x; i < rows * fours; i += p.split * kThreads) {
-        const int r = i / fours, four = i - r * fours, row = rt * ROWS + r;
+// Bytes that join_cluster() needs for `fours` groups of four channels.
+__host__ __device__ inline int join_bytes(int fours) { return (ROWS * fours + MOST_PARTS) * 24 + 4 * MOST_PARTS; }
+// The whole cluster, behind a cluster_arrive() at the kernel's start: joins the parts of the unit's rows and writes them, zeros where a
+// row is not there or attends to nothing.  Every CTA has an even share of the groups of four channels of all rows, and the others
+// store theirs into its memory (`room`), which nobody waits for; reading them instead, 64 loads one after the other, took 4 us.
+// part_of(row, four, sums, maximum, sum of weights) says what this CTA has.
+template <typename T, typename F>
+__device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s, int b, int h, int rt, uint8_t* room, bool bad, const F& part_of) {
+    const int part = blockIdx.x % p.split, fours = p.D / 4, items = min(ROWS, p.T * p.G - rt * ROWS) * fours;
+    const int share = (items + p.split - 1) / p.split, all = share * p.split;
+    const uint32_t sums = smem_at(room), weights = sums + 16 * all, bads = weights + 8 * all;
+    cluster_wait();                                                  // (the others run)
+    for (int i = threadIdx.x; i < items; i += kThreads) {
+        const int owner = i / share, at = part * share + i - owner * share, r = i / fours;
+        float4 x;
+        float m, l;
+        part_of(r, i - r * fours, x, m, l);
+        push4(sm100::map_to_cta(sums, owner) + 16 * at, x);
+        push2(sm100::map_to_cta(weights, owner) + 8 * at, m, l);
+    }
+    if (threadIdx.x < p.split) sm100::st_cluster_u32(sm100::map_to_cta(bads, threadIdx.x) + 4 * part, bad);
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const float4* got = reinterpret_cast<const float4*>(room);
+    const float2* got_weights = reinterpret_cast<const float2*>(got + all);
+    const uint32_t* got_bads = reinterpret_cast<const uint32_t*>(got_weights + all);
+    for (int j = threadIdx.x; j < share && part * share + j < items; j += kThreads) {
+        const int i = part * share + j, r = i / fours, row = rt * ROWS + r;
         float top = -CUDART_INF_F, sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        bool bad = false;
+        bool any_bad = false;
         if (row < s.count * p.G) {
-            // (all of them asked for before the first is used)
-            float m[MOST_PARTS], l[MOST_PARTS];
-            float4 x[MOST_PARTS];
-            uint32_t not_finite[MOST_PARTS];
-#pragma unroll
-            for (int c = 0; c < MOST_PARTS; ++c) {
-                m[c] = -CUDART_INF_F;
-                l[c] = 0.f;
-                not_finite[c] = 0;
-                if (c >= p.split) continue;
-                m[c] = load_cluster(sm100::map_to_cta(tops_at, c) + 4 * r);
-                l[c] = load_cluster(sm100::map_to_cta(weights_at, c) + 4 * r);
-                x[c] = load_cluster4(sm100::map_to_cta(sums_at, c) + 4 * (r * pitch + 4 * four));
-                not_finite[c] = __float_as_uint(load_cluster(sm100::map_to_cta(bads_at, c)));
-            }
-#pragma unroll
-            for (int c = 0; c < MOST_PARTS; ++c) top = fmaxf(top, m[c]);
-#pragma unroll
-            for (int c = 0; c < MOST_PARTS; ++c) {
-                if (c >= p.split || (m[c] == -CUDART_INF_F && l[c] == 0.f)) continue;    // a part without keys
-                const float f = m[c] == top ? 1.f : ex2(m[c] - top);
-                sum = fmaf(l[c], f, sum);
-                y.x = fmaf(x[c].x, f, y.x); y.y = fmaf(x[c].y, f, y.y);
-                y.z = fmaf(x[c].z, f, y.z); y.w = fmaf(x[c].w, f, y.w);
-                bad |= not_finite[c] != 0;
+            for (int c = 0; c < p.split; ++c) top = fmaxf(top, got_weights[c * share + j].x);
+#pragma unroll 4
+            for (int c = 0; c < p.split; ++c) {
+                const float2 w = got_weights[c * share + j];
+                const float4 x = got[c * share + j];
+                const float f = w.x == top ? 1.f : ex2(w.x - top);   // (nothing anywhere: zeros, once each)
+                sum = fmaf(w.y, f, sum);
+                y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y);
+                y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+                any_bad |= got_bads[c] != 0;
             }
         }
-        write_four<T>(p, s, b, h, row, 4 * four, y, sum == 0.f ? 0.f : 1.0f / sum, bad);
+        write_four<T>(p, s, b, h, row, 4 * (i - r * fours), y, sum == 0.f ? 0.f : 1.0f / sum, any_bad);
     }
-    sm100::cluster_sync_all();                                       // (no CTA leaves while others read its memory)
 }
+// A part without keys.
+struct NoPart {
+    __device__ __forceinline__ void operator()(int, int, float4& x, float& m, float& l) const {
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+        m = -CUDART_INF_F;
+        l = 0.f;
+    }
+};
 
 // ---- bfloat16: 16 rows a tile on mma.sync ---------------------------------------------------------------------------------------
 
@@ -145,6 +154,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     float* sL = sM + kWarps * ROWS;                                      // [16] sums
     int* sBad = reinterpret_cast<int*>(sL + ROWS);
     uint8_t* ring = reinterpret_cast<uint8_t*>(sBad + 4);
+    uint8_t* room = ring + kWarps * STAGES * STAGE;                      // (SPLIT)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t own = smem_at(ring) + warp * (STAGES * STAGE);
 
@@ -155,19 +165,14 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         }
         __syncthreads();
     }
+    if (SPLIT) cluster_arrive();
     chain_begin();
 
     Cursor at;
     if (SPLIT) at.start_part(p, blockIdx.x);
     else at.start(p, blockIdx.x);
-    if (at.left == 0) {
-        if (!SPLIT) return;                                              // (the whole CTA)
-        if (threadIdx.x < ROWS) {
-            sM[threadIdx.x] = -CUDART_INF_F;
-            sL[threadIdx.x] = 0.f;
-        }
-        if (threadIdx.x == 0) *sBad = 0;
-        join_cluster<__nv_bfloat16>(p, at.s, at.b, at.h, at.rt, sO, OP, sM, sL, sBad);
+    if (at.left == 0) {                                                  // (the whole CTA)
+        if (SPLIT) join_cluster<__nv_bfloat16>(p, at.s, at.b, at.h, at.rt, room, false, NoPart());
         return;
     }
     Cursor ahead = at;
@@ -200,6 +205,16 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         }
         copies_end();
     };
+    // the rows of q (zeros where a token is not there), with the first slice's copies where there is one unit
+    auto copy_rows = [&]() {
+        for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
+            const int r = i / chunks, col = i - r * chunks, row = at.rt * ROWS + r, t = row / p.G;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
+            if (t < at.s.count) q += at.b * p.qs[0] + t * p.qs[1] + (at.h * p.G + row - t * p.G) * p.qs[2] + col * 8;
+            copy16(smem_at(sQ) + r * PITCH + col * 16, q, t < at.s.count);
+        }
+    };
+    if (SPLIT) copy_rows();
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) {
         if (ahead.left > 0) { fetch(i); ahead.next(p); }
@@ -215,16 +230,18 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         // ---- a unit: its rows
         const Sequence s = at.s;
         const int b = at.b, h = at.h, row0 = at.rt * ROWS, tile0 = at.tile;
-        for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
-            const int r = i / chunks, col = i - r * chunks, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (t < s.count)
-                v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + b * p.qs[0] + t * p.qs[1] +
-                                                    (h * p.G + g) * p.qs[2] + col * 8);
-            *reinterpret_cast<uint4*>(sQ + r * PITCH + col * 16) = v;
-        }
+        if (!SPLIT)
+            for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
+                const int r = i / chunks, col = i - r * chunks, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (t < s.count)
+                    v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + b * p.qs[0] + t * p.qs[1] +
+                                                        (h * p.G + g) * p.qs[2] + col * 8);
+                *reinterpret_cast<uint4*>(sQ + r * PITCH + col * 16) = v;
+            }
         if (threadIdx.x == 0) *sBad = 0;
         const unsigned long long mask0 = seen_by(p, s, b, row0 + lane / 4), mask1 = seen_by(p, s, b, row0 + lane / 4 + 8);
+        if (SPLIT) copies_wait<STAGES - 2>();
         __syncthreads();
         float o[2 * DS][4], m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
 #pragma unroll
@@ -350,6 +367,35 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
             sM[warp * ROWS + r0] = m0;
             sM[warp * ROWS + r1] = m1;
         }
+        if (SPLIT) {
+            // one unit: the ring is free, a warp's own part of it takes its sums
+            float* mine = reinterpret_cast<float*>(ring + warp * (STAGES * STAGE));
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < 2 * DS; ++n) {
+                *reinterpret_cast<float2*>(mine + r0 * OP + n * 8 + (lane & 3) * 2) = make_float2(o[n][0], o[n][1]);
+                *reinterpret_cast<float2*>(mine + r1 * OP + n * 8 + (lane & 3) * 2) = make_float2(o[n][2], o[n][3]);
+            }
+            if ((lane & 3) == 0) {
+                sO[warp * ROWS + r0] = l0;
+                sO[warp * ROWS + r1] = l1;
+            }
+            __syncthreads();
+            join_cluster<__nv_bfloat16>(p, s, b, h, row0 / ROWS, room, *sBad != 0, [&](int r, int four, float4& x, float& m, float& l) {
+                m = fmaxf(fmaxf(sM[r], sM[ROWS + r]), fmaxf(sM[2 * ROWS + r], sM[3 * ROWS + r]));
+                x = make_float4(0.f, 0.f, 0.f, 0.f);
+                l = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(ring + w * (STAGES * STAGE) + 4 * (r * OP + 4 * four));
+                    const float f = sM[w * ROWS + r] == m ? 1.f : ex2(sM[w * ROWS + r] - m);
+                    l = fmaf(sO[w * ROWS + r], f, l);
+                    x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y);
+                    x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+                }
+            });
+            break;
+        }
         __syncthreads();
         float t0 = sM[r0], t1 = sM[r1];
 #pragma unroll
@@ -384,12 +430,6 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
             __syncthreads();
         }
         // ---- handed on, or the result
-        if (SPLIT) {
-            if (threadIdx.x < ROWS)
-                sM[threadIdx.x] = fmaxf(fmaxf(sM[threadIdx.x], sM[ROWS + threadIdx.x]), fmaxf(sM[2 * ROWS + threadIdx.x], sM[3 * ROWS + threadIdx.x]));
-            join_cluster<__nv_bfloat16>(p, s, b, h, row0 / ROWS, sO, OP, sM, sL, sBad);
-            break;
-        }
         const bool whole = tile0 == 0 && at_end;
         float* slot = slot_of(p, blockIdx.x, first_unit);
         const bool any_bad = *sBad;
@@ -448,22 +488,16 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
     float* ring = sP + ROWS * TILE;
     const int stage_floats = 2 * TILE * pitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (SPLIT) cluster_arrive();
     chain_begin();
 
-    // what a cluster's CTAs read from one another: the sums, where the ring was, and beside the queries
-    float *sTop = sP, *sSum = sP + ROWS;
-    int* sBad = reinterpret_cast<int*>(sP + 2 * ROWS);
+    float *sTop = sP, *sSum = sP + ROWS;                                 // (SPLIT, at the end)
+    uint8_t* room = reinterpret_cast<uint8_t*>(ring + STAGES * stage_floats);
     Cursor at;
     if (SPLIT) at.start_part(p, blockIdx.x);
     else at.start(p, blockIdx.x);
     if (at.left == 0) {
-        if (!SPLIT) return;
-        if (threadIdx.x < ROWS) {
-            sTop[threadIdx.x] = -CUDART_INF_F;
-            sSum[threadIdx.x] = 0.f;
-        }
-        if (threadIdx.x == 0) *sBad = 0;
-        join_cluster<float>(p, at.s, at.b, at.h, at.rt, ring, pitch, sTop, sSum, sBad);
+        if (SPLIT) join_cluster<float>(p, at.s, at.b, at.h, at.rt, room, false, NoPart());
         return;
     }
     Cursor ahead = at;
@@ -607,8 +641,12 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
                     sSum[r] = l[i];
                 }
             }
-            if (threadIdx.x == 0) *sBad = 0;
-            join_cluster<float>(p, s, b, h, row0 / ROWS, ring, pitch, sTop, sSum, sBad);
+            __syncthreads();
+            join_cluster<float>(p, s, b, h, row0 / ROWS, room, false, [&](int r, int four, float4& x, float& m_, float& l_) {
+                x = *reinterpret_cast<const float4*>(ring + r * pitch + 4 * four);
+                m_ = sTop[r];
+                l_ = sSum[r];
+            });
             break;
         }
         const bool whole = tile0 == 0 && at_end;
@@ -956,19 +994,20 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
     const long long unit_tiles = (keys + p.tile - 1) / p.tile;
     if (!g.tiles && units * unit_tiles <= 16ll * p.ctas)
         for (p.split = 1; p.split < MOST_PARTS && p.split < unit_tiles && units * p.split * 2 <= p.ctas;) p.split *= 2;
+    const size_t smem = g.smem + (p.split ? (size_t)join_bytes(p.D / 4) : 0);
     int rc;
     if (g.tiles) {
         rc = launch_tree_tiles(p, st);
     } else if (a->dtype == CONVNN_F32) {
-        rc = g.stages == 3 ? launch_scalar<3>(p, (unsigned)units, g.smem, st) : launch_scalar<2>(p, (unsigned)units, g.smem, st);
+        rc = g.stages == 3 ? launch_scalar<3>(p, (unsigned)units, smem, st) : launch_scalar<2>(p, (unsigned)units, smem, st);
     } else {
         switch (steps_of(p.D)) {
-            case 4: rc = launch_rows<4, 4>(p, (unsigned)units, g.smem, st); break;
-            case 5: rc = launch_rows<5, 3>(p, (unsigned)units, g.smem, st); break;
-            case 6: rc = launch_rows<6, 3>(p, (unsigned)units, g.smem, st); break;
-            case 8: rc = launch_rows<8, 2>(p, (unsigned)units, g.smem, st); break;
-            case 12: rc = launch_rows<12, 2>(p, (unsigned)units, g.smem, st); break;
-            default: rc = launch_rows<16, 2>(p, (unsigned)units, g.smem, st); break;
+            case 4: rc = launch_rows<4, 4>(p, (unsigned)units, smem, st); break;
+            case 5: rc = launch_rows<5, 3>(p, (unsigned)units, smem, st); break;
+            case 6: rc = launch_rows<6, 3>(p, (unsigned)units, smem, st); break;
+            case 8: rc = launch_rows<8, 2>(p, (unsigned)units, smem, st); break;
+            case 12: rc = launch_rows<12, 2>(p, (unsigned)units, smem, st); break;
+            default: rc = launch_rows<16, 2>(p, (unsigned)units, smem, st); break;
         }
     }
     if (rc || p.split) return rc;
