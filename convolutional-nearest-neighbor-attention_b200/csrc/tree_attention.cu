@@ -6,10 +6,13 @@
 //
 // rows_kernel (bfloat16): 16 rows on mma.sync.  Each of four warps walks every fourth slice of 16 keys by itself, copies of its next
 // slices in flight, and the four join at the unit's end: no barrier between slices.
-// scalar_kernel (float32): 16 rows, four to a warp, products on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA.
+// scalar_kernel (float32): 16 rows on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA, four rows by four keys or channels a
+// thread.
 // join_kernel: units that several CTAs had, and rows without anything.
 // Where the cache is short, a second kernel would cost more than the even division gains: a cluster of up to sixteen CTAs has a unit, and
 // they join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels).
+#include <type_traits>
+
 #include "paged_attention.cuh"
 #include "sm100.cuh"
 
@@ -47,14 +50,6 @@ __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& rest) {
     const __nv_bfloat162 lo = __floats2bfloat162_rn(x - __uint_as_float(hx & 0xffff0000u), y - __uint_as_float(hy & 0xffff0000u));
     rest = *reinterpret_cast<const uint32_t*>(&lo);
     return __byte_perm(hx, hy, 0x7632);
-}
-
-// The page that holds entry `entry` of sequence b, -1: none.
-__device__ __forceinline__ int page_of(const Params& p, int b, int entry, int& row) {
-    const int slot = p.slot_at(entry);
-    row = entry - slot * p.page_size;
-    const int page = p.table[b * p.table_stride + slot];
-    return (unsigned)page < (unsigned)p.pages ? page : -1;
 }
 
 __device__ __forceinline__ void push4(uint32_t at, const float4& v) {
@@ -95,7 +90,7 @@ __device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s,
     const int share = (items + p.split - 1) / p.split, all = share * p.split;
     const uint32_t sums = smem_at(room), weights = sums + 16 * all, bads = weights + 8 * all;
     cluster_wait();                                                  // (the others run)
-    for (int i = threadIdx.x; i < items; i += kThreads) {
+    for (int i = threadIdx.x; i < items; i += blockDim.x) {
         const int owner = i / share, at = part * share + i - owner * share, r = i / fours;
         float4 x;
         float m, l;
@@ -110,7 +105,7 @@ __device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s,
     const float4* got = reinterpret_cast<const float4*>(room);
     const float2* got_weights = reinterpret_cast<const float2*>(got + all);
     const uint32_t* got_bads = reinterpret_cast<const uint32_t*>(got_weights + all);
-    for (int j = threadIdx.x; j < share && part * share + j < items; j += kThreads) {
+    for (int j = threadIdx.x; j < share && part * share + j < items; j += blockDim.x) {
         const int i = part * share + j, r = i / fours, row = rt * ROWS + r;
         float top = -CUDART_INF_F, sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -179,32 +174,41 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     const int chunks = p.D / 8;
     const bool one_page = p.page_size % 16 == 0;                         // a slice lies in one page
 
+    // The page of a lane's row of this warp's slice of ahead's tile is asked for a slice before it is copied; lanes 16 apart have one row.
+    int next_row = 0, next_page = -1;
+    auto look_up = [&]() {
+        const int first = ahead.tile * 64 + warp * 16, entry = one_page ? first : first + (lane & 15), slot = p.slot_at(entry);
+        next_page = -1;
+        next_row = entry - slot * p.page_size + (one_page ? lane & 15 : 0);
+        if (ahead.left > 0 && entry < ahead.s.total) next_page = p.table[ahead.b * p.table_stride + slot];
+    };
     // this warp's slice of ahead's tile into `stage`
     auto fetch = [&](int stage) {
-        const int first = ahead.tile * 64 + warp * 16;
-        if (first < ahead.s.total) {
+        if (ahead.left > 0) {
+            const int first = ahead.tile * 64 + warp * 16;
+            const bool any = first < ahead.s.total, there = (unsigned)next_page < (unsigned)p.pages && first + (lane & 15) < ahead.s.total;
             const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(p.k) + ahead.h * p.ks[1];
             const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v) + ahead.h * p.vs[1];
             const uint32_t dst = own + stage * STAGE;
-            const int lr = lane & 15;
-            int row = 0, page = -1;
-            if (one_page || first + lr < ahead.s.total) page = page_of(p, ahead.b, one_page ? first : first + lr, row);
-            const bool there = page >= 0 && first + lr < ahead.s.total;
-            const long long kr = there ? page * p.ks[0] + (row + (one_page ? lr : 0)) * p.ks[2] : 0;
-            const long long vr = there ? page * p.vs[0] + (row + (one_page ? lr : 0)) * p.vs[2] : 0;
+            const long long kr = there ? next_page * p.ks[0] + next_row * p.ks[2] : 0, vr = there ? next_page * p.vs[0] + next_row * p.vs[2] : 0;
+            ahead.next(p);
+            look_up();
+            if (any) {
 #pragma unroll
-            for (int i = 0; i < DS; ++i) {
-                const int c = i * 32 + lane, r = c / CH, col = c - r * CH;
-                const long long ko = __shfl_sync(0xffffffffu, kr, r), vo = __shfl_sync(0xffffffffu, vr, r);
-                const bool copied = __shfl_sync(0xffffffffu, (int)there, r);
-                if (col < chunks) {
-                    copy16(dst + r * PITCH + col * 16, k + ko + col * 8, copied);
-                    copy16(dst + SLICE + r * PITCH + col * 16, v + vo + col * 8, copied);
+                for (int i = 0; i < DS; ++i) {
+                    const int c = i * 32 + lane, r = c / CH, col = c - r * CH;
+                    const long long ko = __shfl_sync(0xffffffffu, kr, r), vo = __shfl_sync(0xffffffffu, vr, r);
+                    const bool copied = __shfl_sync(0xffffffffu, (int)there, r);
+                    if (col < chunks) {
+                        copy16(dst + r * PITCH + col * 16, k + ko + col * 8, copied);
+                        copy16(dst + SLICE + r * PITCH + col * 16, v + vo + col * 8, copied);
+                    }
                 }
             }
         }
         copies_end();
     };
+    look_up();
     // the rows of q (zeros where a token is not there), with the first slice's copies where there is one unit
     auto copy_rows = [&]() {
         for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
@@ -216,10 +220,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     };
     if (SPLIT) copy_rows();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (ahead.left > 0) { fetch(i); ahead.next(p); }
-        else copies_end();
-    }
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
     const uint32_t q_at = smem_at(sQ) + (lane & 15) * PITCH + (lane >> 4) * 16;
     const uint32_t k_lane = ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
@@ -251,12 +252,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         bool bad = false, end, at_end;
         do {
             // ---- a tile: this warp's slice of it
-            if (ahead.left > 0) {
-                fetch(stage == 0 ? STAGES - 1 : stage - 1);
-                ahead.next(p);
-            } else {
-                copies_end();
-            }
+            fetch(stage == 0 ? STAGES - 1 : stage - 1);
             copies_wait<STAGES - 1>();
             __syncwarp();
             const int first = at.tile * 64 + warp * 16;
@@ -476,23 +472,31 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
 
 // ---- float32: 16 rows a tile on the fp32 pipes ----------------------------------------------------------------------------------
 
-// A warp owns four rows: a lane's key of the tile for the scores, its four (or twice four) neighbouring channels for the sums.
+// Scores: every warp all 16 x 32 of them, over a part of the channels (a lane four rows by four keys: eight reads of 16 bytes, one
+// wavefront each, for 64 multiply-adds), added by the warp that owns the row, two a warp, a lane a key.  Sums: a lane four rows by four
+// channels, a warp eight such columns, warps that are left over another part of the keys.  A lane with one key or one group of channels for
+// all its rows reads five times as much of shared memory, which then is all that takes time: 4900 cycles a tile of 80 channels.
+constexpr int SW = 8, kScalarThreads = 32 * SW, TILE = 32, SP = 40, PP = 36;   // pitches of the scores and of the weights
 template <int STAGES, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
-    constexpr int TILE = 32;
+__global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     const int pitch = p.D + 4;                                           // floats (rows start on 16-byte boundaries: D is a multiple of 4)
     const int pieces = p.D / 4;
     float* sQ = reinterpret_cast<float*>(smem);                          // [16][pitch]
-    float* sP = sQ + ROWS * pitch;                                       // [16][32]
-    float* ring = sP + ROWS * TILE;
+    float* sS = sQ + ROWS * pitch;                                       // [8][16][SP]
+    float* sP = sS + SW * ROWS * SP;                                     // [16][PP]
+    float *sF = sP + ROWS * PP, *sTop = sF + ROWS, *sSum = sTop + ROWS;  // [16] each
+    float* ring = sSum + ROWS;
     const int stage_floats = 2 * TILE * pitch;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* room = reinterpret_cast<uint8_t*>(ring + STAGES * stage_floats);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 3, lc = lane & 7;   // rows lr + 4 i
+    const int columns = (pieces + 7) / 8, parts = SW / columns;          // warps over the channels; parts of the keys
+    const int my_part = warp / columns, col = (warp - my_part * columns) * 8 + lc;
+    const bool sums_here = my_part < parts && col < pieces;
+    const int keys = TILE / parts / 4 * 4, key0 = my_part * keys, key1 = my_part + 1 == parts ? TILE : key0 + keys;
     if (SPLIT) cluster_arrive();
     chain_begin();
 
-    float *sTop = sP, *sSum = sP + ROWS;                                 // (SPLIT, at the end)
-    uint8_t* room = reinterpret_cast<uint8_t*>(ring + STAGES * stage_floats);
     Cursor at;
     if (SPLIT) at.start_part(p, blockIdx.x);
     else at.start(p, blockIdx.x);
@@ -501,184 +505,196 @@ __global__ void __launch_bounds__(kThreads) scalar_kernel(const Params p) {
         return;
     }
     Cursor ahead = at;
+    // The page of this thread's row (eight threads a row) of ahead's tile is asked for a tile before its row is copied.
+    int next_row = 0, next_page = -1;
+    auto look_up = [&]() {
+        const int entry = ahead.tile * TILE + (threadIdx.x >> 3), slot = p.slot_at(entry);
+        next_page = -1;
+        next_row = entry - slot * p.page_size;
+        if (ahead.left > 0 && entry < ahead.s.total) next_page = p.table[ahead.b * p.table_stride + slot];
+    };
     auto fetch = [&](int stage) {
-        float* dst = ring + stage * stage_floats;
-        const float* k = static_cast<const float*>(p.k) + ahead.h * p.ks[1];
-        const float* v = static_cast<const float*>(p.v) + ahead.h * p.vs[1];
-        // four threads a row
-        const int r = threadIdx.x >> 2, entry = ahead.tile * TILE + r;
-        int row = 0, page = -1;
-        if (entry < ahead.s.total) page = page_of(p, ahead.b, entry, row);
-        const long long ko = page < 0 ? 0 : page * p.ks[0] + row * p.ks[2], vo = page < 0 ? 0 : page * p.vs[0] + row * p.vs[2];
-        for (int c = threadIdx.x & 3; c < pieces; c += 4) {
-            copy16(smem_at(dst + r * pitch + 4 * c), k + ko + 4 * c, page >= 0);
-            copy16(smem_at(dst + (TILE + r) * pitch + 4 * c), v + vo + 4 * c, page >= 0);
+        if (ahead.left > 0) {
+            const bool there = (unsigned)next_page < (unsigned)p.pages;
+            const long long page = there ? next_page : 0, row = there ? next_row : 0;
+            const float* k = static_cast<const float*>(p.k) + ahead.h * p.ks[1] + page * p.ks[0] + row * p.ks[2];
+            const float* v = static_cast<const float*>(p.v) + ahead.h * p.vs[1] + page * p.vs[0] + row * p.vs[2];
+            const uint32_t dst = smem_at(ring + stage * stage_floats + (threadIdx.x >> 3) * pitch);
+            ahead.next(p);
+            look_up();
+            for (int c = threadIdx.x & 7; c < pieces; c += 8) {
+                copy16(dst + 16 * c, k + 4 * c, there);
+                copy16(dst + 4 * TILE * pitch + 16 * c, v + 4 * c, there);
+            }
         }
         copies_end();
     };
+    look_up();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (ahead.left > 0) { fetch(i); ahead.next(p); }
-        else copies_end();
-    }
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
     int stage = 0;
     bool first_unit = true;
     while (at.left > 0) {
         const Sequence s = at.s;
         const int b = at.b, h = at.h, row0 = at.rt * ROWS, tile0 = at.tile;
-        for (int i = threadIdx.x; i < ROWS * pieces; i += kThreads) {
-            const int r = i / pieces, col = i - r * pieces, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+        for (int i = threadIdx.x; i < ROWS * pieces; i += kScalarThreads) {
+            const int r = i / pieces, c = i - r * pieces, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (t < s.count)
                 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + b * p.qs[0] + t * p.qs[1] +
-                                                     (h * p.G + g) * p.qs[2] + col * 4);
-            *reinterpret_cast<float4*>(sQ + r * pitch + col * 4) = v;
+                                                     (h * p.G + g) * p.qs[2] + c * 4);
+            *reinterpret_cast<float4*>(sQ + r * pitch + c * 4) = v;
         }
-        const bool busy = row0 + 4 * warp < s.count * p.G;               // (any of this warp's rows)
-        unsigned long long mask[4];
+        const unsigned long long mask[2] = {seen_by(p, s, b, row0 + 2 * warp), seen_by(p, s, b, row0 + 2 * warp + 1)};
+        float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+        float4 o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mask[i] = seen_by(p, s, b, row0 + 4 * warp + i);
-        float m[4], l[4];
-        float4 o[4][2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = -CUDART_INF_F;
-            l[i] = 0.f;
-            o[i][0] = o[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         bool end, at_end;
         do {
             copies_wait<STAGES - 2>();
             __syncthreads();                                             // the tile is there, and the one before it read
-            if (ahead.left > 0) {
-                fetch(stage == 0 ? STAGES - 1 : stage - 1);
-                ahead.next(p);
-            } else {
-                copies_end();
-            }
-            if (busy) {
-                const float* sk = ring + stage * stage_floats + lane * pitch;
-                const float* sv = ring + stage * stage_floats + TILE * pitch;
-                const float* sq = sQ + 4 * warp * pitch;
-                float c[4] = {};
-#pragma unroll 4
-                for (int d = 0; d < pieces; ++d) {
-                    const float4 kk = *reinterpret_cast<const float4*>(sk + 4 * d);
+            fetch(stage == 0 ? STAGES - 1 : stage - 1);
+            const float* sk = ring + stage * stage_floats;
+            const float* sv = sk + TILE * pitch;
+            {
+                float c[4][4] = {};
+#pragma unroll 2
+                for (int d = warp; d < pieces; d += SW) {
+                    float4 q[4], k[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float4 qq = *reinterpret_cast<const float4*>(sq + i * pitch + 4 * d);
-                        c[i] = fmaf(qq.x, kk.x, c[i]);
-                        c[i] = fmaf(qq.y, kk.y, c[i]);
-                        c[i] = fmaf(qq.z, kk.z, c[i]);
-                        c[i] = fmaf(qq.w, kk.w, c[i]);
+                        q[i] = *reinterpret_cast<const float4*>(sQ + (lr + 4 * i) * pitch + 4 * d);
+                        k[i] = *reinterpret_cast<const float4*>(sk + (lc + 8 * i) * pitch + 4 * d);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            c[i][j] = fmaf(q[i].x, k[j].x, c[i][j]);
+                            c[i][j] = fmaf(q[i].y, k[j].y, c[i][j]);
+                            c[i][j] = fmaf(q[i].z, k[j].z, c[i][j]);
+                            c[i][j] = fmaf(q[i].w, k[j].w, c[i][j]);
+                        }
                 }
-                const int j = at.tile * TILE + lane - s.length;
-                const bool drafts = at.tile * TILE + TILE > s.length;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sS[(warp * ROWS + lr + 4 * i) * SP + lc + 8 * j] = c[i][j];
+            }
+            __syncthreads();
+            const int j = at.tile * TILE + lane - s.length;
+            const bool drafts = at.tile * TILE + TILE > s.length;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 2 * warp + i;
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < SW; ++w) x += sS[(w * ROWS + r) * SP + lane];
+                x *= p.scale_log2;
+                if (drafts && j >= 0 && !(j < s.total - s.length && (mask[i] >> j & 1))) x = -CUDART_INF_F;
+                float top = x;
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                const float n = fmaxf(m[i], top), f = m[i] == n ? 1.f : ex2(m[i] - n);
+                m[i] = n;
+                const float w = ex2(x - (n == -CUDART_INF_F ? 0.f : n));
+                l[i] = fmaf(l[i], f, w);
+                sP[r * PP + lane] = w;
+                if (lane == 0) sF[r] = f;
+            }
+            __syncthreads();
+            auto sums = [&](auto some_hidden) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = c[i] * p.scale_log2;
-                    if (drafts && j >= 0 && !(j < s.total - s.length && (mask[i] >> j & 1))) x = -CUDART_INF_F;
-                    float top = x;
-#pragma unroll
-                    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                    const float n = fmaxf(m[i], top), f = m[i] == n ? 1.f : ex2(m[i] - n);
-                    m[i] = n;
-                    const float w = ex2(x - (n == -CUDART_INF_F ? 0.f : n));
-                    l[i] = fmaf(l[i], f, w);
-                    sP[(4 * warp + i) * TILE + lane] = w;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        o[i][u].x *= f; o[i][u].y *= f; o[i][u].z *= f; o[i][u].w *= f;
-                    }
+                    const float f = sF[lr + 4 * i];
+                    o[i].x *= f; o[i].y *= f; o[i].z *= f; o[i].w *= f;
                 }
-                __syncwarp();
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int col = lane + 32 * u;
-                    if (col >= pieces) continue;
 #pragma unroll 2
-                    for (int e = 0; e < TILE; e += 4) {
-                        float4 w[4], v[4];
+                for (int e = key0; e < key1; e += 4) {
+                    float4 w[4], v[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(sP + (4 * warp + i) * TILE + e);
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = *reinterpret_cast<const float4*>(sP + (lr + 4 * i) * PP + e);
+                        v[i] = *reinterpret_cast<const float4*>(sv + (e + i) * pitch + 4 * col);
+                    }
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const float4*>(sv + (e + x) * pitch + 4 * col);
+                    for (int i = 0; i < 4; ++i) {
+                        const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                if (drafts && ws[x] == 0.f) continue;    // (what a row does not see need not be finite)
-                                o[i][u].x = fmaf(ws[x], v[x].x, o[i][u].x);
-                                o[i][u].y = fmaf(ws[x], v[x].y, o[i][u].y);
-                                o[i][u].z = fmaf(ws[x], v[x].z, o[i][u].z);
-                                o[i][u].w = fmaf(ws[x], v[x].w, o[i][u].w);
-                            }
+                        for (int x = 0; x < 4; ++x) {
+                            if (decltype(some_hidden)::value && ws[x] == 0.f) continue;  // (what a row does not see need not be finite)
+                            o[i].x = fmaf(ws[x], v[x].x, o[i].x);
+                            o[i].y = fmaf(ws[x], v[x].y, o[i].y);
+                            o[i].z = fmaf(ws[x], v[x].z, o[i].z);
+                            o[i].w = fmaf(ws[x], v[x].w, o[i].w);
                         }
                     }
                 }
-                __syncwarp();
+            };
+            if (sums_here) {
+                if (drafts) sums(std::true_type());
+                else sums(std::false_type());
             }
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             end = at.last_of_unit();
             at_end = at.tile + 1 == s.tiles;
             at.next(p);
         } while (!end);
-        if (SPLIT) {
-            copies_wait<0>();
-            __syncthreads();                                             // (the ring and the weights are read)
+
+        // ---- the parts of the keys, then the unit
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+            if (lane == 0) {
+                sTop[2 * warp + i] = m[i];
+                sSum[2 * warp + i] = l[i];
+            }
+        }
+        if (sums_here && my_part)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(sS + ((my_part - 1) * ROWS + lr + 4 * i) * p.D + 4 * col) = o[i];
+        __syncthreads();                                                 // (the scores of the last tile are read)
+        const bool whole = tile0 == 0 && at_end;
+        float* slot = slot_of(p, blockIdx.x, first_unit);
+        if (sums_here && my_part == 0)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = 4 * warp + i;
-#pragma unroll
-                for (int w = 16; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (lane + 32 * u < pieces) *reinterpret_cast<float4*>(ring + r * pitch + 4 * (lane + 32 * u)) = o[i][u];
-                if (lane == 0) {
-                    sTop[r] = m[i];
-                    sSum[r] = l[i];
+                const int r = lr + 4 * i, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
+                float4 y = o[i];
+                for (int w = 0; w < parts - 1; ++w) {
+                    const float4 x = *reinterpret_cast<const float4*>(sS + (w * ROWS + r) * p.D + 4 * col);
+                    y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+                }
+                if (SPLIT) {
+                    *reinterpret_cast<float4*>(sQ + r * pitch + 4 * col) = y;        // (one unit: the queries are read)
+                } else if (!whole) {
+                    *reinterpret_cast<float4*>(slot + r * p.D + 4 * col) = y;
+                } else if (t < s.count) {
+                    const float inv = sSum[r] == 0.f ? 0.f : 1.0f / sSum[r];
+                    y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] +
+                                               4 * col) = y;
                 }
             }
+        if (SPLIT) {
             __syncthreads();
             join_cluster<float>(p, s, b, h, row0 / ROWS, room, false, [&](int r, int four, float4& x, float& m_, float& l_) {
-                x = *reinterpret_cast<const float4*>(ring + r * pitch + 4 * four);
+                x = *reinterpret_cast<const float4*>(sQ + r * pitch + 4 * four);
                 m_ = sTop[r];
                 l_ = sSum[r];
             });
             break;
         }
-        const bool whole = tile0 == 0 && at_end;
-        float* slot = slot_of(p, blockIdx.x, first_unit);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 4 * warp + i, t = (row0 + r) / p.G, g = row0 + r - t * p.G;
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-            const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int col = lane + 32 * u;
-                if (col >= pieces) continue;
-                float4 y = o[i][u];
-                if (whole) {
-                    if (t >= s.count) continue;
-                    y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
-                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] +
-                                               4 * col) = y;
-                } else {
-                    *reinterpret_cast<float4*>(slot + r * p.D + 4 * col) = y;
-                }
-            }
-            if (!whole && lane == 0) {
-                slot[ROWS * p.D + r] = m[i];
-                slot[ROWS * p.D + ROWS + r] = l[i];
-            }
+        if (!whole && threadIdx.x < ROWS) {
+            slot[ROWS * p.D + threadIdx.x] = sTop[threadIdx.x];
+            slot[ROWS * p.D + ROWS + threadIdx.x] = sSum[threadIdx.x];
+            if (threadIdx.x == 0) slot[ROWS * p.D + 2 * ROWS] = 0.f;
         }
-        if (!whole && threadIdx.x == 0) slot[ROWS * p.D + 2 * ROWS] = 0.f;
         first_unit = false;
-        __syncthreads();                                                 // (sQ)
+        __syncthreads();                                                 // (sQ, sS, sTop, sSum)
     }
     copies_wait<0>();
 }
@@ -880,9 +896,9 @@ Plan plan_of(int dtype, int rows, int D, bool tiles) {
     g.rows_per_tile = ROWS;
     if (dtype == CONVNN_F32) {
         g.tile = 32;
-        g.stages = D <= 128 ? 3 : 2;
-        g.smem = 4 * ((size_t)ROWS * (D + 4) + ROWS * 32 + (size_t)g.stages * 64 * (D + 4));
-        g.ctas_per_sm = g.smem <= 74 * 1024 ? 3 : g.smem <= 112 * 1024 ? 2 : 1;
+        g.stages = D <= 64 ? 3 : 2;
+        g.smem = 4 * ((size_t)ROWS * (D + 4) + SW * ROWS * SP + ROWS * PP + 3 * ROWS + (size_t)g.stages * 2 * TILE * (D + 4));
+        g.ctas_per_sm = g.smem <= 112 * 1024 ? 2 : 1;
     } else {
         const int DP = 16 * steps_of(D), pitch = ((DP / 8) | 1) * 16;
         g.tile = 64;
@@ -898,35 +914,46 @@ bool tiles_wanted(int dtype, int rows, int D) { return dtype == CONVNN_BF16 && r
 
 long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
 
-int launch_clusters(void (*kern)(Params), const Params& p, unsigned grid, size_t smem, cudaStream_t st) {
-    // (more than eight CTAs are not every device's: this one's are)
-    static std::atomic<const void*> allowed[16];
-    const void* const me = reinterpret_cast<const void*>(kern);
-    bool seen = false;
-    for (auto& k : allowed) seen = seen || k.load(std::memory_order_relaxed) == me;
-    if (!seen) {
-        const cudaError_t e = cudaFuncSetAttribute(me, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+// What is asked of the driver once: how many clusters of 1, 2, 4, 8, 16 CTAs of a kernel run at once.
+struct Clusters {
+    std::atomic<int> allowed;
+    ClusterLimit fit[5];
+};
+// Up to p.split CTAs a unit, fewer where the clusters would not all run at once.
+int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int threads, size_t smem, cudaStream_t st, Clusters& known) {
+    if (!known.allowed.load(std::memory_order_relaxed)) {            // (more than eight CTAs are not every device's, but this one's)
+        const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "tree_attention: %s", cudaGetErrorString(e));
-        for (auto& k : allowed) {
-            const void* none = nullptr;
-            if (k.compare_exchange_strong(none, me)) break;
-        }
+        known.allowed.store(1, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[2] = {chained_attribute(st), {}};
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.split;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = grid; cfg.blockDim = kThreads; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cfg.attrs = attr; cfg.numAttrs = 2;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1] = chained_attribute(st);
+    cfg.blockDim = threads; cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.attrs = attr;
+    for (int size = 4;; --size) {
+        if ((1 << size) > p.split) continue;
+        attr[0].val.clusterDim.x = (unsigned)(p.split = 1 << size);
+        cfg.gridDim = units * (unsigned)p.split;
+        if (size == 0) break;
+        int clusters = 0;
+        cfg.numAttrs = 1;
+        const int rc = known.fit[size].query(reinterpret_cast<const void*>(kern), &cfg, &clusters);
+        if (rc) return rc;
+        if (units <= (unsigned)clusters) break;
+    }
+    cfg.numAttrs = 2;
     cudaLaunchKernelEx(&cfg, kern, p);               // an error stays the thread's last error (CONVNN_CHECK_LAUNCH)
     return CONVNN_OK;
 }
 template <int DS, int STAGES>
-int launch_rows(const Params& p, unsigned units, size_t smem, cudaStream_t st) {
+int launch_rows(Params& p, unsigned units, size_t smem, cudaStream_t st) {
     if (p.split) {
         CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, true>), smem);
-        const int rc = launch_clusters(rows_kernel<DS, STAGES, true>, p, units * p.split, smem, st);
+        static Clusters known{};
+        const int rc = launch_clusters(rows_kernel<DS, STAGES, true>, p, units, kThreads, smem, st, known);
         if (rc) return rc;
     } else {
         CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, false>), smem);
@@ -936,14 +963,15 @@ int launch_rows(const Params& p, unsigned units, size_t smem, cudaStream_t st) {
     return CONVNN_OK;
 }
 template <int STAGES>
-int launch_scalar(const Params& p, unsigned units, size_t smem, cudaStream_t st) {
+int launch_scalar(Params& p, unsigned units, size_t smem, cudaStream_t st) {
     if (p.split) {
         CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, true>), smem);
-        const int rc = launch_clusters(scalar_kernel<STAGES, true>, p, units * p.split, smem, st);
+        static Clusters known{};
+        const int rc = launch_clusters(scalar_kernel<STAGES, true>, p, units, kScalarThreads, smem, st, known);
         if (rc) return rc;
     } else {
         CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, false>), smem);
-        launch_chained(scalar_kernel<STAGES, false>, p.ctas, kThreads, smem, st, p);
+        launch_chained(scalar_kernel<STAGES, false>, p.ctas, kScalarThreads, smem, st, p);
     }
     CONVNN_CHECK_LAUNCH("tree_attention");
     return CONVNN_OK;
