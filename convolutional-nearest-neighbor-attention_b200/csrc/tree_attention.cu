@@ -11,6 +11,8 @@
 // join_kernel: units that several CTAs had, and rows without anything.
 // Where the cache is short, a second kernel would cost more than the even division gains: a cluster of up to sixteen CTAs has a unit, and
 // they join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels).
+#include <math.h>
+
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -701,8 +703,9 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
 
 // ---- units that several CTAs had ------------------------------------------------------------------------------------------------
 
-// The pieces' maxima, then their sums, in the order of the keys.  What says which pieces there are is read while the kernel before is
-// still at work: it does not write that.
+// The pieces' sums, in the order of the keys, each multiplied by what its maximum is away from the largest so far.  What says which pieces
+// there are, and which rows have none, is read while the kernel before is still at work (it does not write that); behind it a piece's
+// maximum and sums are asked for together, several pieces at a time: one way to memory and back.
 
 // The unit that is cut for the first time where CTA `cta`'s tiles begin: its pieces are c0 .. c1 (c0 == c1: there is none).
 struct Cut {
@@ -727,25 +730,56 @@ __device__ __forceinline__ Cut cut_at(const Params& p, int cta) {
     return u;
 }
 // Rows without anything, of all sequences: zeros, by all warps of the grid.
-template <typename T>
-__device__ __forceinline__ void write_zeros(const Params& p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, blocks = gridDim.x * gridDim.y * gridDim.z;
-    for (int i = block * kWarps + warp; i < p.B * p.T; i += blocks * kWarps) {
-        const int b = i / p.T, t = i - b * p.T;
+__device__ __forceinline__ int next_zero_row(const Params& p, int i) {
+    const int blocks = gridDim.x * gridDim.y * gridDim.z;
+    for (; i < p.B * p.T; i += blocks * kWarps) {
+        const int b = i / p.T;
         const Sequence s = sequence_of(p, b);
-        if (t < s.count && s.total) continue;
-        T* out = static_cast<T*>(p.out) + b * p.os[0] + t * p.os[1];
+        if (i - b * p.T >= s.count || !s.total) break;
+    }
+    return i;
+}
+__device__ __forceinline__ int first_zero_row(const Params& p) {
+    return next_zero_row(p, ((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kWarps + (threadIdx.x >> 5));
+}
+template <typename T>
+__device__ __forceinline__ void write_zeros(const Params& p, int i) {
+    for (; i < p.B * p.T; i = next_zero_row(p, i + gridDim.x * gridDim.y * gridDim.z * kWarps)) {
+        const int b = i / p.T;
+        T* out = static_cast<T*>(p.out) + b * p.os[0] + (i - b * p.T) * p.os[1];
         for (int h = 0; h < p.Hk * p.G; ++h)
-            for (int c = lane; c < p.D; c += 32) out[h * p.os[2] + c] = from_f32<T>(0.f);
+            for (int c = threadIdx.x & 31; c < p.D; c += 32) out[h * p.os[2] + c] = from_f32<T>(0.f);
     }
 }
+// Sums joined so far: N groups of four channels of one row.
+template <int N>
+struct Joined {
+    float top, sum;
+    float4 y[N];
+    __device__ __forceinline__ Joined() : top(-INFINITY), sum(0.f) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) y[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // (a part without keys, m = -inf, has zeros; so has what was joined before any)
+    __device__ __forceinline__ void add(float m, float l, const float4 (&x)[N]) {
+        const float now = fmaxf(top, m), before = top == now ? 1.f : ex2(top - now), f = m == now ? 1.f : ex2(m - now);
+        top = now;
+        sum = sum * before + l * f;
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+            y[v].x = fmaf(x[v].x, f, y[v].x * before); y[v].y = fmaf(x[v].y, f, y[v].y * before);
+            y[v].z = fmaf(x[v].z, f, y[v].z * before); y[v].w = fmaf(x[v].w, f, y[v].w * before);
+        }
+    }
+};
+
 // Tiles of 16 rows.  WARPS of a block's four warps share the pieces of a row: all four where units have several pieces each (a block per
 // unit and row), else a warp goes through every fourth row of 16 of one unit (a block per boundary between two CTAs' tiles).
 constexpr int JOIN_ROWS = 16;
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
     __shared__ float4 sY[WARPS == 4 ? 4 : 1][2][32];
+    __shared__ float sT[4][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Cut u{};
     if (WARPS == 4) {
@@ -765,64 +799,64 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
     } else {
         u = cut_at(p, blockIdx.x);
     }
+    const int zero = first_zero_row(p);
     chain_begin();
-    write_zeros<T>(p);
+    write_zeros<T>(p, zero);
     if (u.c0 == u.c1) return;                    // (written by its CTA, or not this block's)
-    const long long tail = (long long)p.rows_per_tile * p.D;
-    auto piece = [&](int c) { return slot_of(p, c, c > u.c0 || !u.second); };
+    const int tail = p.rows_per_tile * p.D;
+    const bool wide = p.D > 128;
 #pragma unroll 1
     for (int i = 0; i < (WARPS == 4 ? 1 : JOIN_ROWS / kWarps); ++i) {
         const int r = WARPS == 4 ? blockIdx.y : blockIdx.y * JOIN_ROWS + i * kWarps + warp, row = u.rt * p.rows_per_tile + r;
         if (r >= p.rows_per_tile || row >= u.s.count * p.G) return;          // (the whole block, or a warp that meets no other)
-        float top = -CUDART_INF_F, sum = 0.f;
-        bool bad = false;
-        for (int c = u.c0 + lane; c <= u.c1; c += 32) {
-            const float* from = piece(c) + tail;
-            top = fmaxf(top, from[r]);
-            bad |= from[2 * p.rows_per_tile] != 0.f;
-        }
+        Joined<2> all;
+        float bad = 0.f;
+        constexpr int BATCH = 4;
+#pragma unroll 1
+        for (int c = u.c0 + (WARPS == 4 ? warp : 0); c <= u.c1; c += WARPS * BATCH) {
+            float m[BATCH], l[BATCH], hit[BATCH];
+            float4 x[BATCH][2];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        bad = __any_sync(0xffffffffu, bad);
-        if (top == -CUDART_INF_F) top = 0.f;
-        for (int c = u.c0 + lane; c <= u.c1; c += 32) {
-            const float* from = piece(c) + tail;
-            sum = fmaf(from[p.rows_per_tile + r], ex2(from[r] - top), sum);
-        }
+            for (int e = 0; e < BATCH; ++e) {
+                const int at = c + e * WARPS;
+                m[e] = -CUDART_INF_F;
+                l[e] = hit[e] = 0.f;
+                x[e][0] = x[e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at > u.c1) continue;
+                const float* from = slot_of(p, at, at > u.c0 || !u.second);
+                m[e] = from[tail + r];
+                l[e] = from[tail + p.rows_per_tile + r];
+                hit[e] = from[tail + 2 * p.rows_per_tile];
+                if (4 * lane < p.D) x[e][0] = *reinterpret_cast<const float4*>(from + r * p.D + 4 * lane);
+                if (wide && 4 * lane + 128 < p.D) x[e][1] = *reinterpret_cast<const float4*>(from + r * p.D + 4 * lane + 128);
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        float4 y[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 8
-        for (int c = u.c0 + (WARPS == 4 ? warp : 0); c <= u.c1; c += WARPS) {
-            const float* from = piece(c);
-            const float f = ex2(from[tail + r] - top);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const int col = 4 * (lane + 32 * v);
-                if (col >= p.D) continue;
-                const float4 x = *reinterpret_cast<const float4*>(from + r * p.D + col);
-                y[v].x = fmaf(x.x, f, y[v].x); y[v].y = fmaf(x.y, f, y[v].y);
-                y[v].z = fmaf(x.z, f, y[v].z); y[v].w = fmaf(x.w, f, y[v].w);
+            for (int e = 0; e < BATCH; ++e) {
+                all.add(m[e], l[e], x[e]);
+                bad += hit[e];
             }
         }
         if (WARPS == 4) {
-            sY[warp][0][lane] = y[0];
-            sY[warp][1][lane] = y[1];
-            __syncthreads();
+            sY[warp][0][lane] = all.y[0];
+            sY[warp][1][lane] = all.y[1];
+            if (lane == 0) {
+                sT[warp][0] = all.top;
+                sT[warp][1] = all.sum;
+            }
+            bad = __syncthreads_or(bad != 0.f) ? 1.f : 0.f;
             if (warp) return;
+            all = Joined<2>();
 #pragma unroll
-            for (int w = 1; w < 4; ++w)
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const float4 x = sY[w % WARPS][v][lane];
-                    y[v].x += x.x; y[v].y += x.y; y[v].z += x.z; y[v].w += x.w;
-                }
+            for (int w = 0; w < WARPS; ++w) {
+                const float4 x[2] = {sY[w][0][lane], sY[w][1][lane]};
+                all.add(sT[w][0], sT[w][1], x);
+            }
         }
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        const float inv = all.sum == 0.f ? 0.f : 1.0f / all.sum;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int col = 4 * (lane + 32 * v);
-            if (col < p.D) write_four<T>(p, u.s, u.b, u.h, row, col, y[v], inv, bad);
+            if (col < p.D) write_four<T>(p, u.s, u.b, u.h, row, col, all.y[v], inv, bad != 0.f);
         }
     }
 }
@@ -830,42 +864,33 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
 // Tiles of 128 rows and more: a block per boundary, 128 rows and 32 channels, a thread a row (its neighbours' sums lie beside its own).
 __global__ void __launch_bounds__(kThreads) join_tiles_kernel(const Params p) {
     const Cut u = cut_at(p, blockIdx.x);
+    const int zero = first_zero_row(p);
     chain_begin();
-    write_zeros<__nv_bfloat16>(p);
+    write_zeros<__nv_bfloat16>(p, zero);
     const int r = blockIdx.y * 128 + threadIdx.x, row = u.rt * p.rows_per_tile + r;
     if (u.c0 == u.c1 || row >= u.s.count * p.G) return;
-    const long long tail = (long long)p.rows_per_tile * p.D;
-    auto piece = [&](int c) { return slot_of(p, c, c > u.c0 || !u.second); };
-    float top = -CUDART_INF_F, sum = 0.f;
+    const int tail = p.rows_per_tile * p.D;
+    Joined<8> all;
     bool bad = false;
-    for (int c = u.c0; c <= u.c1; ++c) {
-        const float* from = piece(c) + tail;
-        top = fmaxf(top, from[r]);
-        bad |= from[2 * p.rows_per_tile + (r >> 7)] != 0.f;                  // (a word for every 128 rows)
-    }
-    if (top == -CUDART_INF_F) top = 0.f;
-    float4 y[8];
-#pragma unroll
-    for (int v = 0; v < 8; ++v) y[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
     for (int c = u.c0; c <= u.c1; ++c) {
-        const float* from = piece(c);
-        const float f = ex2(from[tail + r] - top);
-        sum = fmaf(from[tail + p.rows_per_tile + r], f, sum);
+        const float* from = slot_of(p, c, c > u.c0 || !u.second);
+        const float m = from[tail + r], l = from[tail + p.rows_per_tile + r];
+        bad |= from[tail + 2 * p.rows_per_tile + (r >> 7)] != 0.f;           // (a word for every 128 rows)
+        float4 x[8];
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
             const int four = blockIdx.z * 8 + v;
-            if (4 * four >= p.D) continue;
-            const float4 x = reinterpret_cast<const float4*>(from)[four * p.rows_per_tile + r];
-            y[v].x = fmaf(x.x, f, y[v].x); y[v].y = fmaf(x.y, f, y[v].y);
-            y[v].z = fmaf(x.z, f, y[v].z); y[v].w = fmaf(x.w, f, y[v].w);
+            x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * four < p.D) x[v] = reinterpret_cast<const float4*>(from)[four * p.rows_per_tile + r];
         }
+        all.add(m, l, x);
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = all.sum == 0.f ? 0.f : 1.0f / all.sum;
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
         const int col = (blockIdx.z * 8 + v) * 4;
-        if (col < p.D) write_four<__nv_bfloat16>(p, u.s, u.b, u.h, row, col, y[v], inv, bad);
+        if (col < p.D) write_four<__nv_bfloat16>(p, u.s, u.b, u.h, row, col, all.y[v], inv, bad);
     }
 }
 
@@ -919,8 +944,10 @@ struct Clusters {
     std::atomic<int> allowed;
     ClusterLimit fit[5];
 };
-// Up to p.split CTAs a unit, fewer where the clusters would not all run at once.
-int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int threads, size_t smem, cudaStream_t st, Clusters& known) {
+// As many CTAs a unit, up to p.split, as leave all clusters room at once; p.split = 0 where the even division is the better one: its second
+// kernel takes as long as a CTA's `worth` tiles.
+int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int unit_tiles, int worth, int threads, size_t smem, cudaStream_t st,
+                    Clusters& known) {
     if (!known.allowed.load(std::memory_order_relaxed)) {            // (more than eight CTAs are not every device's, but this one's)
         const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "tree_attention: %s", cudaGetErrorString(e));
@@ -944,18 +971,25 @@ int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int threads
         if (rc) return rc;
         if (units <= (unsigned)clusters) break;
     }
+    if ((unit_tiles + p.split - 1) / p.split > (long long)units * unit_tiles / p.ctas + worth) {
+        p.split = 0;
+        return CONVNN_OK;
+    }
     cfg.numAttrs = 2;
     cudaLaunchKernelEx(&cfg, kern, p);               // an error stays the thread's last error (CONVNN_CHECK_LAUNCH)
     return CONVNN_OK;
 }
+// p.split: the most CTAs a unit may have, 0: none; on return what it got, 0: the even division.
 template <int DS, int STAGES>
-int launch_rows(Params& p, unsigned units, size_t smem, cudaStream_t st) {
+int launch_rows(Params& p, unsigned units, int unit_tiles, size_t smem, cudaStream_t st) {
     if (p.split) {
-        CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, true>), smem);
+        const size_t joined = smem + join_bytes(p.D / 4);
+        CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, true>), joined);
         static Clusters known{};
-        const int rc = launch_clusters(rows_kernel<DS, STAGES, true>, p, units, kThreads, smem, st, known);
+        const int rc = launch_clusters(rows_kernel<DS, STAGES, true>, p, units, unit_tiles, 6, kThreads, joined, st, known);
         if (rc) return rc;
-    } else {
+    }
+    if (!p.split) {
         CONVNN_ENSURE_SMEM((rows_kernel<DS, STAGES, false>), smem);
         launch_chained(rows_kernel<DS, STAGES, false>, p.ctas, kThreads, smem, st, p);
     }
@@ -963,13 +997,15 @@ int launch_rows(Params& p, unsigned units, size_t smem, cudaStream_t st) {
     return CONVNN_OK;
 }
 template <int STAGES>
-int launch_scalar(Params& p, unsigned units, size_t smem, cudaStream_t st) {
+int launch_scalar(Params& p, unsigned units, int unit_tiles, size_t smem, cudaStream_t st) {
     if (p.split) {
-        CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, true>), smem);
+        const size_t joined = smem + join_bytes(p.D / 4);
+        CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, true>), joined);
         static Clusters known{};
-        const int rc = launch_clusters(scalar_kernel<STAGES, true>, p, units, kScalarThreads, smem, st, known);
+        const int rc = launch_clusters(scalar_kernel<STAGES, true>, p, units, unit_tiles, 2, kScalarThreads, joined, st, known);
         if (rc) return rc;
-    } else {
+    }
+    if (!p.split) {
         CONVNN_ENSURE_SMEM((scalar_kernel<STAGES, false>), smem);
         launch_chained(scalar_kernel<STAGES, false>, p.ctas, kScalarThreads, smem, st, p);
     }
@@ -1018,24 +1054,24 @@ int launch_tree_attention(const convnn_tree_attention* a, const convnn_cache* ca
         return set_error(CONVNN_E_WORKSPACE, "tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
                          (size_t)p.ctas * 2 * p.slot * 4);
     // A unit to a cluster where all tiles that there may be are few for each CTA that runs at once: as many CTAs as run at once, up to
-    // sixteen a unit.
+    // sixteen a unit.  us with clusters and with the even division: 8 units of 65 tiles of 64 keys 11.3 and 17.6, 64 of them 28.5 and 37.0,
+    // 128 units of 9 8.9 and 14.8; 2 units of 257 23.2 and 21.4, in float32 (514 tiles of 32) 80.9 and 30.9.
     const long long unit_tiles = (keys + p.tile - 1) / p.tile;
     if (!g.tiles && units * unit_tiles <= 16ll * p.ctas)
         for (p.split = 1; p.split < MOST_PARTS && p.split < unit_tiles && units * p.split * 2 <= p.ctas;) p.split *= 2;
-    const size_t smem = g.smem + (p.split ? (size_t)join_bytes(p.D / 4) : 0);
     int rc;
     if (g.tiles) {
         rc = launch_tree_tiles(p, st);
     } else if (a->dtype == CONVNN_F32) {
-        rc = g.stages == 3 ? launch_scalar<3>(p, (unsigned)units, smem, st) : launch_scalar<2>(p, (unsigned)units, smem, st);
+        rc = g.stages == 3 ? launch_scalar<3>(p, (unsigned)units, (int)unit_tiles, g.smem, st) : launch_scalar<2>(p, (unsigned)units, (int)unit_tiles, g.smem, st);
     } else {
         switch (steps_of(p.D)) {
-            case 4: rc = launch_rows<4, 4>(p, (unsigned)units, smem, st); break;
-            case 5: rc = launch_rows<5, 3>(p, (unsigned)units, smem, st); break;
-            case 6: rc = launch_rows<6, 3>(p, (unsigned)units, smem, st); break;
-            case 8: rc = launch_rows<8, 2>(p, (unsigned)units, smem, st); break;
-            case 12: rc = launch_rows<12, 2>(p, (unsigned)units, smem, st); break;
-            default: rc = launch_rows<16, 2>(p, (unsigned)units, smem, st); break;
+            case 4: rc = launch_rows<4, 4>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
+            case 5: rc = launch_rows<5, 3>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
+            case 6: rc = launch_rows<6, 3>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
+            case 8: rc = launch_rows<8, 2>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
+            case 12: rc = launch_rows<12, 2>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
+            default: rc = launch_rows<16, 2>(p, (unsigned)units, (int)unit_tiles, g.smem, st); break;
         }
     }
     if (rc || p.split) return rc;
