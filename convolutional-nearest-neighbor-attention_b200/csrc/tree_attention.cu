@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     };
     // this warp's slice of ahead's tile into `stage`
     auto fetch = [&](int stage) {
+        if (!SPLIT) look_up();
         if (ahead.left > 0) {
             const int first = ahead.tile * 64 + warp * 16;
             const bool any = first < ahead.s.total, there = (unsigned)next_page < (unsigned)p.pages && first + (lane & 15) < ahead.s.total;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
             const uint32_t dst = own + stage * STAGE;
             const long long kr = there ? next_page * p.ks[0] + next_row * p.ks[2] : 0, vr = there ? next_page * p.vs[0] + next_row * p.vs[2] : 0;
             ahead.next(p);
-            look_up();
+            if (SPLIT) look_up();
             if (any) {
 #pragma unroll
                 for (int i = 0; i < DS; ++i) {
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
         }
         copies_end();
     };
-    look_up();
+    if (SPLIT) look_up();
     // the rows of q (zeros where a token is not there), with the first slice's copies where there is one unit
     auto copy_rows = [&]() {
         for (int i = threadIdx.x; i < ROWS * chunks; i += kThreads) {
@@ -552,6 +553,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
         float4 o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int live = min(ROWS, s.count * p.G - row0);                // rows; of up to four a lane has one
         bool end, at_end;
         do {
             copies_wait<STAGES - 2>();
@@ -559,18 +561,18 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
             fetch(stage == 0 ? STAGES - 1 : stage - 1);
             const float* sk = ring + stage * stage_floats;
             const float* sv = sk + TILE * pitch;
-            {
-                float c[4][4] = {};
+            auto scores = [&](auto rows) {
+                constexpr int R = decltype(rows)::value;
+                float c[R][4] = {};
 #pragma unroll 2
                 for (int d = warp; d < pieces; d += SW) {
-                    float4 q[4], k[4];
+                    float4 q[R], k[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        q[i] = *reinterpret_cast<const float4*>(sQ + (lr + 4 * i) * pitch + 4 * d);
-                        k[i] = *reinterpret_cast<const float4*>(sk + (lc + 8 * i) * pitch + 4 * d);
-                    }
+                    for (int i = 0; i < R; ++i) q[i] = *reinterpret_cast<const float4*>(sQ + (lr + 4 * i) * pitch + 4 * d);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(sk + (lc + 8 * i) * pitch + 4 * d);
+#pragma unroll
+                    for (int i = 0; i < R; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             c[i][j] = fmaf(q[i].x, k[j].x, c[i][j]);
@@ -580,16 +582,19 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                         }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < R; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sS[(warp * ROWS + lr + 4 * i) * SP + lc + 8 * j] = c[i][j];
-            }
+            };
+            if (live <= 4) scores(std::integral_constant<int, 1>());
+            else scores(std::integral_constant<int, 4>());
             __syncthreads();
             const int j = at.tile * TILE + lane - s.length;
             const bool drafts = at.tile * TILE + TILE > s.length;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = 2 * warp + i;
+                if (r >= live) continue;
                 float x = 0.f;
 #pragma unroll
                 for (int w = 0; w < SW; ++w) x += sS[(w * ROWS + r) * SP + lane];
@@ -606,22 +611,22 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 if (lane == 0) sF[r] = f;
             }
             __syncthreads();
-            auto sums = [&](auto some_hidden) {
+            auto sums = [&](auto some_hidden, auto rows) {
+                constexpr int R = decltype(rows)::value;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < R; ++i) {
                     const float f = sF[lr + 4 * i];
                     o[i].x *= f; o[i].y *= f; o[i].z *= f; o[i].w *= f;
                 }
 #pragma unroll 2
                 for (int e = key0; e < key1; e += 4) {
-                    float4 w[4], v[4];
+                    float4 w[R], v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        w[i] = *reinterpret_cast<const float4*>(sP + (lr + 4 * i) * PP + e);
-                        v[i] = *reinterpret_cast<const float4*>(sv + (e + i) * pitch + 4 * col);
-                    }
+                    for (int i = 0; i < R; ++i) w[i] = *reinterpret_cast<const float4*>(sP + (lr + 4 * i) * PP + e);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float4*>(sv + (e + i) * pitch + 4 * col);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
                         const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
@@ -635,8 +640,9 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 }
             };
             if (sums_here) {
-                if (drafts) sums(std::true_type());
-                else sums(std::false_type());
+                if (live <= 4 && !drafts) sums(std::false_type(), std::integral_constant<int, 1>());
+                else if (!drafts) sums(std::false_type(), std::integral_constant<int, 4>());
+                else sums(std::true_type(), std::integral_constant<int, 4>());
             }
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             end = at.last_of_unit();
