@@ -4,13 +4,18 @@
 // One pass over the keys with a running maximum and sum in float32.  The query heads that share a key head, for all of a sequence's
 // tokens, are the rows of one product, so that keys and values are read once.  With few rows reading them is all that takes time.
 //
-// rows_kernel (bfloat16): 16 rows on mma.sync.  Each of four warps walks every fourth slice of 16 keys by itself, copies of its next
-// slices in flight, and the four join at the unit's end: no barrier between slices.
+// rows_kernel (bfloat16, up to 16 rows): mma.sync.  Each of four warps walks every fourth slice of 16 keys by itself, copies of its next
+// slices in flight, and the four join at the unit's end: no barrier between slices.  48 sequences of 4096 to 16384 entries, 8 key heads of
+// 128: 308 us for 1.87 GB, 6.05 TB/s (92 % of a plain copy's rate; 5.4 after a second of it, when the clock falls to 1700 MHz).  Three slices
+// in flight per warp instead of two (the queries' room for the warps' sums) gain nothing: 324 us; pages asked for a slice ahead 316.
 // scalar_kernel (float32): 16 rows on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA, four rows by four keys or channels a
 // thread.
+// tree_attention_tc.cu (bfloat16, more rows, up to 128 channels, pages of a multiple of 16 entries): tcgen05.  16 sequences of 32 to 64 tokens, 32
+// query heads: 1536 us with rows_kernel, 16 rows at a time.
 // join_kernel: units that several CTAs had, and rows without anything.
-// Where the cache is short, a second kernel would cost more than the even division gains: a cluster of up to sixteen CTAs has a unit, and
-// they join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels).
+// Where the cache is short, the second kernel costs more than the even division gains: a cluster of up to sixteen CTAs has a unit, and they
+// join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels, 5.6 in one, of which 0.6 us
+// are each of the lengths, the table and the first keys, read one after the other).
 #include <math.h>
 
 #include <type_traits>
@@ -945,19 +950,23 @@ bool tiles_wanted(int dtype, int rows, int D) { return dtype == CONVNN_BF16 && r
 
 long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
 
-// What is asked of the driver once: how many clusters of 1, 2, 4, 8, 16 CTAs of a kernel run at once.
+// What is asked of the driver once: that a kernel's clusters may have sixteen CTAs (on each device), and how many clusters of 1, 2, 4, 8, 16
+// run at once.
 struct Clusters {
-    std::atomic<int> allowed;
+    std::atomic<int> allowed[16];
     ClusterLimit fit[5];
 };
 // As many CTAs a unit, up to p.split, as leave all clusters room at once; p.split = 0 where the even division is the better one: its second
 // kernel takes as long as a CTA's `worth` tiles.
 int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int unit_tiles, int worth, int threads, size_t smem, cudaStream_t st,
                     Clusters& known) {
-    if (!known.allowed.load(std::memory_order_relaxed)) {            // (more than eight CTAs are not every device's, but this one's)
+    int device = 0;
+    cudaGetDevice(&device);
+    const bool remembered = device >= 0 && device < 16;
+    if (!remembered || !known.allowed[device].load(std::memory_order_relaxed)) {
         const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return set_error(CONVNN_E_CUDA, "tree_attention: %s", cudaGetErrorString(e));
-        known.allowed.store(1, std::memory_order_relaxed);
+        if (remembered) known.allowed[device].store(1, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[2]{};

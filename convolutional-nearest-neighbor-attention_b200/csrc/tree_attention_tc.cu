@@ -11,6 +11,15 @@
 //              the accumulator multiplied, only when a tile exceeds it by 2^8 (float32 holds what that leaves).
 // A weight is rounded to one bfloat16 for its product (a second part would cost half the tensor cores' time); its sum is of the
 // unrounded ones.
+// 16 sequences of 32 to 64 drafted tokens over 4096 to 16384 entries, 32 query and 8 key heads of 128: 207 us, of which the two products are 77
+// at the tensor cores' nominal rate.  What bounds it is the way round: scores, 2000 cycles of softmax, weights, 1200 cycles of products; a
+// stream's next scores wait for its last weights (they lie where those were), and a period of both streams is 3990 cycles where the tensor
+// cores need 2050 and the exponentials as many.  How it came here: one tile of rows, two streams of keys 325 us (the second tile of rows reads all
+// keys again); two tiles of rows sharing them, registers moved 243; the next unit's queries before the last one's sums, sums side by side 222; one
+// wait a step 218; pieces joined by a thread a row 207.  Tried and slower: a quarter of the exponentials as polynomials with the product
+// in halves 229 (the exponential unit is not what is waited for: without any exponential 240 of 243); one room of scores for both streams,
+// weights apart, so that the next scores are there when the last weights are done: 232, and with the weights kept in registers until
+// their room is free 244 to 286 (216 registers do not hold them).
 #include "f32x2.cuh"
 #include "paged_attention.cuh"
 #include "sm100.cuh"
@@ -92,7 +101,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* sStop = reinterpret_cast<volatile int*>(tmem_slot + 2);    // [2]: a group's
-    int* sBad = reinterpret_cast<int*>(tmem_slot + 4);                       // [4]: a unit's, in turn
+    int* sBad = reinterpret_cast<int*>(tmem_slot + 4);                       // [8]: a unit's, in turn
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -113,7 +122,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
         mbar_init(q_ready + 1, 4);
         mbar_init(drained, 1);
         *abort_flag = 0;
-        sBad[0] = sBad[1] = sBad[2] = sBad[3] = 0;
+        for (int i = 0; i < 8; ++i) sBad[i] = 0;
         fence_barrier_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
@@ -286,8 +295,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
             const Sequence s = at.s;
             const int b = at.b, h = at.h, unit0 = at.rt * (TWO ? 2 : 1) * kRows, row0 = unit0 + (TWO ? group * kRows : 0);
             const int last = TWO ? 2 * n : n;
-            int* unit_bad = sBad + (units & 3);
-            if (threadIdx.x == 128) sBad[(units + 2) & 3] = 0;               // (the groups are less than a unit apart)
+            // (with TWO a group may still write what the unit before the last one was when the other one begins this unit)
+            int* unit_bad = sBad + (units & 7);
+            if (threadIdx.x == 128) sBad[(units + 4) & 7] = 0;
             if (!TWO) load_rows(at);
 
             const unsigned long long drafts = s.total - s.length >= 64 ? ~0ull : (1ull << (s.total - s.length)) - 1;
@@ -512,7 +522,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
 
 template <int DC, int KS, int VS, bool TWO>
 int launch_tiles(const CUtensorMap& k, const CUtensorMap& v, const Params& p, const TileMaps& tm, cudaStream_t st) {
-    const size_t smem = 1024 + (size_t)((TWO ? 2 : 1) + KS + VS) * DC * kChunk + kRows * sizeof(float2) + 8 * (2 * KS + 2 * VS + 9) + 32;
+    const size_t smem = 1024 + (size_t)((TWO ? 2 : 1) + KS + VS) * DC * kChunk + kRows * sizeof(float2) + 8 * (2 * KS + 2 * VS + 9) + 48;
     CONVNN_ENSURE_SMEM((tiles_kernel<DC, KS, VS, TWO>), smem);
     launch_chained(tiles_kernel<DC, KS, VS, TWO>, p.ctas, kTileThreads, smem, st, k, v, p, tm);
     CONVNN_CHECK_LAUNCH("tree_attention");
