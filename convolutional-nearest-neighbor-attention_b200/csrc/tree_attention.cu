@@ -1016,8 +1016,11 @@ int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int unit_ti
         if (size == 0) break;
         int clusters = 0;
         cfg.numAttrs = 1;
-        const int rc = known.fit[size].query(reinterpret_cast<const void*>(kern), &cfg, &clusters);
-        if (rc) return rc;
+        if (known.fit[size].query(reinterpret_cast<const void*>(kern), &cfg, &clusters)) {       // (none fits)
+            clear_error();
+            cudaGetLastError();
+            clusters = 0;
+        }
         if (units <= (unsigned)clusters) break;
     }
     if ((unit_tiles + p.split - 1) / p.split > (long long)units * unit_tiles / p.ctas + worth) {

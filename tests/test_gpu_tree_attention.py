@@ -509,3 +509,86 @@ def test_division_and_clusters_agree(dtype, B, T, H, G, D, length):
     lengths = ints(*[length - (b * 37) % length for b in range(B)])
     for c in (cache, widened(cache)):
         check_attention(ops.tree_attention(q, c, lengths), q, c, lengths)
+
+
+# ---- ways to call -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [4, 12, 20, 36, 60, 68, 100, 132, 160, 188, 252])
+@pytest.mark.parametrize("T,G", [(1, 2), (7, 2)])
+def test_float32_widths(D, T, G):
+    cache = cache_of(2, 2, 16, D, 150 + T, F32)
+    q = randn(2, T, 2 * G, D, seed=9)
+    for c in (cache, widened(cache)):
+        check_attention(ops.tree_attention(q, c, ints(150, 61)), q, c, ints(150, 61))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_calls_through_python_are_the_same(dtype, monkeypatch):
+    """What the host module does, the Python form does, to the bit."""
+    H, Hk, D, T = 6, 2, 64, 3
+    rows = randn(2, T, H + 2 * Hk, D, seed=4, dtype=dtype)
+    q, k, v = rows.split((H, Hk, Hk), 2)
+    w, rope = randn(D, seed=5, dtype=dtype) + 1, rope_table(200, D)
+    lengths, counts, tree = ints(100, 7), ints(T, T - 1), trees(2, T)
+
+    def all_of_them():
+        cache = cache_of(2, Hk, 16, D, 120, dtype)
+        a = ops.qk_norm_rope(q, k, w, None, rope)
+        b = ops.append_kv(cache, k, v, lengths, q=q, q_weight=w, k_weight=w, rope=rope, positions=lengths[:, None] + ints(0, 1, 1), counts=counts)
+        nothing = ops.append_kv(cache, k, v, lengths)
+        c = ops.tree_attention(b, cache, lengths, tree, counts)
+        d = ops.tree_attention(b, cache, lengths, scale=0.3)
+        assert nothing is None
+        return [*a, b, cache.k, cache.v, c, d]
+
+    fast = all_of_them()
+    monkeypatch.setattr(ops, "_calls", ops._GeneralCalls)
+    for x, y in zip(fast, all_of_them()):
+        assert x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y)
+
+
+def test_modes_and_flags():
+    q, cache = randn(1, 1, 4, 64, seed=9, dtype=BF16), cache_of(1, 2, 16, 64, 50)
+    with torch.inference_mode():
+        y = ops.tree_attention(q, cache, ints(30))
+        assert y.is_inference()
+    with torch.enable_grad():
+        z = ops.tree_attention(q, cache, ints(30))
+        assert not z.requires_grad and not z.is_inference() and torch.equal(z, y)
+        with pytest.raises(RuntimeError, match="forward-only"):
+            ops.tree_attention(q.clone().requires_grad_(), cache, ints(30))
+        with pytest.raises(RuntimeError, match="forward-only"):
+            ops.qk_norm_rope(q.clone().requires_grad_(), None)
+    assert z.is_contiguous() and z.add_(1).shape == q.shape
+
+
+def test_no_tokens():
+    cache = cache_of(2, 2, 16, 64, 50)
+    assert ops.tree_attention(torch.empty(2, 0, 4, 64, dtype=BF16, device="cuda"), cache, ints(3, 4)).shape == (2, 0, 4, 64)
+    none = cache._replace(table=cache.table[:0])
+    assert ops.tree_attention(torch.empty(0, 3, 4, 64, dtype=BF16, device="cuda"), none, ints()).shape == (0, 3, 4, 64)
+
+
+@pytest.mark.parametrize("T", [1, 20, 64])
+def test_first_call_under_capture(T):
+    """A width that no other test has: the kernels' limits are set while a graph is captured."""
+    D = {1: 112, 20: 88, 64: 120}[T]
+    cache, q, lengths = cache_of(1, 1, 16, D, 500), randn(1, T, 4, D, seed=9, dtype=BF16), ints(400)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.tree_attention(q, cache, lengths)
+    graph.replay()
+    torch.cuda.synchronize()
+    check_attention(out, q, cache, lengths)
+
+
+def test_many_sequences():
+    B, H, D = 700, 1, 64
+    cache = cache_of(B, H, 16, D, 40)
+    q = randn(B, 2, 2, D, seed=9, dtype=BF16)
+    lengths = torch.arange(B, dtype=torch.int32, device="cuda") % 38
+    for c in (cache, widened(cache)):
+        check_attention(ops.tree_attention(q, c, lengths), q, c, lengths)
+    q = randn(B, 17, 2, D, seed=9, dtype=BF16)
+    lengths = lengths % 20
+    check_attention(ops.tree_attention(q, cache, lengths), q, cache, lengths)
