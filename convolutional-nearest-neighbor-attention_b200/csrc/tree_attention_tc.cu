@@ -19,7 +19,8 @@
 // wait a step 218; pieces joined by a thread a row 207.  Tried and slower: a quarter of the exponentials as polynomials with the product
 // in halves 229 (the exponential unit is not what is waited for: without any exponential 240 of 243); one room of scores for both streams,
 // weights apart, so that the next scores are there when the last weights are done: 232, and with the weights kept in registers until
-// their room is free 244 to 286 (216 registers do not hold them).
+// their room is free 244 to 286 (216 registers do not hold them); steps of 64 keys with two rooms of scores a stream 240 (half the registers, nothing
+// spilled, but twice the hand-overs, and a product of 64 columns reads its 128 rows from shared memory as one of 128 does).
 #include "f32x2.cuh"
 #include "paged_attention.cuh"
 #include "sm100.cuh"
