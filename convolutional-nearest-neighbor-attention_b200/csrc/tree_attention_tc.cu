@@ -11,12 +11,12 @@
 //              the accumulator multiplied, only when a tile exceeds it by 2^8 (float32 holds what that leaves).
 // A weight is rounded to one bfloat16 for its product (a second part would cost half the tensor cores' time); its sum is of the
 // unrounded ones.
-// 16 sequences of 32 to 64 drafted tokens over 4096 to 16384 entries, 32 query and 8 key heads of 128: 207 us, of which the two products are 77
+// 16 sequences of 32 to 64 drafted tokens over 4096 to 16384 entries, 32 query and 8 key heads of 128: 208 us, of which the two products are 77
 // at the tensor cores' nominal rate.  What bounds it is the way round: scores, 2000 cycles of softmax, weights, 1200 cycles of products; a
 // stream's next scores wait for its last weights (they lie where those were), and a period of both streams is 3990 cycles where the tensor
 // cores need 2050 and the exponentials as many.  How it came here: one tile of rows, two streams of keys 325 us (the second tile of rows reads all
 // keys again); two tiles of rows sharing them, registers moved 243; the next unit's queries before the last one's sums, sums side by side 222; one
-// wait a step 218; pieces joined by a thread a row 207.  Tried and slower: a quarter of the exponentials as polynomials with the product
+// wait a step 218; pieces joined by a thread a row 208.  Tried and slower: a quarter of the exponentials as polynomials with the product
 // in halves 229 (the exponential unit is not what is waited for: without any exponential 240 of 243); one room of scores for both streams,
 // weights apart, so that the next scores are there when the last weights are done: 232, and with the weights kept in registers until
 // their room is free 244 to 286 (216 registers do not hold them); steps of 64 keys with two rooms of scores a stream 240 (half the registers, nothing
