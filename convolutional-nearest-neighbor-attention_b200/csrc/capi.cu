@@ -733,6 +733,7 @@ int convnn_b200_tree_attention(const convnn_tree_attention* a, const convnn_cach
     if (a->B < 0 || a->T < 0 || a->Hk < 1 || a->Hq < 1 || a->Hq % a->Hk || a->D < 1)
         return set_error(CONVNN_E_INVALID, "tree_attention: %d query heads over %d key heads of %d channels", a->Hq, a->Hk, a->D);
     if (a->T > 64) return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %d drafted tokens, up to 64 are", a->T);
+    if ((int64_t)a->B * a->T > (1ll << 30)) return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: more than 2^30 tokens");
     if (a->D > kMostHeadChannels)
         return set_error(CONVNN_E_UNSUPPORTED, "tree_attention: %d channels a head, up to %d are", a->D, kMostHeadChannels);
     if (!std::isfinite(a->scale)) return set_error(CONVNN_E_INVALID, "tree_attention: the scale is not finite");

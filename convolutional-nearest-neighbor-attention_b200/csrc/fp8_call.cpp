@@ -443,7 +443,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* pages = plain(PyTuple_GET_ITEM(args[1], 0), device, grad);
     OR_NONE(pages && pages->dim() == 4);
     const int64_t B = q->size(0), T = q->size(1), D = q->size(3), H = pages->size(1), unit = dt == CONVNN_F32 ? 4 : 8;
-    OR_NONE(B >= 1 && B <= MOST && T >= 1 && T <= MOST_DRAFTED && D >= 1 && D <= MOST_CHANNELS && D % unit == 0 && H >= 1 && H <= (1 << 20));
+    OR_NONE(B >= 1 && T >= 1 && T <= MOST_DRAFTED && B <= MOST / T && D >= 1 && D <= MOST_CHANNELS && D % unit == 0 && H >= 1 && H <= (1 << 20));
     a.dtype = dt; a.B = (int32_t)B; a.T = (int32_t)T; a.D = (int32_t)D; a.Hk = (int32_t)H;
     OR_NONE(heads_of(*q, B, T, D, type, a.Hq, a.q_stride) && a.Hq % H == 0 && ints_of(lengths, B) && ints_of(counts, B) &&
             cache_of(args[1], device, grad, B, H, D, type, false, c));

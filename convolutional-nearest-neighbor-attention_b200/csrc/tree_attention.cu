@@ -774,7 +774,8 @@ __device__ __forceinline__ Cut cut_at(const Params& p, int cta) {
     u.second = d.first(u.c0) < begin;
     return u;
 }
-// Rows without anything, of all sequences: zeros, by all warps of the grid.
+// Rows without anything, of all sequences: zeros, by all warps of the grid.  (Up to 2^30 tokens are taken: with a step added they stay
+// below 2^31.)
 __device__ __forceinline__ int next_zero_row(const Params& p, int i) {
     const int blocks = gridDim.x * gridDim.y * gridDim.z;
     for (; i < p.B * p.T; i += blocks * kWarps) {

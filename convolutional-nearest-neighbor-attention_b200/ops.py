@@ -1020,6 +1020,8 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     dt = _dtype_code(q.dtype)
     if T > MOST_DRAFTED:
         raise ValueError(f"tree_attention takes up to {MOST_DRAFTED} drafted tokens, got {T}")
+    if B * T > MOST_CHANNELS:
+        raise ValueError(f"tree_attention takes up to 2^30 tokens, got {B} x {T}")
     Hk = cache[0].shape[1] if cache[0].dim() == 4 else 0
     if Hk < 1 or Hq % Hk:
         raise ValueError(f"{Hq} query heads do not share a cache of shape {tuple(cache[0].shape)} evenly")

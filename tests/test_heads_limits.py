@@ -1,0 +1,23 @@
+"""Sizes and tables at the edge of what heads, the paged cache and the attention over it take, on the CPU: no kernel
+is launched, and no pointer is followed."""
+import pytest
+import torch
+
+from convnn_b200 import _capi, ops
+from test_heads_refusals import BF16, I32, attention, on_any_device, t  # noqa: F401
+
+
+@pytest.mark.parametrize("B,T", [((1 << 30) + 1, 1), ((1 << 24) + 1, 64), (1 << 25, 64), ((1 << 31) - 1, 63), (17895698, 61)])
+def test_attention_of_more_tokens_than_are_counted(B, T):
+    """The rows of a call are counted in 32 bits."""
+    assert B * T > 1 << 30
+    assert attention(B=B, T=T) == _capi.E_UNSUPPORTED
+    assert b"2^30 tokens" in _capi.lib().convnn_b200_last_error()
+
+
+def test_attention_of_more_tokens_from_python(on_any_device):  # noqa: F811
+    B, T = (1 << 24) + 1, 64
+    cache = ops.PagedCache(t(1, 1, 16, 8), t(1, 1, 16, 8), t(1, 1, dtype=I32).expand(B, 1))
+    with pytest.raises(ValueError, match="2\\^30 tokens"):
+        ops.tree_attention(t(1, 1, 1, 8).expand(B, T, 1, 8), cache, t(1, dtype=I32).expand(B))
+    assert not on_any_device
