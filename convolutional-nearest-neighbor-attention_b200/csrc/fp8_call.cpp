@@ -293,7 +293,8 @@ bool rope_of(const at::Tensor* rope, int64_t D, convnn_heads& a) {
     if (rope->scalar_type() != at::kFloat || rope->dim() != 2 || rope->size(1) < 2 || rope->size(1) % 2 || rope->size(1) > D ||
         rope->size(0) > MOST || rope->stride(1) != 1 || rope->stride(0) < rope->size(1))
         return false;
-    a.rope = static_cast<const float*>(rope->data_ptr());
+    // (a table without rows has no address in torch, and none is no rotation: one that is not followed)
+    a.rope = rope->size(0) ? static_cast<const float*>(rope->data_ptr()) : reinterpret_cast<const float*>(16);
     a.rope_stride = rope->stride(0);
     a.rope_rows = (int32_t)rope->size(0);
     a.rotary = (int32_t)rope->size(1);

@@ -792,6 +792,7 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
 # ---- heads, a paged cache, and attention over it --------------------------------------------------------------------
 
 MOST_HEAD_CHANNELS, MOST_DRAFTED = 256, 64
+_NO_ROWS = 16                                     # an address that is not followed
 
 
 class PagedCache(NamedTuple):
@@ -898,7 +899,8 @@ def _heads_arg(q, k, v, q_weight, k_weight, rope, positions, eps, interleaved, l
             raise ValueError(f"rope must be (positions, turned channels), an even number up to {D} of them, got {tuple(rope.shape)}")
         if rope.stride(1) != 1 or rope.stride(0) < rope.shape[1]:
             rope = rope.contiguous()
-        a.rope, a.rope_stride, (a.rope_rows, a.rotary) = rope.data_ptr(), rope.stride(0), rope.shape
+        # (a table without rows has no address in torch, and none is no rotation)
+        a.rope, a.rope_stride, (a.rope_rows, a.rotary) = rope.data_ptr() or _NO_ROWS, rope.stride(0), rope.shape
         kept.append(rope)
     if positions is not None:
         positions = _index_arg(positions, lead, "positions").reshape(a.B, a.T)

@@ -288,7 +288,7 @@ typedef struct convnn_heads {
     const void *q, *k, *v;                    /* v: append_kv only */
     int64_t q_stride[3], k_stride[3], v_stride[3];
     const void *q_weight, *k_weight;          /* (D) in dtype, or NULL */
-    const float* rope;                        /* or NULL: no rotation */
+    const float* rope;                        /* or NULL: no rotation (not NULL where rope_rows is 0: then it is not read) */
     int64_t rope_stride;
     const int32_t* positions;
     int64_t position_stride[2];

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from convnn_b200 import _capi, ops
-from test_heads_refusals import BF16, I32, attention, on_any_device, t  # noqa: F401
+from test_heads_refusals import BF16, I32, attention, on_any_device, paged, t  # noqa: F401
 
 
 @pytest.mark.parametrize("B,T", [((1 << 30) + 1, 1), ((1 << 24) + 1, 64), (1 << 25, 64), ((1 << 31) - 1, 63), (17895698, 61)])
@@ -21,3 +21,14 @@ def test_attention_of_more_tokens_from_python(on_any_device):  # noqa: F811
     with pytest.raises(ValueError, match="2\\^30 tokens"):
         ops.tree_attention(t(1, 1, 1, 8).expand(B, T, 1, 8), cache, t(1, dtype=I32).expand(B))
     assert not on_any_device
+
+
+@pytest.mark.parametrize("call", [lambda rope: ops.qk_norm_rope(t(3, 4, 64), t(3, 2, 64), rope=rope),
+                                  lambda rope: ops.append_kv(paged(), t(2, 1, 2, 64), t(2, 1, 2, 64), t(2, dtype=I32), rope=rope)])
+def test_a_table_without_rows_is_a_table(on_any_device, call):  # noqa: F811
+    """torch gives an empty table no address, and no address is no rotation."""
+    call(torch.empty(0, 32))
+    heads = on_any_device[0][0]._obj
+    assert heads.rope and heads.rotary == 32 and heads.rope_rows == 0
+    call(None)
+    assert not on_any_device[1][0]._obj.rope
