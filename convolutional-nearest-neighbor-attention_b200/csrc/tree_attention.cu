@@ -528,7 +528,8 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
     float* sS = sQ + ROWS * pitch;                                       // [8][16][SP]
     float* sP = sS + SW * ROWS * SP;                                     // [16][PP]
     float *sF = sP + ROWS * PP, *sTop = sF + ROWS, *sSum = sTop + ROWS;  // [16] each
-    float* ring = sSum + ROWS;
+    int* sBad = reinterpret_cast<int*>(sSum + ROWS);                     // (4 words)
+    float* ring = sSum + ROWS + 4;
     const int stage_floats = 2 * TILE * pitch;
     uint8_t* room = reinterpret_cast<uint8_t*>(ring + STAGES * stage_floats);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 3, lc = lane & 7;   // rows lr + 4 i
@@ -587,6 +588,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                                                      (h * p.G + g) * p.qs[2] + c * 4);
             *reinterpret_cast<float4*>(sQ + r * pitch + c * 4) = v;
         }
+        if (threadIdx.x == 0) *sBad = 0;
         const unsigned long long mask[2] = {seen_by(p, s, b, row0 + 2 * warp), seen_by(p, s, b, row0 + 2 * warp + 1)};
         float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
         float4 o[4];
@@ -599,7 +601,19 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
             __syncthreads();                                             // the tile is there, and the one before it read
             fetch(stage == 0 ? STAGES - 1 : stage - 1);
             const float* sk = ring + stage * stage_floats;
-            const float* sv = sk + TILE * pitch;
+            float* sv = ring + stage * stage_floats + TILE * pitch;
+            const bool drafts = at.tile * TILE + TILE > s.length;
+            // what is not finite among the drafted tokens' values: a zero in its place, for now (read behind two more barriers)
+            if (const int entry = at.tile * TILE + (threadIdx.x >> 3); drafts && entry >= s.length && entry < s.total) {
+                for (int c = threadIdx.x & 7; c < pieces; c += 8) {
+                    float4* at16 = reinterpret_cast<float4*>(sv + (threadIdx.x >> 3) * pitch + 4 * c);
+                    const float4 v = *at16;
+                    if (isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w)) continue;
+                    *at16 = make_float4(isfinite(v.x) ? v.x : 0.f, isfinite(v.y) ? v.y : 0.f, isfinite(v.z) ? v.z : 0.f,
+                                        isfinite(v.w) ? v.w : 0.f);
+                    *sBad = 1;
+                }
+            }
             auto scores = [&](auto rows) {
                 constexpr int R = decltype(rows)::value;
                 float c[R][4] = {};
@@ -629,7 +643,6 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
             else scores(std::integral_constant<int, 4>());
             __syncthreads();
             const int j = at.tile * TILE + lane - s.length;
-            const bool drafts = at.tile * TILE + TILE > s.length;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = 2 * warp + i;
@@ -650,7 +663,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 if (lane == 0) sF[r] = f;
             }
             __syncthreads();
-            auto sums = [&](auto some_hidden, auto rows) {
+            auto sums = [&](auto rows) {
                 constexpr int R = decltype(rows)::value;
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
@@ -669,7 +682,6 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                         const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            if (decltype(some_hidden)::value && ws[x] == 0.f) continue;  // (what a row does not see need not be finite)
                             o[i].x = fmaf(ws[x], v[x].x, o[i].x);
                             o[i].y = fmaf(ws[x], v[x].y, o[i].y);
                             o[i].z = fmaf(ws[x], v[x].z, o[i].z);
@@ -679,9 +691,8 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 }
             };
             if (sums_here) {
-                if (live <= 4 && !drafts) sums(std::false_type(), std::integral_constant<int, 1>());
-                else if (!drafts) sums(std::false_type(), std::integral_constant<int, 4>());
-                else sums(std::true_type(), std::integral_constant<int, 4>());
+                if (live <= 4) sums(std::integral_constant<int, 1>());
+                else sums(std::integral_constant<int, 4>());
             }
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             end = at.last_of_unit();
@@ -704,7 +715,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<float4*>(sS + ((my_part - 1) * ROWS + lr + 4 * i) * p.D + 4 * col) = o[i];
         __syncthreads();                                                 // (the scores of the last tile are read)
-        const bool whole = tile0 == 0 && at_end;
+        const bool whole = tile0 == 0 && at_end, any_bad = *sBad != 0;
         float* slot = slot_of(p, blockIdx.x, first_unit);
         if (sums_here && my_part == 0)
 #pragma unroll
@@ -722,13 +733,20 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 } else if (t < s.count) {
                     const float inv = sSum[r] == 0.f ? 0.f : 1.0f / sSum[r];
                     y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
+                    if (any_bad) {
+                        const unsigned long long seen = seen_by(p, s, b, row0 + r);
+                        y.x += not_finite_seen<float>(p, s, b, h, seen, 4 * col);
+                        y.y += not_finite_seen<float>(p, s, b, h, seen, 4 * col + 1);
+                        y.z += not_finite_seen<float>(p, s, b, h, seen, 4 * col + 2);
+                        y.w += not_finite_seen<float>(p, s, b, h, seen, 4 * col + 3);
+                    }
                     *reinterpret_cast<float4*>(static_cast<float*>(p.out) + b * p.os[0] + t * p.os[1] + (h * p.G + g) * p.os[2] +
                                                4 * col) = y;
                 }
             }
         if (SPLIT) {
             __syncthreads();
-            join_cluster<float>(p, s, b, h, row0 / ROWS, room, false, [&](int r, int four, float4& x, float& m_, float& l_) {
+            join_cluster<float>(p, s, b, h, row0 / ROWS, room, any_bad, [&](int r, int four, float4& x, float& m_, float& l_) {
                 x = *reinterpret_cast<const float4*>(sQ + r * pitch + 4 * four);
                 m_ = sTop[r];
                 l_ = sSum[r];
@@ -738,7 +756,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
         if (!whole && threadIdx.x < ROWS) {
             slot[ROWS * p.D + threadIdx.x] = sTop[threadIdx.x];
             slot[ROWS * p.D + ROWS + threadIdx.x] = sSum[threadIdx.x];
-            if (threadIdx.x == 0) slot[ROWS * p.D + 2 * ROWS] = 0.f;
+            if (threadIdx.x == 0) slot[ROWS * p.D + 2 * ROWS] = any_bad ? 1.f : 0.f;
         }
         first_unit = false;
         __syncthreads();                                                 // (sQ, sS, sTop, sSum)
@@ -983,7 +1001,7 @@ Plan plan_of(int dtype, int rows, int D, bool tiles) {
     if (dtype == CONVNN_F32) {
         g.tile = 32;
         g.stages = D <= 64 ? 3 : 2;
-        g.smem = 4 * ((size_t)ROWS * (D + 4) + SW * ROWS * SP + ROWS * PP + 3 * ROWS + (size_t)g.stages * 2 * TILE * (D + 4));
+        g.smem = 4 * ((size_t)ROWS * (D + 4) + SW * ROWS * SP + ROWS * PP + 3 * ROWS + 4 + (size_t)g.stages * 2 * TILE * (D + 4));
         g.ctas_per_sm = g.smem <= 112 * 1024 ? 2 : 1;
     } else {
         const int DP = 16 * steps_of(D), pitch = ((DP / 8) | 1) * 16;

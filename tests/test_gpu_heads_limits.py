@@ -48,3 +48,62 @@ def test_a_rotation_table_without_rows(both_ways, dtype, R):
             page, row = int(cache.table[b, (length + i) // 16]), (length + i) % 16
             check_turned_by_no_row(cache.k[page, :, row], k[b, i], w, R)
             assert torch.equal(cache.v[page, :, row], k[b, i])
+
+
+# ---- values that are not finite -----------------------------------------------------------------------------------------
+
+def place(cache, entry):
+    return int(cache.table[0, entry // cache.k.shape[2]]), entry % cache.k.shape[2]
+
+
+def far_below(dtype, length, T, G, D=64, wide=False):
+    """Queries and a cache in which an entry with the key -40 has a weight that float32 does not hold."""
+    cache = cache_of(1, 2, 16, D, length + T, dtype)
+    if wide:
+        cache = cache._replace(table=torch.cat([cache.table, torch.full((1, 1 << 16), -1, dtype=torch.int32, device="cuda")], 1))
+    return randn(1, T, 2 * G, D, seed=9, dtype=dtype).abs() + 0.5, cache
+
+
+@pytest.mark.parametrize("dtype,T,G", [(F32, 1, 1), (F32, 3, 2), (F32, 7, 4), (BF16, 1, 1), (BF16, 3, 2), (BF16, 20, 2), (BF16, 40, 4)])
+@pytest.mark.parametrize("length", [31, 32, 33, 60, 64, 65, 127, 130, 400])
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_cached_value_that_is_not_finite_shows(dtype, T, G, length, wide):
+    """An entry that all rows see leaves its trace in its channel wherever it lies, however small its weight."""
+    q, cache = far_below(dtype, length, T, G, wide=wide)
+    lengths, D = ints(length), 64
+    for entry in {0, 5, max(0, length // 32 * 32 - 1), length - 1}:
+        page, row = place(cache, entry)
+        key, value = cache.k[page, 1, row].clone(), cache.v[page, 1, row].clone()
+        cache.k[page, 1, row] = -40
+        cache.v[page, 1, row] = 0
+        want = ops.tree_attention(q, cache, lengths)
+        for bad in (float("inf"), float("nan")):
+            cache.v[page, 1, row, 7] = bad
+            got = ops.tree_attention(q, cache, lengths)
+            hit = torch.zeros_like(got, dtype=torch.bool)
+            hit[:, :, G:, 7] = True
+            assert torch.isfinite(want).all() and not torch.isfinite(got[hit]).any(), (entry, bad)
+            assert torch.equal(got[~hit], want[~hit]), (entry, bad)
+        cache.k[page, 1, row], cache.v[page, 1, row] = key, value
+
+
+@pytest.mark.parametrize("dtype,T,G", [(F32, 3, 2), (F32, 7, 4), (F32, 33, 1), (BF16, 3, 2), (BF16, 20, 2), (BF16, 40, 4)])
+@pytest.mark.parametrize("length", [0, 29, 31, 62, 126, 400, 3000])
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_drafted_value_that_is_not_finite_shows_where_it_is_seen(dtype, T, G, length, wide):
+    """The value itself, however small its weight, and nothing of it anywhere else."""
+    q, cache = far_below(dtype, length, T, G, wide=wide)
+    lengths = ints(length)
+    tree = torch.tensor([[1 | 1 << t | (2 if t == 2 else 0) for t in range(T)]], dtype=torch.int64, device="cuda")
+    tree[0, 1] = 1                                           # token 1 is seen by token 2 alone
+    page, row = place(cache, length + 1)
+    cache.k[page, 1, row] = -40
+    cache.v[page, 1, row] = 0
+    want = ops.tree_attention(q, cache, lengths, tree)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        cache.v[page, 1, row, 7] = bad
+        got = ops.tree_attention(q, cache, lengths, tree)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[0, 2, G:, 7] = True
+        assert torch.equal(got[~hit], want[~hit]) and torch.isfinite(want).all()
+        assert torch.isnan(got[hit]).all() if bad != bad else (got[hit] == bad).all()
