@@ -423,6 +423,11 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!ok(append_fn(&a, &c, static_cast<const int32_t*>(lengths->data_ptr()),
                       counts ? static_cast<const int32_t*>(counts->data_ptr()) : nullptr, c10::cuda::getCurrentCUDAStream(device).stream())))
         return nullptr;
+    // (as in-place operations do, so that autograd notices if it has kept them)
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor& pages = THPVariable_Unpack(PyTuple_GET_ITEM(args[0], i));
+        if (!pages.is_inference()) pages.unsafeGetTensorImpl()->bump_version();
+    }
     if (!q) Py_RETURN_FALSE;
     return THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS

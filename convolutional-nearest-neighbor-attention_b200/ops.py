@@ -208,6 +208,7 @@ def out_proj(spec: LayerSpec, o, w_o, out: Optional[torch.Tensor] = None, S: Opt
     res, ldr = _residual_arg(residual, o)
     _capi.check(L.convnn_b200_out_proj(d, o.data_ptr(), w_o.data_ptr(), _capi.ptr(res), ldr, out.data_ptr(), ldo,
                                        scratch.data_ptr(), _stream(o)))
+    _written(out)
     return out
 
 
@@ -245,6 +246,7 @@ def forward(spec: LayerSpec, x: torch.Tensor, packed, cand: Optional[torch.Tenso
     _capi.check(L.convnn_b200_forward(d, x.data_ptr(), ldx, w_qkv.data_ptr(), w_conv.data_ptr(), _capi.ptr(w_pw),
                                       w_o.data_ptr(), _capi.ptr(cand), _capi.ptr(res), ldr, out.data_ptr(), ldo,
                                       workspace.data_ptr(), workspace.numel(), _stream(x)))
+    _written(out)
     return out
 
 
@@ -272,6 +274,7 @@ class LayerForward:
             view, ldo = _rows_view(out)
             if view is not out:
                 raise ValueError("out must have unit channel stride and evenly strided rows")
+            _written(out)
         res, ldr = (None, 0) if residual is None else _residual_arg(residual, x)
         w = self.w
         rc = _capi.lib().convnn_b200_forward(
@@ -425,12 +428,14 @@ def outproj_mlp(o: torch.Tensor, w_o: torch.Tensor, x: torch.Tensor, eps: float,
 # ---- the other halves of the branching wrappers ------------------------------------------------
 
 def _out_slice(out: Optional[torch.Tensor], like: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """-> (what the caller is about to write, its row stride)"""
     B, T, D = like.shape
     if out is None:
         out = torch.empty(B, T, D, dtype=like.dtype, device=like.device)
     view, ldo = _rows_view(out)
     if view is not out:
         raise ValueError("out must have unit channel stride and evenly strided rows")
+    _written(out)
     return out, ldo
 
 
@@ -530,6 +535,10 @@ def _forward_only(*tensors) -> None:
         if t is not None and t.requires_grad:
             raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
                                "(training / backward is outside this library)")
+
+
+# For tensors of the caller's that a kernel has written: autograd notices if it has kept one of them.
+_written = torch.autograd.graph.increment_version
 
 
 def _device_of(like: torch.Tensor, *tensors) -> int:
@@ -938,7 +947,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     if done is not None:
         return done
     if torch.is_grad_enabled():
-        _forward_only(q, k, q_weight, k_weight, rope)
+        _forward_only(q, k, q_weight, k_weight, rope, *(() if out is None else out))
     like = q if q is not None else k
     if like is None:
         raise ValueError("qk_norm_rope needs queries or keys")
@@ -960,6 +969,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
         results.append(o)
     if a.B and a.T:
         _launch(index, _capi.lib().convnn_b200_qk_norm_rope, ctypes.byref(a))
+        _written([o for o in into if o is not None])
     return tuple(results)
 
 
@@ -991,6 +1001,7 @@ def append_kv(cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, q:
     if a.B and a.T:
         _launch(index, _capi.lib().convnn_b200_append_kv, ctypes.byref(a), ctypes.byref(c), lengths.data_ptr(),
                 None if counts is None else counts.data_ptr())
+        _written(cache[:2])
     return result
 
 
@@ -1013,7 +1024,7 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     if done is not None:
         return done
     if torch.is_grad_enabled():
-        _forward_only(q, cache[0], cache[1])
+        _forward_only(q, cache[0], cache[1], out)
     index = _device_of(q, lengths, tree, counts, out, *cache)
     if q.dim() != 4:
         raise ValueError(f"queries must be (sequences, tokens, heads, channels), got {tuple(q.shape)}")
@@ -1048,6 +1059,8 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
             need = L.convnn_b200_tree_attention_workspace_bytes(dt, T, Hq, Hk, D)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         _launch(index, L.convnn_b200_tree_attention, ctypes.byref(a), ctypes.byref(c), workspace.data_ptr(), need)
+        if out is not None:
+            _written(out)
     if room is not result:
         result.copy_(room)
     return result

@@ -107,3 +107,61 @@ def test_a_drafted_value_that_is_not_finite_shows_where_it_is_seen(dtype, T, G, 
         hit[0, 2, G:, 7] = True
         assert torch.equal(got[~hit], want[~hit]) and torch.isfinite(want).all()
         assert torch.isnan(got[hit]).all() if bad != bad else (got[hit] == bad).all()
+
+
+# ---- tensors that autograd watches --------------------------------------------------------------------------------------
+
+def appended(cache, n=2):
+    new = randn(2, n, 2, 64, seed=3, dtype=cache.k.dtype)
+    ops.append_kv(cache, new, new, ints(5, 30))
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_cache_that_autograd_has_kept(both_ways, which):
+    cache = cache_of(2, 2, 16, 64, 60)
+    w = torch.ones(64, dtype=BF16, device="cuda", requires_grad=True)
+    with torch.enable_grad():
+        y = (getattr(cache, which) * w).sum()
+    appended(cache)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # slices of one buffer: its own version
+    both = randn(2, 9, 2, 16, 64, seed=1, dtype=BF16)
+    before = both._version
+    appended(cache._replace(k=both[0], v=both[1]))
+    assert both._version > before
+    # no version to move
+    with torch.inference_mode():
+        cache = cache_of(2, 2, 16, 64, 60)
+    appended(cache)
+    with torch.inference_mode():
+        appended(cache)
+        appended(cache_of(2, 2, 16, 64, 60))
+
+
+def test_results_that_autograd_has_kept(both_ways):
+    cache, q = cache_of(2, 2, 16, 64, 60), randn(2, 1, 4, 64, seed=9, dtype=BF16)
+    w = torch.ones(64, dtype=BF16, device="cuda", requires_grad=True)
+    odd = torch.empty(q.numel() + 1, dtype=BF16, device="cuda")[1:].view(q.shape)
+    for out in (torch.ones_like(q), odd.fill_(1)):
+        for write in (lambda: ops.tree_attention(q, cache, ints(5, 30), out=out), lambda: ops.qk_norm_rope(q, None, out=(out, None))):
+            with torch.enable_grad():
+                y = (out * w).sum()
+            write()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    with torch.enable_grad():
+        for write in (lambda o: ops.tree_attention(q, cache, ints(5, 30), out=o), lambda o: ops.qk_norm_rope(q, None, out=(o, None))):
+            with pytest.raises(RuntimeError, match="forward-only"):
+                write(torch.ones_like(q).requires_grad_())
+
+
+def test_a_layers_result_that_autograd_has_kept():
+    x, w = randn(2, 40, 64, seed=1, dtype=BF16), torch.ones(64, dtype=BF16, device="cuda", requires_grad=True)
+    w_qkv, w_o = randn(3, 64, 64, seed=2, dtype=BF16, scale=0.1), randn(64, 64, seed=3, dtype=BF16, scale=0.1)
+    out = torch.ones_like(x)
+    with torch.enable_grad():
+        y = (out * w).sum()
+    ops.softmax_attention(x, w_qkv, w_o, 2, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -32,3 +32,17 @@ def test_a_table_without_rows_is_a_table(on_any_device, call):  # noqa: F811
     assert heads.rope and heads.rotary == 32 and heads.rope_rows == 0
     call(None)
     assert not on_any_device[1][0]._obj.rope
+
+
+def test_what_is_written_moves_its_version(on_any_device):  # noqa: F811
+    c, q, lengths = paged(), t(2, 1, 4, 64), t(2, dtype=I32)
+    ops.append_kv(c, t(2, 1, 2, 64), t(2, 1, 2, 64), lengths)
+    assert c.k._version > 0 and c.v._version > 0 and c.table._version == 0
+    y, z = t(2, 1, 4, 64), t(2, 1, 4, 64)
+    assert ops.qk_norm_rope(q, None, out=(y, None))[0] is y and y._version > 0 and q._version == 0
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="forward-only"):
+        ops.qk_norm_rope(q, None, out=(z.requires_grad_(), None))
+    # nothing is written
+    c = paged()
+    ops.append_kv(c, t(2, 0, 2, 64), t(2, 0, 2, 64), lengths)
+    assert c.k._version == 0
