@@ -4,12 +4,14 @@
 // rms_norm with a residual and an 8-bit result takes 14 us of host time through Python, linear_fp8 12, qk_norm_rope 20, append_kv 32 and
 // tree_attention 30; their kernels for a few rows take less.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -71,11 +73,21 @@ PyObject* bind_heads(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-// A plain tensor on `device` (-1: on any CUDA device, which is then the one); no gradient wanted.
-const at::Tensor* plain(PyObject* o, int& device, bool grad) {
+// What autograd watches for at this call: gradients that are wanted, tangents (where a level of forward mode is open; there is but one).
+struct Watch {
+    bool grad, tangents;
+};
+Watch watching() {
+    return {c10::GradMode::is_enabled(),
+            c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr};
+}
+// A plain tensor on `device` (-1: on any CUDA device, which is then the one); no gradient wanted, and no tangent with it.
+const at::Tensor* plain(PyObject* o, int& device, const Watch& watch) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.layout() != at::kStrided || (grad && t.requires_grad())) return nullptr;
+    if (!t.is_cuda() || t.layout() != at::kStrided || (watch.grad && t.requires_grad()) ||
+        (watch.tangents && t._fw_grad(0).defined()))
+        return nullptr;
     if (device < 0) device = t.get_device();
     return t.get_device() == device ? &t : nullptr;
 }
@@ -140,10 +152,11 @@ bool ok(int status) {
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     OR_NONE(n == 5 && norm_fn && PyFloat_CheckExact(args[2]) && PyBool_Check(args[4]));
-    const bool grad = c10::GradMode::is_enabled(), quantize = args[4] == Py_True, with_residual = args[3] != Py_None;
+    const Watch watch = watching();
+    const bool quantize = args[4] == Py_True, with_residual = args[3] != Py_None;
     int device = -1;
-    const at::Tensor *x = plain(args[0], device, grad), *w = x ? plain(args[1], device, grad) : nullptr;
-    const at::Tensor* res = w && with_residual ? plain(args[3], device, grad) : nullptr;
+    const at::Tensor *x = plain(args[0], device, watch), *w = x ? plain(args[1], device, watch) : nullptr;
+    const at::Tensor* res = w && with_residual ? plain(args[3], device, watch) : nullptr;
     int64_t rows, ldx, ldr = 0, res_rows;
     OR_NONE(w && (res || !with_residual) && device == c10::cuda::current_device());
     const auto type = x->scalar_type();
@@ -190,7 +203,7 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_RETURN_NONE;
     }
     int device = -1;
-    const at::Tensor* x = plain(args[0], device, c10::GradMode::is_enabled());
+    const at::Tensor* x = plain(args[0], device, watching());
     int64_t rows, ldx, ld, row, block;
     OR_NONE(x && device == c10::cuda::current_device() && (block_rows == 1 || (block_rows == BLOCK && x->dim() == 2)));
     const int dt = dtype_code(x->scalar_type());
@@ -219,17 +232,18 @@ PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     OR_NONE(n == 7 && linear_fn && PyTuple_Check(args[0]) && PyTuple_GET_SIZE(args[0]) == 2 && PyTuple_Check(args[1]) &&
             PyTuple_GET_SIZE(args[1]) == 2 && PyBool_Check(args[3]) && PyLong_CheckExact(args[5]) && PyBool_Check(args[6]));
-    const bool grad = c10::GradMode::is_enabled(), gelu = args[3] == Py_True, quantize = args[6] == Py_True;
+    const Watch watch = watching();
+    const bool gelu = args[3] == Py_True, quantize = args[6] == Py_True;
     const bool with_bias = args[2] != Py_None, with_residual = args[4] != Py_None;
     const int io = (int)PyLong_AsLong(args[5]);
     int device = -1;
-    const at::Tensor* a = plain(PyTuple_GET_ITEM(args[0], 0), device, grad);
-    const at::Tensor* sa = a ? plain(PyTuple_GET_ITEM(args[0], 1), device, grad) : nullptr;
-    const at::Tensor* w = sa ? plain(PyTuple_GET_ITEM(args[1], 0), device, grad) : nullptr;
-    const at::Tensor* sw = w ? plain(PyTuple_GET_ITEM(args[1], 1), device, grad) : nullptr;
+    const at::Tensor* a = plain(PyTuple_GET_ITEM(args[0], 0), device, watch);
+    const at::Tensor* sa = a ? plain(PyTuple_GET_ITEM(args[0], 1), device, watch) : nullptr;
+    const at::Tensor* w = sa ? plain(PyTuple_GET_ITEM(args[1], 0), device, watch) : nullptr;
+    const at::Tensor* sw = w ? plain(PyTuple_GET_ITEM(args[1], 1), device, watch) : nullptr;
     OR_NONE(sw && device == c10::cuda::current_device());
-    const at::Tensor* bias = with_bias ? plain(args[2], device, grad) : nullptr;
-    const at::Tensor* res = with_residual ? plain(args[4], device, grad) : nullptr;
+    const at::Tensor* bias = with_bias ? plain(args[2], device, watch) : nullptr;
+    const at::Tensor* res = with_residual ? plain(args[4], device, watch) : nullptr;
     OR_NONE((bias || !with_bias) && (res || !with_residual));
     const auto type = io == CONVNN_BF16 ? at::kBFloat16 : at::kFloat;
     // (values of more dimensions go through Python, which looks at how their scales are strided)
@@ -269,8 +283,8 @@ at::Tensor room_for(at::IntArrayRef shape, at::ScalarType type) {
                                      std::nullopt);
 }
 // None, or a plain tensor.
-bool maybe(PyObject* o, const at::Tensor*& t, int& device, bool grad) {
-    t = o == Py_None ? nullptr : plain(o, device, grad);
+bool maybe(PyObject* o, const at::Tensor*& t, int& device, const Watch& watch) {
+    t = o == Py_None ? nullptr : plain(o, device, watch);
     return t || o == Py_None;
 }
 // (B, T, H, D) or (T, H, D), channels side by side.
@@ -303,11 +317,11 @@ bool rope_of(const at::Tensor* rope, int64_t D, convnn_heads& a) {
 bool ints_of(const at::Tensor* t, int64_t n) {
     return !t || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && (t->stride(0) == 1 || n == 1));
 }
-bool cache_of(PyObject* o, int& device, bool grad, int64_t B, int64_t H, int64_t D, at::ScalarType type, bool written, convnn_cache& c) {
+bool cache_of(PyObject* o, int& device, const Watch& watch, int64_t B, int64_t H, int64_t D, at::ScalarType type, bool written, convnn_cache& c) {
     if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 3) return false;
-    const at::Tensor* k = plain(PyTuple_GET_ITEM(o, 0), device, grad);
-    const at::Tensor* v = k ? plain(PyTuple_GET_ITEM(o, 1), device, grad) : nullptr;
-    const at::Tensor* table = v ? plain(PyTuple_GET_ITEM(o, 2), device, grad) : nullptr;
+    const at::Tensor* k = plain(PyTuple_GET_ITEM(o, 0), device, watch);
+    const at::Tensor* v = k ? plain(PyTuple_GET_ITEM(o, 1), device, watch) : nullptr;
+    const at::Tensor* table = v ? plain(PyTuple_GET_ITEM(o, 2), device, watch) : nullptr;
     if (!table || k->scalar_type() != type || v->scalar_type() != type || table->scalar_type() != at::kInt || k->dim() != 4 ||
         v->sizes() != k->sizes() || k->size(1) != H || k->size(3) != D || k->size(0) < 1 || k->size(2) < 1 || k->size(0) > MOST ||
         k->size(2) > MOST || table->dim() != 2 || table->size(0) != B || table->size(1) > MOST || table->size(1) * k->size(2) > MOST ||
@@ -346,11 +360,11 @@ void dense_strides(int64_t (&stride)[3], int64_t T, int64_t H, int64_t D) {
 PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     OR_NONE(n == 9 && heads_fn && PyFloat_CheckExact(args[6]) && PyBool_Check(args[7]) && args[8] == Py_None);
-    const bool grad = c10::GradMode::is_enabled();
+    const Watch watch = watching();
     int device = -1;
-    const at::Tensor *q = plain(args[0], device, grad), *k, *wq, *wk, *rope, *at_;
-    OR_NONE(q && maybe(args[1], k, device, grad) && maybe(args[2], wq, device, grad) && maybe(args[3], wk, device, grad) &&
-            maybe(args[4], rope, device, grad) && maybe(args[5], at_, device, grad) && device == c10::cuda::current_device());
+    const at::Tensor *q = plain(args[0], device, watch), *k, *wq, *wk, *rope, *at_;
+    OR_NONE(q && maybe(args[1], k, device, watch) && maybe(args[2], wq, device, watch) && maybe(args[3], wk, device, watch) &&
+            maybe(args[4], rope, device, watch) && maybe(args[5], at_, device, watch) && device == c10::cuda::current_device());
     convnn_heads a{};
     const auto type = q->scalar_type();
     const int64_t dim = q->dim();
@@ -388,12 +402,12 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     OR_NONE(n == 12 && append_fn && PyFloat_CheckExact(args[10]) && PyBool_Check(args[11]));
-    const bool grad = c10::GradMode::is_enabled();
+    const Watch watch = watching();
     int device = -1;
-    const at::Tensor *k = plain(args[1], device, grad), *v = k ? plain(args[2], device, grad) : nullptr;
-    const at::Tensor *lengths = v ? plain(args[3], device, grad) : nullptr, *q, *wq, *wk, *rope, *at_, *counts;
-    OR_NONE(lengths && maybe(args[4], q, device, grad) && maybe(args[5], wq, device, grad) && maybe(args[6], wk, device, grad) &&
-            maybe(args[7], rope, device, grad) && maybe(args[8], at_, device, grad) && maybe(args[9], counts, device, grad) &&
+    const at::Tensor *k = plain(args[1], device, watch), *v = k ? plain(args[2], device, watch) : nullptr;
+    const at::Tensor *lengths = v ? plain(args[3], device, watch) : nullptr, *q, *wq, *wk, *rope, *at_, *counts;
+    OR_NONE(lengths && maybe(args[4], q, device, watch) && maybe(args[5], wq, device, watch) && maybe(args[6], wk, device, watch) &&
+            maybe(args[7], rope, device, watch) && maybe(args[8], at_, device, watch) && maybe(args[9], counts, device, watch) &&
             device == c10::cuda::current_device());
     convnn_heads a{};
     convnn_cache c{};
@@ -408,7 +422,7 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     OR_NONE(heads_of(*k, B, T, D, type, a.Hk, a.k_stride) && heads_of(*v, B, T, D, type, Hv, a.v_stride) && Hv == a.Hk &&
             (!q || heads_of(*q, B, T, D, type, a.Hq, a.q_stride)) && weight_of(wq, D, type) && weight_of(wk, D, type) &&
             rope_of(rope, D, a) && positions_of(at_, B, T, 2, a) && ints_of(lengths, B) && ints_of(counts, B) &&
-            cache_of(args[0], device, grad, B, a.Hk, D, type, true, c));
+            cache_of(args[0], device, watch, B, a.Hk, D, type, true, c));
     a.k = k->data_ptr();
     a.v = v->data_ptr();
     a.q_weight = wq ? wq->data_ptr() : nullptr;
@@ -437,22 +451,22 @@ PyObject* append_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     OR_NONE(n == 7 && attention_fn && (args[5] == Py_None || PyFloat_CheckExact(args[5])) && args[6] == Py_None);
-    const bool grad = c10::GradMode::is_enabled();
+    const Watch watch = watching();
     int device = -1;
-    const at::Tensor *q = plain(args[0], device, grad), *lengths = q ? plain(args[2], device, grad) : nullptr, *tree, *counts;
-    OR_NONE(lengths && maybe(args[3], tree, device, grad) && maybe(args[4], counts, device, grad) && device == c10::cuda::current_device());
+    const at::Tensor *q = plain(args[0], device, watch), *lengths = q ? plain(args[2], device, watch) : nullptr, *tree, *counts;
+    OR_NONE(lengths && maybe(args[3], tree, device, watch) && maybe(args[4], counts, device, watch) && device == c10::cuda::current_device());
     convnn_tree_attention a{};
     convnn_cache c{};
     const auto type = q->scalar_type();
     const int dt = dtype_code(type);
     OR_NONE(q->dim() == 4 && dt >= 0 && PyTuple_Check(args[1]) && PyTuple_GET_SIZE(args[1]) == 3);
-    const at::Tensor* pages = plain(PyTuple_GET_ITEM(args[1], 0), device, grad);
+    const at::Tensor* pages = plain(PyTuple_GET_ITEM(args[1], 0), device, watch);
     OR_NONE(pages && pages->dim() == 4);
     const int64_t B = q->size(0), T = q->size(1), D = q->size(3), H = pages->size(1), unit = dt == CONVNN_F32 ? 4 : 8;
     OR_NONE(B >= 1 && T >= 1 && T <= MOST_DRAFTED && B <= MOST / T && D >= 1 && D <= MOST_CHANNELS && D % unit == 0 && H >= 1 && H <= (1 << 20));
     a.dtype = dt; a.B = (int32_t)B; a.T = (int32_t)T; a.D = (int32_t)D; a.Hk = (int32_t)H;
     OR_NONE(heads_of(*q, B, T, D, type, a.Hq, a.q_stride) && a.Hq % H == 0 && ints_of(lengths, B) && ints_of(counts, B) &&
-            cache_of(args[1], device, grad, B, H, D, type, false, c));
+            cache_of(args[1], device, watch, B, H, D, type, false, c));
     if (tree) {
         OR_NONE(tree->scalar_type() == at::kLong && tree->dim() == 2 && tree->size(0) == B && tree->size(1) == T);
         a.tree = static_cast<const int64_t*>(tree->data_ptr());

@@ -309,6 +309,7 @@ class MultiHeadConvNNAttention(WatchedModule):
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
                                "(training / backward is outside this library)")
+        ops._forward_only(x)
         if self.training and self.attention_dropout > 0:
             raise RuntimeError("convnn_b200 is forward-only: dropout > 0 needs module.eval()")
         if self.magnitude_type not in ('cosine', 'matmul', 'euclidean'):
@@ -403,9 +404,7 @@ class MultiHeadConvNNAttention(WatchedModule):
 def _library_call(x: torch.Tensor, what: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"convnn_b200.{what} runs on CUDA (sm_100a) only; there is no CPU path")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
-                           "(training / backward is outside this library)")
+    ops._forward_only(x)
 
 
 class _PackedParams:

@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 from . import build as _build
@@ -531,10 +532,20 @@ FP8_BLOCK = 128
 
 
 def _forward_only(*tensors) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
-                               "(training / backward is outside this library)")
+    """Refuses what would want a gradient, or hands a tangent on, of the result."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("convnn_b200 is forward-only: call it under torch.no_grad() "
+                                   "(training / backward is outside this library)")
+    _refuse_tangents(*tensors)
+
+
+def _refuse_tangents(*tensors) -> None:
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():      # (torch.no_grad() does not end this mode)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("convnn_b200 is forward-only: its results carry no tangents, got a dual tensor")
 
 
 # For tensors of the caller's that a kernel has written: autograd notices if it has kept one of them.
@@ -656,8 +667,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     done = (_calls or _bind_calls()).rms_norm(x, weight, eps, residual, quantize)
     if done is not None:
         return done
-    if torch.is_grad_enabled():
-        _forward_only(x, weight, residual)
+    _forward_only(x, weight, residual)
     index = _device_of(x, weight, residual)
     shape, dtype = x.shape, x.dtype
     D = _channels(shape, "rms_norm")
@@ -698,8 +708,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> Fp8Blocks:
     done = (_calls or _bind_calls()).quantize_fp8(x, block_rows)
     if done is not None:
         return done
-    if torch.is_grad_enabled():
-        _forward_only(x)
+    _forward_only(x)
     index = _device_of(x)
     shape = x.shape
     D = _channels(shape, "quantize_fp8")
@@ -747,8 +756,7 @@ def linear_fp8(a, w, bias: Optional[torch.Tensor] = None, gelu: bool = False, re
     if done is not None:
         return done
     (av, sa), (wv, sw) = a, w
-    if torch.is_grad_enabled():
-        _forward_only(av, sa, wv, sw, bias, residual)
+    _forward_only(av, sa, wv, sw, bias, residual)
     index = _device_of(av, sa, wv, sw, bias, residual)
     io = _dtype_code(dtype)
     if av.dtype is not _E4M3 or wv.dtype is not _E4M3:
@@ -946,8 +954,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     done = (_calls or _bind_calls()).qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved, out)
     if done is not None:
         return done
-    if torch.is_grad_enabled():
-        _forward_only(q, k, q_weight, k_weight, rope, *(() if out is None else out))
+    _forward_only(q, k, q_weight, k_weight, rope, *(() if out is None else out))
     like = q if q is not None else k
     if like is None:
         raise ValueError("qk_norm_rope needs queries or keys")
@@ -985,8 +992,7 @@ def append_kv(cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, q:
     done = (_calls or _bind_calls()).append_kv(cache, k, v, lengths, q, q_weight, k_weight, rope, positions, counts, eps, interleaved)
     if done is not None:
         return None if done is False else done
-    if torch.is_grad_enabled():
-        _forward_only(q, k, v, q_weight, k_weight, rope, cache[0], cache[1])
+    _forward_only(q, k, v, q_weight, k_weight, rope, cache[0], cache[1])
     index = _device_of(k, v, lengths, q, q_weight, k_weight, rope, positions, counts, *cache)
     if k.dim() != 4:
         raise ValueError(f"keys must be (sequences, tokens, heads, channels), got {tuple(k.shape)}")
@@ -1023,8 +1029,7 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     done = (_calls or _bind_calls()).tree_attention(q, cache, lengths, tree, counts, scale, out)
     if done is not None:
         return done
-    if torch.is_grad_enabled():
-        _forward_only(q, cache[0], cache[1], out)
+    _forward_only(q, cache[0], cache[1], out)
     index = _device_of(q, lengths, tree, counts, out, *cache)
     if q.dim() != 4:
         raise ValueError(f"queries must be (sequences, tokens, heads, channels), got {tuple(q.shape)}")

@@ -48,7 +48,10 @@ class PatchEmbedding(WatchedModule):
 def _library_path(x: torch.Tensor) -> bool:
     """The fused encoder ops cover CUDA float32 / bfloat16 inference (and, for the model input,
     8-bit images that the patch unfold normalises on the way)."""
-    return x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.uint8) and not torch.is_grad_enabled()
+    if not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16, torch.uint8) or torch.is_grad_enabled():
+        return False
+    ops._refuse_tangents(x)
+    return True
 
 
 class PositionalEncoding(WatchedModule):

@@ -2,6 +2,7 @@
 tables without rows, values that are not finite under weights that vanish, tensors that autograd watches."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from convnn_b200 import _capi, ops
 from heads_util import HALF, randn, turned
@@ -165,3 +166,35 @@ def test_a_layers_result_that_autograd_has_kept():
     ops.softmax_attention(x, w_qkv, w_o, 2, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(both_ways, grad):
+    cache, q, k, w = cache_of(2, 2, 16, 64, 60), randn(2, 1, 4, 64, seed=9, dtype=BF16), randn(2, 1, 2, 64, seed=8, dtype=BF16), randn(64, dtype=BF16)
+    lengths = ints(5, 30)
+    want = ops.tree_attention(q, cache, lengths)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.qk_norm_rope(dual(q), k, w, w), lambda: ops.qk_norm_rope(q, dual(k)[:, :, :1]),
+                     lambda: ops.append_kv(cache, k, k, lengths, q=dual(q)), lambda: ops.append_kv(cache, k, dual(k), lengths),
+                     lambda: ops.tree_attention(dual(q), cache, lengths), lambda: ops.rms_norm(dual(q), w), lambda: ops.rms_norm(q, w, residual=dual(q)),
+                     lambda: ops.quantize_fp8(dual(q)),
+                     lambda: ops.linear_fp8(ops.quantize_fp8(q[:, 0, 0]), ops.quantize_fp8(q[:, 0, 0], 128), bias=dual(w[:2]))):
+            with pytest.raises(RuntimeError, match="no tangents"):
+                call()
+        assert torch.equal(ops.tree_attention(q, cache, lengths), want)
+        # without forward mode a dual tensor is what it holds
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(ops.tree_attention(dual(q), cache, lengths), want)
+
+
+def test_layers_refuse_tangents():
+    import convnn_b200
+    layer = convnn_b200.MultiHeadAttention(64, 2, 0.0).cuda().to(BF16).eval()
+    x = randn(2, 40, 64, seed=1, dtype=BF16)
+    want = layer(x)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no tangents"):
+            layer(forward_ad.make_dual(x, torch.ones_like(x)))
+        assert torch.equal(layer(x), want)

@@ -2,6 +2,7 @@
 is launched, and no pointer is followed."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from convnn_b200 import _capi, ops
 from test_heads_refusals import BF16, I32, attention, on_any_device, paged, t  # noqa: F401
@@ -46,3 +47,26 @@ def test_what_is_written_moves_its_version(on_any_device):  # noqa: F811
     c = paged()
     ops.append_kv(c, t(2, 0, 2, 64), t(2, 0, 2, 64), lengths)
     assert c.k._version == 0
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", range(10))
+def test_tangents_are_refused(on_any_device, which, grad):  # noqa: F811
+    """Forward-only is said of forward mode too: a result would come without its tangent.  torch.no_grad() does not end that mode."""
+    q, k, w = t(2, 1, 4, 64), t(2, 1, 2, 64), t(64)
+    lengths, c = t(2, dtype=I32), paged()
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+        calls = [lambda: ops.qk_norm_rope(dual(q), None), lambda: ops.qk_norm_rope(q, dual(k)), lambda: ops.qk_norm_rope(q, None, dual(w)),
+                 lambda: ops.append_kv(c, dual(k), k, lengths), lambda: ops.append_kv(c._replace(v=dual(c.v)), k, k, lengths),
+                 lambda: ops.append_kv(c, k, k, lengths, q=dual(q)), lambda: ops.tree_attention(dual(q), c, lengths),
+                 lambda: ops.tree_attention(q, c._replace(k=dual(c.k)), lengths), lambda: ops.rms_norm(dual(t(3, 64)), w),
+                 lambda: ops.quantize_fp8(dual(t(3, 64)))]
+        with pytest.raises(RuntimeError, match="no tangents"):
+            calls[which]()
+        assert not on_any_device
+        with forward_ad._set_fwd_grad_enabled(False):
+            if 3 > which or which > 7:
+                calls[which]()
+                assert len(on_any_device) == 1
