@@ -1018,11 +1018,11 @@ bool tiles_wanted(int dtype, int rows, int D) { return dtype == CONVNN_BF16 && r
 
 long long slot_floats(const Plan& g, int D) { return (long long)g.rows_per_tile * (D + 2) + 4; }
 
-// What is asked of the driver once: that a kernel's clusters may have sixteen CTAs (on each device), and how many clusters of 1, 2, 4, 8, 16
-// run at once.
+// What is asked of the driver once on each device: that a kernel's clusters may have sixteen CTAs, and how many clusters of 1, 2, 4, 8, 16 run
+// at once, which goes by its shared memory and so by the channels, a multiple of 4 (one more than that; 0: not asked).
 struct Clusters {
     std::atomic<int> allowed[16];
-    ClusterLimit fit[5];
+    std::atomic<short> fit[16][64][5];
 };
 // As many CTAs a unit, up to p.split, as leave all clusters room at once; p.split = 0 where the even division is the better one: its second
 // kernel takes as long as a CTA's `worth` tiles.
@@ -1048,12 +1048,15 @@ int launch_clusters(void (*kern)(Params), Params& p, unsigned units, int unit_ti
         attr[0].val.clusterDim.x = (unsigned)(p.split = 1 << size);
         cfg.gridDim = units * (unsigned)p.split;
         if (size == 0) break;
-        int clusters = 0;
-        cfg.numAttrs = 1;
-        if (known.fit[size].query(reinterpret_cast<const void*>(kern), &cfg, &clusters)) {       // (none fits)
-            clear_error();
-            cudaGetLastError();
-            clusters = 0;
+        std::atomic<short>* fit = remembered ? &known.fit[device][p.D / 4 - 1][size] : nullptr;
+        int clusters = fit ? fit->load(std::memory_order_relaxed) - 1 : -1;
+        if (clusters < 0) {
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(kern), &cfg) != cudaSuccess) {   // (none fits)
+                cudaGetLastError();
+                clusters = 0;
+            }
+            if (fit) fit->store((short)(clusters + 1), std::memory_order_relaxed);
         }
         if (units <= (unsigned)clusters) break;
     }

@@ -198,3 +198,28 @@ def test_layers_refuse_tangents():
         with pytest.raises(RuntimeError, match="no tangents"):
             layer(forward_ad.make_dual(x, torch.ones_like(x)))
         assert torch.equal(layer(x), want)
+
+
+# ---- what a call asks and launches --------------------------------------------------------------------------------------
+
+def recorded(*calls):
+    """Names of what the calls launch and of what they ask of the driver."""
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU, torch.profiler.ProfilerActivity.CUDA]) as seen:
+        for call in calls:
+            call()
+        torch.cuda.synchronize()
+    return [e.name for e in seen.events()]
+
+
+@pytest.mark.parametrize("dtype,widths", [(F32, range(68, 257, 12)), (BF16, range(136, 257, 8))])
+def test_the_driver_is_asked_once_for_every_width(dtype, widths):
+    """How many clusters run at once goes by the heads' width; a size that does not fit is remembered too."""
+    calls = []
+    for D in widths:
+        cache, q, lengths = cache_of(1, 12, 16, D, 1000, dtype), randn(1, 1, 12, D, dtype=dtype), ints(900)
+        calls.append(lambda q=q, cache=cache, lengths=lengths: ops.tree_attention(q, cache, lengths))
+        calls[-1]()
+    names = recorded(*calls)
+    assert sum("rows_kernel" in n or "scalar_kernel" in n for n in names) == len(calls), set(names)
+    assert not [n for n in names if "Occupancy" in n or "FuncSetAttribute" in n]
