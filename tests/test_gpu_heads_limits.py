@@ -1,11 +1,15 @@
 """Calls of the heads' norm and rotation, the paged cache and the attention over it that their documentation allows and that lie at an edge:
 tables without rows, values that are not finite under weights that vanish, tensors that autograd watches."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from convnn_b200 import _capi, ops
-from heads_util import HALF, randn, turned
+from heads_util import HALF, check_attention, randn, rope_table, turned
 from test_gpu_tree_attention import cache_of, ints
 
 pytestmark = pytest.mark.gpu
@@ -223,3 +227,101 @@ def test_the_driver_is_asked_once_for_every_width(dtype, widths):
     names = recorded(*calls)
     assert sum("rows_kernel" in n or "scalar_kernel" in n for n in names) == len(calls), set(names)
     assert not [n for n in names if "Occupancy" in n or "FuncSetAttribute" in n]
+
+
+def kernels(call):
+    return [n for n in recorded(call) if "_kernel" in n]
+
+
+@pytest.mark.parametrize("dtype,tiles,worth", [(BF16, 64, 6), (F32, 32, 2)])
+def test_clusters_on_one_side_of_the_line_and_the_even_division_on_the_other(dtype, tiles, worth):
+    """Two units: sixteen CTAs each, while those have no more than `worth` tiles of what the table could hold."""
+    q, lengths = randn(1, 2, 2, 64, seed=9, dtype=dtype), ints(500)
+    for room, clusters in ((16 * worth * tiles, True), (16 * worth * tiles + 16, False)):
+        cache = cache_of(1, 2, 16, 64, room, dtype)
+        call = lambda: ops.tree_attention(q, cache, lengths)         # noqa: E731
+        check_attention(call(), q, cache, lengths)
+        names = kernels(call)
+        assert len(names) == (1 if clusters else 2), names
+        assert ("true>" if clusters else "false>") in names[0] and ("rows_kernel" if dtype == BF16 else "scalar_kernel") in names[0]
+        assert clusters or "join_kernel" in names[1]
+
+
+@pytest.mark.parametrize("T,G,D,P,kernel", [(16, 1, 128, 16, "rows_kernel"), (17, 1, 128, 16, "tiles_kernel<2, 3, 3, false>"),
+                                            (32, 4, 64, 16, "tiles_kernel<1, 6, 6, false>"), (43, 3, 64, 48, "tiles_kernel<1, 6, 5, true>"),
+                                            (43, 3, 72, 128, "tiles_kernel<2, 3, 2, true>"), (17, 1, 136, 16, "rows_kernel"),
+                                            (17, 1, 128, 20, "rows_kernel"), (17, 1, 128, 8, "rows_kernel")])
+def test_rows_channels_and_pages_decide_which_kernel(T, G, D, P, kernel):
+    cache, q, lengths = cache_of(2, 2, P, D, 300 + T), randn(2, T, 2 * G, D, seed=9, dtype=BF16), ints(300, 41)
+    call = lambda: ops.tree_attention(q, cache, lengths)             # noqa: E731
+    check_attention(call(), q, cache, lengths)
+    names = kernels(call)
+    assert kernel in names[0] and ("join_tiles_kernel" in names[1] if "tiles" in kernel else True), names
+
+
+# ---- ways to call -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_host_module_answers(dtype):
+    """Ordinary calls are its, and its results those of the Python form."""
+    calls = ops._bind_calls()
+    assert calls is not ops._GeneralCalls
+    rows = randn(2, 3, 10, 64, seed=4, dtype=dtype)
+    q, k, v = rows.split((6, 2, 2), 2)
+    w, rope, lengths, counts = randn(64, seed=5, dtype=dtype) + 1, rope_table(200, 64), ints(100, 7), ints(3, 2)
+    tree, positions = torch.ones(2, 3, dtype=torch.int64, device="cuda"), lengths[:, None] + ints(0, 1, 1)
+
+    def answers(by):
+        cache = cache_of(2, 2, 16, 64, 120, dtype)
+        a = by.qk_norm_rope(q, k, w, None, rope, None, 1e-6, False, None)
+        b = by.append_kv(cache, k, v, lengths, q, w, w, rope, positions, counts, 1e-6, True)
+        nothing = by.append_kv(cache, k, v, lengths, None, None, None, None, None, None, 1e-6, False)
+        c = by.tree_attention(q, cache, lengths, tree, counts, None, None)
+        d = by.tree_attention(q, cache, lengths, None, None, 0.3, None)
+        assert a is not None and b is not None and c is not None and d is not None and not nothing
+        return [*a, b, *cache[:2], c, d], nothing
+
+    (host, done), (python, none) = answers(calls), answers(ops)
+    assert done is False and none is None
+    for x, y in zip(host, python):
+        assert x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y)
+
+
+CAPTURE = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+from convnn_b200 import _capi, ops
+from heads_util import check_attention, randn, rope_table
+torch.set_grad_enabled(False)
+def ints(*x): return torch.tensor(x, dtype=torch.int32, device="cuda")
+made = []
+# one call of each kernel; the width of the table decides between clusters and the even division
+for name, dtype, T, G, D, width in (("rows", torch.bfloat16, 1, 2, 256, 32), ("rows, divided", torch.bfloat16, 1, 2, 64, 4096),
+                                    ("float32", torch.float32, 2, 2, 256, 32), ("float32, divided", torch.float32, 2, 2, 64, 4096),
+                                    ("tiles", torch.bfloat16, 20, 2, 128, 32), ("two tiles", torch.bfloat16, 64, 4, 64, 32)):
+    k = randn(64, 2, 16, D, seed=1, dtype=dtype)
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :32] = torch.arange(32, 64)
+    made.append((name, randn(1, T, 2 * G, D, seed=3, dtype=dtype), ops.PagedCache(k, k.flip(0).contiguous(), table), ints(400)))
+rope, new = rope_table(512, 64), randn(1, 3, 2, 64, seed=4, dtype=torch.bfloat16)
+cache = ops.PagedCache(*(torch.zeros(64, 2, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)), made[0][2].table)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [ops.tree_attention(q, c, lengths) for _, q, c, lengths in made]
+    turned = ops.append_kv(cache, new, new, made[0][3], q=new, rope=rope)
+graph.replay()
+torch.cuda.synchronize()
+for (name, q, c, lengths), out in zip(made, outs):
+    check_attention(out, q, c, lengths)
+assert torch.equal(turned[:, 0].transpose(0, 1), cache.k[32 + 25, :, :1]) and torch.equal(cache.v[32 + 25, :, :3], new[0].transpose(0, 1))
+assert _capi.device_status() == 0
+print("captured", len(outs))
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """Kernels are loaded, their limits raised and the driver asked while a graph is captured."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", CAPTURE.format(path=[os.path.dirname(here), here])], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured 6" in done.stdout, done.stdout + done.stderr
