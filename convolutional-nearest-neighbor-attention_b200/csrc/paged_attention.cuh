@@ -165,6 +165,16 @@ __device__ __forceinline__ unsigned long long seen_by(const Params& p, const Seq
     return (unsigned long long)p.tree[b * p.tree_stride[0] + t * p.tree_stride[1]];
 }
 
+// One over a row's sum of weights, the largest of which is 1.  There is none where a row is not there or sees nothing, whose result is zeros, and
+// where all that it sees has a score of minus infinity, which has no softmax: NaN.
+__device__ __forceinline__ float inverse_of(const Params& p, const Sequence& s, int b, int row, float sum) {
+    if (sum != 0.f) return 1.0f / sum;
+    if (row >= s.count * p.G) return 0.f;
+    const int drafted = s.total - s.length;
+    const unsigned long long there = drafted >= 64 ? ~0ull : (1ull << drafted) - 1;
+    return s.length > 0 || (seen_by(p, s, b, row) & there) ? CUDART_NAN_F : 0.f;
+}
+
 // Values that are not finite do not stay in a product with zero: those of drafted tokens, which some rows see and others do not, are
 // taken out before it (a zero in their place) and added to the rows that see them here, at the end.
 template <typename T>

@@ -130,7 +130,7 @@ __device__ __forceinline__ void join_cluster(const Params& p, const Sequence& s,
                 any_bad |= got_bads[c] != 0;
             }
         }
-        write_four<T>(p, s, b, h, row, 4 * (i - r * fours), y, sum == 0.f ? 0.f : 1.0f / sum, any_bad);
+        write_four<T>(p, s, b, h, row, 4 * (i - r * fours), y, inverse_of(p, s, b, row, sum), any_bad);
     }
 }
 // A part without keys.
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
             if (whole) {
                 const int t = (row0 + r) / p.G, g = row0 + r - t * p.G;
                 if (t >= s.count) continue;
-                const float inv = sL[r] == 0.f ? 0.f : 1.0f / sL[r];
+                const float inv = inverse_of(p, s, b, row0 + r, sL[r]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] *= inv;
                 if (any_bad) {
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                 } else if (!whole) {
                     *reinterpret_cast<float4*>(slot + r * p.D + 4 * col) = y;
                 } else if (t < s.count) {
-                    const float inv = sSum[r] == 0.f ? 0.f : 1.0f / sSum[r];
+                    const float inv = inverse_of(p, s, b, row0 + r, sSum[r]);
                     y.x *= inv; y.y *= inv; y.z *= inv; y.w *= inv;
                     if (any_bad) {
                         const unsigned long long seen = seen_by(p, s, b, row0 + r);
@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
                 all.add(sT[w][0], sT[w][1], x);
             }
         }
-        const float inv = all.sum == 0.f ? 0.f : 1.0f / all.sum;
+        const float inv = inverse_of(p, u.s, u.b, row, all.sum);
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int col = 4 * (lane + 32 * v);
@@ -965,7 +965,7 @@ __global__ void __launch_bounds__(kThreads) join_tiles_kernel(const Params p) {
             bad |= hit[e] != 0.f;
         }
     }
-    const float inv = all.sum == 0.f ? 0.f : 1.0f / all.sum;
+    const float inv = inverse_of(p, u.s, u.b, row, all.sum);
 #pragma unroll
     for (int v = 0; v < FOURS; ++v) {
         const int col = (blockIdx.z * FOURS + v) * 4;

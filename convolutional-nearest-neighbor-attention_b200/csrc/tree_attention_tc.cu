@@ -444,7 +444,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CU
                 f.y = other.x == -CUDART_INF_F ? 0.f : ex2((other.x - top) * tm.factor);
                 const float sum = l * f.x + other.y * f.y;
                 if (whole) {
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                    const float inv = inverse_of(p, s, b, row0 + r, sum);
                     f.x *= inv;
                     f.y *= inv;
                 } else {

@@ -1024,7 +1024,7 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     them and to drafted token ``j`` where bit ``j`` of ``tree[b, t]`` (int64) is set, of which there are ``counts[b]`` (default:
     T); without ``tree`` to every ``j <= t``, so that one token is ordinary decoding.  The heads of ``q`` share the cache's evenly,
     neighbours the same; ``scale`` is by default ``channels ** -0.5``.  Zeros for tokens that are not there or have nothing to attend
-    to; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels, float32 of 4, rows of the
+    to, NaN where every score is minus infinity; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels, float32 of 4, rows of the
     cache on 16-byte boundaries.  -> (B, T, heads, channels) in ``q``'s type, or ``out``."""
     done = (_calls or _bind_calls()).tree_attention(q, cache, lengths, tree, counts, scale, out)
     if done is not None:

@@ -321,7 +321,7 @@ int convnn_b200_append_kv(const convnn_heads* heads, const convnn_cache* cache, 
  * lengths[b] entries.  Token t attends to all entries before them and to drafted token j where bit j of
  * tree[b][t] (int64, strides tree_stride) is set, of the first counts[b]; tree NULL: to j <= t.  Query head h
  * reads key head h / (Hq / Hk).  out (B, T, Hq, D): zeros for tokens from counts[b] on and for those that
- * have nothing to attend to.  What a token does not see may hold anything, infinities and NaN included.
+ * have nothing to attend to; NaN where every score is minus infinity.  What a token does not see may hold anything, infinities and NaN included.
  * Rows of q, out and the cache start on 16-byte boundaries (D a multiple of 8, in float32 of 4). */
 typedef struct convnn_tree_attention {
     int32_t dtype, B, T, Hq, Hk, D;

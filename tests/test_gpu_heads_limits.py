@@ -114,6 +114,28 @@ def test_a_drafted_value_that_is_not_finite_shows_where_it_is_seen(dtype, T, G, 
         assert torch.isnan(got[hit]).all() if bad != bad else (got[hit] == bad).all()
 
 
+@pytest.mark.parametrize("dtype,T,G", [(F32, 3, 2), (F32, 7, 4), (BF16, 3, 2), (BF16, 20, 2), (BF16, 40, 4)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_scores_of_minus_infinity(dtype, T, G, wide):
+    """Among others they are weights of zero; where a token sees nothing else there is no softmax, and the result says so."""
+    B, D = 5, 64
+    cache = cache_of(B, 2, 16, D, 200 + T, dtype)
+    if wide:
+        cache = cache._replace(table=torch.cat([cache.table, torch.full((B, 1 << 16), -1, dtype=torch.int32, device="cuda")], 1))
+    q = randn(B, T, 2 * G, D, seed=9, dtype=dtype).abs() + 0.5
+    lengths, counts = ints(1, 1, 0, 200, 0), ints(T, T - 1, T, T, T)
+    tree = torch.zeros(B, T, dtype=torch.int64, device="cuda")
+    tree[0] = torch.arange(T, device="cuda") % 2            # one or two entries
+    tree[2, 1] = 4                                          # a token that sees the third alone
+    for b, entry in ((0, 0), (1, 0), (2, 2), (3, 7)):
+        cache.k[int(cache.table[b, entry // 16]), 1, entry % 16, 3] = -float("inf")
+    got = ops.tree_attention(q, cache, lengths, tree, counts)
+    check_attention(got, q, cache, lengths, tree, counts)
+    assert torch.isnan(got[0, ::2, G:]).all() and torch.isfinite(got[0, 1::2]).all() and torch.isnan(got[1, :T - 1, G:]).all()
+    assert not got[1, T - 1:].any() and torch.isnan(got[2, 1, G:]).all() and torch.isfinite(got[3]).all()
+    assert not got[2, [t for t in range(T) if t != 1]].any() and not got[4].any()
+
+
 # ---- tensors that autograd watches --------------------------------------------------------------------------------------
 
 def appended(cache, n=2):
