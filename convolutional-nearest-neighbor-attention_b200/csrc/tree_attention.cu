@@ -665,10 +665,12 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
             __syncthreads();
             auto sums = [&](auto rows) {
                 constexpr int R = decltype(rows)::value;
+                float4 part[R];                                          // (a tile's own, so that what is added to a long sum is not small)
+                float f[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
-                    const float f = sF[lr + 4 * i];
-                    o[i].x *= f; o[i].y *= f; o[i].z *= f; o[i].w *= f;
+                    part[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    f[i] = sF[lr + 4 * i];
                 }
 #pragma unroll 2
                 for (int e = key0; e < key1; e += 4) {
@@ -682,12 +684,17 @@ __global__ void __launch_bounds__(kScalarThreads) scalar_kernel(const Params p) 
                         const float ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            o[i].x = fmaf(ws[x], v[x].x, o[i].x);
-                            o[i].y = fmaf(ws[x], v[x].y, o[i].y);
-                            o[i].z = fmaf(ws[x], v[x].z, o[i].z);
-                            o[i].w = fmaf(ws[x], v[x].w, o[i].w);
+                            part[i].x = fmaf(ws[x], v[x].x, part[i].x);
+                            part[i].y = fmaf(ws[x], v[x].y, part[i].y);
+                            part[i].z = fmaf(ws[x], v[x].z, part[i].z);
+                            part[i].w = fmaf(ws[x], v[x].w, part[i].w);
                         }
                     }
+                }
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    o[i].x = fmaf(o[i].x, f[i], part[i].x); o[i].y = fmaf(o[i].y, f[i], part[i].y);
+                    o[i].z = fmaf(o[i].z, f[i], part[i].z); o[i].w = fmaf(o[i].w, f[i], part[i].w);
                 }
             };
             if (sums_here) {

@@ -136,6 +136,20 @@ def test_scores_of_minus_infinity(dtype, T, G, wide):
     assert not got[2, [t for t in range(T) if t != 1]].any() and not got[4].any()
 
 
+# ---- long sums ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("G,T", [(1, 1), (4, 1), (8, 1), (3, 5)])
+def test_long_sums_in_float32(G, T):
+    """Equal weights and values that a sum of thousands of them rounds the same way each time.  Tiles of 32 keys are summed before they are
+    added to what came before: 32 roundings of a tile's sum, one for each of 512 tiles, and at most 40 of pieces and of what follows, half a
+    step of 2^-24 each; 16384 of them one after the other are off by more than three times that."""
+    n, D, B, v = 16384, 256, 160, 1 + 2.0 ** -12
+    k = randn(n // 64, 1, 64, D, seed=1)
+    cache = ops.PagedCache(k, torch.full_like(k, v), torch.arange(n // 64, dtype=torch.int32, device="cuda").repeat(B, 1))
+    got = ops.tree_attention(torch.zeros(B, T, G, D, device="cuda"), cache, torch.full((B,), n - T, dtype=torch.int32, device="cuda"))
+    assert float((got.double() / v - 1).abs().max()) <= (32 + n // 32 + 40) * 2.0 ** -24
+
+
 # ---- tensors that autograd watches --------------------------------------------------------------------------------------
 
 def appended(cache, n=2):
