@@ -9,13 +9,14 @@
 // 128: 308 us for 1.87 GB, 6.05 TB/s (92 % of a plain copy's rate; 5.4 after a second of it, when the clock falls to 1700 MHz).  Three slices
 // in flight per warp instead of two (the queries' room for the warps' sums) gain nothing: 324 us; pages asked for a slice ahead 316.
 // scalar_kernel (float32): 16 rows on the fp32 pipes, tiles of 32 keys through a ring of the whole CTA, four rows by four keys or channels a
-// thread.
+// thread; 64 units of 4096 entries of 128 channels 81 us, twice what their bytes take.  Three barriers a tile are what is waited for.
 // tree_attention_tc.cu (bfloat16, more rows, up to 128 channels, pages of a multiple of 16 entries): tcgen05.  16 sequences of 32 to 64 tokens, 32
 // query heads: 1536 us with rows_kernel, 16 rows at a time.
 // join_kernel: units that several CTAs had, and rows without anything.
 // Where the cache is short, the second kernel costs more than the even division gains: a cluster of up to sixteen CTAs has a unit, and they
 // join through their shared memories (one token of 12 heads over 1000 entries: 10.6 us with two kernels, 5.6 in one, of which 0.6 us
-// are each of the lengths, the table and the first keys, read one after the other).
+// are each of the lengths, the table and the first keys, read one after the other).  The host goes by what the tables could hold: a table
+// 64 times as wide as those entries need is divided evenly (9.3 us).
 #include <math.h>
 
 #include <type_traits>
@@ -183,7 +184,8 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
     const bool one_page = p.page_size % 16 == 0 && p.ks[2] < (1 << 26) && p.vs[2] < (1 << 26);
     const int k_row = (int)p.ks[2], v_row = (int)p.vs[2];
 
-    // The page of a lane's row of this warp's slice of ahead's tile is asked for a slice before it is copied; lanes 16 apart have one row.
+    // The page of a lane's row of this warp's slice of ahead's tile; lanes 16 apart have one row.  In a cluster it is asked for a slice before
+    // it is copied, in the even division where it is (sooner is slower there, see above).
     int next_row = 0, next_page = -1;
     auto look_up = [&]() {
         const int first = ahead.tile * 64 + warp * 16, entry = one_page ? first : first + (lane & 15), slot = p.slot_at(entry);
@@ -210,7 +212,6 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const Params p) {
                     v += page * p.vs[0] + row * p.vs[2];
                 }
                 ahead.next(p);
-                if (SPLIT) look_up();
                 if (rows >= 16) {
 #pragma unroll
                     for (int i = 0; i < DS; ++i) {

@@ -950,7 +950,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     R / 2)``, with ``interleaved`` ``(2 i, 2 i + 1)``, of its first ``R`` channels are turned by the angle whose cosine and sine are in
     ``rope`` (positions, R) float32, cosines first, at row ``positions`` (..., tokens) int32, by default the token's index.  A
     position outside ``rope`` makes NaN of the turned channels.  -> (q, k), rounded once; ``out`` a pair to write to, which may be
-    ``q`` and ``k``."""
+    ``q`` and ``k``, and else lies apart from them."""
     done = (_calls or _bind_calls()).qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved, out)
     if done is not None:
         return done
@@ -1024,8 +1024,8 @@ def tree_attention(q: torch.Tensor, cache, lengths: torch.Tensor, tree: Optional
     them and to drafted token ``j`` where bit ``j`` of ``tree[b, t]`` (int64) is set, of which there are ``counts[b]`` (default:
     T); without ``tree`` to every ``j <= t``, so that one token is ordinary decoding.  The heads of ``q`` share the cache's evenly,
     neighbours the same; ``scale`` is by default ``channels ** -0.5``.  Zeros for tokens that are not there or have nothing to attend
-    to, NaN where every score is minus infinity; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels, float32 of 4, rows of the
-    cache on 16-byte boundaries.  -> (B, T, heads, channels) in ``q``'s type, or ``out``."""
+    to, NaN where every score is minus infinity; what a token does not see may hold anything.  bfloat16 heads of a multiple of 8 channels,
+    float32 of 4, rows of the cache on 16-byte boundaries.  Up to 2^30 tokens.  -> (B, T, heads, channels) in ``q``'s type, or ``out``."""
     done = (_calls or _bind_calls()).tree_attention(q, cache, lengths, tree, counts, scale, out)
     if done is not None:
         return done

@@ -322,7 +322,8 @@ int convnn_b200_append_kv(const convnn_heads* heads, const convnn_cache* cache, 
  * tree[b][t] (int64, strides tree_stride) is set, of the first counts[b]; tree NULL: to j <= t.  Query head h
  * reads key head h / (Hq / Hk).  out (B, T, Hq, D): zeros for tokens from counts[b] on and for those that
  * have nothing to attend to; NaN where every score is minus infinity.  What a token does not see may hold anything, infinities and NaN included.
- * Rows of q, out and the cache start on 16-byte boundaries (D a multiple of 8, in float32 of 4). */
+ * Rows of q, out and the cache start on 16-byte boundaries (D a multiple of 8, in float32 of 4).  Up to 2^30
+ * tokens, B * T.  lengths, counts and the table may not change while the call runs.  out may be q. */
 typedef struct convnn_tree_attention {
     int32_t dtype, B, T, Hq, Hk, D;
     float scale;

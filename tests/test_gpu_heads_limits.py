@@ -323,6 +323,19 @@ def test_the_host_module_answers(dtype):
         assert x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype,T,G", [(BF16, 1, 4), (BF16, 3, 3), (BF16, 20, 2), (BF16, 64, 4), (F32, 1, 4), (F32, 9, 3)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_results_over_the_queries(dtype, T, G, wide):
+    cache = cache_of(3, 2, 16, 64, 3000, dtype)
+    if wide:
+        cache = cache._replace(table=torch.cat([cache.table, torch.full((3, 1 << 16), -1, dtype=torch.int32, device="cuda")], 1))
+    rows, lengths, counts = randn(3, T, 2 * G + 1, 64, seed=9, dtype=dtype), ints(2900, 0, 40), ints(T, T, max(0, T - 1))
+    q, last = rows[:, :, :-1], rows[:, :, -1].clone()
+    want = ops.tree_attention(q, cache, lengths, counts=counts)
+    got = ops.tree_attention(q, cache, lengths, counts=counts, out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(rows[:, :, -1], last)
+
+
 CAPTURE = """
 import sys
 sys.path[:0] = {path!r}
