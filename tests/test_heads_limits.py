@@ -1,11 +1,11 @@
-"""Sizes and tables at the edge of what heads, the paged cache and the attention over it take, on the CPU: no kernel
-is launched, and no pointer is followed."""
+"""Sizes and tables at the edge of what heads, the paged cache and the attention over it take, and tensors that autograd watches, on the
+CPU: no kernel is launched, and no pointer is followed."""
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from convnn_b200 import _capi, ops
-from test_heads_refusals import BF16, I32, attention, on_any_device, paged, t  # noqa: F401
+from test_heads_refusals import I32, attention, on_any_device, paged, t  # noqa: F401
 
 
 @pytest.mark.parametrize("B,T", [((1 << 30) + 1, 1), ((1 << 24) + 1, 64), (1 << 25, 64), ((1 << 31) - 1, 63), (17895698, 61)])
